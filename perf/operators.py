@@ -357,6 +357,7 @@ def _plain_sample(state):
     cum = w.cumsum(-1)
     n = live.sum(-1)
     k = torch.where(state["top_k"] > 0, torch.minimum(state["top_k"].long(), n), n)
+    k = torch.where(t[:, 0] > 0, k, 1)
     mass = cum.gather(1, k[:, None] - 1)
     p = state["top_p"].double()[:, None]
     n_p = torch.where(state["top_p"] < 1, (cum < p * mass).sum(-1) + 1, k)
