@@ -19,7 +19,8 @@
  *
  * Numerics: binary32 accumulation with a fixed, documented reduction order (see
  * the kernel sources), outputs rounded to nearest even.  Results are bit-for-bit
- * reproducible on the CPU.
+ * reproducible on the CPU, except where an entry point says otherwise (the matrix-core
+ * GEMMs and the operators of the last section: tolerances, or results stated exactly).
  */
 #ifndef THINTENSOR_HIP_H
 #define THINTENSOR_HIP_H
@@ -759,6 +760,97 @@ const uint8_t* tt_archive_data(const tt_archive* archive);
  * Returns once the last chunk is queued; calls on one archive are serialized. */
 int tt_archive_upload(tt_archive* archive, int64_t offset, int64_t nbytes, void* dst, void* stream);
 int tt_archive_close(tt_archive* archive);
+
+/* ---------------------------------------------------------------- a decode step around its weights
+ * Rotary positions, a KV cache of 4 bits and sampling for rows of requests with their own
+ * positions, lengths and settings.  No reference kernel: the reference rotates whole heads
+ * from a table, keeps 16-bit caches and takes the argmax (gpu_runtime.py:8754-8785,
+ * 3929-4769; triton_kernels.py:2248-2537). */
+
+/* Rotates q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (kv_heads may be 0)
+ * to their positions: for i < rotary/2, t = positions[token] inv_freq[i], the pair (a, b) of
+ * dims (i, i + rotary/2) -- (2i, 2i + 1) with `interleaved` -- becomes amplitude times
+ * (a cos t - b sin t, b cos t + a sin t); dims past `rotary` are copied.  Outputs may be the
+ * inputs themselves, but not overlap them otherwise.  inv_freq is binary64 (radians per
+ * position): t is formed and reduced in binary64, the rotation in binary32, rounded once.
+ * Strides of tokens and heads are free, the last axis is contiguous.  positions are int32 or
+ * int64 (position_bytes 4 or 8), negative ones included. */
+int tt_rotary_rows(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                   int dtype, const void* positions, int position_bytes, const double* inv_freq, float amplitude,
+                   int interleaved, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rotary,
+                   void* q_out, int64_t qo_token, int64_t qo_head, void* k_out, int64_t ko_token, int64_t ko_head,
+                   void* stream);
+
+/* A KV cache of 4 bits for `batch` sequences.  Groups of group_size (32, 64 or 128) dims of one
+ * token and KV head share a step s and a minimum m (fp16): value = code s + m, code 0 .. 15.
+ *   k_codes  uint32 [batch, kv_heads, capacity, head_dim/8], dim d in nibble d % 8 of word d/8
+ *   k_scales fp16   [batch, kv_heads, capacity, groups, 2]   (s, m)
+ *   v_codes  uint32 [batch, kv_heads, capacity/8, head_dim], token t of a block of eight in
+ *            nibble t/2 + 4 (t % 2) of the dim's word
+ *   v_scales fp16   [batch, kv_heads, capacity/8, groups, 2, 8]   (s of eight tokens, m of eight)
+ * Strides of sequences and heads are free, the inner axes contiguous; codes and v_scales start on
+ * 16-byte boundaries in every sequence and head, k_scales on 4 times groups / 8 bytes (4 at least).
+ * head_dim 64, 128 or 256; capacity a multiple of 32.  s has at most seven significant bits, so
+ * that code s is exact in fp16. */
+typedef struct {
+  void *k_codes, *k_scales, *v_codes, *v_scales;
+  int64_t kc_seq, kc_head, ks_seq, ks_head; /* in elements of each array */
+  int64_t vc_seq, vc_head, vs_seq, vs_head;
+  int64_t batch, kv_heads, capacity, head_dim, group_size;
+} tt_int4_cache;
+
+int64_t tt_int4_cache_size(void); /* sizeof(tt_int4_cache), for bindings */
+
+/* Packs `tokens` tokens of k and v [rows, tokens, kv_heads, head_dim] into sequences 0 .. rows - 1
+ * of the cache from position starts[row] on; counts (or NULL: all) says how many of a row's tokens
+ * count.  Tokens that would lie before position 0 or past the capacity are left out.  A group's m
+ * is its minimum rounded to fp16 (limited to the finite values), s the smallest value of seven
+ * significant bits (a multiple of 2^-24, at most 4352) with 15 s >= maximum - m, and codes are
+ * (x - m) / s rounded to the nearest, ties to even, limited to 0 .. 15, all as if in exact
+ * arithmetic.  A group that holds an infinity or a NaN reads as NaN.  Strides of rows, tokens and
+ * heads are free. */
+int tt_kv_append_int4(const tt_int4_cache* cache, const void* k, int64_t k_row, int64_t k_token, int64_t k_head,
+                      const void* v, int64_t v_row, int64_t v_token, int64_t v_head, int dtype,
+                      const int32_t* starts, const int32_t* counts, int64_t rows, int64_t tokens, void* stream);
+
+/* The inverse: tokens starts[row] .. of rows 0 .. rows - 1 as code s + m (rounded to binary32, then
+ * to the output type) to k_out and v_out, laid out as tt_kv_append_int4 takes them.  Tokens outside
+ * 0 .. capacity - 1 or past counts[row] are left as they were. */
+int tt_kv_read_int4(const tt_int4_cache* cache, void* k_out, int64_t k_row, int64_t k_token, int64_t k_head, void* v_out,
+                    int64_t v_row, int64_t v_token, int64_t v_head, int dtype, const int32_t* starts,
+                    const int32_t* counts, int64_t rows, int64_t tokens, void* stream);
+
+/* Attention of one query token per sequence to the cache's sequences 0 .. rows - 1: q and out
+ * [rows, heads, head_dim], heads a multiple of the cache's kv_heads.  Row r sees token t where
+ * t < n = min(max(lengths[r], 0), capacity, max_length) and, with window > 0, t >= n - window or
+ * t < first_tokens.  out = sum p v with p the softmax of scale q.k and, where sinks [heads] is
+ * given, of the sink's logit, which carries no value.  A row that sees nothing is 0; a row whose q
+ * is not finite is NaN.  max_length bounds what the launch is sized for.
+ * scratch: tt_gqa_attention_int4_scratch_floats of the same arguments (0: none is needed), for one
+ * call at a time. */
+int64_t tt_gqa_attention_int4_scratch_floats(const tt_int4_cache* cache, int64_t rows, int64_t heads, int64_t window,
+                                             int64_t first_tokens, int64_t max_length);
+int tt_gqa_attention_int4(const tt_int4_cache* cache, const void* q, int64_t q_row, int64_t q_head, int dtype,
+                          const int32_t* lengths, int64_t rows, int64_t heads, int64_t window, int64_t first_tokens,
+                          int64_t max_length, const void* sinks, int sink_dtype, float scale, float* scratch,
+                          int64_t scratch_floats, void* out, int64_t out_row, int64_t out_head, void* stream);
+
+/* One token per row of logits [rows, vocab] from uniforms[row] in [0, 1).  Order: logits
+ * descending, equal ones (+0 and -0 among them) by index; -inf and NaN are left out.  Weights
+ * w = exp((x - max) / temperature); kept: the first top_k of the order, of these the shortest
+ * beginning whose weight is at least top_p of theirs, of these the ones with w >= min_p (the first
+ * always).  The token is the first whose cumulative weight exceeds uniforms[row] times that of the
+ * kept ones; its share of them goes to probs (or NULL).  Settings are per row, or NULL for none:
+ * temperature <= 0 takes the first of the order, top_k <= 0, top_p >= 1 and min_p <= 0 keep all,
+ * NaN settings count as none (NaN temperature as 0); uniforms outside [0, 1) count as the nearest
+ * value inside.  A row without a logit above -inf gives token -1 and share 0.
+ * Weights are binary64 and are added in units of 2^-43 of the largest, so that no order of adding
+ * changes a result.  scratch: tt_sample_rows_scratch_bytes, 16-byte aligned, for one call at a time. */
+int64_t tt_sample_rows_scratch_bytes(int64_t rows, int64_t vocab);
+int tt_sample_rows(const void* logits, int64_t row_stride, int dtype, int64_t rows, int64_t vocab,
+                   const float* uniforms, const float* temperature, const int32_t* top_k, const float* top_p,
+                   const float* min_p, void* scratch, int64_t scratch_bytes, int64_t* tokens, float* probs,
+                   void* stream);
 
 #ifdef __cplusplus
 }

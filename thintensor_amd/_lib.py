@@ -73,6 +73,19 @@ class ArchiveRecord(ctypes.Structure):
         ("checksum", ctypes.c_uint8 * 32),
     ]
 
+
+class Int4Cache(ctypes.Structure):
+    """tt_int4_cache: pointers, strides (elements) and sizes of a 4-bit KV cache."""
+    _fields_ = [
+        ("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P),
+        ("kc_seq", _L), ("kc_head", _L), ("ks_seq", _L), ("ks_head", _L),
+        ("vc_seq", _L), ("vc_head", _L), ("vs_seq", _L), ("vs_head", _L),
+        ("batch", _L), ("kv_heads", _L), ("capacity", _L), ("head_dim", _L), ("group_size", _L),
+    ]
+
+
+_CP = ctypes.POINTER(Int4Cache)
+
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES: dict[str, list] = {
     "tt_version": [],
@@ -152,6 +165,14 @@ SIGNATURES: dict[str, list] = {
     "tt_requantize_mxfp4_lowbit": [_P, _P, _L, _I, _P, _P, _P],
     "tt_quantize_dense_lowbit": [_P, _I, _L, _L, _L, _I, _P, _P, _P],
     "tt_pack_mxfp4_ternary": [_P, _L, _L, _P, _P],
+    "tt_rotary_rows": [_P, _L, _L, _P, _L, _L, _I, _P, _I, _P, _F, _I, _L, _L, _L, _L, _L, _P, _L, _L, _P, _L, _L, _P],
+    "tt_int4_cache_size": [],
+    "tt_kv_append_int4": [_CP, _P, _L, _L, _L, _P, _L, _L, _L, _I, _P, _P, _L, _L, _P],
+    "tt_kv_read_int4": [_CP, _P, _L, _L, _L, _P, _L, _L, _L, _I, _P, _P, _L, _L, _P],
+    "tt_gqa_attention_int4_scratch_floats": [_CP, _L, _L, _L, _L, _L],
+    "tt_gqa_attention_int4": [_CP, _P, _L, _L, _I, _P, _L, _L, _L, _L, _L, _P, _I, _F, _P, _L, _P, _L, _L, _P],
+    "tt_sample_rows_scratch_bytes": [_L, _L],
+    "tt_sample_rows": [_P, _L, _I, _L, _L, _P, _P, _P, _P, _P, _P, _L, _P, _P, _P],
     "tt_archive_open": [ctypes.c_char_p, ctypes.POINTER(_P)],
     "tt_archive_parse_pages": [_P],
     "tt_archive_check_overlaps": [_P],
@@ -163,7 +184,8 @@ SIGNATURES: dict[str, list] = {
     "tt_archive_close": [_P],
 }
 _RESTYPES = {"tt_last_error": ctypes.c_char_p, "tt_matvec_argmax_partials": ctypes.c_int64,
-             "tt_batched_workspace_floats": ctypes.c_int64,
+             "tt_batched_workspace_floats": ctypes.c_int64, "tt_int4_cache_size": ctypes.c_int64,
+             "tt_gqa_attention_int4_scratch_floats": ctypes.c_int64, "tt_sample_rows_scratch_bytes": ctypes.c_int64,
              "tt_norm_router_workspace_bytes": ctypes.c_int64,
              "tt_stream_read_waves": ctypes.c_int64,
              "tt_matvec_argmax_batched_partials": ctypes.c_int64, "tt_archive_find": ctypes.c_int64,
@@ -210,6 +232,9 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         if (seg.value, desc.value) != (ctypes.sizeof(FusedSegment), ctypes.sizeof(FusedGemv)):
             raise KernelLibraryError(f"fused descriptor layout mismatch: library {seg.value}/{desc.value} bytes, "
                                      f"binding {ctypes.sizeof(FusedSegment)}/{ctypes.sizeof(FusedGemv)}")
+        if lib.tt_int4_cache_size() != ctypes.sizeof(Int4Cache):
+            raise KernelLibraryError(f"4-bit cache descriptor mismatch: library {lib.tt_int4_cache_size()} bytes, binding "
+                                     f"{ctypes.sizeof(Int4Cache)}")
         _lib = lib
         return lib
 

@@ -15,6 +15,7 @@ depends only on the tensor shapes.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import Any
@@ -22,6 +23,7 @@ from typing import Any
 import torch
 
 from . import _lib
+from .kv_cache import Int4KvCache
 
 _DTYPE_CODE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
@@ -50,6 +52,14 @@ def _stream(t: torch.Tensor) -> int:
     if not t.is_cuda:
         raise ValueError("HipDecodeBackend operates on device tensors only")
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _device_of(t: torch.Tensor):
+    """Makes the tensor's GPU the current one, where it is not already."""
+    return _NO_GUARD if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _require_cuda(*tensors: torch.Tensor) -> None:
@@ -1537,6 +1547,163 @@ class HipDecodeBackend:
         )
         _lib.check(rc, "fused_lm_head_argmax")
         return self._argmax_out_idx
+
+    # ------------------------------------------------------------ a decode step around its weights (no reference counterpart)
+    @staticmethod
+    def _on_device(t: torch.Tensor, *others: torch.Tensor | None) -> None:
+        """Every tensor on the first one's GPU."""
+        _require_cuda(t)
+        device = t.device
+        for o in others:
+            if o is not None and o.device != device:
+                raise ValueError(f"tensors on different devices: {device} and {o.device}")
+
+    def rotary_rows(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                    q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, *,
+                    interleaved: bool = False, amplitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """Rotate q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] to ``positions``
+        [tokens] (int32 or int64): the first 2 * len(inv_freq) dims of every head in pairs
+        (i, i + half), or (2i, 2i + 1) with ``interleaved``, by position * inv_freq[i] radians and
+        times ``amplitude``; the other dims are copied.  ``inv_freq`` is float64
+        (:func:`thintensor_amd.rotary.rotary_frequencies`).  Without outputs in place; an output may be
+        its input but not overlap one otherwise."""
+        q_out = q if q_out is None else q_out
+        k_out = k if k_out is None else k_out
+        if q.ndim != 3 or (k is not None and (k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+            raise ValueError("rotary_rows takes q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim]")
+        if q_out.shape != q.shape or (k is not None and k_out.shape != k.shape) or (k is None and k_out is not None):
+            raise ValueError("rotary_rows outputs must have their inputs' shapes")
+        if q_out.dtype != q.dtype or (k is not None and (k.dtype != q.dtype or k_out.dtype != q.dtype)):
+            raise ValueError("rotary_rows operands must share a dtype")
+        tokens, heads, head_dim = q.shape
+        if positions.numel() != tokens or not positions.is_contiguous() or \
+                positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError("rotary_rows takes one int32 or int64 position per token")
+        if inv_freq.dtype != torch.float64 or inv_freq.ndim != 1 or not inv_freq.is_contiguous():
+            raise ValueError("rotary_rows frequencies must be a contiguous float64 vector")
+        if any(t is not None and t.stride(2) != 1 for t in (q, k, q_out, k_out)):
+            raise ValueError("rotary_rows operands must be contiguous in their last axis")
+        self._on_device(q, k, positions, inv_freq, q_out, k_out)
+        with _device_of(q):
+            rc = self.lib.tt_rotary_rows(
+                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr() if k is not None else None,
+                k.stride(0) if k is not None else 0, k.stride(1) if k is not None else 0, _code(q, "rotary_rows"),
+                positions.data_ptr(), positions.element_size(), inv_freq.data_ptr(), float(amplitude), int(interleaved),
+                tokens, heads, int(k.shape[1]) if k is not None else 0, head_dim, 2 * inv_freq.numel(),
+                q_out.data_ptr(), q_out.stride(0), q_out.stride(1), k_out.data_ptr() if k is not None else None,
+                k_out.stride(0) if k is not None else 0, k_out.stride(1) if k is not None else 0, _stream(q))
+        _lib.check(rc, "rotary_rows")
+        return q_out, k_out
+
+    def _kv_rows(self, entry, what: str, cache: Int4KvCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+                 counts: torch.Tensor | None) -> None:
+        if k.ndim not in (3, 4) or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError(f"{what} takes k and v [rows, tokens, kv_heads, head_dim] (or [rows, kv_heads, head_dim])")
+        rows, tokens = int(k.shape[0]), int(k.shape[1]) if k.ndim == 4 else 1
+        if rows > cache.batch or k.shape[-2] != cache.kv_heads or k.shape[-1] != cache.head_dim:
+            raise ValueError(f"{what}: {tuple(k.shape)} does not fit a cache of {cache.batch} sequences, "
+                             f"{cache.kv_heads} KV heads of {cache.head_dim}")
+        if k.stride(-1) != 1 or v.stride(-1) != 1:
+            raise ValueError(f"{what}: k and v must be contiguous in their last axis")
+        for t in (starts, counts):
+            if t is not None and (t.dtype != torch.int32 or t.numel() != rows or not t.is_contiguous()):
+                raise ValueError(f"{what}: starts and counts must be int32, one per row")
+        self._on_device(k, v, starts, counts, cache.k_codes)
+        with _device_of(k):
+            rc = entry(
+                cache.desc, k.data_ptr(), k.stride(0), k.stride(1) if k.ndim == 4 else 0, k.stride(-2), v.data_ptr(),
+                v.stride(0), v.stride(1) if v.ndim == 4 else 0, v.stride(-2), _code(k, what), starts.data_ptr(),
+                counts.data_ptr() if counts is not None else None, rows, tokens, _stream(k))
+        _lib.check(rc, what)
+
+    def kv_append_int4(self, cache: Int4KvCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+                       counts: torch.Tensor | None = None) -> None:
+        """Pack k and v [rows, tokens, kv_heads, head_dim] (one token: [rows, kv_heads, head_dim]),
+        fp16, bf16 or fp32, into sequences 0 .. rows - 1 of ``cache`` from positions ``starts`` (int32
+        [rows]) on; ``counts`` (int32 [rows]) limits how many of a row's tokens are taken.  Tokens that
+        would lie outside the cache are left out; others of the cache keep their contents."""
+        self._kv_rows(self.lib.tt_kv_append_int4, "kv_append_int4", cache, k, v, starts, counts)
+
+    def kv_read_int4(self, cache: Int4KvCache, k_out: torch.Tensor, v_out: torch.Tensor, starts: torch.Tensor,
+                     counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The inverse of :meth:`kv_append_int4`: the values that the cache holds, to outputs laid out
+        as its inputs.  Tokens outside the cache or past ``counts`` are left as they were."""
+        self._kv_rows(self.lib.tt_kv_read_int4, "kv_read_int4", cache, k_out, v_out, starts, counts)
+        return k_out, v_out
+
+    def gqa_attention_int4(self, q: torch.Tensor, cache: Int4KvCache, out: torch.Tensor, lengths: torch.Tensor, *,
+                           window: int = 0, first_tokens: int = 0, sinks: torch.Tensor | None = None,
+                           scale: float | None = None, max_length: int | None = None) -> torch.Tensor:
+        """Attention of one query token per sequence over a 4-bit cache: q and out [rows, heads,
+        head_dim] fp16 or bf16, ``lengths`` int32 [rows] the tokens that a row's sequence holds (its
+        own included).  With ``window`` > 0 a row sees its last ``window`` tokens and the sequence's
+        first ``first_tokens``; ``sinks`` [heads] are logits that join the softmax and carry no value.
+        ``scale`` is head_dim ** -0.5 by default.  ``max_length`` (by default the capacity) bounds the
+        lengths, longer ones count as it, and sizes the launch.  A row that sees nothing is 0.  Scratch
+        of long contexts comes from the current stream's allocator with every call."""
+        if q.ndim != 3 or out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("gqa_attention_int4 takes q and out [rows, heads, head_dim] of one dtype")
+        rows, heads, head_dim = q.shape
+        if head_dim != cache.head_dim or heads == 0 or heads % cache.kv_heads or rows > cache.batch:
+            raise ValueError(f"gqa_attention_int4: q {tuple(q.shape)} does not fit a cache of {cache.batch} sequences, "
+                             f"{cache.kv_heads} KV heads of {cache.head_dim}")
+        if q.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"gqa_attention_int4 takes fp16 or bf16 queries, got {q.dtype}")
+        if q.stride(2) != 1 or out.stride(2) != 1:
+            raise ValueError("gqa_attention_int4: q and out must be contiguous in their last axis")
+        if lengths.dtype != torch.int32 or lengths.numel() != rows or not lengths.is_contiguous():
+            raise ValueError("gqa_attention_int4: lengths must be int32, one per row")
+        if sinks is not None and (sinks.numel() != heads or not sinks.is_contiguous()):
+            raise ValueError("gqa_attention_int4: sinks must hold one logit per query head")
+        limit = cache.capacity if max_length is None else int(max_length)
+        self._on_device(q, out, lengths, sinks, cache.k_codes)
+        with _device_of(q):
+            need = self.lib.tt_gqa_attention_int4_scratch_floats(cache.desc, rows, heads, int(window), int(first_tokens), limit)
+            if need < 0:
+                _lib.check(int(need), "gqa_attention_int4")
+            scratch = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
+            rc = self.lib.tt_gqa_attention_int4(
+                cache.desc, q.data_ptr(), q.stride(0), q.stride(1), _code(q, "gqa_attention_int4"), lengths.data_ptr(), rows,
+                heads, int(window), int(first_tokens), limit, sinks.data_ptr() if sinks is not None else None,
+                _code(sinks, "sinks") if sinks is not None else _lib.F32,
+                float(scale) if scale is not None else head_dim ** -0.5, scratch.data_ptr() if scratch is not None else None,
+                need, out.data_ptr(), out.stride(0), out.stride(1), _stream(q))
+        _lib.check(rc, "gqa_attention_int4")
+        return out
+
+    def sample_rows(self, logits: torch.Tensor, uniforms: torch.Tensor, tokens: torch.Tensor, *,
+                    temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+                    top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
+                    probs: torch.Tensor | None = None) -> torch.Tensor:
+        """One token per row of ``logits`` [rows, vocab] (fp16, bf16 or fp32) from ``uniforms``
+        (float32 [rows], in [0, 1)) to ``tokens`` (int64 [rows]).  Tokens are ordered by logit, equal
+        ones by index; of exp(logit / temperature) are kept the first ``top_k``, of these the shortest
+        beginning that holds ``top_p`` of their weight, of these the ones of at least ``min_p`` times the
+        largest; the token is where the cumulative weight passes uniforms times that of the kept.
+        Settings are per row (float32, ``top_k`` int32) or None; a temperature of 0 is greedy, a top_k
+        of 0 keeps all.  ``probs`` (float32 [rows]) takes the token's share of the kept weight.  Logits
+        of -inf and NaN are never taken; a row without others gives token -1 and share 0."""
+        if logits.ndim != 2 or logits.stride(1) != 1 or logits.shape[1] == 0:
+            raise ValueError("sample_rows takes logits [rows, vocab], contiguous in the vocabulary")
+        rows, vocab = logits.shape
+        if tokens.dtype != torch.int64 or tokens.numel() != rows or not tokens.is_contiguous():
+            raise ValueError("sample_rows: tokens must be a contiguous int64 tensor, one per row")
+        for name, t, dtype in (("uniforms", uniforms, torch.float32), ("temperature", temperature, torch.float32),
+                               ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                               ("min_p", min_p, torch.float32), ("probs", probs, torch.float32)):
+            if t is not None and (t.dtype != dtype or t.numel() != rows or not t.is_contiguous()):
+                raise ValueError(f"sample_rows: {name} must be contiguous {dtype}, one per row")
+        self._on_device(logits, uniforms, tokens, temperature, top_k, top_p, min_p, probs)
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        with _device_of(logits):
+            need = self.lib.tt_sample_rows_scratch_bytes(rows, vocab)
+            scratch = torch.empty(need, device=logits.device, dtype=torch.uint8)
+            rc = self.lib.tt_sample_rows(
+                logits.data_ptr(), logits.stride(0), _code(logits, "sample_rows"), rows, vocab, uniforms.data_ptr(),
+                ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), scratch.data_ptr(), need, tokens.data_ptr(),
+                ptr(probs), _stream(logits))
+        _lib.check(rc, "sample_rows")
+        return tokens
 
     # ------------------------------------------------------------ decode-step helpers (no reference counterpart)
     def embedding(self, embed: torch.Tensor, token: torch.Tensor | int, out: torch.Tensor) -> torch.Tensor:

@@ -1,0 +1,479 @@
+// Decode attention over the 4-bit KV cache (tt_int4_cache in thintensor_hip.h), one query token per
+// sequence, with a window and first tokens, on the 16-bit matrix cores.
+//
+// A stored value is c s + m with s of seven significant bits, so f16(c s) is exact and
+//   q.k_t  = sum_d q_d (c s)_td + sum_groups m_tg (sum of q over the group),
+//   out_d  = sum_t p_t (c s)_td + sum_t p_t m_tg
+// are products of exact f16 operands added in binary32 (v_mfma_f32_16x16x32_f16):
+//   * q is scaled by a power of two per head (its largest element to [2^7, 2^8)), which rounds only
+//     what lies 2^-31 below that element; a group's sum of q goes in as three f16 parts;
+//   * p is kept as 2^15 exp(score - running maximum), split into an f16 and the f16 of what that
+//     leaves, so a weight is off by 2^-22 of itself or 2^-40 of the largest.
+// Scores come out as rows = tokens, columns = query heads: a lane holds eight consecutive tokens of
+// one head, which is the operand that the product with V takes, so p never leaves its registers.  The
+// product with V is formed transposed (rows = dims, columns = heads), so that a head's running
+// maximum, sum and rescaling stay in its column's lanes as well.
+//
+// One wave takes 32 tokens at a time for up to sixteen query heads of a KV head; the waves of a
+// workgroup take turns and are joined in LDS; a long sequence is split over workgroups that leave
+// (m, l, o) for a second kernel.
+#include "kv_int4.h"
+#include "tt_common.h"
+
+namespace tt {
+
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 32;          // tokens per step of a wave
+constexpr int kHeadBlock = 16;     // query heads per workgroup
+constexpr int kWaves = 4;
+constexpr float kPScale = 15.0f;   // weights are 2^15 exp(s - m)
+
+struct Attn4Params {
+  tt_int4_cache c;
+  const void* q;
+  int64_t q_row, q_head;
+  const int32_t* lengths;
+  const void* sinks;
+  int sink_dtype, q_bf16;
+  int heads, per_kv, head_blocks, splits;
+  int window, first, max_length;
+  float scale_log2;                // scale * log2(e)
+  float* part;                     // [rows, heads, splits, D + 2]: o, m, l
+  void* out;
+  int64_t out_row, out_head;
+};
+
+// The visible 32-token tiles of a row: [0, a) and [b, e); tile i of them.
+struct Visible {
+  int n, start, a, b, e;
+  __device__ Visible(const Attn4Params& P, int row) {
+    n = min(max(P.lengths[row], 0), P.max_length);
+    start = P.window > 0 ? max(0, n - P.window) : 0;
+    e = (n + kTile - 1) / kTile;
+    b = start / kTile;
+    a = min((min(P.first, n) + kTile - 1) / kTile, b);
+  }
+  __device__ int tiles() const { return a + e - b; }
+  __device__ int tile(int i) const { return i < a ? i : b + i - a; }
+  // workgroups of `splits` that have tiles, and how many each takes
+  __device__ int share(int splits) const { return max(kWaves, (tiles() + splits - 1) / splits); }
+};
+
+// (__builtin_bit_cast of a vector's element takes element 0: a value of its own, always)
+__device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) { return f32_to_f16_bits(a) | ((uint32_t)f32_to_f16_bits(b) << 16); }
+
+// Eight codes as f16 times (s0, s1, s2, s3), packed pairs: register p holds nibbles p and p + 4.
+__device__ __forceinline__ h8_t scaled_codes(uint32_t w, h2 s0, h2 s1, h2 s2, h2 s3) {
+  const h2 s[4] = {s0, s1, s2, s3};
+  const h2 off = {(_Float16)1024.0f, (_Float16)1024.0f};
+  u4_t r;
+#pragma unroll
+  for (int p = 0; p < 4; p++) {
+    const uint32_t x = ((w >> (4 * p)) & 0x000f000fu) | 0x64006400u;   // 1024 + code
+    const h2 v = (as_h2(x) - off) * s[p];
+    r[p] = __builtin_bit_cast(uint32_t, v);
+  }
+  return __builtin_bit_cast(h8_t, r);
+}
+
+// Orders this wave's LDS accesses for its other lanes: a wave's LDS operations execute in order, the
+// compiler has to keep them so.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+__device__ __forceinline__ float col_max(float v) {   // over the four lanes of a column
+  v = fmaxf(v, xor_partner<16>(v));
+  return fmaxf(v, xor_partner<32>(v));
+}
+__device__ __forceinline__ float col_sum(float v) { return bfly<32>(bfly<16>(v)); }
+
+__device__ __forceinline__ float sink_log2(const Attn4Params& P, int h) {
+  const float v = P.sink_dtype == TT_F32    ? reinterpret_cast<const float*>(P.sinks)[h]
+                  : P.sink_dtype == TT_BF16 ? to_f32(reinterpret_cast<const bf16_t*>(P.sinks)[h])
+                                            : to_f32(reinterpret_cast<const f16_t*>(P.sinks)[h]);
+  return v * 0x1.715476p+0f;
+}
+
+__device__ __forceinline__ void store_out(const Attn4Params& P, int row, int h, int d, float v) {
+  const int64_t at = row * P.out_row + h * P.out_head + d;
+  if (P.q_bf16) store<bf16_t>(reinterpret_cast<bf16_t*>(P.out) + at, v);
+  else store<f16_t>(reinterpret_cast<f16_t*>(P.out) + at, v);
+}
+
+// o / (l + sink), where l and o carry the maximum M; a row that saw nothing is 0.
+__device__ __forceinline__ float finish(const Attn4Params& P, int h, float o, float l, float M, bool any) {
+  if (!any) return 0.0f;
+  if (P.sinks) {
+    const float sk = sink_log2(P, h);
+    const float top = fmaxf(M, sk);
+    const float e = __builtin_amdgcn_exp2f(M - top);
+    return o * e / (l * e + __builtin_amdgcn_exp2f(sk - top + kPScale));
+  }
+  return o / l;
+}
+
+template <int D, int G>
+__global__ __launch_bounds__(64 * kWaves) void attn4_kernel(Attn4Params P) {
+  constexpr int NG = D / G;                    // groups of a token
+  constexpr int KW = D / 32;                   // K words of a lane: its quarter of the dims
+  constexpr int LG = D / 4 > G ? D / 4 / G : 1;   // groups in that quarter (1 or 2)
+  constexpr int VT = D / 16;                   // tiles of 16 dims
+  constexpr int VJ = D / 64;
+  constexpr int OS = D + 4;                    // LDS row of a head
+  const int row = blockIdx.z, split = blockIdx.x;
+  const int kvh = blockIdx.y / P.head_blocks, hb = blockIdx.y % P.head_blocks;
+  const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int h0 = kvh * P.per_kv + hb * kHeadBlock;
+  const int heads = min(kHeadBlock, P.per_kv - hb * kHeadBlock);
+  __shared__ __attribute__((aligned(16))) float o_s[kWaves][16][OS];
+  __shared__ float m_s[kWaves][16], l_s[kWaves][16];
+
+  const Visible vis(P, row);
+  const int nt = vis.tiles(), share = vis.share(P.splits);
+  const int first_tile = split * share;
+  if (first_tile >= nt && !(nt == 0 && split == 0)) return;
+  const int end_tile = min(first_tile + share, nt);
+
+  // ---- q as f16 operands: element e of step i is dim quad D/4 + 8 i + (e/2) + 4 (e%2)
+  const int hq = h0 + min(n, heads - 1);
+  float qf[KW * 8];
+  {
+    const int64_t at = row * P.q_row + hq * P.q_head + quad * (D / 4);
+#pragma unroll
+    for (int i = 0; i < KW * 8; i++)
+      qf[i] = P.q_bf16 ? to_f32(reinterpret_cast<const bf16_t*>(P.q)[at + i]) : to_f32(reinterpret_cast<const f16_t*>(P.q)[at + i]);
+  }
+  float big = 0.0f, poison = 0.0f;
+#pragma unroll
+  for (int i = 0; i < KW * 8; i++) {
+    big = fmaxf(big, __builtin_fabsf(qf[i]));
+    poison += qf[i] * 0.0f;
+  }
+  big = col_max(big);
+  poison = col_sum(poison);
+  // the exponent of the largest element, limited so that both powers of two are normal
+  int ex = (int)(__builtin_bit_cast(uint32_t, big) >> 23) - 127 - 7;
+  if (ex < -110) ex = -110;
+  const float down = poison == poison ? pow2i(-ex) : poison;
+  const float score_scale = P.scale_log2 * pow2i(ex);
+  h8_t qb[KW], qm;
+  {
+    float part[LG];
+#pragma unroll
+    for (int j = 0; j < LG; j++) part[j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KW; i++) {
+      u4_t r;
+#pragma unroll
+      for (int p = 0; p < 4; p++) r[p] = pack_h2(qf[8 * i + p] * down, qf[8 * i + p + 4] * down);
+      qb[i] = __builtin_bit_cast(h8_t, r);
+#pragma unroll
+      for (int e = 0; e < 8; e++) part[i * LG / KW] += (float)qb[i][e];
+    }
+    uint16_t limb[6] = {0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < LG; j++)
+#pragma unroll
+      for (int k = 0; k < 3; k++) {
+        limb[3 * j + k] = f32_to_f16_bits(part[j]);
+        part[j] -= to_f32(f16_t{limb[3 * j + k]});
+      }
+    const u4_t r = {limb[0] | ((uint32_t)limb[1] << 16), limb[2] | ((uint32_t)limb[3] << 16), limb[4] | ((uint32_t)limb[5] << 16), 0u};
+    qm = __builtin_bit_cast(h8_t, r);
+  }
+
+  const uint32_t* kc = reinterpret_cast<const uint32_t*>(P.c.k_codes) + row * P.c.kc_seq + kvh * P.c.kc_head + quad * KW;
+  const uint16_t* ks = reinterpret_cast<const uint16_t*>(P.c.k_scales) + row * P.c.ks_seq + kvh * P.c.ks_head + (quad * (D / 4) / G) * 2;
+  const uint32_t* vc = reinterpret_cast<const uint32_t*>(P.c.v_codes) + row * P.c.vc_seq + kvh * P.c.vc_head;
+  const uint16_t* vs = reinterpret_cast<const uint16_t*>(P.c.v_scales) + row * P.c.vs_seq + kvh * P.c.vs_head;
+
+  const float ninf = __builtin_bit_cast(float, 0xff800000u);
+  f4_t o[VT], om = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < VT; i++) o[i] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
+  float m_run = ninf, l_run = 0.0f;
+
+  for (int i = first_tile + wave; i < end_tile; i += kWaves) {
+    const int t0 = vis.tile(i) * kTile;
+    // ---- loads: K rows of this lane's token in both halves, V words of its block of eight tokens
+    uint32_t kw[2][KW], ksm[2][LG];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int64_t t = t0 + 8 * (n >> 2) + 4 * h + (n & 3);
+#pragma unroll
+      for (int x = 0; x < KW; x++) kw[h][x] = kc[t * (D / 8) + x];
+#pragma unroll
+      for (int j = 0; j < LG; j++) ksm[h][j] = *reinterpret_cast<const uint32_t*>(ks + t * (2 * NG) + 2 * j);
+    }
+    const int64_t blk = t0 / 8 + quad;
+    u4_t vw[VJ], vsp[VJ], vm = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < VJ; j++) {
+      vw[j] = *reinterpret_cast<const u4_t*>(vc + blk * D + 64 * j + 4 * n);
+      vsp[j] = *reinterpret_cast<const u4_t*>(vs + ((blk * NG + (64 * j + 4 * n) / G) * 2) * 8);
+    }
+    if (n < NG) vm = *reinterpret_cast<const u4_t*>(vs + ((blk * NG + n) * 2 + 1) * 8);
+
+    // ---- scores: register e of half h is token t0 + 8 quad + 4 h + e of head n
+    f4_t sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      sc[h] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int x = 0; x < KW; x++) {
+        const uint32_t sm = ksm[h][x * LG / KW];
+        const h2 s = {as_h2(sm)[0], as_h2(sm)[0]};
+        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_codes(kw[h][x], s, s, s, s), qb[x], sc[h], 0, 0, 0);
+      }
+      const uint32_t ma = ksm[h][0] >> 16, mb = LG > 1 ? ksm[h][LG - 1] >> 16 : 0u;
+      const u4_t r = {ma | (ma << 16), ma | (mb << 16), mb | (mb << 16), 0u};
+      sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, r), qm, sc[h], 0, 0, 0);
+    }
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) s[e] = sc[e >> 2][e & 3] * score_scale;
+    const bool whole = t0 + kTile <= vis.n && (t0 >= vis.start || t0 + kTile <= P.first);
+    if (!whole) {
+      // tokens out of sight: no score, and V's step and minimum 0 (what lies there may be NaN)
+      uint32_t keep[4];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int t = t0 + 8 * quad + e;
+        const bool in = t < vis.n && (t >= vis.start || t < P.first);
+        if (!in) s[e] = ninf;
+        if ((e & 1) == 0) keep[e >> 1] = in ? 0xffffu : 0u;
+        else keep[e >> 1] |= in ? 0xffff0000u : 0u;
+      }
+#pragma unroll
+      for (int p = 0; p < 4; p++) {
+        vm[p] &= keep[p];
+#pragma unroll
+        for (int j = 0; j < VJ; j++) vsp[j][p] &= keep[p];
+      }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
+    const float m_new = fmaxf(m_run, col_max(top));
+    const float m_use = m_new == ninf ? 0.0f : m_new;
+    if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
+      const float a = __builtin_amdgcn_exp2f(m_run - m_use);
+      l_run *= a;
+#pragma unroll
+      for (int x = 0; x < VT; x++) o[x] *= a;
+      om *= a;
+      m_run = m_new;
+    }
+    u4_t hi, lo;
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+      const float pa = __builtin_amdgcn_exp2f(s[2 * p] - m_use + kPScale);
+      const float pb = __builtin_amdgcn_exp2f(s[2 * p + 1] - m_use + kPScale);
+      l_run += pa + pb;
+      hi[p] = pack_h2(pa, pb);
+      const h2 hh = as_h2(hi[p]);
+      lo[p] = pack_h2(pa - (float)hh[0], pb - (float)hh[1]);
+    }
+    const h8_t ph = __builtin_bit_cast(h8_t, hi), pl = __builtin_bit_cast(h8_t, lo);
+
+    // ---- values: register r of o[4 j + x] is dim 64 j + 4 (4 quad + r) + x of head n
+#pragma unroll
+    for (int j = 0; j < VJ; j++) {
+      const h2 s0 = as_h2(vsp[j][0]), s1 = as_h2(vsp[j][1]), s2 = as_h2(vsp[j][2]), s3 = as_h2(vsp[j][3]);
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        const h8_t v = scaled_codes(vw[j][x], s0, s1, s2, s3);
+        o[4 * j + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[4 * j + x], 0, 0, 0);
+        o[4 * j + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[4 * j + x], 0, 0, 0);
+      }
+    }
+    const h8_t vmh = __builtin_bit_cast(h8_t, vm);   // rows = groups
+    om = __builtin_amdgcn_mfma_f32_16x16x32_f16(vmh, ph, om, 0, 0, 0);
+    om = __builtin_amdgcn_mfma_f32_16x16x32_f16(vmh, pl, om, 0, 0, 0);
+  }
+
+  // ---- join the waves.  The groups' sums of p m sit in the column's lanes of quads 0 and 1.
+  const float l_col = col_sum(l_run);
+  {
+    float* mine = o_s[wave][n];
+    if (4 * quad < NG) {   // staged through the row, read back by its four lanes below
+#pragma unroll
+      for (int r = 0; r < 4; r++) mine[4 * quad + r] = om[r];
+    }
+    wave_lds_fence();
+    float gm[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) gm[g] = mine[g];
+    wave_lds_fence();
+#pragma unroll
+    for (int j = 0; j < VJ; j++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int d = 64 * j + 16 * quad + 4 * r;
+        float add = gm[0];
+#pragma unroll
+        for (int g = 1; g < NG; g++) add = d / G == g ? gm[g] : add;
+        f4_t v;
+#pragma unroll
+        for (int x = 0; x < 4; x++) v[x] = o[4 * j + x][r] + add;
+        *reinterpret_cast<f4_t*>(mine + d) = v;
+      }
+    if (quad == 0) {
+      m_s[wave][n] = m_run;
+      l_s[wave][n] = l_col;
+    }
+  }
+  __syncthreads();
+  const bool only = nt <= share;
+  for (int u = threadIdx.x; u < heads * D; u += 64 * kWaves) {
+    const int hh = u / D, d = u % D;
+    float M = m_s[0][hh];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) M = fmaxf(M, m_s[w][hh]);
+    const float base = M == ninf ? 0.0f : M;
+    float acc = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      const float e = __builtin_amdgcn_exp2f(m_s[w][hh] - base);
+      acc = __builtin_fmaf(o_s[w][hh][d], e, acc);
+      l = __builtin_fmaf(l_s[w][hh], e, l);
+    }
+    if (only) {
+      store_out(P, row, h0 + hh, d, finish(P, h0 + hh, acc, l, M, nt > 0));
+    } else {
+      float* part = P.part + (((int64_t)row * P.heads + h0 + hh) * P.splits + split) * (D + 2);
+      part[d] = acc;
+      if (d == 0) {
+        part[D] = M;
+        part[D + 1] = l;
+      }
+    }
+  }
+}
+
+// Joins the splits of one (row, head); rows that one workgroup finished are left alone.
+template <int D>
+__global__ __launch_bounds__(D) void attn4_fold_kernel(Attn4Params P) {
+  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
+  const Visible vis(P, row);
+  const int nt = vis.tiles(), share = vis.share(P.splits);
+  if (nt <= share) return;
+  const int parts = (nt + share - 1) / share;
+  const float* part = P.part + ((int64_t)row * P.heads + h) * P.splits * (D + 2);
+  float M = part[D];
+  for (int i = 1; i < parts; i++) M = fmaxf(M, part[i * (D + 2) + D]);
+  const float base = M == __builtin_bit_cast(float, 0xff800000u) ? 0.0f : M;
+  float acc = 0.0f, l = 0.0f;
+  for (int i = 0; i < parts; i++) {
+    const float e = __builtin_amdgcn_exp2f(part[i * (D + 2) + D] - base);
+    acc = __builtin_fmaf(part[i * (D + 2) + d], e, acc);
+    l = __builtin_fmaf(part[i * (D + 2) + D + 1], e, l);
+  }
+  store_out(P, row, h, d, finish(P, h, acc, l, M, true));
+}
+
+// Tiles that a row may see at most, and the workgroups that share them.
+static int64_t most_tiles(int64_t limit, int64_t window, int64_t first) {
+  const int64_t all = (limit + kTile - 1) / kTile;
+  if (window <= 0) return all;
+  const int64_t some = (first + kTile - 1) / kTile + (window + kTile - 1) / kTile + 1;
+  return some < all ? some : all;
+}
+
+static int64_t split_count(int64_t groups, int64_t tiles) {
+  const int64_t fill = (4 * 256 + groups - 1) / groups;      // workgroups that fill the chip
+  const int64_t most = (tiles + kWaves - 1) / kWaves;        // a tile for every wave
+  int64_t s = fill < most ? fill : most;
+  if (s > 128) s = 128;
+  return s < 1 ? 1 : s;
+}
+
+struct Attn4Plan {
+  int64_t limit, window, first, head_blocks, splits;
+};
+
+static Attn4Plan plan(const tt_int4_cache* c, int64_t rows, int64_t heads, int64_t window, int64_t first, int64_t max_length) {
+  Attn4Plan p;
+  p.limit = max_length < c->capacity ? max_length : c->capacity;
+  p.window = window > p.limit ? 0 : (window > 0 ? window : 0);
+  p.first = p.window == 0 ? 0 : (first < p.limit ? first : p.limit);
+  p.head_blocks = (heads / c->kv_heads + kHeadBlock - 1) / kHeadBlock;
+  p.splits = split_count(rows * c->kv_heads * p.head_blocks, most_tiles(p.limit, p.window, p.first));
+  return p;
+}
+
+template <int D, int G>
+static int launch_attn4(const Attn4Params& P, int64_t rows, hipStream_t st, const char* what) {
+  const dim3 grid((unsigned)P.splits, (unsigned)(P.c.kv_heads * P.head_blocks), (unsigned)rows);
+  hipLaunchKernelGGL((attn4_kernel<D, G>), grid, dim3(64 * kWaves), 0, st, P);
+  const int rc = check_launch(what);
+  if (rc || P.splits == 1) return rc;
+  hipLaunchKernelGGL((attn4_fold_kernel<D>), dim3((unsigned)P.heads, (unsigned)rows), dim3(D), 0, st, P);
+  return check_launch(what);
+}
+
+static int check_attention(const tt_int4_cache* c, int64_t rows, int64_t heads, int64_t window, int64_t first,
+                           int64_t max_length, const char* what) {
+  const int rc = check_cache(c, rows, what);
+  if (rc) return rc;
+  TT_REQUIRE(heads > 0 && heads % c->kv_heads == 0, "%s: heads must be a multiple of kv_heads", what);
+  TT_REQUIRE(heads <= 65535 && c->kv_heads * ((heads / c->kv_heads + kHeadBlock - 1) / kHeadBlock) <= 65535, "%s: too many heads", what);
+  TT_REQUIRE(window >= 0 && first >= 0 && max_length > 0, "%s: window, first_tokens and max_length must not be negative (max_length at least 1)", what);
+  return TT_OK;
+}
+
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" int64_t tt_gqa_attention_int4_scratch_floats(const tt_int4_cache* cache, int64_t rows, int64_t heads,
+                                                        int64_t window, int64_t first_tokens, int64_t max_length) {
+  if (check_attention(cache, rows, heads, window, first_tokens, max_length, "gqa_attention_int4") != TT_OK) return TT_ERR_INVALID;
+  if (rows == 0) return 0;
+  const Attn4Plan p = plan(cache, rows, heads, window, first_tokens, max_length);
+  return p.splits == 1 ? 0 : rows * heads * p.splits * (cache->head_dim + 2);
+}
+
+extern "C" int tt_gqa_attention_int4(const tt_int4_cache* cache, const void* q, int64_t q_row, int64_t q_head, int dtype,
+                                     const int32_t* lengths, int64_t rows, int64_t heads, int64_t window,
+                                     int64_t first_tokens, int64_t max_length, const void* sinks, int sink_dtype,
+                                     float scale, float* scratch, int64_t scratch_floats, void* out, int64_t out_row,
+                                     int64_t out_head, void* stream) {
+  const char* what = "gqa_attention_int4";
+  const int rc = check_attention(cache, rows, heads, window, first_tokens, max_length, what);
+  if (rc) return rc;
+  TT_REQUIRE(valid_act_dtype(dtype), "%s: q must be fp16 or bf16", what);
+  TT_REQUIRE(sinks == nullptr || valid_out_dtype(sink_dtype), "%s: sinks must be fp16, bf16 or fp32", what);
+  if (rows == 0) return TT_OK;
+  TT_REQUIRE(q && out && lengths, "%s: null pointer", what);
+  const Attn4Plan p = plan(cache, rows, heads, window, first_tokens, max_length);
+  TT_REQUIRE(p.splits == 1 || (scratch && scratch_floats >= rows * heads * p.splits * (cache->head_dim + 2)),
+             "%s: scratch too small", what);
+  Attn4Params P{};
+  P.c = *cache;
+  P.q = q; P.q_row = q_row; P.q_head = q_head; P.q_bf16 = dtype == TT_BF16;
+  P.lengths = lengths;
+  P.sinks = sinks; P.sink_dtype = sink_dtype;
+  P.heads = (int)heads; P.per_kv = (int)(heads / cache->kv_heads);
+  P.head_blocks = (int)p.head_blocks; P.splits = (int)p.splits;
+  P.window = (int)p.window; P.first = (int)p.first; P.max_length = (int)p.limit;
+  P.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  P.part = scratch;
+  P.out = out; P.out_row = out_row; P.out_head = out_head;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define TT_ATTN4(D, G) \
+  if (cache->head_dim == D && cache->group_size == G) return launch_attn4<D, G>(P, rows, st, what);
+  TT_ATTN4(64, 32) TT_ATTN4(64, 64) TT_ATTN4(128, 32) TT_ATTN4(128, 64) TT_ATTN4(128, 128) TT_ATTN4(256, 32)
+  TT_ATTN4(256, 64) TT_ATTN4(256, 128)
+#undef TT_ATTN4
+  set_error("%s: unsupported head_dim / group_size", what);
+  return TT_ERR_UNSUPPORTED;
+}
