@@ -805,7 +805,7 @@ int64_t tt_int4_cache_size(void); /* sizeof(tt_int4_cache), for bindings */
  * of the cache from position starts[row] on; counts (or NULL: all) says how many of a row's tokens
  * count.  Tokens that would lie before position 0 or past the capacity are left out.  A group's m
  * is its minimum rounded to fp16 (limited to the finite values), s the smallest value of seven
- * significant bits (a multiple of 2^-24, at most 4352) with 15 s >= maximum - m, and codes are
+ * significant bits (a multiple of 2^-24, at most 4064) with 15 s >= maximum - m, and codes are
  * (x - m) / s rounded to the nearest, ties to even, limited to 0 .. 15, all as if in exact
  * arithmetic.  A group that holds an infinity or a NaN reads as NaN.  Strides of rows, tokens and
  * heads are free. */
@@ -827,7 +827,7 @@ int tt_kv_read_int4(const tt_int4_cache* cache, void* k_out, int64_t k_row, int6
  * given, of the sink's logit, which carries no value.  A row that sees nothing is 0; a row whose q
  * is not finite is NaN.  max_length bounds what the launch is sized for.
  * scratch: tt_gqa_attention_int4_scratch_floats of the same arguments (0: none is needed), for one
- * call at a time. */
+ * call at a time, 16-byte aligned. */
 int64_t tt_gqa_attention_int4_scratch_floats(const tt_int4_cache* cache, int64_t rows, int64_t heads, int64_t window,
                                              int64_t first_tokens, int64_t max_length);
 int tt_gqa_attention_int4(const tt_int4_cache* cache, const void* q, int64_t q_row, int64_t q_head, int dtype,

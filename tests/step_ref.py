@@ -22,9 +22,9 @@ def rotary(x, positions, inv_freq, interleaved, amplitude):
 # ------------------------------------------------------------------ the 4-bit cache
 def steps():
     """Every step that the format has, in increasing order: seven significant bits, multiples of
-    2^-24, at most 4352."""
+    2^-24, at most 4064."""
     v = {n * 2.0 ** e for e in range(-24, 7) for n in range(1, 129)}
-    return np.array(sorted(x for x in v if x <= 4352.0))
+    return np.array(sorted(x for x in v if x <= 4064.0))
 
 
 _STEPS = steps()

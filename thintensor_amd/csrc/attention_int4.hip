@@ -7,8 +7,8 @@
 // are products of exact f16 operands added in binary32 (v_mfma_f32_16x16x32_f16):
 //   * q is scaled by a power of two per head (its largest element to [2^7, 2^8)), which rounds only
 //     what lies 2^-31 below that element; a group's sum of q goes in as three f16 parts;
-//   * p is kept as 2^15 exp(score - running maximum), split into an f16 and the f16 of what that
-//     leaves, so a weight is off by 2^-22 of itself or 2^-40 of the largest.
+//   * p is split into an f16 and the f16 of what that leaves, so a weight is off by 2^-21 of itself or
+//     2^-31 of the largest.
 // Scores come out as rows = tokens, columns = query heads: a lane holds eight consecutive tokens of
 // one head, which is the operand that the product with V takes, so p never leaves its registers.  The
 // product with V is formed transposed (rows = dims, columns = heads), so that a head's running
@@ -29,7 +29,11 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 constexpr int kTile = 32;          // tokens per step of a wave
 constexpr int kHeadBlock = 16;     // query heads per workgroup
 constexpr int kWaves = 4;
-constexpr float kPScale = 15.0f;   // weights are 2^15 exp(s - m)
+constexpr int kMostSplits = 128;
+// Weights are 2^7 exp(s - m), where m follows the running maximum only when that is more than 2^8 past it:
+// they stay below 2^15.
+constexpr float kPScale = 7.0f;
+constexpr float kSlack = 8.0f;
 
 struct Attn4Params {
   tt_int4_cache c;
@@ -37,11 +41,12 @@ struct Attn4Params {
   int64_t q_row, q_head;
   const int32_t* lengths;
   const void* sinks;
-  int sink_dtype, q_bf16;
+  int sink_dtype, q_bf16, q_vec;      // q_vec: rows of q start on 16-byte boundaries
   int heads, per_kv, head_blocks, splits;
   int window, first, max_length;
   float scale_log2;                // scale * log2(e)
-  float* part;                     // [rows, heads, splits, D + 2]: o, m, l
+  float* part_o;                   // [rows, heads, splits, D]
+  float2* part_ml;                 // [rows, heads, splits]: (m, l)
   void* out;
   int64_t out_row, out_head;
 };
@@ -66,16 +71,18 @@ struct Visible {
 __device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) { return f32_to_f16_bits(a) | ((uint32_t)f32_to_f16_bits(b) << 16); }
 
-// Eight codes as f16 times (s0, s1, s2, s3), packed pairs: register p holds nibbles p and p + 4.
-__device__ __forceinline__ h8_t scaled_codes(uint32_t w, h2 s0, h2 s1, h2 s2, h2 s3) {
-  const h2 s[4] = {s0, s1, s2, s3};
-  const h2 off = {(_Float16)1024.0f, (_Float16)1024.0f};
+// Eight codes as f16(c s), exactly: register p holds nibbles p and p + 4 (times s[p]).  The nibble goes
+// to the top of the mantissa of 16, which makes 16 + c, and one packed fma takes c s from it (off = -16 s;
+// steps are at most 4064, so that it is finite).  `mask` sits in a register of its own: an instruction
+// takes one constant.
+__device__ __forceinline__ h8_t scaled_codes(uint32_t w, const h2 s[4], const h2 off[4], uint32_t mask) {
+  const uint32_t x[4] = {w << 6, w << 2, w >> 2, w >> 6};
   u4_t r;
 #pragma unroll
   for (int p = 0; p < 4; p++) {
-    const uint32_t x = ((w >> (4 * p)) & 0x000f000fu) | 0x64006400u;   // 1024 + code
-    const h2 v = (as_h2(x) - off) * s[p];
-    r[p] = __builtin_bit_cast(uint32_t, v);
+    const uint32_t v = (x[p] & mask) | 0x4c004c00u;
+    const h2 c = __builtin_elementwise_fma(as_h2(v), s[p], off[p]);
+    r[p] = __builtin_bit_cast(uint32_t, c);
   }
   return __builtin_bit_cast(h8_t, r);
 }
@@ -119,11 +126,56 @@ __device__ __forceinline__ float finish(const Attn4Params& P, int h, float o, fl
   return o / l;
 }
 
+// What a wave needs of 32 tokens, in registers: K rows of its lane's token in both halves (its quarter
+// of the dims) with their steps and minima, V words of its lane's block of eight tokens with theirs.
 template <int D, int G>
-__global__ __launch_bounds__(64 * kWaves) void attn4_kernel(Attn4Params P) {
+struct Tile {
+  static constexpr int KW = D / 32, VJ = D / 64;
+  static constexpr int LG = D / 4 > G ? D / 4 / G : 1;   // groups in a quarter (1 or 2)
+  uint32_t kw[2][KW], ks[2][LG];
+  u4_t vw[VJ], vs[VJ], vm;
+  static constexpr int NG = D / G;
+  // kc, ksp: this lane's quarter
+  __device__ __forceinline__ void load_k(const uint32_t* kc, const uint16_t* ksp, int t0, int n) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int64_t t = t0 + 8 * (n >> 2) + 4 * h + (n & 3);
+      const uint32_t* p = kc + t * (D / 8);
+      if constexpr (KW == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        kw[h][0] = v.x; kw[h][1] = v.y;
+      } else {
+#pragma unroll
+        for (int x = 0; x < KW / 4; x++) {
+          const u4_t v = *reinterpret_cast<const u4_t*>(p + 4 * x);
+#pragma unroll
+          for (int e = 0; e < 4; e++) kw[h][4 * x + e] = v[e];
+        }
+      }
+      if constexpr (LG == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(ksp + t * (2 * NG));
+        ks[h][0] = v.x; ks[h][1] = v.y;
+      } else {
+        ks[h][0] = *reinterpret_cast<const uint32_t*>(ksp + t * (2 * NG));
+      }
+    }
+  }
+  __device__ __forceinline__ void load_v(const uint32_t* vc, const uint16_t* vsp, int t0, int n, int quad) {
+    const int64_t blk = t0 / 8 + quad;
+#pragma unroll
+    for (int j = 0; j < VJ; j++) {
+      vw[j] = *reinterpret_cast<const u4_t*>(vc + blk * D + 64 * j + 4 * n);
+      vs[j] = *reinterpret_cast<const u4_t*>(vsp + ((blk * NG + (64 * j + 4 * n) / G) * 2) * 8);
+    }
+    // rows past the groups repeat the last one; their products are not used
+    vm = *reinterpret_cast<const u4_t*>(vsp + ((blk * NG + (n < NG ? n : NG - 1)) * 2 + 1) * 8);
+  }
+};
+
+template <typename T, int D, int G>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : 3))) void attn4_kernel(Attn4Params P) {
   constexpr int NG = D / G;                    // groups of a token
-  constexpr int KW = D / 32;                   // K words of a lane: its quarter of the dims
-  constexpr int LG = D / 4 > G ? D / 4 / G : 1;   // groups in that quarter (1 or 2)
+  constexpr int KW = Tile<D, G>::KW, LG = Tile<D, G>::LG;
   constexpr int VT = D / 16;                   // tiles of 16 dims
   constexpr int VJ = D / 64;
   constexpr int OS = D + 4;                    // LDS row of a head
@@ -144,26 +196,40 @@ __global__ __launch_bounds__(64 * kWaves) void attn4_kernel(Attn4Params P) {
 
   // ---- q as f16 operands: element e of step i is dim quad D/4 + 8 i + (e/2) + 4 (e%2)
   const int hq = h0 + min(n, heads - 1);
-  float qf[KW * 8];
+  uint32_t qw[KW * 4];                         // pairs of elements as they are stored
   {
-    const int64_t at = row * P.q_row + hq * P.q_head + quad * (D / 4);
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(P.q) + row * P.q_row + hq * P.q_head + quad * (D / 4);
+    if (P.q_vec) {
 #pragma unroll
-    for (int i = 0; i < KW * 8; i++)
-      qf[i] = P.q_bf16 ? to_f32(reinterpret_cast<const bf16_t*>(P.q)[at + i]) : to_f32(reinterpret_cast<const f16_t*>(P.q)[at + i]);
+      for (int i = 0; i < KW; i++) {
+        const u4_t v = reinterpret_cast<const u4_t*>(q)[i];
+#pragma unroll
+        for (int e = 0; e < 4; e++) qw[4 * i + e] = v[e];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KW * 4; i++) qw[i] = q[2 * i] | ((uint32_t)q[2 * i + 1] << 16);
+    }
   }
+  auto qf = [&](int i) __attribute__((always_inline)) {
+    return (i & 1) ? hi_f32<T>(qw[i / 2]) : lo_f32<T>(qw[i / 2]);
+  };
   float big = 0.0f, poison = 0.0f;
 #pragma unroll
   for (int i = 0; i < KW * 8; i++) {
-    big = fmaxf(big, __builtin_fabsf(qf[i]));
-    poison += qf[i] * 0.0f;
+    const float v = qf(i);
+    big = fmaxf(big, __builtin_fabsf(v));
+    poison += v * 0.0f;
   }
   big = col_max(big);
   poison = col_sum(poison);
   // the exponent of the largest element, limited so that both powers of two are normal
   int ex = (int)(__builtin_bit_cast(uint32_t, big) >> 23) - 127 - 7;
   if (ex < -110) ex = -110;
-  const float down = poison == poison ? pow2i(-ex) : poison;
-  const float score_scale = P.scale_log2 * pow2i(ex);
+  // the sign of the scale goes to q, so that the largest product is the largest score
+  float down = poison == poison ? pow2i(-ex) : poison;
+  if (P.scale_log2 < 0.0f) down = -down;
+  const float score_scale = fmaxf(__builtin_fabsf(P.scale_log2) * pow2i(ex), 0x1p-126f);
   h8_t qb[KW], qm;
   {
     float part[LG];
@@ -173,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn4_kernel(Attn4Params P) {
     for (int i = 0; i < KW; i++) {
       u4_t r;
 #pragma unroll
-      for (int p = 0; p < 4; p++) r[p] = pack_h2(qf[8 * i + p] * down, qf[8 * i + p + 4] * down);
+      for (int p = 0; p < 4; p++) r[p] = pack_h2(qf(8 * i + p) * down, qf(8 * i + p + 4) * down);
       qb[i] = __builtin_bit_cast(h8_t, r);
 #pragma unroll
       for (int e = 0; e < 8; e++) part[i * LG / KW] += (float)qb[i][e];
@@ -201,45 +267,34 @@ __global__ __launch_bounds__(64 * kWaves) void attn4_kernel(Attn4Params P) {
   for (int i = 0; i < VT; i++) o[i] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
   float m_run = ninf, l_run = 0.0f;
 
-  for (int i = first_tile + wave; i < end_tile; i += kWaves) {
-    const int t0 = vis.tile(i) * kTile;
-    // ---- loads: K rows of this lane's token in both halves, V words of its block of eight tokens
-    uint32_t kw[2][KW], ksm[2][LG];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int64_t t = t0 + 8 * (n >> 2) + 4 * h + (n & 3);
-#pragma unroll
-      for (int x = 0; x < KW; x++) kw[h][x] = kc[t * (D / 8) + x];
-#pragma unroll
-      for (int j = 0; j < LG; j++) ksm[h][j] = *reinterpret_cast<const uint32_t*>(ks + t * (2 * NG) + 2 * j);
-    }
-    const int64_t blk = t0 / 8 + quad;
-    u4_t vw[VJ], vsp[VJ], vm = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int j = 0; j < VJ; j++) {
-      vw[j] = *reinterpret_cast<const u4_t*>(vc + blk * D + 64 * j + 4 * n);
-      vsp[j] = *reinterpret_cast<const u4_t*>(vs + ((blk * NG + (64 * j + 4 * n) / G) * 2) * 8);
-    }
-    if (n < NG) vm = *reinterpret_cast<const u4_t*>(vs + ((blk * NG + n) * 2 + 1) * 8);
+  uint32_t mask = 0x03c003c0u;
+  asm volatile("" : "+v"(mask));
 
+    Tile<D, G> tile;
+  auto step = [&](int t0, int next) __attribute__((always_inline)) {
     // ---- scores: register e of half h is token t0 + 8 quad + 4 h + e of head n
     f4_t sc[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       sc[h] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int x = 0; x < KW; x++) {
-        const uint32_t sm = ksm[h][x * LG / KW];
-        const h2 s = {as_h2(sm)[0], as_h2(sm)[0]};
-        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_codes(kw[h][x], s, s, s, s), qb[x], sc[h], 0, 0, 0);
-      }
-      const uint32_t ma = ksm[h][0] >> 16, mb = LG > 1 ? ksm[h][LG - 1] >> 16 : 0u;
+      const uint32_t ma = tile.ks[h][0] >> 16, mb = LG > 1 ? tile.ks[h][LG - 1] >> 16 : 0u;
       const u4_t r = {ma | (ma << 16), ma | (mb << 16), mb | (mb << 16), 0u};
       sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, r), qm, sc[h], 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < LG; j++) {
+        const h2 sm = as_h2(tile.ks[h][j]);
+        const h2 s1 = {sm[0], sm[0]};
+        const h2 o1 = s1 * (h2){(_Float16)-16.0f, (_Float16)-16.0f};
+        const h2 s4[4] = {s1, s1, s1, s1}, o4[4] = {o1, o1, o1, o1};
+#pragma unroll
+        for (int x = j * KW / LG; x < (j + 1) * KW / LG; x++)
+          sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_codes(tile.kw[h][x], s4, o4, mask), qb[x], sc[h], 0, 0, 0);
+      }
     }
+    tile.load_k(kc, ks, next, n);
     float s[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) s[e] = sc[e >> 2][e & 3] * score_scale;
+    for (int e = 0; e < 8; e++) s[e] = sc[e >> 2][e & 3];
     const bool whole = t0 + kTile <= vis.n && (t0 >= vis.start || t0 + kTile <= P.first);
     if (!whole) {
       // tokens out of sight: no score, and V's step and minimum 0 (what lies there may be NaN)
@@ -254,50 +309,71 @@ __global__ __launch_bounds__(64 * kWaves) void attn4_kernel(Attn4Params P) {
       }
 #pragma unroll
       for (int p = 0; p < 4; p++) {
-        vm[p] &= keep[p];
+        tile.vm[p] &= keep[p];
 #pragma unroll
-        for (int j = 0; j < VJ; j++) vsp[j][p] &= keep[p];
+        for (int j = 0; j < VJ; j++) tile.vs[j][p] &= keep[p];
       }
     }
     float top = s[0];
 #pragma unroll
     for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
-    const float m_new = fmaxf(m_run, col_max(top));
-    const float m_use = m_new == ninf ? 0.0f : m_new;
-    if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
-      const float a = __builtin_amdgcn_exp2f(m_run - m_use);
+    top = col_max(top) * score_scale;
+    if (__builtin_amdgcn_ballot_w64(top > m_run + kSlack) != 0) {
+      const float m_new = fmaxf(m_run, top);
+      const float a = m_new == ninf ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       l_run *= a;
 #pragma unroll
       for (int x = 0; x < VT; x++) o[x] *= a;
       om *= a;
       m_run = m_new;
     }
+    const float base = kPScale - (m_run == ninf ? 0.0f : m_run);
     u4_t hi, lo;
 #pragma unroll
     for (int p = 0; p < 4; p++) {
-      const float pa = __builtin_amdgcn_exp2f(s[2 * p] - m_use + kPScale);
-      const float pb = __builtin_amdgcn_exp2f(s[2 * p + 1] - m_use + kPScale);
+      const float pa = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * p], score_scale, base));
+      const float pb = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * p + 1], score_scale, base));
       l_run += pa + pb;
-      hi[p] = pack_h2(pa, pb);
-      const h2 hh = as_h2(hi[p]);
-      lo[p] = pack_h2(pa - (float)hh[0], pb - (float)hh[1]);
+      // both parts towards zero: the second one takes what the first leaves
+      const uint32_t hw = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(pa, pb));
+      const h2 hh = as_h2(hw);
+      hi[p] = hw;
+      lo[p] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(pa - (float)hh[0], pb - (float)hh[1]));
     }
     const h8_t ph = __builtin_bit_cast(h8_t, hi), pl = __builtin_bit_cast(h8_t, lo);
 
     // ---- values: register r of o[4 j + x] is dim 64 j + 4 (4 quad + r) + x of head n
+    const h8_t vmh = __builtin_bit_cast(h8_t, tile.vm);   // rows = groups
+    om = __builtin_amdgcn_mfma_f32_16x16x32_f16(vmh, ph, om, 0, 0, 0);
+    om = __builtin_amdgcn_mfma_f32_16x16x32_f16(vmh, pl, om, 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < VJ; j++) {
-      const h2 s0 = as_h2(vsp[j][0]), s1 = as_h2(vsp[j][1]), s2 = as_h2(vsp[j][2]), s3 = as_h2(vsp[j][3]);
+      const h2 s4[4] = {as_h2(tile.vs[j][0]), as_h2(tile.vs[j][1]), as_h2(tile.vs[j][2]), as_h2(tile.vs[j][3])};
+      h2 o4[4];
+#pragma unroll
+      for (int p = 0; p < 4; p++) o4[p] = s4[p] * (h2){(_Float16)-16.0f, (_Float16)-16.0f};
 #pragma unroll
       for (int x = 0; x < 4; x++) {
-        const h8_t v = scaled_codes(vw[j][x], s0, s1, s2, s3);
+        const h8_t v = scaled_codes(tile.vw[j][x], s4, o4, mask);
         o[4 * j + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[4 * j + x], 0, 0, 0);
         o[4 * j + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[4 * j + x], 0, 0, 0);
       }
     }
-    const h8_t vmh = __builtin_bit_cast(h8_t, vm);   // rows = groups
-    om = __builtin_amdgcn_mfma_f32_16x16x32_f16(vmh, ph, om, 0, 0, 0);
-    om = __builtin_amdgcn_mfma_f32_16x16x32_f16(vmh, pl, om, 0, 0, 0);
+    tile.load_v(vc, vs, next, n, quad);
+  };
+
+  // K of the next tile is requested as soon as the scores have taken the present one's, V after the
+  // products with it (past the end: the last tile once more)
+  int i = first_tile + wave;
+  if (i < end_tile) {
+    int t0 = vis.tile(i) * kTile;
+    tile.load_k(kc, ks, t0, n);
+    tile.load_v(vc, vs, t0, n, quad);
+    for (; i < end_tile; i += kWaves) {
+      const int next = vis.tile(min(i + kWaves, end_tile - 1)) * kTile;
+      step(t0, next);
+      t0 = next;
+    }
   }
 
   // ---- join the waves.  The groups' sums of p m sit in the column's lanes of quads 0 and 1.
@@ -349,35 +425,62 @@ __global__ __launch_bounds__(64 * kWaves) void attn4_kernel(Attn4Params P) {
     if (only) {
       store_out(P, row, h0 + hh, d, finish(P, h0 + hh, acc, l, M, nt > 0));
     } else {
-      float* part = P.part + (((int64_t)row * P.heads + h0 + hh) * P.splits + split) * (D + 2);
-      part[d] = acc;
-      if (d == 0) {
-        part[D] = M;
-        part[D + 1] = l;
-      }
+      const int64_t at = ((int64_t)row * P.heads + h0 + hh) * P.splits + split;
+      P.part_o[at * D + d] = acc;
+      if (d == 0) P.part_ml[at] = make_float2(M, l);
     }
   }
 }
 
-// Joins the splits of one (row, head); rows that one workgroup finished are left alone.
+// Joins the splits of one (row, head), two or more; rows that one workgroup finished are left alone.
+// Every wave forms all weights (a split per lane); sixteen bytes of a split's o per thread, the splits
+// dealt over the threads' rows and joined in LDS.
 template <int D>
-__global__ __launch_bounds__(D) void attn4_fold_kernel(Attn4Params P) {
-  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
+__global__ __launch_bounds__(256) void attn4_fold_kernel(Attn4Params P) {
+  constexpr int PIECES = D / 4, ROWS = 256 / PIECES;
+  const int h = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 63;
+  const int piece = threadIdx.x % PIECES, r = threadIdx.x / PIECES;
+  __shared__ float e_s[kMostSplits];
+  __shared__ __attribute__((aligned(16))) f4_t sum[ROWS][PIECES];
+  const int64_t at = ((int64_t)row * P.heads + h) * P.splits;
+  const float2* ml = P.part_ml + at;
+  const f4_t* po = reinterpret_cast<const f4_t*>(P.part_o + at * D);
   const Visible vis(P, row);
   const int nt = vis.tiles(), share = vis.share(P.splits);
   if (nt <= share) return;
   const int parts = (nt + share - 1) / share;
-  const float* part = P.part + ((int64_t)row * P.heads + h) * P.splits * (D + 2);
-  float M = part[D];
-  for (int i = 1; i < parts; i++) M = fmaxf(M, part[i * (D + 2) + D]);
-  const float base = M == __builtin_bit_cast(float, 0xff800000u) ? 0.0f : M;
-  float acc = 0.0f, l = 0.0f;
-  for (int i = 0; i < parts; i++) {
-    const float e = __builtin_amdgcn_exp2f(part[i * (D + 2) + D] - base);
-    acc = __builtin_fmaf(part[i * (D + 2) + d], e, acc);
-    l = __builtin_fmaf(part[i * (D + 2) + D + 1], e, l);
+  const float ninf = __builtin_bit_cast(float, 0xff800000u);
+  constexpr int PER = kMostSplits / 64;
+  float2 v[PER];
+#pragma unroll
+  for (int k = 0; k < PER; k++) v[k] = lane + 64 * k < parts ? ml[lane + 64 * k] : make_float2(ninf, 0.0f);
+  float M = ninf;
+#pragma unroll
+  for (int k = 0; k < PER; k++) M = fmaxf(M, v[k].x);
+#define TT_LEVEL(X) M = fmaxf(M, xor_partner<X>(M));
+  TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8) TT_LEVEL(16) TT_LEVEL(32)
+#undef TT_LEVEL
+  const float base = M == ninf ? 0.0f : M;
+  float l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < PER; k++) {
+    const float e = __builtin_amdgcn_exp2f(v[k].x - base);
+    l = __builtin_fmaf(v[k].y, e, l);
+    if (threadIdx.x < 64) e_s[lane + 64 * k] = e;
   }
-  store_out(P, row, h, d, finish(P, h, acc, l, M, true));
+  l = xor_sum(l, 1, 64);
+  __syncthreads();
+  f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int i = r; i < parts; i += ROWS) acc += po[(int64_t)i * PIECES + piece] * e_s[i];
+  sum[r][piece] = acc;
+  __syncthreads();
+  if (r == 0) {
+#pragma unroll
+    for (int k = 1; k < ROWS; k++) acc += sum[k][piece];
+#pragma unroll
+    for (int x = 0; x < 4; x++) store_out(P, row, h, 4 * piece + x, finish(P, h, acc[x], l, M, true));
+  }
 }
 
 // Tiles that a row may see at most, and the workgroups that share them.
@@ -392,7 +495,7 @@ static int64_t split_count(int64_t groups, int64_t tiles) {
   const int64_t fill = (4 * 256 + groups - 1) / groups;      // workgroups that fill the chip
   const int64_t most = (tiles + kWaves - 1) / kWaves;        // a tile for every wave
   int64_t s = fill < most ? fill : most;
-  if (s > 128) s = 128;
+  if (s > kMostSplits) s = kMostSplits;
   return s < 1 ? 1 : s;
 }
 
@@ -413,10 +516,11 @@ static Attn4Plan plan(const tt_int4_cache* c, int64_t rows, int64_t heads, int64
 template <int D, int G>
 static int launch_attn4(const Attn4Params& P, int64_t rows, hipStream_t st, const char* what) {
   const dim3 grid((unsigned)P.splits, (unsigned)(P.c.kv_heads * P.head_blocks), (unsigned)rows);
-  hipLaunchKernelGGL((attn4_kernel<D, G>), grid, dim3(64 * kWaves), 0, st, P);
+  if (P.q_bf16) hipLaunchKernelGGL((attn4_kernel<bf16_t, D, G>), grid, dim3(64 * kWaves), 0, st, P);
+  else hipLaunchKernelGGL((attn4_kernel<f16_t, D, G>), grid, dim3(64 * kWaves), 0, st, P);
   const int rc = check_launch(what);
   if (rc || P.splits == 1) return rc;
-  hipLaunchKernelGGL((attn4_fold_kernel<D>), dim3((unsigned)P.heads, (unsigned)rows), dim3(D), 0, st, P);
+  hipLaunchKernelGGL((attn4_fold_kernel<D>), dim3((unsigned)P.heads, (unsigned)rows), dim3(256), 0, st, P);
   return check_launch(what);
 }
 
@@ -455,18 +559,20 @@ extern "C" int tt_gqa_attention_int4(const tt_int4_cache* cache, const void* q, 
   if (rows == 0) return TT_OK;
   TT_REQUIRE(q && out && lengths, "%s: null pointer", what);
   const Attn4Plan p = plan(cache, rows, heads, window, first_tokens, max_length);
-  TT_REQUIRE(p.splits == 1 || (scratch && scratch_floats >= rows * heads * p.splits * (cache->head_dim + 2)),
-             "%s: scratch too small", what);
+  TT_REQUIRE(p.splits == 1 || (scratch && aligned(scratch, 16) && scratch_floats >= rows * heads * p.splits * (cache->head_dim + 2)),
+             "%s: scratch too small or not 16-byte aligned", what);
   Attn4Params P{};
   P.c = *cache;
   P.q = q; P.q_row = q_row; P.q_head = q_head; P.q_bf16 = dtype == TT_BF16;
+  P.q_vec = aligned(q, 16) && q_row % 8 == 0 && q_head % 8 == 0;
   P.lengths = lengths;
   P.sinks = sinks; P.sink_dtype = sink_dtype;
   P.heads = (int)heads; P.per_kv = (int)(heads / cache->kv_heads);
   P.head_blocks = (int)p.head_blocks; P.splits = (int)p.splits;
   P.window = (int)p.window; P.first = (int)p.first; P.max_length = (int)p.limit;
   P.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  P.part = scratch;
+  P.part_o = scratch;
+  P.part_ml = reinterpret_cast<float2*>(scratch + rows * heads * p.splits * cache->head_dim);
   P.out = out; P.out_row = out_row; P.out_head = out_head;
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define TT_ATTN4(D, G) \

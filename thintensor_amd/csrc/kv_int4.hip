@@ -37,7 +37,7 @@ __device__ __forceinline__ void group_step(float lo, float hi, bool finite, uint
     s = __builtin_ceil(raw / lsb) * lsb;
     if (15.0 * (s - lsb) >= reach) s -= lsb;
     if (15.0 * s < reach) s += lsb;
-    s = __builtin_fmin(s, 4352.0);
+    s = __builtin_fmin(s, 4064.0);
   }
   *m_bits = f32_to_f16_bits(m);
   *s_bits = f32_to_f16_bits((float)s);
