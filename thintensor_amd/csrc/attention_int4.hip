@@ -491,12 +491,16 @@ static int64_t most_tiles(int64_t limit, int64_t window, int64_t first) {
   return some < all ? some : all;
 }
 
+// Workgroups that share a row: few tiles are taken by one, since a second launch has to join several
+// (8 groups of sequence and KV head, head_dim 64: 19 tiles 6.6 us by one and 8.0 shared, 32 tiles 8.3 and
+// 7.8, 64 tiles 13.4 and 7.9), and more of them while there are groups for the chip (256 groups: 16 tiles
+// 6.5 and 10.4, 64 tiles 13.9 and 16.0).  Shared, 512 workgroups and eight tiles each (32768 tokens of 8 x
+// 64: 1024 workgroups 11.7, 512 9.8; four tiles each, 130 tiles, 10 x 128, 4 rows: 15.5 and 14.1).
 static int64_t split_count(int64_t groups, int64_t tiles) {
-  const int64_t fill = (4 * 256 + groups - 1) / groups;      // workgroups that fill the chip
-  const int64_t most = (tiles + kWaves - 1) / kWaves;        // a tile for every wave
-  int64_t s = fill < most ? fill : most;
-  if (s > kMostSplits) s = kMostSplits;
-  return s < 1 ? 1 : s;
+  if (tiles <= 24 || (groups >= 256 && tiles <= 64)) return 1;
+  const int64_t fill = (512 + groups - 1) / groups, most = (tiles + 7) / 8;
+  const int64_t s = fill < most ? fill : most;
+  return s < kMostSplits ? s : kMostSplits;
 }
 
 struct Attn4Plan {
