@@ -6,8 +6,8 @@
 // a histogram over z = (max - x) / temperature says which bins the cuts and the target can fall into,
 // and only the candidates in those bins are put in order.
 //   1. every chunk of a row: largest and smallest logit;
-//   2. every chunk: count and weight of each bin;
-//   3. every chunk: the candidates, gathered from the bins that the row's cuts can fall into;
+//   2. every chunk: weight (and, for top-k, count) of each bin;
+//   3. every chunk: the bins that the row's cuts can fall into, and their candidates;
 //   4. one workgroup per row: candidates sorted, cuts and target resolved among them.
 // Weights are exp(-z) in units of 2^-43, 64-bit integers: sums have no order, and a total is exact to
 // 2^-43 of the largest weight per token, far below what tells two cumulative sums apart.
@@ -19,315 +19,534 @@ namespace tt {
 constexpr int kBins = 2048;             // the last one: weights below 2^-43, which count as 0
 constexpr double kReach = 64.0;         // z that the bins reach to at most
 constexpr double kUnit = 8796093022208.0;   // 2^43
-constexpr int kMostChunks = 64;
+constexpr int kThreads = 256;           // of a chunk's workgroup
+constexpr int kStep = 8 * kThreads;     // logits that it takes at a time
+constexpr int kMostChunks = 256;
 constexpr int kMostCandidates = 4096;   // that the last step sorts in LDS
 constexpr int kFinalThreads = 1024;
+constexpr int kCuts = 4;                // intervals of bins: top-k, top-p, min-p, the target
 
-struct SampleRow {                      // scratch of one row
+// What step 3 leaves for step 4: disjoint intervals of bins in increasing order (n of them), the
+// weight and count before each and the weight up to its end; the bins of top-k and min-p.
+struct alignas(16) SamplePlan {
+  int n;
+  int lo[kCuts], hi[kCuts];
+  uint64_t before[kCuts], upto[kCuts];
+  uint32_t rank_before[kCuts];
+  int k_cut;                            // whether top-k divides a bin
+  uint32_t k;
+  uint64_t k_mass;                      // otherwise: the weight that it keeps
+  uint64_t total, m_before;             // all weight; the weight before min-p's interval
+};
+
+struct alignas(16) SampleRow {                      // scratch of one row
   uint64_t mass[kBins];
   uint32_t count[kBins];
   float2 range[kMostChunks];            // largest, smallest finite
+  SamplePlan plan;
   uint32_t candidates;
   uint32_t pad[3];
   uint64_t list[kMostCandidates];
 };
+static_assert(sizeof(SampleRow) % 16 == 0, "rows keep their alignment");
 
 struct SampleParams {
   const void* logits;
   int64_t row_stride;
-  int64_t vocab;
+  int vocab, vec;                       // vec: rows start on 16-byte boundaries
   const float* uniforms;
   const float* temperature;
   const int32_t* top_k;
   const float* top_p;
   const float* min_p;
   SampleRow* rows;
-  int chunks, chunk;                    // chunks of a row and their elements
+  int chunks, chunk;                    // chunks of a row and their logits, a multiple of kStep
   int64_t* tokens;
   float* probs;
 };
 
-// Order-preserving key of a logit; NaN and -inf as 0 (never taken), -0 as +0.
+// Order-preserving key of a logit above -inf, -0 as +0.
 __device__ __forceinline__ uint32_t key_of(float x) {
   x = x + 0.0f;
   const uint32_t b = __builtin_bit_cast(uint32_t, x);
-  if (!(x > __builtin_bit_cast(float, 0xff800000u))) return 0u;
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(uint32_t k) {
   return __builtin_bit_cast(float, (k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
-__device__ __forceinline__ bool live(float x) { return x > __builtin_bit_cast(float, 0xff800000u); }
+constexpr uint32_t kNegInf = 0xff800000u;
+__device__ __forceinline__ bool live(float x) { return x > __builtin_bit_cast(float, kNegInf); }
+
+// e^-z for z >= 0 in binary64, as p 2^n: z log2 e = -n + f, p = e^(f ln 2) by its Taylor polynomial
+// (|f ln 2| <= 0.3466: the first term left out is below 2^-57 of it).
+__device__ __forceinline__ double exp_neg(double z, int* n) {
+  const double y = z * -1.4426950408889634074;
+  const double r = __builtin_rint(y);
+  const double g = __builtin_fma(r, -0.69314718055994530942, -z);
+  const double g2 = __builtin_fma(r, -2.3190468138462996e-17, g);   // the rest of ln 2
+  double p = 1.6059043836821613e-10;                                 // 1/13!
+  p = __builtin_fma(p, g2, 2.08767569878681e-09);
+  p = __builtin_fma(p, g2, 2.505210838544172e-08);
+  p = __builtin_fma(p, g2, 2.755731922398589e-07);
+  p = __builtin_fma(p, g2, 2.7557319223985893e-06);
+  p = __builtin_fma(p, g2, 2.48015873015873e-05);
+  p = __builtin_fma(p, g2, 0.0001984126984126984);
+  p = __builtin_fma(p, g2, 0.001388888888888889);
+  p = __builtin_fma(p, g2, 0.008333333333333333);
+  p = __builtin_fma(p, g2, 0.041666666666666664);
+  p = __builtin_fma(p, g2, 0.16666666666666666);
+  p = __builtin_fma(p, g2, 0.5);
+  p = __builtin_fma(p, g2, 1.0);
+  p = __builtin_fma(p, g2, 1.0);
+  *n = (int)r;
+  return p;
+}
 
 // What a row's settings and range make of a logit.
 struct RowScale {
   double top, inv_t, bins_per_z;
   bool greedy;
-  __device__ RowScale(const SampleParams& P, int row, float largest, float smallest) {
+  __device__ RowScale(const SampleParams& P, int row, float2 range) {
     const float t = P.temperature ? P.temperature[row] : 1.0f;
     greedy = !(t > 0.0f);
-    top = (double)largest;
+    top = (double)range.x;
     inv_t = greedy ? 0.0 : 1.0 / (double)t;
-    const double far = greedy ? kReach : z_of(smallest);
+    const double far = greedy ? kReach : z_of(range.y);
     // all of the range in bins 0 .. kBins - 2, or what lies below kReach of it
     const double most = far < kReach ? far : kReach;
     bins_per_z = most > 0.0 ? (kBins - 2) / most : 0.0;
   }
   __device__ double z_of(float x) const {
-    if ((double)x == top) return 0.0;
-    if (greedy) return __builtin_inf();
-    return (top - (double)x) * inv_t;
+    const double d = top - (double)x;
+    if ((double)x == top) return 0.0;   // (infinities among them)
+    return greedy ? __builtin_inf() : d * inv_t;
   }
   __device__ int bin_of(double z) const {
     const double b = z == 0.0 ? 0.0 : z * bins_per_z;
     return b < (double)(kBins - 1) ? (int)b : kBins - 1;
   }
-  __device__ double weight_of(double z) const { return exp(-z); }
-  __device__ uint64_t mass_of(double z) const { return (uint64_t)(weight_of(z) * kUnit + 0.5); }
+  __device__ double weight_of(double z) const {
+    if (!(z < 700.0)) return 0.0;
+    int n;
+    const double p = exp_neg(z, &n);
+    return __builtin_amdgcn_ldexp(p, n);
+  }
+  // in units: 2^52 added leaves the rounded integer in the low bits
+  __device__ uint64_t mass_of(double z) const {
+    if (!(z < 31.0)) return 0;
+    int n;
+    const double p = exp_neg(z, &n);
+    const double v = __builtin_amdgcn_ldexp(p, n + 43) + 4503599627370496.0;
+    return __builtin_bit_cast(uint64_t, v) - 0x4330000000000000ull;
+  }
 };
 
 template <typename T>
-__device__ __forceinline__ float logit(const SampleParams& P, int row, int64_t i) {
+__device__ __forceinline__ float logit(const SampleParams& P, int row, int i) {
   return to_f32(reinterpret_cast<const T*>(P.logits)[row * P.row_stride + i]);
 }
 
-__device__ __forceinline__ float2 row_range(const SampleParams& P, int row) {
-  const float2* r = P.rows[row].range;
-  float hi = __builtin_bit_cast(float, 0xff800000u), lo = __builtin_bit_cast(float, 0x7f800000u);
-  for (int c = 0; c < P.chunks; c++) {
-    hi = fmaxf(hi, r[c].x);
-    lo = fminf(lo, r[c].y);
+// Eight logits from i on, -inf past the vocabulary.
+template <typename T>
+__device__ __forceinline__ void logits8(const SampleParams& P, int row, int i, float x[8]) {
+  const T* p = reinterpret_cast<const T*>(P.logits) + row * P.row_stride + i;
+  if (P.vec && i + 8 <= P.vocab) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = piece_f32<T>(v, e);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = i + e < P.vocab ? to_f32(p[e]) : __builtin_bit_cast(float, kNegInf);
   }
+}
+
+__device__ __forceinline__ float2 wave_range(float hi, float lo) {
+#define TT_LEVEL(M) hi = fmaxf(hi, xor_partner<M>(hi)); lo = fminf(lo, xor_partner<M>(lo));
+  TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8) TT_LEVEL(16) TT_LEVEL(32)
+#undef TT_LEVEL
   return make_float2(hi, lo);
 }
 
+// The row's range from its chunks'; by every wave, all lanes.
+__device__ __forceinline__ float2 row_range(const SampleParams& P, int row) {
+  const float2* r = P.rows[row].range;
+  const float inf = __builtin_bit_cast(float, 0x7f800000u);
+  float2 v[kMostChunks / 64];
+#pragma unroll
+  for (int k = 0; k < kMostChunks / 64; k++) {
+    const int c = (threadIdx.x & 63) + 64 * k;
+    v[k] = c < P.chunks ? r[c] : make_float2(-inf, inf);
+  }
+  float hi = -inf, lo = inf;
+#pragma unroll
+  for (int k = 0; k < kMostChunks / 64; k++) {
+    hi = fmaxf(hi, v[k].x);
+    lo = fminf(lo, v[k].y);
+  }
+  return wave_range(hi, lo);
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void sample_range_kernel(SampleParams P) {
+__global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleParams P) {
   const int row = blockIdx.y, c = blockIdx.x;
   SampleRow& R = P.rows[row];
-  for (int b = c * 256 + threadIdx.x; b < kBins; b += 256 * P.chunks) {
+  for (int b = c * kThreads + threadIdx.x; b < kBins; b += kThreads * P.chunks) {
     R.mass[b] = 0;
     R.count[b] = 0;
   }
   if (c == 0 && threadIdx.x == 0) R.candidates = 0;
   const float inf = __builtin_bit_cast(float, 0x7f800000u);
   float hi = -inf, lo = inf;
-  const int64_t end = min(P.vocab, (int64_t)(c + 1) * P.chunk);
-  for (int64_t i = (int64_t)c * P.chunk + threadIdx.x; i < end; i += 256) {
-    const float x = logit<T>(P, row, i);
-    hi = fmaxf(hi, x);
-    if (live(x)) lo = fminf(lo, x);
+  const int end = min(P.vocab, (c + 1) * P.chunk);
+#pragma unroll 2
+  for (int i = c * P.chunk + 8 * (int)threadIdx.x; i < end; i += kStep) {
+    float x[8];
+    logits8<T>(P, row, i, x);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      hi = fmaxf(hi, x[e]);
+      lo = fminf(lo, live(x[e]) ? x[e] : inf);
+    }
   }
-  __shared__ float hs[4], ls[4];
-#define TT_LEVEL(M) hi = fmaxf(hi, xor_partner<M>(hi)); lo = fminf(lo, xor_partner<M>(lo));
-  TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8) TT_LEVEL(16) TT_LEVEL(32)
-#undef TT_LEVEL
-  if ((threadIdx.x & 63) == 0) {
-    hs[threadIdx.x >> 6] = hi;
-    ls[threadIdx.x >> 6] = lo;
-  }
+  __shared__ float2 ws[kThreads / 64];
+  const float2 w = wave_range(hi, lo);
+  if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = w;
   __syncthreads();
   if (threadIdx.x == 0) {
-    R.range[c] = make_float2(fmaxf(fmaxf(hs[0], hs[1]), fmaxf(hs[2], hs[3])),
-                             fminf(fminf(ls[0], ls[1]), fminf(ls[2], ls[3])));
+    R.range[c] = make_float2(fmaxf(fmaxf(ws[0].x, ws[1].x), fmaxf(ws[2].x, ws[3].x)),
+                             fminf(fminf(ws[0].y, ws[1].y), fminf(ws[2].y, ws[3].y)));
   }
+}
+
+// Whether top-k cuts a row's order (a greedy row keeps the first).
+__device__ __forceinline__ uint32_t row_top_k(const SampleParams& P, int row, bool greedy) {
+  const int32_t k = greedy ? 1 : P.top_k ? P.top_k[row] : 0;
+  return k > 0 && k < P.vocab ? (uint32_t)k : 0u;
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams P) {
+__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams P) {
   const int row = blockIdx.y, c = blockIdx.x;
   SampleRow& R = P.rows[row];
-  __shared__ uint64_t mass[kBins];
-  __shared__ uint32_t count[kBins];
-  for (int b = threadIdx.x; b < kBins; b += 256) {
-    mass[b] = 0;
-    count[b] = 0;
-  }
+  __shared__ __attribute__((aligned(16))) uint64_t mass[kBins];
+  __shared__ __attribute__((aligned(16))) uint32_t count[kBins];
+  const int end = min(P.vocab, (c + 1) * P.chunk);
+  int i = c * P.chunk + 8 * (int)threadIdx.x;
+  float x[8];
+  if (i < end) logits8<T>(P, row, i, x);
   const float2 range = row_range(P, row);
-  const RowScale S(P, row, range.x, range.y);
-  __syncthreads();
-  const int64_t end = min(P.vocab, (int64_t)(c + 1) * P.chunk);
-  for (int64_t i = (int64_t)c * P.chunk + threadIdx.x; i < end; i += 256) {
-    const float x = logit<T>(P, row, i);
-    if (!live(x)) continue;
-    const double z = S.z_of(x);
-    const int b = S.bin_of(z);
-    atomicAdd(&count[b], 1u);
-    if (b < kBins - 1) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)S.mass_of(z));
+  for (int b = threadIdx.x; b < kBins / 2; b += kThreads) {
+    reinterpret_cast<ulonglong2*>(mass)[b] = make_ulonglong2(0, 0);
+    reinterpret_cast<uint2*>(count)[b] = make_uint2(0, 0);
   }
+  const RowScale S(P, row, range);
+  const bool counts = row_top_k(P, row, S.greedy) != 0;
+  uint32_t far = 0;                     // of the last bin
   __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += 256)
-    if (count[b]) {
-      atomicAdd(&R.count[b], count[b]);
-      atomicAdd((unsigned long long*)&R.mass[b], (unsigned long long)mass[b]);
+  while (i < end) {
+    double z[8];
+    int b[8];
+    uint64_t m[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      z[e] = live(x[e]) ? S.z_of(x[e]) : __builtin_inf();
+      b[e] = S.bin_of(z[e]);
+      m[e] = S.mass_of(z[e]);
+      far += live(x[e]) && b[e] == kBins - 1;
     }
+    const int next = i + kStep;
+    if (next < end) logits8<T>(P, row, next, x);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if (m[e]) atomicAdd((unsigned long long*)&mass[b[e]], (unsigned long long)m[e]);
+      if (counts && b[e] < kBins - 1) atomicAdd(&count[b[e]], 1u);
+    }
+    i = next;
+  }
+  if (counts && far) atomicAdd(&count[kBins - 1], far);
+  __syncthreads();
+  for (int k = threadIdx.x; k < kBins; k += kThreads) {
+    if (mass[k]) atomicAdd((unsigned long long*)&R.mass[k], (unsigned long long)mass[k]);
+    if (counts && count[k]) atomicAdd(&R.count[k], count[k]);
+  }
 }
 
-// The cumulative histogram of a row and the bins that its cuts and target can fall into.
-struct Bins {
-  uint64_t mass[kBins + 1];             // before each bin
-  uint32_t count[kBins + 1];
-  uint64_t wave_mass[kFinalThreads / 64];
-  uint32_t wave_count[kFinalThreads / 64];
-  int at;                               // answer of a search
+// A row's cumulative histogram, eight bins per thread, and searches in it.  An answer is a bin with
+// the weight and count before it and up to its end.
+struct BinAt {
+  int bin;
+  uint32_t n0, n1;
+  uint64_t m0, m1;
 };
 
-// Fills B from the row's histogram; THREADS threads, kBins / THREADS bins each.
-template <int THREADS>
-__device__ void cumulate(const SampleRow& R, Bins& B) {
-  constexpr int PER = kBins / THREADS;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  uint64_t m[PER], ms = 0;
-  uint32_t n[PER], ns = 0;
+struct CumBins {
+  static constexpr int PER = kBins / kThreads;
+  uint64_t m[PER + 1], total;           // before each of this thread's bins, and after the last
+  uint32_t n[PER + 1], all;
+  uint64_t* wave_m;
+  uint32_t* wave_n;
+  __device__ void load(const SampleRow& R) {
+    const int t = threadIdx.x;
+    const ulonglong2* rm = reinterpret_cast<const ulonglong2*>(R.mass + t * PER);
+    const uint4* rn = reinterpret_cast<const uint4*>(R.count + t * PER);
 #pragma unroll
-  for (int k = 0; k < PER; k++) {
-    m[k] = ms;
-    n[k] = ns;
-    ms += R.mass[t * PER + k];
-    ns += R.count[t * PER + k];
-  }
-  uint64_t mi = ms;
-  uint32_t ni = ns;
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t mo = __shfl_up((unsigned long long)mi, d);
-    const uint32_t no = __shfl_up(ni, d);
-    if (lane >= d) {
-      mi += mo;
-      ni += no;
+    for (int k = 0; k < PER / 2; k++) {
+      const ulonglong2 v = rm[k];
+      m[2 * k] = v.x; m[2 * k + 1] = v.y;
+    }
+#pragma unroll
+    for (int k = 0; k < PER / 4; k++) {
+      const uint4 v = rn[k];
+      n[4 * k] = v.x; n[4 * k + 1] = v.y; n[4 * k + 2] = v.z; n[4 * k + 3] = v.w;
     }
   }
-  if (lane == 63) {
-    B.wave_mass[wave] = mi;
-    B.wave_count[wave] = ni;
-  }
-  __syncthreads();
-  uint64_t mb = mi - ms;
-  uint32_t nb = ni - ns;
-  for (int w = 0; w < wave; w++) {
-    mb += B.wave_mass[w];
-    nb += B.wave_count[w];
-  }
+  __device__ void sum() {               // one barrier
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    uint64_t ms = 0;
+    uint32_t ns = 0;
 #pragma unroll
-  for (int k = 0; k < PER; k++) {
-    B.mass[t * PER + k] = mb + m[k];
-    B.count[t * PER + k] = nb + n[k];
+    for (int k = 0; k < PER; k++) {
+      const uint64_t a = m[k];
+      const uint32_t b = n[k];
+      m[k] = ms;
+      n[k] = ns;
+      ms += a;
+      ns += b;
+    }
+    uint64_t mi = ms;
+    uint32_t ni = ns;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t mo = __shfl_up((unsigned long long)mi, d);
+      const uint32_t no = __shfl_up(ni, d);
+      if (lane >= d) {
+        mi += mo;
+        ni += no;
+      }
+    }
+    if (lane == 63) {
+      wave_m[wave] = mi;
+      wave_n[wave] = ni;
+    }
+    __syncthreads();
+    uint64_t mb = mi - ms;
+    uint32_t nb = ni - ns;
+    total = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; w++) {
+      if (w < wave) {
+        mb += wave_m[w];
+        nb += wave_n[w];
+      }
+      total += wave_m[w];
+      all += wave_n[w];
+    }
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      m[k] += mb;
+      n[k] += nb;
+    }
+    m[PER] = mb + ms;
+    n[PER] = nb + ns;
   }
-  if (t == THREADS - 1) {
-    B.mass[kBins] = mb + ms;
-    B.count[kBins] = nb + ns;
+  // The thread that holds the answer writes it: before a barrier that the caller makes, into a place
+  // that holds the default.
+  template <typename Cond>              // cond(m0, m1, n0, n1): this bin is the answer
+  __device__ void find(Cond cond, BinAt* out) const {
+    if (!cond(m[0], m[PER], n[0], n[PER])) return;
+#pragma unroll
+    for (int k = 0; k < PER; k++)
+      if (cond(m[k], m[k + 1], n[k], n[k + 1])) *out = BinAt{(int)threadIdx.x * PER + k, n[k], n[k + 1], m[k], m[k + 1]};
   }
-  __syncthreads();
-}
+  __device__ void get(int bin, BinAt* out) const {
+    if (bin / PER != (int)threadIdx.x) return;
+#pragma unroll
+    for (int k = 0; k < PER; k++)
+      if (bin % PER == k) *out = BinAt{bin, n[k], n[k + 1], m[k], m[k + 1]};
+  }
+};
 
-// First bin whose cumulative weight (the bin's own included) is at least / more than target;
-// kBins - 1 if none is.  The same for every thread.
-__device__ __forceinline__ int bin_at_least(const Bins& B, double target) {
-  int lo = 0, hi = kBins - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if ((double)B.mass[mid + 1] >= target) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
-}
-__device__ __forceinline__ int bin_above(const Bins& B, double target) {
-  int lo = 0, hi = kBins - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if ((double)B.mass[mid + 1] > target) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
-}
-__device__ __forceinline__ int bin_of_rank(const Bins& B, uint32_t rank) {   // rank 1 .. count
-  int lo = 0, hi = kBins - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (B.count[mid + 1] >= rank) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
-}
-
-// A row's cuts as intervals of bins; an interval is empty where nothing needs resolving.
-struct Cuts {
-  uint32_t k;                           // rank of the last kept by top-k; 0: no cut
+// A row's settings.
+struct Settings {
+  uint32_t k;                           // 0: none
   double p, min_p, u;
   bool use_p, use_m;
-  int k_bin, p_lo, p_hi, m_lo, m_hi, u_lo, u_hi;
-  uint64_t k_mass;                      // where k_bin < 0: the weight kept by top-k
-  __device__ Cuts(const SampleParams& P, int row, const RowScale& S, const Bins& B) {
-    const uint32_t total = B.count[kBins];
-    const int32_t tk = S.greedy ? 1 : P.top_k ? P.top_k[row] : 0;
-    const float tp = P.top_p ? P.top_p[row] : 1.0f, mp = P.min_p ? P.min_p[row] : 0.0f;
-    const float un = P.uniforms[row];
+  __device__ Settings(const SampleParams& P, int row, bool greedy) {
+    k = row_top_k(P, row, greedy);
+    const float tp = P.top_p ? P.top_p[row] : 1.0f, mp = P.min_p ? P.min_p[row] : 0.0f, un = P.uniforms[row];
     u = un > 0.0f ? (un < 1.0f ? (double)un : 1.0 - 0x1p-24) : 0.0;
-    k = tk > 0 && (uint32_t)tk < total ? (uint32_t)tk : 0;
     use_p = tp < 1.0f;
     p = tp > 0.0f ? (double)tp : 0.0;
     use_m = mp > 0.0f;
     min_p = (double)mp;
-    // top-k: a bin it divides has to be resolved; the last bin weighs nothing
-    k_bin = -1;
-    k_mass = B.mass[kBins];
-    uint64_t lo = k_mass, hi = k_mass;
-    if (k) {
-      const int b = bin_of_rank(B, k);
-      if (B.count[b + 1] == k || b == kBins - 1) {
-        k_mass = lo = hi = B.mass[b + 1];
-      } else {
-        k_bin = b;
-        lo = B.mass[b];
-        hi = B.mass[b + 1];
-      }
-    }
-    p_lo = p_hi = -1;
-    uint64_t kept_lo = lo, kept_hi = hi;
-    if (use_p) {
-      p_lo = bin_at_least(B, p * (double)lo);
-      p_hi = bin_at_least(B, p * (double)hi);
-      kept_lo = min(kept_lo, B.mass[p_lo]);
-      kept_hi = min(kept_hi, B.mass[p_hi + 1]);
-    }
-    m_lo = m_hi = -1;
-    if (use_m) {
-      const double z = min_p < 1.0 ? -log(min_p) : 0.0;
-      const int b = S.greedy ? 0 : S.bin_of(z);
-      m_lo = max(0, b - 1);
-      m_hi = min(kBins - 1, b + 1);
-      kept_lo = min(kept_lo, B.mass[m_lo]);
-      kept_hi = min(kept_hi, B.mass[m_hi + 1]);
-    }
-    u_lo = bin_above(B, u * (double)kept_lo);
-    u_hi = bin_above(B, u * (double)kept_hi);
-  }
-  __device__ bool needs(int b) const {
-    return b < kBins - 1 && (b == k_bin || (b >= p_lo && b <= p_hi) || (b >= m_lo && b <= m_hi) || (b >= u_lo && b <= u_hi));
   }
 };
 
 template <typename T>
-__global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams P) {
+__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams P) {
   const int row = blockIdx.y, c = blockIdx.x;
   SampleRow& R = P.rows[row];
-  __shared__ Bins B;
-  __shared__ uint64_t found[1024];
+  __shared__ uint64_t wave_m[kThreads / 64];
+  __shared__ uint32_t wave_n[kThreads / 64];
+  __shared__ BinAt at[4 * kCuts];
+  __shared__ uint64_t found[kStep];
   __shared__ uint32_t n_found, base;
-  if (threadIdx.x == 0) n_found = 0;
+  const int end = min(P.vocab, (c + 1) * P.chunk);
+  int i = c * P.chunk + 8 * (int)threadIdx.x;
+  float x[8];
+  if (i < end) logits8<T>(P, row, i, x);
+  CumBins B;
+  B.wave_m = wave_m;
+  B.wave_n = wave_n;
+  B.load(R);
   const float2 range = row_range(P, row);
   if (!live(range.x)) return;
-  const RowScale S(P, row, range.x, range.y);
-  cumulate<256>(R, B);
-  const Cuts C(P, row, S, B);
-  const int64_t end = min(P.vocab, (int64_t)(c + 1) * P.chunk);
-  for (int64_t i0 = (int64_t)c * P.chunk; i0 < end; i0 += 1024) {
+  const RowScale S(P, row, range);
+  const Settings C(P, row, S.greedy);
+  if (threadIdx.x == 0) n_found = 0;
+  // where nothing answers, the last bin does
+  if (threadIdx.x < 4 * kCuts) at[threadIdx.x].bin = kBins - 1;
+  B.sum();
+
+  // ---- top-k: the bin of its last one; whole bins and the last bin (no weight) need no resolving
+  uint64_t k_lo = B.total, k_hi = B.total;
+  int k_bin = -1;
+  if (C.k && C.k < B.all) {
+    B.find([&](uint64_t, uint64_t, uint32_t n0, uint32_t n1) { return n0 < C.k && C.k <= n1; }, &at[0]);
+    __syncthreads();
+    const BinAt a = at[0];
+    k_lo = k_hi = a.m1;
+    if (a.n1 != C.k && a.bin != kBins - 1) {
+      k_bin = a.bin;
+      k_lo = a.m0;
+    }
+  }
+  // ---- top-p and min-p, as far as the weight of top-k is known
+  uint64_t kept_lo = k_lo, kept_hi = k_hi, m_before = 0;
+  int p_lo = -1, p_hi = -2, m_lo = -1, m_hi = -2;
+  if (C.use_p || C.use_m) {
+    const double t_lo = C.p * (double)k_lo, t_hi = C.p * (double)k_hi;
+    auto at_least = [](double t) { return [t](uint64_t m0, uint64_t m1, uint32_t, uint32_t) { return (double)m0 < t && (double)m1 >= t; }; };
+    if (C.use_p) {
+      if (t_lo > 0.0) B.find(at_least(t_lo), &at[1]);
+      else B.get(0, &at[1]);
+      if (t_hi > 0.0) B.find(at_least(t_hi), &at[2]);
+      else B.get(0, &at[2]);
+    }
+    if (C.use_m) {
+      const int b = S.greedy || !(C.min_p < 1.0) ? 0 : S.bin_of(-log(C.min_p));
+      m_lo = max(0, b - 1);
+      m_hi = min(kBins - 1, b + 1);
+      B.get(m_lo, &at[3]);
+      B.get(m_hi, &at[4]);
+    }
+    __syncthreads();
+    if (C.use_p) {
+      p_lo = at[1].bin;
+      p_hi = at[2].bin;
+      if (p_lo < kBins - 1) kept_lo = min(kept_lo, at[1].m0);
+      if (p_hi < kBins - 1) kept_hi = min(kept_hi, at[2].m1);
+    }
+    if (C.use_m) {
+      m_before = at[3].m0;
+      kept_lo = min(kept_lo, at[3].m0);
+      kept_hi = min(kept_hi, at[4].m1);
+    }
+  }
+  // ---- the target
+  {
+    const double t_lo = C.u * (double)kept_lo, t_hi = C.u * (double)kept_hi;
+    auto above = [](double t) { return [t](uint64_t m0, uint64_t m1, uint32_t, uint32_t) { return (double)m0 <= t && (double)m1 > t; }; };
+    B.find(above(t_lo), &at[5]);
+    B.find(above(t_hi), &at[6]);
+    __syncthreads();
+  }
+  // ---- disjoint intervals in order
+  int lo[kCuts] = {k_bin < 0 ? kBins : k_bin, p_hi < p_lo ? kBins : p_lo, m_hi < m_lo ? kBins : m_lo, at[5].bin};
+  int hi[kCuts] = {k_bin, p_hi, m_hi, at[6].bin};
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int64_t i = i0 + 256 * k + threadIdx.x;
-      const float x = i < end ? logit<T>(P, row, i) : __builtin_bit_cast(float, 0xff800000u);
-      if (live(x) && C.needs(S.bin_of(S.z_of(x)))) {
-        const uint32_t at = atomicAdd(&n_found, 1u);
-        found[at] = ((uint64_t)key_of(x) << 32) | (uint32_t)~(uint32_t)i;
+  for (int a = 0; a < kCuts; a++) {
+    hi[a] = min(hi[a], kBins - 2);      // the last bin weighs nothing
+    if (hi[a] < lo[a]) lo[a] = kBins;
+  }
+#pragma unroll
+  for (int a = 0; a < kCuts - 1; a++)
+#pragma unroll
+    for (int b = 0; b < kCuts - 1 - a; b++)
+      if (lo[b + 1] < lo[b]) {
+        const int l = lo[b], h = hi[b];
+        lo[b] = lo[b + 1]; hi[b] = hi[b + 1];
+        lo[b + 1] = l; hi[b + 1] = h;
+      }
+#pragma unroll
+  for (int a = 1; a < kCuts; a++)
+    if (lo[a] < kBins) {
+      // joined with the one before where they touch; that one takes this place
+      const bool touch = lo[a - 1] < kBins && lo[a] <= hi[a - 1] + 1;
+      if (touch) {
+        lo[a] = lo[a - 1];
+        hi[a] = max(hi[a], hi[a - 1]);
+        lo[a - 1] = kBins;
+      }
+    }
+  if (c == 0) {                         // the plan, for the last step
+#pragma unroll
+    for (int a = 0; a < kCuts; a++)
+      if (lo[a] < kBins) {
+        B.get(lo[a], &at[2 * kCuts + a]);
+        B.get(hi[a], &at[3 * kCuts + a]);
+      }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      SamplePlan& L = R.plan;
+      int n = 0;
+#pragma unroll
+      for (int a = 0; a < kCuts; a++)
+        if (lo[a] < kBins) {
+          L.lo[n] = lo[a];
+          L.hi[n] = hi[a];
+          L.before[n] = at[2 * kCuts + a].m0;
+          L.rank_before[n] = at[2 * kCuts + a].n0;
+          L.upto[n] = at[3 * kCuts + a].m1;
+          n++;
+        }
+      L.n = n;
+      L.k_cut = k_bin >= 0;
+      L.k = C.k;
+      L.k_mass = k_hi;
+      L.total = B.total;
+      L.m_before = m_before;
+    }
+  }
+  // ---- this chunk's candidates
+  int first = kBins;                    // most logits are past every interval
+  int last = -1;
+#pragma unroll
+  for (int a = 0; a < kCuts; a++)
+    if (lo[a] < kBins) {
+      first = min(first, lo[a]);
+      last = max(last, hi[a]);
+    }
+  for (int i0 = c * P.chunk; i0 < end; i0 += kStep) {
+    i = i0 + 8 * (int)threadIdx.x;
+    if (i0 > c * P.chunk && i < end) logits8<T>(P, row, i, x);
+    if (i < end) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (!live(x[e])) continue;
+        const int b = S.bin_of(S.z_of(x[e]));
+        if (b < first || b > last) continue;
+        bool in = false;
+#pragma unroll
+        for (int a = 0; a < kCuts; a++) in |= b >= lo[a] && b <= hi[a];
+        if (in) found[atomicAdd(&n_found, 1u)] = ((uint64_t)key_of(x[e]) << 32) | (uint32_t)~(uint32_t)(i + e);
       }
     }
     __syncthreads();
@@ -339,15 +558,55 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleParams P) {
         n_found = 0;
       }
       __syncthreads();
-      for (uint32_t j = threadIdx.x; j < n; j += 256)
+      for (uint32_t j = threadIdx.x; j < n; j += kThreads)
         if (base + j < (uint32_t)kMostCandidates) R.list[base + j] = found[j];
       __syncthreads();
     }
   }
 }
 
+// Value of lane ^ M of a 64-bit integer.
+template <int M>
+__device__ __forceinline__ uint64_t xor64(uint64_t v) {
+  const uint32_t hi = __builtin_bit_cast(uint32_t, xor_partner<M>(__builtin_bit_cast(float, (uint32_t)(v >> 32))));
+  const uint32_t lo = __builtin_bit_cast(uint32_t, xor_partner<M>(__builtin_bit_cast(float, (uint32_t)v)));
+  return ((uint64_t)hi << 32) | lo;
+}
+
+// Sorts up to 1024 keys, one per thread, largest first: n is a power of two, 64 at least, and threads
+// past it only meet the barriers.  Bitonic: partners within a wave by lane exchange, others in LDS.
+__device__ uint64_t sort_one(uint64_t v, int n, uint64_t* buf) {
+  const int t = threadIdx.x;
+  auto keep = [&](uint64_t mine, uint64_t other, int j, int k) {
+    const bool larger = ((t & j) == 0) == ((t & k) == 0);   // this thread keeps the larger one
+    return (mine < other) == larger ? other : mine;
+  };
+  auto within = [&](int k, int from) {
+    if (from >= 32) v = keep(v, xor64<32>(v), 32, k);
+    if (from >= 16) v = keep(v, xor64<16>(v), 16, k);
+    if (from >= 8) v = keep(v, xor64<8>(v), 8, k);
+    if (from >= 4) v = keep(v, xor64<4>(v), 4, k);
+    if (from >= 2) v = keep(v, xor64<2>(v), 2, k);
+    v = keep(v, xor64<1>(v), 1, k);
+  };
+  const bool on = t < n;                // whole waves
+  if (on)
+    for (int k = 2; k <= 64; k <<= 1) within(k, k >> 1);
+  for (int k = 128; k <= n; k <<= 1) {
+    for (int j = k >> 1; j >= 64; j >>= 1) {
+      if (on) buf[t] = v;
+      __syncthreads();
+      const uint64_t o = on ? buf[t ^ j] : 0;
+      __syncthreads();
+      if (on) v = keep(v, o, j, k);
+    }
+    if (on) within(k, 32);
+  }
+  return v;
+}
+
 // Sorts n (a power of two, at most kMostCandidates) keys in LDS, largest first.
-__device__ void sort_descending(uint64_t* a, int n) {
+__device__ void sort_many(uint64_t* a, int n) {
   for (int k = 2; k <= n; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
       for (int i = threadIdx.x; i < n / 2; i += kFinalThreads) {
@@ -363,26 +622,27 @@ __device__ void sort_descending(uint64_t* a, int n) {
     }
 }
 
-struct Found {           // answers of the last step's searches
+struct Found {           // answer of a search
   uint64_t mass;         // cumulative weight up to and including the element
   uint64_t key;          // the element
 };
 
-// A candidate list that does not fit: the elements of bins lo .. hi are searched by the digits of
+// A candidate list that does not fit: the elements of one interval are searched by the digits of
 // their keys and indexes, over the row itself.  mode 0: the element of rank `rank`; 1: the first
 // whose cumulative weight is at least target; 2: the first whose is more.
 template <typename T>
-__device__ Found search_digits(const SampleParams& P, int row, const RowScale& S, const Bins& B, int lo, int hi, int mode,
+__device__ Found search_digits(const SampleParams& P, int row, const RowScale& S, const SamplePlan& L, int a, int mode,
                                uint32_t rank, double target, uint64_t* dm, uint32_t* dn, uint64_t* answer) {
-  uint64_t prefix = 0, mass = B.mass[lo];
-  uint32_t count = B.count[lo];
+  const int lo = L.lo[a], hi = L.hi[a];
+  uint64_t prefix = 0, mass = L.before[a];
+  uint32_t count = L.rank_before[a];
   for (int shift = 56; shift >= 0; shift -= 8) {
     for (int b = threadIdx.x; b < 256; b += kFinalThreads) {
       dm[b] = 0;
       dn[b] = 0;
     }
     __syncthreads();
-    for (int64_t i = threadIdx.x; i < P.vocab; i += kFinalThreads) {
+    for (int i = threadIdx.x; i < P.vocab; i += kFinalThreads) {
       const float x = logit<T>(P, row, i);
       if (!live(x)) continue;
       const double z = S.z_of(x);
@@ -423,12 +683,17 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
 
 template <typename T>
 __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParams P) {
-  const int row = blockIdx.x, t = threadIdx.x;
+  constexpr int PER = kMostCandidates / kFinalThreads;
+  const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
   SampleRow& R = P.rows[row];
-  __shared__ Bins B;
+  __shared__ SamplePlan L;
   __shared__ uint64_t list[kMostCandidates], cum[kMostCandidates];   // cum: weight up to and including
-  __shared__ uint64_t wave_sum[kFinalThreads / 64], answer[4];
+  __shared__ uint64_t wave_sum[kFinalThreads / 64], answer[4], start_sum[kCuts];
+  __shared__ int start[kCuts];
   __shared__ unsigned long long kept_m;
+  uint64_t mine = R.list[t];            // (used where the list is that long)
+  const uint32_t n = R.candidates;
+  if (t < (int)(sizeof(SamplePlan) / 4)) reinterpret_cast<uint32_t*>(&L)[t] = reinterpret_cast<const uint32_t*>(&R.plan)[t];
   const float2 range = row_range(P, row);
   if (!live(range.x)) {
     if (t == 0) {
@@ -437,141 +702,174 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
     }
     return;
   }
-  const RowScale S(P, row, range.x, range.y);
-  cumulate<kFinalThreads>(R, B);
-  const Cuts C(P, row, S, B);
-  const uint32_t n = R.candidates;
+  const RowScale S(P, row, range);
+  const Settings C(P, row, S.greedy);
   const bool fits = n <= (uint32_t)kMostCandidates;
-  if (t == 0) kept_m = 0;
   __syncthreads();
-  int size = 2;
+  if (t == 0) kept_m = L.m_before;
+  uint64_t k_mass = L.k_mass, kept, key = 0;
   if (fits) {
+    // ---- the candidates in order: thread t holds entries t PER' .. in `list`
+    const bool one = n <= (uint32_t)kFinalThreads;
+    const int per = one ? 1 : PER;
+    int size = 64;
     while (size < (int)n) size <<= 1;
-    for (int i = t; i < size; i += kFinalThreads) list[i] = i < (int)n ? R.list[i] : 0;
-    __syncthreads();
-    sort_descending(list, size);
-    // cumulative weights: those of the whole bins that were not gathered come in between
-    constexpr int PER = kMostCandidates / kFinalThreads;
+    if (one) {
+      if (t >= (int)n) mine = 0;
+      mine = sort_one(mine, size, list);
+      if (t < size) list[t] = mine;
+      __syncthreads();
+    } else {
+      for (int i = t; i < size; i += kFinalThreads) list[i] = i < (int)n ? R.list[i] : 0;
+      __syncthreads();
+      sort_many(list, size);
+    }
+    // ---- their cumulative weights; an interval begins with the weight of all bins before it
     uint64_t w[PER], sum = 0;
+    int bins[PER];
 #pragma unroll
     for (int k = 0; k < PER; k++) {
-      const int i = t * PER + k;
-      if (i < (int)n) sum += S.mass_of(S.z_of(of_key((uint32_t)(list[i] >> 32))));
+      const int i = t * per + k;
+      bins[k] = -1;
+      if (k < per && i < (int)n) {
+        const double z = S.z_of(of_key((uint32_t)(list[i] >> 32)));
+        bins[k] = S.bin_of(z);
+        sum += S.mass_of(z);
+      }
       w[k] = sum;
     }
     uint64_t incl = sum;
+#pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint64_t o = __shfl_up((unsigned long long)incl, d);
-      if ((t & 63) >= d) incl += o;
+      if (lane >= d) incl += o;
     }
-    if ((t & 63) == 63) wave_sum[t >> 6] = incl;
+    if (lane == 63) wave_sum[wave] = incl;
     __syncthreads();
     uint64_t before = incl - sum;
-    for (int v = 0; v < (t >> 6); v++) before += wave_sum[v];
+    for (int v = 0; v < wave; v++) before += wave_sum[v];
+    int own[PER];                       // the interval of each entry
 #pragma unroll
-    for (int k = 0; k < PER; k++)
-      if (t * PER + k < (int)n) cum[t * PER + k] = before + w[k];
+    for (int k = 0; k < PER; k++) {
+      own[k] = -1;
+      const int i = t * per + k;
+      if (bins[k] < 0) continue;
+      for (int a = 0; a < L.n; a++)
+        if (bins[k] >= L.lo[a] && bins[k] <= L.hi[a]) own[k] = a;
+      // the first of its interval: the one before lies in an earlier interval
+      const int prev = i > 0 ? S.bin_of(S.z_of(of_key((uint32_t)(list[i - 1] >> 32)))) : -1;
+      if (prev < L.lo[own[k]]) {
+        start[own[k]] = i;
+        start_sum[own[k]] = before + (k > 0 ? w[k - 1] : 0);
+      }
+    }
     __syncthreads();
     uint64_t full[PER];
 #pragma unroll
     for (int k = 0; k < PER; k++) {
-      const int i = t * PER + k;
-      if (i >= (int)n) continue;
-      const int b = S.bin_of(S.z_of(of_key((uint32_t)(list[i] >> 32))));
-      // the first candidate of this bin: bins are whole in the list
-      int lo = 0, hi = i;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (S.bin_of(S.z_of(of_key((uint32_t)(list[mid] >> 32)))) >= b) hi = mid;
-        else lo = mid + 1;
-      }
-      full[k] = B.mass[b] + cum[i] - (lo > 0 ? cum[lo - 1] : 0);
+      const int i = t * per + k;
+      full[k] = 0;
+      if (own[k] < 0) continue;
+      full[k] = L.before[own[k]] + (before + w[k] - start_sum[own[k]]);
+      cum[i] = full[k];
     }
     __syncthreads();
+    auto before_of = [&](int k) {       // the weight before entry k of this thread
+      const int i = t * per + k;
+      return i == start[own[k]] ? L.before[own[k]] : cum[i - 1];
+    };
+    // ---- top-k
+    if (L.k_cut) {
+#pragma unroll
+      for (int k = 0; k < PER; k++)
+        if (own[k] >= 0 && L.rank_before[own[k]] + (uint32_t)(t * per + k - start[own[k]]) + 1 == L.k) answer[0] = full[k];
+      __syncthreads();
+      k_mass = answer[0];
+    }
+    kept = k_mass;
+    // ---- top-p and min-p
+    const double p_target = C.p * (double)k_mass;
+    if (C.use_p) {
+      if (t == 0) answer[1] = L.total;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < PER; k++)
+        if (own[k] >= 0 && (double)full[k] >= p_target) {
+          const uint64_t b = before_of(k);
+          if (b == 0 || (double)b < p_target) answer[1] = full[k];
+        }
+    }
+    if (C.use_m) {
+#pragma unroll
+      for (int k = 0; k < PER; k++)
+        if (own[k] >= 0) {
+          const double z = S.z_of(of_key((uint32_t)(list[t * per + k] >> 32)));
+          if (z == 0.0 || S.weight_of(z) >= C.min_p) atomicMax(&kept_m, (unsigned long long)full[k]);
+        }
+    }
+    if (C.use_p || C.use_m) {
+      __syncthreads();
+      if (C.use_p) kept = min(kept, answer[1]);
+      // a min_p above 1 keeps the first alone
+      if (C.use_m) kept = min(kept, C.min_p > 1.0 ? (uint64_t)kUnit : (uint64_t)kept_m);
+    }
+    // ---- the token
+    const double target = C.u * (double)kept;
 #pragma unroll
     for (int k = 0; k < PER; k++)
-      if (t * PER + k < (int)n) cum[t * PER + k] = full[k];
-    __syncthreads();
-  }
-  auto bin_at = [&](int i) { return S.bin_of(S.z_of(of_key((uint32_t)(list[i] >> 32)))); };
-  // first candidate from bin `b` on that satisfies a monotone condition on the cumulative weight
-  auto first_in = [&](int b, auto cond) {
-    int lo = 0, hi = (int)n;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      const int bm = bin_at(mid);
-      if (bm > b || (bm == b && cond(mid))) hi = mid;
-      else lo = mid + 1;
-    }
-    return lo < (int)n ? lo : (int)n - 1;
-  };
-  // ---- top-k
-  uint64_t k_mass = C.k_mass;
-  if (C.k_bin >= 0) {
-    if (fits) {
-      const int start = first_in(C.k_bin, [&](int) { return true; });
-      k_mass = cum[start + (int)(C.k - B.count[C.k_bin]) - 1];
-    } else {
-      k_mass = search_digits<T>(P, row, S, B, C.k_bin, C.k_bin, 0, C.k, 0.0, cum, (uint32_t*)list, answer).mass;
-    }
-  }
-  uint64_t kept = k_mass;
-  // ---- top-p
-  if (C.use_p) {
-    const double target = C.p * (double)k_mass;
-    const int b = bin_at_least(B, target);
-    uint64_t mass;
-    if (b == kBins - 1) mass = B.mass[kBins];
-    else if (fits) mass = cum[first_in(b, [&](int i) { return (double)cum[i] >= target; })];
-    else mass = search_digits<T>(P, row, S, B, b, b, 1, 0, target, cum, (uint32_t*)list, answer).mass;
-    kept = min(kept, mass);
-  }
-  // ---- min-p: the weights of the interval's elements that pass
-  if (C.use_m) {
-    uint64_t some = 0;
-    auto add = [&](float x) {
-      const double z = S.z_of(x);
-      const int b = S.bin_of(z);
-      if (b >= C.m_lo && b <= C.m_hi && b < kBins - 1 && (z == 0.0 || S.weight_of(z) >= C.min_p)) some += S.mass_of(z);
-    };
-    if (fits) {
-      for (int i = t; i < (int)n; i += kFinalThreads) add(of_key((uint32_t)(list[i] >> 32)));
-    } else {
-      for (int64_t i = t; i < P.vocab; i += kFinalThreads) {
-        const float x = logit<T>(P, row, i);
-        if (live(x)) add(x);
+      if (own[k] >= 0 && (double)full[k] > target) {
+        const uint64_t b = before_of(k);
+        if (b == 0 || (double)b <= target) answer[2] = list[t * per + k];
       }
-    }
-    if (some) atomicAdd(&kept_m, (unsigned long long)some);
     __syncthreads();
-    // a min_p above 1 keeps the first alone
-    const uint64_t mass = C.min_p > 1.0 ? (uint64_t)kUnit : B.mass[C.m_lo] + (uint64_t)kept_m;
-    kept = min(kept, mass);
+    key = answer[2];
+  } else {
+    // the interval that an answer lies in
+    auto holding = [&](double target, bool above) {
+      int a = 0;
+      while (a + 1 < L.n && !(above ? (double)L.upto[a] > target : (double)L.upto[a] >= target)) a++;
+      return a;
+    };
+    uint32_t* dn = reinterpret_cast<uint32_t*>(list);
+    if (L.k_cut) {
+      int a = 0;
+      while (a + 1 < L.n && L.rank_before[a + 1] < L.k) a++;
+      k_mass = search_digits<T>(P, row, S, L, a, 0, L.k, 0.0, cum, dn, answer).mass;
+    }
+    kept = k_mass;
+    if (C.use_p) {
+      const double target = C.p * (double)k_mass;
+      kept = min(kept, search_digits<T>(P, row, S, L, holding(target, false), 1, 0, target, cum, dn, answer).mass);
+    }
+    if (C.use_m) {
+      // every logit from min-p's interval on that passes
+      uint64_t some = 0;
+      const int b = S.greedy || !(C.min_p < 1.0) ? 0 : S.bin_of(-log(C.min_p));
+      const int m_lo = max(0, b - 1), m_hi = min(kBins - 1, b + 1);
+      for (int i = t; i < P.vocab; i += kFinalThreads) {
+        const float x = logit<T>(P, row, i);
+        if (!live(x)) continue;
+        const double z = S.z_of(x);
+        const int bz = S.bin_of(z);
+        if (bz >= m_lo && bz <= m_hi && (z == 0.0 || S.weight_of(z) >= C.min_p)) some += S.mass_of(z);
+      }
+      __syncthreads();
+      if (some) atomicAdd(&kept_m, (unsigned long long)some);
+      __syncthreads();
+      kept = min(kept, C.min_p > 1.0 ? (uint64_t)kUnit : (uint64_t)kept_m);
+    }
+    const double target = C.u * (double)kept;
+    key = search_digits<T>(P, row, S, L, holding(target, true), 2, 0, target, cum, dn, answer).key;
   }
-  // ---- the token
-  const double target = C.u * (double)kept;
-  const int b = bin_above(B, target);
-  uint64_t key;
-  if (fits) key = list[first_in(b, [&](int i) { return (double)cum[i] > target; })];
-  else key = search_digits<T>(P, row, S, B, b, b, 2, 0, target, cum, (uint32_t*)list, answer).key;
   if (t == 0) {
     P.tokens[row] = (int64_t)(uint32_t)~(uint32_t)key;
     if (P.probs) P.probs[row] = (float)(S.weight_of(S.z_of(of_key((uint32_t)(key >> 32)))) * kUnit / (double)kept);
   }
 }
 
-// Chunks of a row: enough workgroups for the chip, at least 1024 logits each.
-static int sample_chunks(int64_t rows, int64_t vocab) {
-  int64_t c = (vocab + 1023) / 1024;
-  const int64_t fill = (4 * 256 + rows - 1) / rows;
-  if (c > fill) c = fill;
-  if (c > kMostChunks) c = kMostChunks;
-  return c < 1 ? 1 : (int)c;
-}
-
 template <typename T>
 static int launch_sample(const SampleParams& P, int64_t rows, hipStream_t st) {
-  const dim3 grid((unsigned)P.chunks, (unsigned)rows), block(256);
+  const dim3 grid((unsigned)P.chunks, (unsigned)rows), block(kThreads);
   hipLaunchKernelGGL((sample_range_kernel<T>), grid, block, 0, st, P);
   int rc = check_launch("sample_rows");
   if (rc) return rc;
@@ -604,11 +902,17 @@ extern "C" int tt_sample_rows(const void* logits, int64_t row_stride, int dtype,
   TT_REQUIRE(logits && uniforms && tokens && scratch, "%s: null pointer", what);
   TT_REQUIRE(aligned(scratch, 16) && scratch_bytes >= rows * (int64_t)sizeof(SampleRow), "%s: scratch too small", what);
   SampleParams P{};
-  P.logits = logits; P.row_stride = row_stride; P.vocab = vocab;
+  P.logits = logits; P.row_stride = row_stride; P.vocab = (int)vocab;
+  P.vec = aligned(logits, 16) && row_stride % (dtype == TT_F32 ? 4 : 8) == 0;
   P.uniforms = uniforms; P.temperature = temperature; P.top_k = top_k; P.top_p = top_p; P.min_p = min_p;
   P.rows = reinterpret_cast<SampleRow*>(scratch);
-  P.chunks = sample_chunks(rows, vocab);
-  P.chunk = (int)(((vocab + P.chunks - 1) / P.chunks + 7) / 8 * 8);
+  // chunks: a step of logits each while that leaves the chip four workgroups per CU
+  const int64_t steps = (vocab + kStep - 1) / kStep;
+  int64_t chunks = (4 * 256 + rows - 1) / rows;
+  if (chunks > kMostChunks) chunks = kMostChunks;
+  const int64_t per = (steps + chunks - 1) / chunks;
+  P.chunk = (int)(per * kStep);
+  P.chunks = (int)((steps + per - 1) / per);
   P.tokens = tokens; P.probs = probs;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == TT_F16) return launch_sample<f16_t>(P, rows, st);
