@@ -10,6 +10,25 @@
 
 namespace tt {
 
+// Eight elements of a 16-byte aligned piece (two pieces of binary32).
+template <typename T> __device__ __forceinline__ void load8(const T* p, float x[8]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+  for (int e = 0; e < 8; e++) x[e] = piece_f32<T>(v, e);
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, float x[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float x[8]) {
+  *reinterpret_cast<uint4*>(p) = pack_piece<T>(x);
+}
+template <> __device__ __forceinline__ void store8<float>(float* p, const float x[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
 struct RotaryParams {
   const void* x[2];        // q, k
   void* out[2];
@@ -56,8 +75,88 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams P) {
   }
 }
 
+// Rows whose parts start on 16-byte boundaries and come in whole pieces of eight dims: a thread takes
+// eight pairs of the half layout (two pieces) or four of the interleaved one, or copies a piece.
+// `tokens_per` tokens share a workgroup where one has few pieces.
+template <typename T, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_vec_kernel(RotaryParams P, int tokens_per) {
+  extern __shared__ __attribute__((aligned(16))) float turn_s[];   // cosines, then sines, of each token
+  const int half = P.rotary >> 1;
+  const int64_t t0 = (int64_t)blockIdx.x * tokens_per;
+  const int tokens = (int)min((int64_t)tokens_per, P.tokens - t0);
+  for (int u = threadIdx.x; u < tokens * half; u += 256) {
+    const int tk = u / half, i = u - tk * half;
+    const double t = (double)load_expert(P.positions, P.position_shift, t0 + tk) * P.inv_freq[i] * 0.15915494309189533577;
+    float s, c;
+    sincospif(2.0f * (float)(t - __builtin_rint(t)), &s, &c);
+    turn_s[tk * P.rotary + i] = c * P.amplitude;
+    turn_s[tk * P.rotary + half + i] = s * P.amplitude;
+  }
+  __syncthreads();
+  const int turns = INTERLEAVED ? P.rotary / 8 : half / 8;
+  const int units = turns + (P.head_dim - P.rotary) / 8;
+  const int heads = P.heads[0] + P.heads[1];
+  for (int w = threadIdx.x; w < tokens * heads * units; w += 256) {
+    const int hu = w / units, u = w - hu * units;
+    const int tk = hu / heads, hh = hu - tk * heads;
+    const bool second = hh >= P.heads[0];
+    const int h = second ? hh - P.heads[0] : hh;
+    const T* x = reinterpret_cast<const T*>(second ? P.x[1] : P.x[0]) + (t0 + tk) * (second ? P.x_token[1] : P.x_token[0]) +
+                 h * (second ? P.x_head[1] : P.x_head[0]);
+    T* o = reinterpret_cast<T*>(second ? P.out[1] : P.out[0]) + (t0 + tk) * (second ? P.o_token[1] : P.o_token[0]) +
+           h * (second ? P.o_head[1] : P.o_head[0]);
+    const float* cs = turn_s + tk * P.rotary;
+    if (u >= turns) {
+      const int d = P.rotary + 8 * (u - turns);
+      if (x != o) {
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(T) / 2; k++) reinterpret_cast<uint4*>(o + d)[k] = reinterpret_cast<const uint4*>(x + d)[k];
+      }
+    } else if (INTERLEAVED) {
+      float a[8], r[8];
+      load8<T>(x + 8 * u, a);
+      const float4 c = *reinterpret_cast<const float4*>(cs + 4 * u), s = *reinterpret_cast<const float4*>(cs + half + 4 * u);
+      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        r[2 * k] = a[2 * k] * cc[k] - a[2 * k + 1] * ss[k];
+        r[2 * k + 1] = a[2 * k + 1] * cc[k] + a[2 * k] * ss[k];
+      }
+      store8<T>(o + 8 * u, r);
+    } else {
+      float a[8], b[8], ra[8], rb[8];
+      load8<T>(x + 8 * u, a);
+      load8<T>(x + half + 8 * u, b);
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const float c = cs[8 * u + k], s = cs[half + 8 * u + k];
+        ra[k] = a[k] * c - b[k] * s;
+        rb[k] = b[k] * c + a[k] * s;
+      }
+      store8<T>(o + 8 * u, ra);
+      store8<T>(o + half + 8 * u, rb);
+    }
+  }
+}
+
 template <typename T>
 static int launch_rotary(const RotaryParams& P, bool interleaved, hipStream_t st) {
+  constexpr uintptr_t step = 16 / sizeof(T);
+  bool vec = P.head_dim % 8 == 0 && P.rotary % (interleaved ? 8 : 16) == 0;
+  for (int w = 0; w < (P.heads[1] > 0 ? 2 : 1); w++)
+    vec = vec && aligned(P.x[w], 16) && aligned(P.out[w], 16) &&
+          ((P.x_token[w] | P.x_head[w] | P.o_token[w] | P.o_head[w]) & (int64_t)(step - 1)) == 0;
+  if (vec) {
+    // a round of the workgroup's threads, at most eight tokens
+    const int pieces = (P.heads[0] + P.heads[1]) * ((interleaved ? P.rotary / 8 : P.rotary / 16) + (P.head_dim - P.rotary) / 8);
+    int per = 256 / pieces;
+    per = per < 1 ? 1 : per > 8 ? 8 : per;
+    const dim3 grid((unsigned)((P.tokens + per - 1) / per));
+    const size_t lds = sizeof(float) * (size_t)(per * P.rotary);
+    if (interleaved) hipLaunchKernelGGL((rotary_vec_kernel<T, true>), grid, dim3(256), lds, st, P, per);
+    else hipLaunchKernelGGL((rotary_vec_kernel<T, false>), grid, dim3(256), lds, st, P, per);
+    return check_launch("rotary_rows");
+  }
   const dim3 grid((unsigned)P.tokens), block(256);
   const size_t lds = sizeof(float2) * (size_t)(P.rotary / 2);
   if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, true>), grid, block, lds, st, P);

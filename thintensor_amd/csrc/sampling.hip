@@ -21,6 +21,9 @@ constexpr double kReach = 64.0;         // z that the bins reach to at most
 constexpr double kUnit = 8796093022208.0;   // 2^43
 constexpr int kThreads = 256;           // of a chunk's workgroup
 constexpr int kStep = 8 * kThreads;     // logits that it takes at a time
+// of step 2, where fewer workgroups leave fewer bins to add (8 rows of 201088: 256 threads 30.5 us a call,
+// 512 27.5, 1024 27.1; 64 rows of 152064: 62, 61, 68)
+constexpr int kBinThreads = 512;
 constexpr int kMostChunks = 256;
 constexpr int kMostCandidates = 4096;   // that the last step sorts in LDS
 constexpr int kFinalThreads = 1024;
@@ -61,6 +64,7 @@ struct SampleParams {
   const float* min_p;
   SampleRow* rows;
   int chunks, chunk;                    // chunks of a row and their logits, a multiple of kStep
+  int bin_chunks, bin_chunk;            // those of step 2
   int64_t* tokens;
   float* probs;
 };
@@ -231,17 +235,17 @@ __device__ __forceinline__ uint32_t row_top_k(const SampleParams& P, int row, bo
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams P) {
+__global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleParams P) {
   const int row = blockIdx.y, c = blockIdx.x;
   SampleRow& R = P.rows[row];
   __shared__ __attribute__((aligned(16))) uint64_t mass[kBins];
   __shared__ __attribute__((aligned(16))) uint32_t count[kBins];
-  const int end = min(P.vocab, (c + 1) * P.chunk);
-  int i = c * P.chunk + 8 * (int)threadIdx.x;
+  const int end = min(P.vocab, (c + 1) * P.bin_chunk);
+  int i = c * P.bin_chunk + 8 * (int)threadIdx.x;
   float x[8];
   if (i < end) logits8<T>(P, row, i, x);
   const float2 range = row_range(P, row);
-  for (int b = threadIdx.x; b < kBins / 2; b += kThreads) {
+  for (int b = threadIdx.x; b < kBins / 2; b += kBinThreads) {
     reinterpret_cast<ulonglong2*>(mass)[b] = make_ulonglong2(0, 0);
     reinterpret_cast<uint2*>(count)[b] = make_uint2(0, 0);
   }
@@ -260,7 +264,7 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams P) {
       m[e] = S.mass_of(z[e]);
       far += live(x[e]) && b[e] == kBins - 1;
     }
-    const int next = i + kStep;
+    const int next = i + 8 * kBinThreads;
     if (next < end) logits8<T>(P, row, next, x);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -271,7 +275,7 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleParams P) {
   }
   if (counts && far) atomicAdd(&count[kBins - 1], far);
   __syncthreads();
-  for (int k = threadIdx.x; k < kBins; k += kThreads) {
+  for (int k = threadIdx.x; k < kBins; k += kBinThreads) {
     if (mass[k]) atomicAdd((unsigned long long*)&R.mass[k], (unsigned long long)mass[k]);
     if (counts && count[k]) atomicAdd(&R.count[k], count[k]);
   }
@@ -873,7 +877,7 @@ static int launch_sample(const SampleParams& P, int64_t rows, hipStream_t st) {
   hipLaunchKernelGGL((sample_range_kernel<T>), grid, block, 0, st, P);
   int rc = check_launch("sample_rows");
   if (rc) return rc;
-  hipLaunchKernelGGL((sample_bins_kernel<T>), grid, block, 0, st, P);
+  hipLaunchKernelGGL((sample_bins_kernel<T>), dim3((unsigned)P.bin_chunks, (unsigned)rows), dim3(kBinThreads), 0, st, P);
   if ((rc = check_launch("sample_rows"))) return rc;
   hipLaunchKernelGGL((sample_gather_kernel<T>), grid, block, 0, st, P);
   if ((rc = check_launch("sample_rows"))) return rc;
@@ -906,13 +910,15 @@ extern "C" int tt_sample_rows(const void* logits, int64_t row_stride, int dtype,
   P.vec = aligned(logits, 16) && row_stride % (dtype == TT_F32 ? 4 : 8) == 0;
   P.uniforms = uniforms; P.temperature = temperature; P.top_k = top_k; P.top_p = top_p; P.min_p = min_p;
   P.rows = reinterpret_cast<SampleRow*>(scratch);
-  // chunks: a step of logits each while that leaves the chip four workgroups per CU
-  const int64_t steps = (vocab + kStep - 1) / kStep;
-  int64_t chunks = (4 * 256 + rows - 1) / rows;
-  if (chunks > kMostChunks) chunks = kMostChunks;
-  const int64_t per = (steps + chunks - 1) / chunks;
-  P.chunk = (int)(per * kStep);
-  P.chunks = (int)((steps + per - 1) / per);
+  // chunks: a step of logits each while that leaves the chip four workgroups per CU (two larger ones)
+  auto cut = [&](int64_t step, int64_t groups, int* chunks, int* chunk) {
+    const int64_t steps = (vocab + step - 1) / step, most = (groups + rows - 1) / rows;
+    const int64_t fit = most < kMostChunks ? most : kMostChunks, per = (steps + fit - 1) / fit;
+    *chunk = (int)(per * step);
+    *chunks = (int)((steps + per - 1) / per);
+  };
+  cut(kStep, 1024, &P.chunks, &P.chunk);
+  cut(8 * kBinThreads, 512, &P.bin_chunks, &P.bin_chunk);
   P.tokens = tokens; P.probs = probs;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == TT_F16) return launch_sample<f16_t>(P, rows, st);
