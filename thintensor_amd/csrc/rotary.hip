@@ -10,24 +10,31 @@
 
 namespace tt {
 
-// Eight elements of a 16-byte aligned piece (two pieces of binary32).
-template <typename T> __device__ __forceinline__ void load8(const T* p, float x[8]) {
-  const uint4 v = *reinterpret_cast<const uint4*>(p);
+// Eight elements as they are stored: one 16-byte piece, two of binary32.
+template <typename T> struct Eight {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = v; }
+  __device__ __forceinline__ float get(int e) const { return piece_f32<T>(v, e); }
+  __device__ __forceinline__ void set(const float* x) { v = pack_piece<T>(x); }
+};
+template <> struct Eight<float> {
+  float x[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+  __device__ __forceinline__ float get(int e) const { return x[e]; }
+  __device__ __forceinline__ void set(const float* y) {
 #pragma unroll
-  for (int e = 0; e < 8; e++) x[e] = piece_f32<T>(v, e);
-}
-template <> __device__ __forceinline__ void load8<float>(const float* p, float x[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-template <typename T> __device__ __forceinline__ void store8(T* p, const float x[8]) {
-  *reinterpret_cast<uint4*>(p) = pack_piece<T>(x);
-}
-template <> __device__ __forceinline__ void store8<float>(float* p, const float x[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
+    for (int e = 0; e < 8; e++) x[e] = y[e];
+  }
+};
 
 struct RotaryParams {
   const void* x[2];        // q, k
@@ -75,66 +82,92 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams P) {
   }
 }
 
-// Rows whose parts start on 16-byte boundaries and come in whole pieces of eight dims: a thread takes
-// eight pairs of the half layout (two pieces) or four of the interleaved one, or copies a piece.
-// `tokens_per` tokens share a workgroup where one has few pieces.
+// Rows whose parts start on 16-byte boundaries and come in whole pieces of eight dims: a thread keeps
+// one place of the head -- eight pairs of the half layout (two pieces), four of the interleaved one, or
+// a piece to copy -- and walks over the heads of its workgroup's tokens (`tokens_per`, more than one
+// where a token has few pieces), kAhead at a time: requested together, the first before the angles are
+// formed, and written together, because a load that was issued after a store waits for it.
+constexpr int kAhead = 4;
 template <typename T, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void rotary_vec_kernel(RotaryParams P, int tokens_per) {
+__global__ __launch_bounds__(1024) void rotary_vec_kernel(RotaryParams P, int tokens_per, int units) {
   extern __shared__ __attribute__((aligned(16))) float turn_s[];   // cosines, then sines, of each token
+  constexpr int NP = INTERLEAVED ? 1 : 2;      // pieces of a place
   const int half = P.rotary >> 1;
+  const int turns = INTERLEAVED ? P.rotary / 8 : half / 8;
   const int64_t t0 = (int64_t)blockIdx.x * tokens_per;
   const int tokens = (int)min((int64_t)tokens_per, P.tokens - t0);
-  for (int u = threadIdx.x; u < tokens * half; u += 256) {
-    const int tk = u / half, i = u - tk * half;
+  const int heads = P.heads[0] + P.heads[1];
+  const int rows = (int)blockDim.x / units;                // heads in flight
+  const int r0 = (int)threadIdx.x / units, u = (int)threadIdx.x - r0 * units;
+  const int total = r0 < rows ? tokens * heads : 0;
+  const bool copy = u >= turns;
+  const int d0 = copy ? P.rotary + 8 * (u - turns) : 8 * u, d1 = INTERLEAVED || copy ? d0 : d0 + half;
+  struct Place {
+    const T* x;
+    T* o;
+    int token;
+  };
+  auto place = [&](int r) __attribute__((always_inline)) {
+    const int tk = tokens_per == 1 ? 0 : r / heads, hh = r - tk * heads;
+    const bool second = hh >= P.heads[0];
+    const int h = second ? hh - P.heads[0] : hh;
+    return Place{reinterpret_cast<const T*>(second ? P.x[1] : P.x[0]) + (t0 + tk) * (second ? P.x_token[1] : P.x_token[0]) +
+                     h * (second ? P.x_head[1] : P.x_head[0]),
+                 reinterpret_cast<T*>(second ? P.out[1] : P.out[0]) + (t0 + tk) * (second ? P.o_token[1] : P.o_token[0]) +
+                     h * (second ? P.o_head[1] : P.o_head[0]), tk};
+  };
+  Eight<T> a[kAhead], b[kAhead];
+  auto load = [&](int r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+      if (r + k * rows < total) {
+        const Place p = place(r + k * rows);
+        a[k].load(p.x + d0);
+        if (NP == 2 && !copy) b[k].load(p.x + d1);
+      }
+  };
+  load(r0);
+  for (int v = threadIdx.x; v < tokens * half; v += (int)blockDim.x) {
+    const int tk = tokens_per == 1 ? 0 : v / half, i = v - tk * half;
     const double t = (double)load_expert(P.positions, P.position_shift, t0 + tk) * P.inv_freq[i] * 0.15915494309189533577;
     float s, c;
     sincospif(2.0f * (float)(t - __builtin_rint(t)), &s, &c);
     turn_s[tk * P.rotary + i] = c * P.amplitude;
     turn_s[tk * P.rotary + half + i] = s * P.amplitude;
   }
-  __syncthreads();
-  const int turns = INTERLEAVED ? P.rotary / 8 : half / 8;
-  const int units = turns + (P.head_dim - P.rotary) / 8;
-  const int heads = P.heads[0] + P.heads[1];
-  for (int w = threadIdx.x; w < tokens * heads * units; w += 256) {
-    const int hu = w / units, u = w - hu * units;
-    const int tk = hu / heads, hh = hu - tk * heads;
-    const bool second = hh >= P.heads[0];
-    const int h = second ? hh - P.heads[0] : hh;
-    const T* x = reinterpret_cast<const T*>(second ? P.x[1] : P.x[0]) + (t0 + tk) * (second ? P.x_token[1] : P.x_token[0]) +
-                 h * (second ? P.x_head[1] : P.x_head[0]);
-    T* o = reinterpret_cast<T*>(second ? P.out[1] : P.out[0]) + (t0 + tk) * (second ? P.o_token[1] : P.o_token[0]) +
-           h * (second ? P.o_head[1] : P.o_head[0]);
-    const float* cs = turn_s + tk * P.rotary;
-    if (u >= turns) {
-      const int d = P.rotary + 8 * (u - turns);
-      if (x != o) {
+  lds_barrier();
+  for (int r = r0; r < total; r += kAhead * rows) {
+    if (r != r0) load(r);
 #pragma unroll
-        for (int k = 0; k < (int)sizeof(T) / 2; k++) reinterpret_cast<uint4*>(o + d)[k] = reinterpret_cast<const uint4*>(x + d)[k];
-      }
-    } else if (INTERLEAVED) {
-      float a[8], r[8];
-      load8<T>(x + 8 * u, a);
-      const float4 c = *reinterpret_cast<const float4*>(cs + 4 * u), s = *reinterpret_cast<const float4*>(cs + half + 4 * u);
-      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+    for (int k = 0; k < kAhead; k++) {
+      if (r + k * rows >= total) break;
+      const Place p = place(r + k * rows);
+      if (!copy) {
+        const float* cs = turn_s + p.token * P.rotary;
+        float ra[8], rb[8];
+        if (INTERLEAVED) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        r[2 * k] = a[2 * k] * cc[k] - a[2 * k + 1] * ss[k];
-        r[2 * k + 1] = a[2 * k + 1] * cc[k] + a[2 * k] * ss[k];
-      }
-      store8<T>(o + 8 * u, r);
-    } else {
-      float a[8], b[8], ra[8], rb[8];
-      load8<T>(x + 8 * u, a);
-      load8<T>(x + half + 8 * u, b);
+          for (int e = 0; e < 4; e++) {
+            const float c = cs[4 * u + e], s = cs[half + 4 * u + e];
+            const float x = a[k].get(2 * e), y = a[k].get(2 * e + 1);
+            ra[2 * e] = x * c - y * s;
+            ra[2 * e + 1] = y * c + x * s;
+          }
+        } else {
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const float c = cs[8 * u + k], s = cs[half + 8 * u + k];
-        ra[k] = a[k] * c - b[k] * s;
-        rb[k] = b[k] * c + a[k] * s;
+          for (int e = 0; e < 8; e++) {
+            const float c = cs[8 * u + e], s = cs[half + 8 * u + e];
+            const float x = a[k].get(e), y = b[k].get(e);
+            ra[e] = x * c - y * s;
+            rb[e] = y * c + x * s;
+          }
+          b[k].set(rb);
+          b[k].store(p.o + d1);
+        }
+        a[k].set(ra);
       }
-      store8<T>(o + 8 * u, ra);
-      store8<T>(o + half + 8 * u, rb);
+      // one store for turned and copied pieces of a wave (in place, a copied one is what it was)
+      a[k].store(p.o + d0);
     }
   }
 }
@@ -147,14 +180,23 @@ static int launch_rotary(const RotaryParams& P, bool interleaved, hipStream_t st
     vec = vec && aligned(P.x[w], 16) && aligned(P.out[w], 16) &&
           ((P.x_token[w] | P.x_head[w] | P.o_token[w] | P.o_head[w]) & (int64_t)(step - 1)) == 0;
   if (vec) {
-    // a round of the workgroup's threads, at most eight tokens
-    const int pieces = (P.heads[0] + P.heads[1]) * ((interleaved ? P.rotary / 8 : P.rotary / 16) + (P.head_dim - P.rotary) / 8);
-    int per = 256 / pieces;
+    const int units = (interleaved ? P.rotary / 8 : P.rotary / 16) + (P.head_dim - P.rotary) / 8;   // 128 at most
+    const int64_t pieces = (int64_t)units * (P.heads[0] + P.heads[1]);
+    // Few pieces: a thread for each.  Many: kAhead for each thread, so that every load comes before the
+    // first store (8191 tokens of 72 heads of 128, 64 dims turned: 256 threads, which take some pieces in a
+    // second turn, 67.8 us, 320 without one 65.6; 61.8, 4.9 TB/s, since turned and copied pieces share a
+    // store).  Several tokens together where a token has few (4096 tokens of 3 heads of 64: 5.0 us with
+    // one token per workgroup, 4.0 with eight).
+    const bool many = P.tokens * pieces > 4 * 65536;
+    int64_t per = (many ? 1024 : P.tokens >= 1024 ? 256 : 0) / pieces;
     per = per < 1 ? 1 : per > 8 ? 8 : per;
-    const dim3 grid((unsigned)((P.tokens + per - 1) / per));
+    int64_t threads = (per * pieces + (many ? kAhead : 1) - 1) / (many ? kAhead : 1);
+    threads = (threads + units - 1) / units * units;
+    threads = threads < 64 ? 64 : threads > 960 ? 960 : (threads + 63) / 64 * 64;
+    const dim3 grid((unsigned)((P.tokens + per - 1) / per)), block((unsigned)threads);
     const size_t lds = sizeof(float) * (size_t)(per * P.rotary);
-    if (interleaved) hipLaunchKernelGGL((rotary_vec_kernel<T, true>), grid, dim3(256), lds, st, P, per);
-    else hipLaunchKernelGGL((rotary_vec_kernel<T, false>), grid, dim3(256), lds, st, P, per);
+    if (interleaved) hipLaunchKernelGGL((rotary_vec_kernel<T, true>), grid, block, lds, st, P, (int)per, units);
+    else hipLaunchKernelGGL((rotary_vec_kernel<T, false>), grid, block, lds, st, P, (int)per, units);
     return check_launch("rotary_rows");
   }
   const dim3 grid((unsigned)P.tokens), block(256);
