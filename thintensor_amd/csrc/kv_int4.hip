@@ -7,6 +7,7 @@
 // exact under any order, taken over its 4, 8 or 16 lanes.
 #include "kv_int4.h"
 #include "tt_common.h"
+#include "tt_eight.h"
 
 namespace tt {
 
@@ -16,43 +17,55 @@ struct KvRowsParams {
   int64_t x_row[2], x_token[2], x_head[2];
   const int32_t* starts;
   const int32_t* counts;
-  int tokens;
+  int tokens, vec;         // vec: eight elements of k and v start on 16-byte boundaries
 };
 
-// A group's m and s (f16 bits) from its extremes, in binary64: hi - m is exact there.  The
-// division only proposes s; 15 s against hi - m decides.
-__device__ __forceinline__ void group_step(float lo, float hi, bool finite, uint16_t* m_bits, uint16_t* s_bits) {
-  if (!finite) {
-    *m_bits = *s_bits = 0x7e00u;   // reads as NaN
-    return;
-  }
-  const float m = (float)(_Float16)pin_f32(__builtin_fminf(__builtin_fmaxf(lo, -65504.0f), 65504.0f));
+// The exact decisions below are made in binary64, where hi - m, x - m and what a code leaves of them are
+// exact.  They are only reached next to a border: binary32 is off by less than 2^-18 of a step, and
+// whatever is further than that from a border has the same answer there.
+
+// The smallest s of seven significant bits with 15 s >= hi - m; a division only proposes it.
+__device__ __noinline__ float exact_step(float hi, float m) {
   const double reach = (double)hi - (double)m;
-  double s = 0.0;
-  if (reach > 0.0) {
-    const double raw = reach / 15.0;
-    int e = (int)((__builtin_bit_cast(uint64_t, raw) >> 52) & 2047) - 1022 - 7;   // lsb of 7 bits
-    if (e < -24) e = -24;
-    const double lsb = __builtin_bit_cast(double, (uint64_t)(e + 1023) << 52);
-    s = __builtin_ceil(raw / lsb) * lsb;
-    if (15.0 * (s - lsb) >= reach) s -= lsb;
-    if (15.0 * s < reach) s += lsb;
-    s = __builtin_fmin(s, 4064.0);
-  }
-  *m_bits = f32_to_f16_bits(m);
-  *s_bits = f32_to_f16_bits((float)s);
+  if (!(reach > 0.0)) return 0.0f;
+  const double raw = reach / 15.0;
+  int e = (int)((__builtin_bit_cast(uint64_t, raw) >> 52) & 2047) - 1022 - 7;   // lsb of 7 bits
+  if (e < -24) e = -24;
+  const double lsb = __builtin_bit_cast(double, (uint64_t)(e + 1023) << 52);
+  double s = __builtin_ceil(raw / lsb) * lsb;
+  if (15.0 * (s - lsb) >= reach) s -= lsb;
+  if (15.0 * s < reach) s += lsb;
+  return (float)__builtin_fmin(s, 4064.0);
 }
 
-// (x - m) / s to the nearest code, ties to even: the product with 1/s proposes, the exact residual
-// decides.
-__device__ __forceinline__ uint32_t code_of(float x, double m, double s, double inv) {
-  const double d = (double)x - m;
-  double q = __builtin_rint(d * inv);
-  const double r2 = 2.0 * __builtin_fma(-q, s, d);
+// (x - m) / s to the nearest code, ties to even: the product with 1/s proposes, the residual decides.
+__device__ __noinline__ uint32_t exact_code(float x, float m, float s) {
+  const double d = (double)x - (double)m, sd = (double)s;
+  double q = __builtin_rint(d / sd);
+  const double r2 = 2.0 * __builtin_fma(-q, sd, d);
   const bool odd = ((int64_t)q & 1) != 0;
-  if (r2 > s || (r2 == s && odd)) q += 1.0;
-  else if (r2 < -s || (r2 == -s && odd)) q -= 1.0;
+  if (r2 > sd || (r2 == sd && odd)) q += 1.0;
+  else if (r2 < -sd || (r2 == -sd && odd)) q -= 1.0;
   return (uint32_t)(int)__builtin_fmin(__builtin_fmax(q, 0.0), 15.0);
+}
+
+// A group's m and s from its extremes.
+__device__ __forceinline__ float group_step(float hi, float m) {
+  const float raw = (hi - m) * (1.0f / 15.0f);
+  int e = (int)((__builtin_bit_cast(uint32_t, raw) >> 23) & 255) - 126 - 7;   // lsb of 7 bits
+  if (e < -24) e = -24;
+  const float t = __builtin_amdgcn_ldexpf(raw, -e);                           // at most 128
+  const float n = __builtin_ceilf(t);
+  // next to a whole number of units, or where the range is none or past the format's end
+  if (!(n - t > 0x1p-10f && n - t < 1.0f - 0x1p-10f && raw < 4000.0f)) return exact_step(hi, m);
+  return __builtin_amdgcn_ldexpf(n, e);
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
+  const float y = (x - m) * inv;
+  const float q = __builtin_rintf(y);
+  if (__builtin_expect(__builtin_fabsf(y - q) > 0.5f - 0x1p-12f, 0)) return exact_code(x, m, s);
+  return (uint32_t)(int)__builtin_fminf(__builtin_fmaxf(q, 0.0f), 15.0f);
 }
 
 template <int G>   // over G / 8 neighbouring lanes
@@ -85,8 +98,15 @@ __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
   float x[8];
   const T* src = reinterpret_cast<const T*>(P.x[which]) + row * P.x_row[which] + (valid ? t : 0) * P.x_token[which] +
                  head * P.x_head[which] + 8 * word;
+  if (P.vec) {
+    Eight<T> v;
+    v.load(src);
 #pragma unroll
-  for (int e = 0; e < 8; e++) x[e] = valid ? to_f32(src[e]) : 0.0f;
+    for (int e = 0; e < 8; e++) x[e] = valid ? v.get(e) : 0.0f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = valid ? to_f32(src[e]) : 0.0f;
+  }
   float lo = x[0], hi = x[0], poison = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
@@ -95,12 +115,14 @@ __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
     poison += x[e] * 0.0f;                         // NaN where x is not finite
   }
   group_extremes<G>(lo, hi, poison);
-  uint16_t mb, sb;
-  group_step(lo, hi, poison == poison, &mb, &sb);
-  const double m = (double)to_f32(f16_t{mb}), s = (double)to_f32(f16_t{sb});
+  const bool finite = poison == poison;
+  const float m = round_f16(__builtin_fminf(__builtin_fmaxf(lo, -65504.0f), 65504.0f));
+  const float s = finite ? group_step(hi, m) : 0.0f;
+  // a group that is not finite reads as NaN
+  const uint16_t mb = finite ? f32_to_f16_bits(m) : 0x7e00u, sb = finite ? f32_to_f16_bits(s) : 0x7e00u;
   uint32_t codes = 0;
-  if (s > 0.0) {
-    const double inv = 1.0 / s;
+  if (s > 0.0f) {
+    const float inv = 1.0f / s;
 #pragma unroll
     for (int e = 0; e < 8; e++) codes |= code_of(x[e], m, s, inv) << (4 * e);
   }
@@ -155,21 +177,33 @@ __global__ __launch_bounds__(2 * D) void kv_read_int4_kernel(KvRowsParams P) {
   const int64_t t = pos - start;
   if (!(t >= 0 && t < count && pos >= 0 && pos < P.c.capacity)) return;
   T* dst = reinterpret_cast<T*>(P.x[which]) + row * P.x_row[which] + t * P.x_token[which] + head * P.x_head[which] + 8 * word;
+  float y[8];
   if (which == 0) {
     const uint32_t w = reinterpret_cast<const uint32_t*>(P.c.k_codes)[row * P.c.kc_seq + head * P.c.kc_head + pos * W + word];
     const uint32_t sm = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(P.c.k_scales) + row * P.c.ks_seq +
                                                            head * P.c.ks_head + (pos * NG + word / (G / 8)) * 2);
     const float s = lo_f32<f16_t>(sm), m = hi_f32<f16_t>(sm);
 #pragma unroll
-    for (int e = 0; e < 8; e++) store<T>(dst + e, __builtin_fmaf((float)((w >> (4 * e)) & 15u), s, m));
+    for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)((w >> (4 * e)) & 15u), s, m);
   } else {
-    const uint32_t* vc = reinterpret_cast<const uint32_t*>(P.c.v_codes) + row * P.c.vc_seq + head * P.c.vc_head + block * D + 8 * word;
+    const uint4* vc = reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(P.c.v_codes) + row * P.c.vc_seq +
+                                                     head * P.c.vc_head + block * D + 8 * word);
+    const uint4 w0 = vc[0], w1 = vc[1];
     const f16_t* vs = reinterpret_cast<const f16_t*>(P.c.v_scales) + row * P.c.vs_seq + head * P.c.vs_head +
                       ((block * NG + word / (G / 8)) * 2) * 8 + token;
     const float s = to_f32(vs[0]), m = to_f32(vs[8]);
     const int nib = 4 * ((token >> 1) + 4 * (token & 1));
+    const uint32_t ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-    for (int e = 0; e < 8; e++) store<T>(dst + e, __builtin_fmaf((float)((vc[e] >> nib) & 15u), s, m));
+    for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)((ws[e] >> nib) & 15u), s, m);
+  }
+  if (P.vec) {
+    Eight<T> v;
+    v.set(y);
+    v.store(dst);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) store<T>(dst + e, y[e]);
   }
 }
 
@@ -208,6 +242,9 @@ static int rows_entry(const tt_int4_cache* cache, void* k, int64_t k_row, int64_
   P.x_token[0] = k_token; P.x_token[1] = v_token;
   P.x_head[0] = k_head; P.x_head[1] = v_head;
   P.starts = starts; P.counts = counts; P.tokens = (int)tokens;
+  const int64_t whole = dtype == TT_F32 ? 4 : 8;
+  P.vec = aligned(k, 16) && aligned(v, 16) &&
+          ((k_row | k_token | k_head | v_row | v_token | v_head) & (whole - 1)) == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == TT_F16) return launch_rows<f16_t, APPEND>(P, rows, st, what);
   if (dtype == TT_BF16) return launch_rows<bf16_t, APPEND>(P, rows, st, what);
