@@ -11,155 +11,181 @@
 
 namespace tt {
 
+constexpr int kMostBlocks = 8;
+constexpr int kAhead = 4;
+
 struct KvRowsParams {
   tt_int4_cache c;
   void* x[2];              // k, v
   int64_t x_row[2], x_token[2], x_head[2];
   const int32_t* starts;
   const int32_t* counts;
+  int blocks_per;          // blocks of eight cache tokens that a workgroup takes
   int tokens, vec;         // vec: eight elements of k and v start on 16-byte boundaries
 };
 
-// The exact decisions below are made in binary64, where hi - m, x - m and what a code leaves of them are
-// exact.  They are only reached next to a border: binary32 is off by less than 2^-18 of a step, and
-// whatever is further than that from a border has the same answer there.
+// A group's step, and codes, are decided in binary64, which costs what binary32 does here and where
+// hi - m, x - m and what a code leaves of them are exact.
 
-// The smallest s of seven significant bits with 15 s >= hi - m; a division only proposes it.
-__device__ __noinline__ float exact_step(float hi, float m) {
+// The smallest s of seven significant bits with 15 s >= hi - m; the product with 1/15 only proposes it.
+__device__ __forceinline__ double group_step(float hi, float m) {
   const double reach = (double)hi - (double)m;
-  if (!(reach > 0.0)) return 0.0f;
-  const double raw = reach / 15.0;
+  const double raw = reach * (1.0 / 15.0);
   int e = (int)((__builtin_bit_cast(uint64_t, raw) >> 52) & 2047) - 1022 - 7;   // lsb of 7 bits
   if (e < -24) e = -24;
-  const double lsb = __builtin_bit_cast(double, (uint64_t)(e + 1023) << 52);
-  double s = __builtin_ceil(raw / lsb) * lsb;
+  const double lsb = __builtin_amdgcn_ldexp(1.0, e);
+  double s = __builtin_ceil(__builtin_amdgcn_ldexp(raw, -e)) * lsb;
   if (15.0 * (s - lsb) >= reach) s -= lsb;
   if (15.0 * s < reach) s += lsb;
-  return (float)__builtin_fmin(s, 4064.0);
+  return reach > 0.0 ? __builtin_fmin(s, 4064.0) : 0.0;
 }
 
-// (x - m) / s to the nearest code, ties to even: the product with 1/s proposes, the residual decides.
-__device__ __noinline__ uint32_t exact_code(float x, float m, float s) {
-  const double d = (double)x - (double)m, sd = (double)s;
-  double q = __builtin_rint(d / sd);
-  const double r2 = 2.0 * __builtin_fma(-q, sd, d);
-  const bool odd = ((int64_t)q & 1) != 0;
-  if (r2 > sd || (r2 == sd && odd)) q += 1.0;
-  else if (r2 < -sd || (r2 == -sd && odd)) q -= 1.0;
-  return (uint32_t)(int)__builtin_fmin(__builtin_fmax(q, 0.0), 15.0);
+// (x - m) / s to the nearest code, ties to even.  The quotient is corrected by its residual, which
+// makes it exact where it has few bits (a tie is j + 1/2) and keeps every other off the ties; 1.5 2^52
+// added leaves its nearest integer in the low word.  x is limited to [m, top], top = m + 16 s.
+__device__ __forceinline__ uint32_t code_of(float x, float m, float top, double md, double s, double inv) {
+  const double d = (double)__builtin_amdgcn_fmed3f(x, m, top) - md;
+  const double y0 = d * inv;
+  const double y = __builtin_fma(__builtin_fma(-y0, s, d), inv, y0);
+  const uint32_t q = (uint32_t)__builtin_bit_cast(uint64_t, y + 6755399441055744.0);
+  return q < 15u ? q : 15u;
 }
 
-// A group's m and s from its extremes.
-__device__ __forceinline__ float group_step(float hi, float m) {
-  const float raw = (hi - m) * (1.0f / 15.0f);
-  int e = (int)((__builtin_bit_cast(uint32_t, raw) >> 23) & 255) - 126 - 7;   // lsb of 7 bits
-  if (e < -24) e = -24;
-  const float t = __builtin_amdgcn_ldexpf(raw, -e);                           // at most 128
-  const float n = __builtin_ceilf(t);
-  // next to a whole number of units, or where the range is none or past the format's end
-  if (!(n - t > 0x1p-10f && n - t < 1.0f - 0x1p-10f && raw < 4000.0f)) return exact_step(hi, m);
-  return __builtin_amdgcn_ldexpf(n, e);
+// Extremes of a group over G / 8 neighbouring lanes, as integers in the order of the values.
+__device__ __forceinline__ int ordered(float x) {
+  const int b = __builtin_bit_cast(int, x);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float of_ordered(int k) { return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff)); }
+
+template <int M> __device__ __forceinline__ int xor_int(int v) {
+  return __builtin_bit_cast(int, xor_partner<M>(__builtin_bit_cast(float, v)));
 }
 
-__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
-  const float y = (x - m) * inv;
-  const float q = __builtin_rintf(y);
-  if (__builtin_expect(__builtin_fabsf(y - q) > 0.5f - 0x1p-12f, 0)) return exact_code(x, m, s);
-  return (uint32_t)(int)__builtin_fminf(__builtin_fmaxf(q, 0.0f), 15.0f);
-}
-
-template <int G>   // over G / 8 neighbouring lanes
-__device__ __forceinline__ void group_extremes(float& lo, float& hi, float& poison) {
-#define TT_LEVEL(M)                                   \
-  if (G / 8 > M) {                                    \
-    lo = __builtin_fminf(lo, xor_partner<M>(lo));     \
-    hi = __builtin_fmaxf(hi, xor_partner<M>(hi));     \
-    poison = poison + xor_partner<M>(poison);         \
+template <int G>
+__device__ __forceinline__ void group_extremes(int& lo, int& hi) {
+#define TT_LEVEL(M)                   \
+  if (G / 8 > M) {                    \
+    lo = min(lo, xor_int<M>(lo));     \
+    hi = max(hi, xor_int<M>(hi));     \
   }
   TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8)
 #undef TT_LEVEL
 }
 
+// The cache tokens of this workgroup: blocks of eight from `block` up to `end`, and which of a row's
+// tokens lie there.
+struct BlockRows {
+  int start, count, block, end;
+  __device__ BlockRows(const KvRowsParams& P, int row, int part) {
+    start = P.starts[row];
+    count = P.counts ? min(P.counts[row], P.tokens) : P.tokens;
+    // beyond these no token is inside the cache, within them positions fit 32 bits
+    if (start >= P.c.capacity || start <= -(1 << 30)) count = 0;
+    const int first = (start >> 3) + part * P.blocks_per;
+    const int64_t past = min((int64_t)start + max(count, 0) + 7, (int64_t)P.c.capacity) >> 3;
+    block = max(first, 0);
+    end = (int)min((int64_t)first + P.blocks_per, past);
+    if (count <= 0) end = block;
+  }
+};
+
 template <typename T, int D, int G>
 __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
   constexpr int W = D / 8;                         // words (and lanes) per token
   constexpr int NG = D / G;
-  __shared__ uint32_t vw[8][W];
+  __shared__ uint32_t vw[2][8][W];
   const int row = blockIdx.z, head = blockIdx.y;
-  const int start = P.starts[row];
-  const int count = P.counts ? min(P.counts[row], P.tokens) : P.tokens;
-  const int64_t block = (int64_t)(start >> 3) + blockIdx.x;
-  const int which = threadIdx.x / D;               // 0: K, 1: V
-  const int tid = threadIdx.x % D;
+  const BlockRows R(P, row, (int)blockIdx.x);
+  if (R.block >= R.end) return;
+  const int which = __builtin_amdgcn_readfirstlane((int)threadIdx.x / D);   // 0: K, 1: V; whole waves
+  const int tid = (int)threadIdx.x % D;
   const int token = tid / W, word = tid % W;
-  const int64_t pos = 8 * block + token;
-  const int64_t t = pos - start;
-  const bool valid = t >= 0 && t < count && pos >= 0 && pos < P.c.capacity;
-  float x[8];
-  const T* src = reinterpret_cast<const T*>(P.x[which]) + row * P.x_row[which] + (valid ? t : 0) * P.x_token[which] +
-                 head * P.x_head[which] + 8 * word;
-  if (P.vec) {
-    Eight<T> v;
-    v.load(src);
+  const bool first = word % (G / 8) == 0;          // writes the group's scales
+  const T* src = reinterpret_cast<const T*>(P.x[which]) + row * P.x_row[which] + head * P.x_head[which] + 8 * word;
+  const int64_t x_token = P.x_token[which];
+  // this thread's words of a block: of K its token's, of V its dim's
+  uint32_t* out = which == 0 ? reinterpret_cast<uint32_t*>(P.c.k_codes) + row * P.c.kc_seq + head * P.c.kc_head + tid
+                             : reinterpret_cast<uint32_t*>(P.c.v_codes) + row * P.c.vc_seq + head * P.c.vc_head + tid;
+  uint16_t* scales = which == 0 ? reinterpret_cast<uint16_t*>(P.c.k_scales) + row * P.c.ks_seq + head * P.c.ks_head +
+                                      (token * NG + word / (G / 8)) * 2
+                                : reinterpret_cast<uint16_t*>(P.c.v_scales) + row * P.c.vs_seq + head * P.c.vs_head +
+                                      word / (G / 8) * 16 + token;
+  Eight<T> next;
+  auto request = [&](int block) __attribute__((always_inline)) {
+    const int t = 8 * block + token - R.start;
+    const T* p = src + min(max(t, 0), R.count - 1) * x_token;
+    if (P.vec) {
+      next.load(p);
+    } else {
+      float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = valid ? v.get(e) : 0.0f;
-  } else {
+      for (int e = 0; e < 8; e++) y[e] = to_f32(p[e]);
+      next.set(y);                                 // back to what was stored
+    }
+  };
+  request(R.block);
+  for (int block = R.block; block < R.end; block++) {
+    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = valid ? to_f32(src[e]) : 0.0f;
-  }
-  float lo = x[0], hi = x[0], poison = 0.0f;
+    for (int e = 0; e < 8; e++) x[e] = next.get(e);
+    if (block + 1 < R.end) request(block + 1);
+    const int t = 8 * block + token - R.start;
+    const bool valid = t >= 0 && t < R.count;      // (positions of the block are inside the cache)
+    // extremes; a NaN, which those leave out, counts as an infinity
+    float lof = x[0], hif = x[0], poison = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    lo = __builtin_fminf(lo, x[e]);
-    hi = __builtin_fmaxf(hi, x[e]);
-    poison += x[e] * 0.0f;                         // NaN where x is not finite
-  }
-  group_extremes<G>(lo, hi, poison);
-  const bool finite = poison == poison;
-  const float m = round_f16(__builtin_fminf(__builtin_fmaxf(lo, -65504.0f), 65504.0f));
-  const float s = finite ? group_step(hi, m) : 0.0f;
-  // a group that is not finite reads as NaN
-  const uint16_t mb = finite ? f32_to_f16_bits(m) : 0x7e00u, sb = finite ? f32_to_f16_bits(s) : 0x7e00u;
-  uint32_t codes = 0;
-  if (s > 0.0f) {
-    const float inv = 1.0f / s;
+    for (int e = 0; e < 8; e++) {
+      lof = __builtin_fminf(lof, x[e]);
+      hif = __builtin_fmaxf(hif, x[e]);
+      poison = __builtin_fmaf(x[e], 0.0f, poison);
+    }
+    int lo = ordered(lof), hi = poison == poison ? ordered(hif) : 0x7f800000;
+    group_extremes<G>(lo, hi);
+    const bool finite = hi < 0x7f800000 && lo > ordered(__builtin_bit_cast(float, 0xff800000u));
+    const float m = round_f16(__builtin_amdgcn_fmed3f(of_ordered(lo), -65504.0f, 65504.0f));
+    const double s = finite ? group_step(of_ordered(hi), m) : 0.0;
+    const float sf = (float)s;
+    uint32_t codes = 0;
+    if (s > 0.0) {
+      const double md = (double)m;
+      const float top = m + 16.0f * sf;
+      double inv = __builtin_amdgcn_rcp(s);
+      inv = __builtin_fma(__builtin_fma(-s, inv, 1.0), inv, inv);
+      inv = __builtin_fma(__builtin_fma(-s, inv, 1.0), inv, inv);
 #pragma unroll
-    for (int e = 0; e < 8; e++) codes |= code_of(x[e], m, s, inv) << (4 * e);
-  }
-  if (which == 0) {
-    if (valid) {
-      const int64_t at = row * P.c.kc_seq + head * P.c.kc_head + pos * W + word;
-      reinterpret_cast<uint32_t*>(P.c.k_codes)[at] = codes;
-      if (word % (G / 8) == 0) {
-        const int64_t sat = row * P.c.ks_seq + head * P.c.ks_head + (pos * NG + word / (G / 8)) * 2;
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(P.c.k_scales) + sat) = sb | ((uint32_t)mb << 16);
+      for (int e = 0; e < 8; e++) codes |= code_of(x[e], m, top, md, s, inv) << (4 * e);
+    }
+    // a group that is not finite reads as NaN
+    const uint32_t mb = finite ? f32_to_f16_bits(m) : 0x7e00u, sb = finite ? f32_to_f16_bits(sf) : 0x7e00u;
+    if (which == 0) {
+      if (valid) {
+        out[(int64_t)block * D] = codes;
+        if (first) *reinterpret_cast<uint32_t*>(scales + (int64_t)block * (16 * NG)) = sb | (mb << 16);
+      }
+    } else {
+      vw[block & 1][token][word] = codes;
+      if (valid && first) {
+        scales[(int64_t)block * (16 * NG)] = (uint16_t)sb;
+        scales[(int64_t)block * (16 * NG) + 8] = (uint16_t)mb;
       }
     }
-  } else {
-    vw[token][word] = codes;
-    if (valid && word % (G / 8) == 0) {
-      uint16_t* vs = reinterpret_cast<uint16_t*>(P.c.v_scales) + row * P.c.vs_seq + head * P.c.vs_head +
-                     ((block * NG + word / (G / 8)) * 2) * 8 + token;
-      vs[0] = sb;
-      vs[8] = mb;
+    lds_barrier();                                 // the other buffer's readers are past it as well
+    if (which == 1) {
+      // this thread's dim of the eight tokens; the tokens that were not given keep their codes
+      uint32_t word_out = 0, keep = 0;
+#pragma unroll
+      for (int k = 0; k < 8; k++) word_out |= ((vw[block & 1][k][tid / 8] >> (4 * (tid % 8))) & 15u) << (4 * ((k >> 1) + 4 * (k & 1)));
+      const int t0 = 8 * block - R.start;
+      if (t0 < 0 || t0 + 8 > R.count) {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (t0 + k < 0 || t0 + k >= R.count) keep |= 15u << (4 * ((k >> 1) + 4 * (k & 1)));
+        word_out = (word_out & ~keep) | (out[(int64_t)block * D] & keep);
+      }
+      out[(int64_t)block * D] = word_out;
     }
   }
-  __syncthreads();
-  if (which == 0 || block < 0 || block >= P.c.capacity / 8) return;
-  // this thread's dim of the eight tokens; the tokens that were not given keep their codes
-  const int d = tid;
-  uint32_t word_out = 0, keep = 0;
-#pragma unroll
-  for (int k = 0; k < 8; k++) {
-    const int64_t pk = 8 * block + k, tk = pk - start;
-    const int nib = 4 * ((k >> 1) + 4 * (k & 1));
-    if (tk >= 0 && tk < count) word_out |= ((vw[k][d / 8] >> (4 * (d % 8))) & 15u) << nib;
-    else keep |= 15u << nib;
-  }
-  if (keep == 0xffffffffu) return;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(P.c.v_codes) + row * P.c.vc_seq + head * P.c.vc_head + block * D + d;
-  if (keep) word_out |= *dst & keep;
-  *dst = word_out;
 }
 
 template <typename T, int D, int G>
@@ -167,50 +193,72 @@ __global__ __launch_bounds__(2 * D) void kv_read_int4_kernel(KvRowsParams P) {
   constexpr int W = D / 8;
   constexpr int NG = D / G;
   const int row = blockIdx.z, head = blockIdx.y;
-  const int start = P.starts[row];
-  const int count = P.counts ? min(P.counts[row], P.tokens) : P.tokens;
-  const int64_t block = (int64_t)(start >> 3) + blockIdx.x;
-  const int which = threadIdx.x / D;
-  const int tid = threadIdx.x % D;
+  const BlockRows R(P, row, (int)blockIdx.x);
+  if (R.block >= R.end) return;
+  const int which = __builtin_amdgcn_readfirstlane((int)threadIdx.x / D);
+  const int tid = (int)threadIdx.x % D;
   const int token = tid / W, word = tid % W;
-  const int64_t pos = 8 * block + token;
-  const int64_t t = pos - start;
-  if (!(t >= 0 && t < count && pos >= 0 && pos < P.c.capacity)) return;
-  T* dst = reinterpret_cast<T*>(P.x[which]) + row * P.x_row[which] + t * P.x_token[which] + head * P.x_head[which] + 8 * word;
-  float y[8];
-  if (which == 0) {
-    const uint32_t w = reinterpret_cast<const uint32_t*>(P.c.k_codes)[row * P.c.kc_seq + head * P.c.kc_head + pos * W + word];
-    const uint32_t sm = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(P.c.k_scales) + row * P.c.ks_seq +
-                                                           head * P.c.ks_head + (pos * NG + word / (G / 8)) * 2);
-    const float s = lo_f32<f16_t>(sm), m = hi_f32<f16_t>(sm);
+  T* dst = reinterpret_cast<T*>(P.x[which]) + row * P.x_row[which] + head * P.x_head[which] + 8 * word;
+  const int64_t x_token = P.x_token[which];
+  const uint32_t* codes = which == 0 ? reinterpret_cast<const uint32_t*>(P.c.k_codes) + row * P.c.kc_seq + head * P.c.kc_head + tid
+                                     : reinterpret_cast<const uint32_t*>(P.c.v_codes) + row * P.c.vc_seq + head * P.c.vc_head + 8 * word;
+  const uint16_t* scales = which == 0 ? reinterpret_cast<const uint16_t*>(P.c.k_scales) + row * P.c.ks_seq + head * P.c.ks_head +
+                                            (token * NG + word / (G / 8)) * 2
+                                      : reinterpret_cast<const uint16_t*>(P.c.v_scales) + row * P.c.vs_seq + head * P.c.vs_head +
+                                            word / (G / 8) * 16 + token;
+  const int m_at = which == 0 ? 1 : 8;
+  const int nib = 4 * ((token >> 1) + 4 * (token & 1));
+  // up to kAhead blocks are requested together, before the first store, which a later load would wait for
+  for (int b0 = R.block; b0 < R.end; b0 += kAhead) {
+    uint16_t s_bits[kAhead], m_bits[kAhead];
+    uint4 w0[kAhead], w1[kAhead];                  // K: the word in w0.x
 #pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)((w >> (4 * e)) & 15u), s, m);
-  } else {
-    const uint4* vc = reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(P.c.v_codes) + row * P.c.vc_seq +
-                                                     head * P.c.vc_head + block * D + 8 * word);
-    const uint4 w0 = vc[0], w1 = vc[1];
-    const f16_t* vs = reinterpret_cast<const f16_t*>(P.c.v_scales) + row * P.c.vs_seq + head * P.c.vs_head +
-                      ((block * NG + word / (G / 8)) * 2) * 8 + token;
-    const float s = to_f32(vs[0]), m = to_f32(vs[8]);
-    const int nib = 4 * ((token >> 1) + 4 * (token & 1));
-    const uint32_t ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+    for (int k = 0; k < kAhead; k++) {
+      const int block = min(b0 + k, R.end - 1);
+      const uint32_t* c = codes + (int64_t)block * D;
+      s_bits[k] = scales[(int64_t)block * (16 * NG)];
+      m_bits[k] = scales[(int64_t)block * (16 * NG) + m_at];
+      if (which == 0) {
+        w0[k].x = *c;
+      } else {
+        w0[k] = reinterpret_cast<const uint4*>(c)[0];
+        w1[k] = reinterpret_cast<const uint4*>(c)[1];
+      }
+    }
 #pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)((ws[e] >> nib) & 15u), s, m);
-  }
-  if (P.vec) {
-    Eight<T> v;
-    v.set(y);
-    v.store(dst);
-  } else {
+    for (int k = 0; k < kAhead; k++) {
+      const float s = to_f32(f16_t{s_bits[k]}), m = to_f32(f16_t{m_bits[k]});
+      float y[8];
+      if (which == 0) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) store<T>(dst + e, y[e]);
+        for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)((w0[k].x >> (4 * e)) & 15u), s, m);
+      } else {
+        const uint32_t ws[8] = {w0[k].x, w0[k].y, w0[k].z, w0[k].w, w1[k].x, w1[k].y, w1[k].z, w1[k].w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf((float)((ws[e] >> nib) & 15u), s, m);
+      }
+      const int t = 8 * (b0 + k) + token - R.start;
+      if (b0 + k >= R.end || t < 0 || t >= R.count) continue;
+      T* o = dst + t * x_token;
+      if (P.vec) {
+        Eight<T> v;
+        v.set(y);
+        v.store(o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) store<T>(o + e, y[e]);
+      }
+    }
   }
 }
 
 template <typename T, bool APPEND>
-static int launch_rows(const KvRowsParams& P, int64_t rows, hipStream_t st, const char* what) {
+static int launch_rows(KvRowsParams P, int64_t rows, hipStream_t st, const char* what) {
   // any start inside a block: one block more than the tokens fill
-  const dim3 grid((unsigned)((P.tokens + 14) / 8), (unsigned)P.c.kv_heads, (unsigned)rows);
+  const int64_t blocks = (P.tokens + 14) / 8;
+  const int64_t fill = blocks * P.c.kv_heads * rows * P.c.head_dim / (256 * 2048);
+  P.blocks_per = (int)(fill < 1 ? 1 : fill > kMostBlocks ? kMostBlocks : fill);
+  const dim3 grid((unsigned)((blocks + P.blocks_per - 1) / P.blocks_per), (unsigned)P.c.kv_heads, (unsigned)rows);
   const dim3 block((unsigned)(2 * P.c.head_dim));
 #define TT_ROWS(D, G)                                                                                     \
   if (P.c.head_dim == D && P.c.group_size == G) {                                                         \
