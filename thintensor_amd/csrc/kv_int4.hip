@@ -1,10 +1,10 @@
 // Packing tokens into the 4-bit KV cache and reading them back (layout and rounding: tt_int4_cache
 // and tt_kv_append_int4 in thintensor_hip.h).
 //
-// A workgroup owns one block of eight cache tokens of one sequence and KV head: the V words hold
+// A workgroup owns whole blocks of eight cache tokens of one sequence and KV head: the V words hold
 // eight tokens, so a word has one writer, which merges the tokens it was not given from memory.  Half
-// of its threads pack K, half V; a thread holds eight dims of one token, and a group's extremes are
-// exact under any order, taken over its 4, 8 or 16 lanes.
+// of its threads pack K, half V, two blocks at a time; a thread holds sixteen dims of one token, and a
+// group's extremes are exact under any order, taken over its 2, 4 or 8 lanes.
 #include "kv_int4.h"
 #include "tt_common.h"
 #include "tt_eight.h"
@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t code_of(float x, float m, float top, double 
   return q < 15u ? q : 15u;
 }
 
-// Extremes of a group over G / 8 neighbouring lanes, as integers in the order of the values.
+// Extremes of a group over G / 16 neighbouring lanes, as integers in the order of the values.
 __device__ __forceinline__ int ordered(float x) {
   const int b = __builtin_bit_cast(int, x);
   return b ^ ((b >> 31) & 0x7fffffff);
@@ -65,11 +65,11 @@ template <int M> __device__ __forceinline__ int xor_int(int v) {
 template <int G>
 __device__ __forceinline__ void group_extremes(int& lo, int& hi) {
 #define TT_LEVEL(M)                   \
-  if (G / 8 > M) {                    \
+  if (G / 16 > M) {                   \
     lo = min(lo, xor_int<M>(lo));     \
     hi = max(hi, xor_int<M>(hi));     \
   }
-  TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8)
+  TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4)
 #undef TT_LEVEL
 }
 
@@ -92,50 +92,54 @@ struct BlockRows {
 
 template <typename T, int D, int G>
 __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
-  constexpr int W = D / 8;                         // words (and lanes) per token
+  constexpr int W = D / 16;                        // lanes per token, two words each
   constexpr int NG = D / G;
-  __shared__ uint32_t vw[2][8][W];
+  __shared__ uint2 vw[2][16][W];
   const int row = blockIdx.z, head = blockIdx.y;
   const BlockRows R(P, row, (int)blockIdx.x);
   if (R.block >= R.end) return;
   const int which = __builtin_amdgcn_readfirstlane((int)threadIdx.x / D);   // 0: K, 1: V; whole waves
   const int tid = (int)threadIdx.x % D;
-  const int token = tid / W, word = tid % W;
-  const bool first = word % (G / 8) == 0;          // writes the group's scales
-  const T* src = reinterpret_cast<const T*>(P.x[which]) + row * P.x_row[which] + head * P.x_head[which] + 8 * word;
+  const int token = tid / W, word = tid % W;       // of two blocks' sixteen
+  const bool first = word % (G / 16) == 0;         // writes the group's scales
+  const T* src = reinterpret_cast<const T*>(P.x[which]) + row * P.x_row[which] + head * P.x_head[which] + 16 * word;
   const int64_t x_token = P.x_token[which];
   // this thread's words of a block: of K its token's, of V its dim's
-  uint32_t* out = which == 0 ? reinterpret_cast<uint32_t*>(P.c.k_codes) + row * P.c.kc_seq + head * P.c.kc_head + tid
+  uint32_t* out = which == 0 ? reinterpret_cast<uint32_t*>(P.c.k_codes) + row * P.c.kc_seq + head * P.c.kc_head + 2 * tid
                              : reinterpret_cast<uint32_t*>(P.c.v_codes) + row * P.c.vc_seq + head * P.c.vc_head + tid;
   uint16_t* scales = which == 0 ? reinterpret_cast<uint16_t*>(P.c.k_scales) + row * P.c.ks_seq + head * P.c.ks_head +
-                                      (token * NG + word / (G / 8)) * 2
+                                      (token * NG + word / (G / 16)) * 2
                                 : reinterpret_cast<uint16_t*>(P.c.v_scales) + row * P.c.vs_seq + head * P.c.vs_head +
-                                      word / (G / 8) * 16 + token;
-  Eight<T> next;
+                                      (token / 8 * NG + word / (G / 16)) * 16 + token % 8;
+  Eight<T> next[2];
   auto request = [&](int block) __attribute__((always_inline)) {
     const int t = 8 * block + token - R.start;
     const T* p = src + min(max(t, 0), R.count - 1) * x_token;
-    if (P.vec) {
-      next.load(p);
-    } else {
-      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = to_f32(p[e]);
-      next.set(y);                                 // back to what was stored
+    for (int h = 0; h < 2; h++) {
+      if (P.vec) {
+        next[h].load(p + 8 * h);
+      } else {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = to_f32(p[8 * h + e]);
+        next[h].set(y);                            // back to what was stored
+      }
     }
   };
   request(R.block);
-  for (int block = R.block; block < R.end; block++) {
-    float x[8];
+  int buffer = 0;
+  for (int block = R.block; block < R.end; block += 2, buffer ^= 1) {
+    float x[16];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = next.get(e);
-    if (block + 1 < R.end) request(block + 1);
+    for (int e = 0; e < 16; e++) x[e] = next[e >> 3].get(e & 7);
+    if (block + 2 < R.end) request(block + 2);
     const int t = 8 * block + token - R.start;
-    const bool valid = t >= 0 && t < R.count;      // (positions of the block are inside the cache)
+    const bool valid = t >= 0 && t < R.count && block + token / 8 < R.end;
     // extremes; a NaN, which those leave out, counts as an infinity
     float lof = x[0], hif = x[0], poison = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
+    for (int e = 0; e < 16; e++) {
       lof = __builtin_fminf(lof, x[e]);
       hif = __builtin_fmaxf(hif, x[e]);
       poison = __builtin_fmaf(x[e], 0.0f, poison);
@@ -146,7 +150,7 @@ __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
     const float m = round_f16(__builtin_amdgcn_fmed3f(of_ordered(lo), -65504.0f, 65504.0f));
     const double s = finite ? group_step(of_ordered(hi), m) : 0.0;
     const float sf = (float)s;
-    uint32_t codes = 0;
+    uint2 codes = make_uint2(0, 0);
     if (s > 0.0) {
       const double md = (double)m;
       const float top = m + 16.0f * sf;
@@ -154,17 +158,20 @@ __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
       inv = __builtin_fma(__builtin_fma(-s, inv, 1.0), inv, inv);
       inv = __builtin_fma(__builtin_fma(-s, inv, 1.0), inv, inv);
 #pragma unroll
-      for (int e = 0; e < 8; e++) codes |= code_of(x[e], m, top, md, s, inv) << (4 * e);
+      for (int e = 0; e < 8; e++) {
+        codes.x |= code_of(x[e], m, top, md, s, inv) << (4 * e);
+        codes.y |= code_of(x[8 + e], m, top, md, s, inv) << (4 * e);
+      }
     }
     // a group that is not finite reads as NaN
     const uint32_t mb = finite ? f32_to_f16_bits(m) : 0x7e00u, sb = finite ? f32_to_f16_bits(sf) : 0x7e00u;
     if (which == 0) {
       if (valid) {
-        out[(int64_t)block * D] = codes;
+        *reinterpret_cast<uint2*>(out + (int64_t)block * D) = codes;
         if (first) *reinterpret_cast<uint32_t*>(scales + (int64_t)block * (16 * NG)) = sb | (mb << 16);
       }
     } else {
-      vw[block & 1][token][word] = codes;
+      vw[buffer][token][word] = codes;
       if (valid && first) {
         scales[(int64_t)block * (16 * NG)] = (uint16_t)sb;
         scales[(int64_t)block * (16 * NG) + 8] = (uint16_t)mb;
@@ -172,18 +179,24 @@ __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
     }
     lds_barrier();                                 // the other buffer's readers are past it as well
     if (which == 1) {
-      // this thread's dim of the eight tokens; the tokens that were not given keep their codes
-      uint32_t word_out = 0, keep = 0;
+      // this thread's dim of a block's eight tokens; the tokens that were not given keep their codes
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(&vw[buffer][0][0]);
 #pragma unroll
-      for (int k = 0; k < 8; k++) word_out |= ((vw[block & 1][k][tid / 8] >> (4 * (tid % 8))) & 15u) << (4 * ((k >> 1) + 4 * (k & 1)));
-      const int t0 = 8 * block - R.start;
-      if (t0 < 0 || t0 + 8 > R.count) {
+      for (int h = 0; h < 2; h++) {
+        if (block + h >= R.end) break;
+        uint32_t word_out = 0, keep = 0;
 #pragma unroll
         for (int k = 0; k < 8; k++)
-          if (t0 + k < 0 || t0 + k >= R.count) keep |= 15u << (4 * ((k >> 1) + 4 * (k & 1)));
-        word_out = (word_out & ~keep) | (out[(int64_t)block * D] & keep);
+          word_out |= ((words[(8 * h + k) * (D / 8) + tid / 8] >> (4 * (tid % 8))) & 15u) << (4 * ((k >> 1) + 4 * (k & 1)));
+        const int t0 = 8 * (block + h) - R.start;
+        if (t0 < 0 || t0 + 8 > R.count) {
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (t0 + k < 0 || t0 + k >= R.count) keep |= 15u << (4 * ((k >> 1) + 4 * (k & 1)));
+          word_out = (word_out & ~keep) | (out[(int64_t)(block + h) * D] & keep);
+        }
+        out[(int64_t)(block + h) * D] = word_out;
       }
-      out[(int64_t)block * D] = word_out;
     }
   }
 }
@@ -257,7 +270,7 @@ static int launch_rows(KvRowsParams P, int64_t rows, hipStream_t st, const char*
   // any start inside a block: one block more than the tokens fill
   const int64_t blocks = (P.tokens + 14) / 8;
   const int64_t fill = blocks * P.c.kv_heads * rows * P.c.head_dim / (256 * 2048);
-  P.blocks_per = (int)(fill < 1 ? 1 : fill > kMostBlocks ? kMostBlocks : fill);
+  P.blocks_per = (int)(fill < 2 ? (APPEND ? 2 : 1) : fill > kMostBlocks ? kMostBlocks : fill & ~1);
   const dim3 grid((unsigned)((blocks + P.blocks_per - 1) / P.blocks_per), (unsigned)P.c.kv_heads, (unsigned)rows);
   const dim3 block((unsigned)(2 * P.c.head_dim));
 #define TT_ROWS(D, G)                                                                                     \
