@@ -1552,8 +1552,9 @@ class HipDecodeBackend:
     @staticmethod
     def _on_device(t: torch.Tensor, *others: torch.Tensor | None) -> None:
         """Every tensor on the first one's GPU."""
-        _require_cuda(t)
         device = t.device
+        if device.type != "cuda":
+            raise ValueError("HipDecodeBackend operates on device tensors only")
         for o in others:
             if o is not None and o.device != device:
                 raise ValueError(f"tensors on different devices: {device} and {o.device}")
@@ -1568,53 +1569,74 @@ class HipDecodeBackend:
         (:func:`thintensor_amd.rotary.rotary_frequencies`).  Without outputs in place; an output may be
         its input but not overlap one otherwise."""
         q_out = q if q_out is None else q_out
-        k_out = k if k_out is None else k_out
-        if q.ndim != 3 or (k is not None and (k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
-            raise ValueError("rotary_rows takes q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim]")
-        if q_out.shape != q.shape or (k is not None and k_out.shape != k.shape) or (k is None and k_out is not None):
-            raise ValueError("rotary_rows outputs must have their inputs' shapes")
-        if q_out.dtype != q.dtype or (k is not None and (k.dtype != q.dtype or k_out.dtype != q.dtype)):
-            raise ValueError("rotary_rows operands must share a dtype")
+        if k is None:
+            if k_out is not None:
+                raise ValueError("rotary_rows: k_out without k")
+        elif k_out is None:
+            k_out = k
+        qs, qos = q.stride(), q_out.stride()
+        if q.ndim != 3 or q_out.shape != q.shape:
+            raise ValueError("rotary_rows takes q and its output [tokens, heads, head_dim]")
         tokens, heads, head_dim = q.shape
+        dtype = q.dtype
+        if q_out.dtype != dtype:
+            raise ValueError("rotary_rows operands must share a dtype")
         if positions.numel() != tokens or not positions.is_contiguous() or \
                 positions.dtype not in (torch.int32, torch.int64):
             raise ValueError("rotary_rows takes one int32 or int64 position per token")
         if inv_freq.dtype != torch.float64 or inv_freq.ndim != 1 or not inv_freq.is_contiguous():
             raise ValueError("rotary_rows frequencies must be a contiguous float64 vector")
-        if any(t is not None and t.stride(2) != 1 for t in (q, k, q_out, k_out)):
+        if qs[2] != 1 or qos[2] != 1:
             raise ValueError("rotary_rows operands must be contiguous in their last axis")
+        if k is not None:
+            ks, kos, shape = k.stride(), k_out.stride(), k.shape
+            if k.ndim != 3 or shape[0] != tokens or shape[2] != head_dim or k_out.shape != shape:
+                raise ValueError("rotary_rows takes k and its output [tokens, kv_heads, head_dim]")
+            if k.dtype != dtype or k_out.dtype != dtype:
+                raise ValueError("rotary_rows operands must share a dtype")
+            if ks[2] != 1 or kos[2] != 1:
+                raise ValueError("rotary_rows operands must be contiguous in their last axis")
+            k_args = (k.data_ptr(), ks[0], ks[1])
+            ko_args = (k_out.data_ptr(), kos[0], kos[1])
+            kv_heads = shape[1]
+        else:
+            k_args, ko_args, kv_heads = (None, 0, 0), (None, 0, 0), 0
         self._on_device(q, k, positions, inv_freq, q_out, k_out)
         with _device_of(q):
             rc = self.lib.tt_rotary_rows(
-                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr() if k is not None else None,
-                k.stride(0) if k is not None else 0, k.stride(1) if k is not None else 0, _code(q, "rotary_rows"),
-                positions.data_ptr(), positions.element_size(), inv_freq.data_ptr(), float(amplitude), int(interleaved),
-                tokens, heads, int(k.shape[1]) if k is not None else 0, head_dim, 2 * inv_freq.numel(),
-                q_out.data_ptr(), q_out.stride(0), q_out.stride(1), k_out.data_ptr() if k is not None else None,
-                k_out.stride(0) if k is not None else 0, k_out.stride(1) if k is not None else 0, _stream(q))
-        _lib.check(rc, "rotary_rows")
+                q.data_ptr(), qs[0], qs[1], *k_args, _code(q, "rotary_rows"), positions.data_ptr(),
+                positions.element_size(), inv_freq.data_ptr(), amplitude, int(interleaved), tokens, heads, kv_heads,
+                head_dim, 2 * inv_freq.numel(), q_out.data_ptr(), qos[0], qos[1], *ko_args, _stream(q))
+        if rc:
+            _lib.check(rc, "rotary_rows")
         return q_out, k_out
 
     def _kv_rows(self, entry, what: str, cache: Int4KvCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
                  counts: torch.Tensor | None) -> None:
-        if k.ndim not in (3, 4) or k.shape != v.shape or k.dtype != v.dtype:
+        shape, ks, vs = k.shape, k.stride(), v.stride()
+        if len(shape) not in (3, 4) or v.shape != shape or k.dtype != v.dtype:
             raise ValueError(f"{what} takes k and v [rows, tokens, kv_heads, head_dim] (or [rows, kv_heads, head_dim])")
-        rows, tokens = int(k.shape[0]), int(k.shape[1]) if k.ndim == 4 else 1
-        if rows > cache.batch or k.shape[-2] != cache.kv_heads or k.shape[-1] != cache.head_dim:
-            raise ValueError(f"{what}: {tuple(k.shape)} does not fit a cache of {cache.batch} sequences, "
+        rows = shape[0]
+        if len(shape) == 4:
+            tokens, k_token, v_token = shape[1], ks[1], vs[1]
+        else:
+            tokens, k_token, v_token = 1, 0, 0
+        if rows > cache.batch or shape[-2] != cache.kv_heads or shape[-1] != cache.head_dim:
+            raise ValueError(f"{what}: {tuple(shape)} does not fit a cache of {cache.batch} sequences, "
                              f"{cache.kv_heads} KV heads of {cache.head_dim}")
-        if k.stride(-1) != 1 or v.stride(-1) != 1:
+        if ks[-1] != 1 or vs[-1] != 1:
             raise ValueError(f"{what}: k and v must be contiguous in their last axis")
-        for t in (starts, counts):
-            if t is not None and (t.dtype != torch.int32 or t.numel() != rows or not t.is_contiguous()):
-                raise ValueError(f"{what}: starts and counts must be int32, one per row")
+        if starts.dtype != torch.int32 or starts.numel() != rows or not starts.is_contiguous():
+            raise ValueError(f"{what}: starts must be int32, one per row")
+        if counts is not None and (counts.dtype != torch.int32 or counts.numel() != rows or not counts.is_contiguous()):
+            raise ValueError(f"{what}: counts must be int32, one per row")
         self._on_device(k, v, starts, counts, cache.k_codes)
         with _device_of(k):
             rc = entry(
-                cache.desc, k.data_ptr(), k.stride(0), k.stride(1) if k.ndim == 4 else 0, k.stride(-2), v.data_ptr(),
-                v.stride(0), v.stride(1) if v.ndim == 4 else 0, v.stride(-2), _code(k, what), starts.data_ptr(),
-                counts.data_ptr() if counts is not None else None, rows, tokens, _stream(k))
-        _lib.check(rc, what)
+                cache.desc, k.data_ptr(), ks[0], k_token, ks[-2], v.data_ptr(), vs[0], v_token, vs[-2], _code(k, what),
+                starts.data_ptr(), counts.data_ptr() if counts is not None else None, rows, tokens, _stream(k))
+        if rc:
+            _lib.check(rc, what)
 
     def kv_append_int4(self, cache: Int4KvCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
                        counts: torch.Tensor | None = None) -> None:
@@ -1641,34 +1663,37 @@ class HipDecodeBackend:
         ``scale`` is head_dim ** -0.5 by default.  ``max_length`` (by default the capacity) bounds the
         lengths, longer ones count as it, and sizes the launch.  A row that sees nothing is 0.  Scratch
         of long contexts comes from the current stream's allocator with every call."""
-        if q.ndim != 3 or out.shape != q.shape or out.dtype != q.dtype:
+        shape, qs, os, dtype = q.shape, q.stride(), out.stride(), q.dtype
+        if len(shape) != 3 or out.shape != shape or out.dtype != dtype:
             raise ValueError("gqa_attention_int4 takes q and out [rows, heads, head_dim] of one dtype")
-        rows, heads, head_dim = q.shape
+        rows, heads, head_dim = shape
         if head_dim != cache.head_dim or heads == 0 or heads % cache.kv_heads or rows > cache.batch:
-            raise ValueError(f"gqa_attention_int4: q {tuple(q.shape)} does not fit a cache of {cache.batch} sequences, "
+            raise ValueError(f"gqa_attention_int4: q {tuple(shape)} does not fit a cache of {cache.batch} sequences, "
                              f"{cache.kv_heads} KV heads of {cache.head_dim}")
-        if q.dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f"gqa_attention_int4 takes fp16 or bf16 queries, got {q.dtype}")
-        if q.stride(2) != 1 or out.stride(2) != 1:
+        if dtype != torch.float16 and dtype != torch.bfloat16:
+            raise ValueError(f"gqa_attention_int4 takes fp16 or bf16 queries, got {dtype}")
+        if qs[2] != 1 or os[2] != 1:
             raise ValueError("gqa_attention_int4: q and out must be contiguous in their last axis")
         if lengths.dtype != torch.int32 or lengths.numel() != rows or not lengths.is_contiguous():
             raise ValueError("gqa_attention_int4: lengths must be int32, one per row")
-        if sinks is not None and (sinks.numel() != heads or not sinks.is_contiguous()):
-            raise ValueError("gqa_attention_int4: sinks must hold one logit per query head")
-        limit = cache.capacity if max_length is None else int(max_length)
+        sink_ptr, sink_code = None, _lib.F32
+        if sinks is not None:
+            if sinks.numel() != heads or not sinks.is_contiguous():
+                raise ValueError("gqa_attention_int4: sinks must hold one logit per query head")
+            sink_ptr, sink_code = sinks.data_ptr(), _code(sinks, "sinks")
+        limit = cache.capacity if max_length is None else max_length
         self._on_device(q, out, lengths, sinks, cache.k_codes)
         with _device_of(q):
-            need = self.lib.tt_gqa_attention_int4_scratch_floats(cache.desc, rows, heads, int(window), int(first_tokens), limit)
+            need = self.lib.tt_gqa_attention_int4_scratch_floats(cache.desc, rows, heads, window, first_tokens, limit)
             if need < 0:
                 _lib.check(int(need), "gqa_attention_int4")
             scratch = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
             rc = self.lib.tt_gqa_attention_int4(
-                cache.desc, q.data_ptr(), q.stride(0), q.stride(1), _code(q, "gqa_attention_int4"), lengths.data_ptr(), rows,
-                heads, int(window), int(first_tokens), limit, sinks.data_ptr() if sinks is not None else None,
-                _code(sinks, "sinks") if sinks is not None else _lib.F32,
-                float(scale) if scale is not None else head_dim ** -0.5, scratch.data_ptr() if scratch is not None else None,
-                need, out.data_ptr(), out.stride(0), out.stride(1), _stream(q))
-        _lib.check(rc, "gqa_attention_int4")
+                cache.desc, q.data_ptr(), qs[0], qs[1], _code(q, "gqa_attention_int4"), lengths.data_ptr(), rows, heads,
+                window, first_tokens, limit, sink_ptr, sink_code, scale if scale is not None else head_dim ** -0.5,
+                scratch.data_ptr() if need else None, need, out.data_ptr(), os[0], os[1], _stream(q))
+        if rc:
+            _lib.check(rc, "gqa_attention_int4")
         return out
 
     def sample_rows(self, logits: torch.Tensor, uniforms: torch.Tensor, tokens: torch.Tensor, *,
@@ -1688,21 +1713,24 @@ class HipDecodeBackend:
         rows, vocab = logits.shape
         if tokens.dtype != torch.int64 or tokens.numel() != rows or not tokens.is_contiguous():
             raise ValueError("sample_rows: tokens must be a contiguous int64 tensor, one per row")
-        for name, t, dtype in (("uniforms", uniforms, torch.float32), ("temperature", temperature, torch.float32),
-                               ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                               ("min_p", min_p, torch.float32), ("probs", probs, torch.float32)):
-            if t is not None and (t.dtype != dtype or t.numel() != rows or not t.is_contiguous()):
-                raise ValueError(f"sample_rows: {name} must be contiguous {dtype}, one per row")
+        ptrs = []
+        for name, t in (("uniforms", uniforms), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
+                        ("min_p", min_p), ("probs", probs)):
+            if t is None:
+                ptrs.append(None)
+                continue
+            if t.dtype != (torch.int32 if name == "top_k" else torch.float32) or t.numel() != rows or not t.is_contiguous():
+                raise ValueError(f"sample_rows: {name} must be contiguous {'int32' if name == 'top_k' else 'float32'}, one per row")
+            ptrs.append(t.data_ptr())
         self._on_device(logits, uniforms, tokens, temperature, top_k, top_p, min_p, probs)
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         with _device_of(logits):
             need = self.lib.tt_sample_rows_scratch_bytes(rows, vocab)
             scratch = torch.empty(need, device=logits.device, dtype=torch.uint8)
             rc = self.lib.tt_sample_rows(
-                logits.data_ptr(), logits.stride(0), _code(logits, "sample_rows"), rows, vocab, uniforms.data_ptr(),
-                ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), scratch.data_ptr(), need, tokens.data_ptr(),
-                ptr(probs), _stream(logits))
-        _lib.check(rc, "sample_rows")
+                logits.data_ptr(), logits.stride(0), _code(logits, "sample_rows"), rows, vocab, *ptrs[:5],
+                scratch.data_ptr(), need, tokens.data_ptr(), ptrs[5], _stream(logits))
+        if rc:
+            _lib.check(rc, "sample_rows")
         return tokens
 
     # ------------------------------------------------------------ decode-step helpers (no reference counterpart)
