@@ -31,6 +31,8 @@ import torch
 
 from . import _lib
 from .backend import HipDecodeBackend
+from .kv_cache import Int4KvCache
+from .rotary import rotary_frequencies
 from .synth import DenseWeights, MoEWeights
 
 _ACT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -545,3 +547,133 @@ class MoEBatchDecoder:
                 self.step()
         torch.cuda.synchronize(self.device)
         return self.history[:, :steps].cpu().tolist()
+
+
+class DenseBatchDecoder:
+    """Requests of a dense int4 model decoded together, each at its own position over a KV cache of
+    4 bits, their tokens sampled from given uniform numbers.
+
+    Every launch covers the batch: batched int4 GEMMs, rotary positions from frequencies (``rotary``:
+    frequencies and amplitude of :func:`~thintensor_amd.rotary.rotary_frequencies`, by default the
+    model's theta), the append to each layer's cache, attention (optionally a window of ``window``
+    tokens and ``first_tokens`` first ones), the lm_head's logits and ``sample_rows``.  Sampling settings
+    are per request (:meth:`set_sampling`, greedy at first).  A request that has reached the capacity
+    keeps decoding without storing further tokens; one whose logits leave nothing gets token -1."""
+
+    def __init__(self, backend: HipDecodeBackend, weights: DenseWeights, batch: int, capacity: int, *,
+                 group_size: int = 32, window: int = 0, first_tokens: int = 0,
+                 rotary: tuple[torch.Tensor, float] | None = None) -> None:
+        s = weights.shape
+        if batch < 1 or capacity < 1:
+            raise ValueError("batch and capacity must be at least 1")
+        self.be, self.w, self.s, self.batch = backend, weights, s, batch
+        dev = weights.embed.device
+        self.device, dt = dev, torch.float16
+        self.window, self.first_tokens = window, first_tokens
+        self.inv_freq, self.amplitude = rotary or rotary_frequencies(s.head_dim, s.rope_theta, device=dev)
+        self.caches = [Int4KvCache.allocate(batch, s.kv_heads, capacity, s.head_dim, group_size, dev)
+                       for _ in weights.layers]
+        self.capacity = self.caches[0].capacity
+        self.tokens = torch.zeros(batch, device=dev, dtype=torch.int64)
+        self.positions = torch.zeros(batch, device=dev, dtype=torch.int32)   # of the tokens to come
+        self.lengths = torch.ones(batch, device=dev, dtype=torch.int32)      # positions + 1
+        self.uniforms = torch.zeros(batch, device=dev)
+        self.temperature = torch.zeros(batch, device=dev)
+        self.top_k = torch.zeros(batch, device=dev, dtype=torch.int32)
+        self.top_p = torch.ones(batch, device=dev)
+        self.min_p = torch.zeros(batch, device=dev)
+        self.probs = torch.zeros(batch, device=dev)
+        empty = lambda n: torch.empty((batch, n), device=dev, dtype=dt)  # noqa: E731
+        self.zeros = torch.zeros((batch, s.hidden), device=dev, dtype=dt)
+        self.embedded, self.hidden_a, self.hidden_b = empty(s.hidden), empty(s.hidden), empty(s.hidden)
+        self.normed, self.attn_out, self.mlp = empty(s.hidden), empty(s.hidden), empty(s.hidden)
+        self.q, self.k, self.v, self.attn = empty(s.q_dim), empty(s.kv_dim), empty(s.kv_dim), empty(s.q_dim)
+        self.gate, self.up, self.act = empty(s.intermediate), empty(s.intermediate), empty(s.intermediate)
+        self.greedy = torch.zeros(batch, device=dev, dtype=torch.int64)
+        self.logits = empty(int(weights.lm_head.shape[0]))
+        self.graph: torch.cuda.CUDAGraph | None = None
+        self._graph_stream: torch.cuda.Stream | None = None
+
+    def set_sampling(self, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0) -> None:
+        """Settings of every request: a number for all of them, or one per request."""
+        for buf, value in ((self.temperature, temperature), (self.top_k, top_k), (self.top_p, top_p), (self.min_p, min_p)):
+            buf.copy_(torch.as_tensor(value, dtype=buf.dtype).expand(self.batch))
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+               counts: torch.Tensor | None = None) -> None:
+        """Tokens that the requests already hold (rotated k, v [batch, tokens, kv_heads, head_dim])."""
+        self.be.kv_append_int4(self.caches[layer], k, v, starts, counts)
+
+    def step(self) -> None:
+        """One token of every request from ``uniforms``; advances the positions."""
+        be, w, s, B = self.be, self.w, self.s, self.batch
+        heads = self.q.view(B, s.heads, s.head_dim)
+        k, v = self.k.view(B, s.kv_heads, s.head_dim), self.v.view(B, s.kv_heads, s.head_dim)
+        for b in range(B):
+            be.embedding(w.embed, self.tokens[b], self.embedded[b])
+        left, right = self.embedded, self.zeros
+        for li, L in enumerate(w.layers):
+            be.add_then_rms_norm_rows(left, right, self.hidden_a, L.ln1, self.normed, s.eps)
+            for (packed, scales), out in ((L.q, self.q), (L.k, self.k), (L.v, self.v)):
+                be.int4_batched_matvec(packed, scales, self.normed, out, group_size=s.group)
+            be.rotary_rows(heads, k, self.positions, self.inv_freq, amplitude=self.amplitude)
+            be.kv_append_int4(self.caches[li], k, v, self.positions)
+            be.gqa_attention_int4(heads, self.caches[li], self.attn.view(B, s.heads, s.head_dim), self.lengths,
+                                  window=self.window, first_tokens=self.first_tokens)
+            be.int4_batched_matvec(L.o[0], L.o[1], self.attn, self.attn_out, group_size=s.group)
+            be.add_then_rms_norm_rows(self.hidden_a, self.attn_out, self.hidden_b, L.ln2, self.normed, s.eps)
+            be.int4_batched_matvec(L.gate[0], L.gate[1], self.normed, self.gate, group_size=s.group)
+            be.int4_batched_matvec(L.up[0], L.up[1], self.normed, self.up, group_size=s.group)
+            be.silu_mul(self.gate, self.up, self.act)
+            be.int4_batched_matvec(L.down[0], L.down[1], self.act, self.mlp, group_size=s.group)
+            left, right = self.hidden_b, self.mlp
+        be.add_then_rms_norm_rows(left, right, self.hidden_a, w.final_norm, self.normed, s.eps)
+        be.matvec_argmax_batched(w.lm_head, self.normed, logits=self.logits, out=self.greedy)
+        be.sample_rows(self.logits, self.uniforms, self.tokens, temperature=self.temperature, top_k=self.top_k,
+                       top_p=self.top_p, min_p=self.min_p, probs=self.probs)
+        self.positions.add_(1)
+        self.lengths.add_(1)
+
+    def capture(self) -> None:
+        """Record one step into a HIP graph.  Scratch of the operators that keep theirs is reserved
+        first; the others take it from the graph's own pool."""
+        self.be._batched_argmax_scratch(self.batch, int(self.w.lm_head.shape[0]), self.s.hidden)
+        for rows, cols in ((self.s.intermediate, self.s.hidden), (self.s.hidden, self.s.intermediate)):
+            self.be._batched_workspace(self.batch, rows, cols)
+        torch.cuda.synchronize(self.device)
+        self._graph_stream = torch.cuda.Stream(self.device)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph, stream=self._graph_stream):
+            self.step()
+
+    def prime(self, tokens: list[int], positions: list[int]) -> None:
+        """The requests' next input tokens and the positions that these take."""
+        if len(tokens) != self.batch or len(positions) != self.batch:
+            raise ValueError("one start token and position per request")
+        if not all(0 <= p < self.capacity for p in positions):
+            raise ValueError("position outside the KV cache")
+        self.tokens.copy_(torch.tensor(tokens, dtype=torch.int64))
+        self.positions.copy_(torch.tensor(positions, dtype=torch.int32))
+        self.lengths.copy_(torch.tensor(positions, dtype=torch.int32) + 1)
+
+    def generate(self, tokens: list[int], positions: list[int], uniforms: torch.Tensor, use_graph: bool = True) -> list[list[int]]:
+        """One token per row of ``uniforms`` [steps, batch] for every request; one id list per request."""
+        steps = int(uniforms.shape[0])
+        if uniforms.ndim != 2 or uniforms.shape[1] != self.batch or uniforms.dtype != torch.float32:
+            raise ValueError("uniforms must be float32 [steps, batch]")
+        if max(positions) + steps > self.capacity:
+            raise ValueError("not enough KV capacity for the requested steps")
+        if use_graph and self.graph is None:
+            self.capture()
+        self.prime(tokens, positions)
+        history = torch.empty((steps, self.batch), device=self.device, dtype=torch.int64)
+        uniforms = uniforms.to(self.device)
+        for i in range(steps):
+            self.uniforms.copy_(uniforms[i])
+            if use_graph:
+                self.graph.replay()
+            else:
+                self.step()
+            history[i].copy_(self.tokens)
+        torch.cuda.synchronize(self.device)
+        return history.t().cpu().tolist()
