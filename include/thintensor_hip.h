@@ -774,7 +774,7 @@ int tt_archive_close(tt_archive* archive);
  * inputs themselves, but not overlap them otherwise.  inv_freq is binary64 (radians per
  * position): t is formed and reduced in binary64, the rotation in binary32, rounded once.
  * Strides of tokens and heads are free, the last axis is contiguous.  positions are int32 or
- * int64 (position_bytes 4 or 8), negative ones included. */
+ * int64 (position_bytes 4 or 8), negative ones included.  At most 2^22 tokens. */
 int tt_rotary_rows(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
                    int dtype, const void* positions, int position_bytes, const double* inv_freq, float amplitude,
                    int interleaved, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rotary,
@@ -808,7 +808,7 @@ int64_t tt_int4_cache_size(void); /* sizeof(tt_int4_cache), for bindings */
  * significant bits (a multiple of 2^-24, at most 4064) with 15 s >= maximum - m, and codes are
  * (x - m) / s rounded to the nearest, ties to even, limited to 0 .. 15, all as if in exact
  * arithmetic.  A group that holds an infinity or a NaN reads as NaN.  Strides of rows, tokens and
- * heads are free. */
+ * heads are free.  At most 2^26 tokens of a row. */
 int tt_kv_append_int4(const tt_int4_cache* cache, const void* k, int64_t k_row, int64_t k_token, int64_t k_head,
                       const void* v, int64_t v_row, int64_t v_token, int64_t v_head, int dtype,
                       const int32_t* starts, const int32_t* counts, int64_t rows, int64_t tokens, void* stream);

@@ -445,15 +445,22 @@ __global__ __launch_bounds__(256) void attn4_fold_kernel(Attn4Params P) {
   const int64_t at = ((int64_t)row * P.heads + h) * P.splits;
   const float2* ml = P.part_ml + at;
   const f4_t* po = reinterpret_cast<const f4_t*>(P.part_o + at * D);
+  // requested before the row's length is known, all inside the scratch: what no workgroup wrote is not used
+  constexpr int PER = kMostSplits / 64, PRE = 4;
+  float2 v[PER];
+  f4_t pre[PRE];
+#pragma unroll
+  for (int k = 0; k < PER; k++) v[k] = ml[min(lane + 64 * k, P.splits - 1)];
+#pragma unroll
+  for (int k = 0; k < PRE; k++) pre[k] = po[(int64_t)min(r + k * ROWS, P.splits - 1) * PIECES + piece];
   const Visible vis(P, row);
   const int nt = vis.tiles(), share = vis.share(P.splits);
   if (nt <= share) return;
   const int parts = (nt + share - 1) / share;
   const float ninf = __builtin_bit_cast(float, 0xff800000u);
-  constexpr int PER = kMostSplits / 64;
-  float2 v[PER];
 #pragma unroll
-  for (int k = 0; k < PER; k++) v[k] = lane + 64 * k < parts ? ml[lane + 64 * k] : make_float2(ninf, 0.0f);
+  for (int k = 0; k < PER; k++)
+    if (lane + 64 * k >= parts) v[k] = make_float2(ninf, 0.0f);
   float M = ninf;
 #pragma unroll
   for (int k = 0; k < PER; k++) M = fmaxf(M, v[k].x);
@@ -471,8 +478,11 @@ __global__ __launch_bounds__(256) void attn4_fold_kernel(Attn4Params P) {
   l = xor_sum(l, 1, 64);
   __syncthreads();
   f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int k = 0; k < PRE; k++)
+    if (r + k * ROWS < parts) acc += pre[k] * e_s[r + k * ROWS];
 #pragma unroll 4
-  for (int i = r; i < parts; i += ROWS) acc += po[(int64_t)i * PIECES + piece] * e_s[i];
+  for (int i = r + PRE * ROWS; i < parts; i += ROWS) acc += po[(int64_t)i * PIECES + piece] * e_s[i];
   sum[r][piece] = acc;
   __syncthreads();
   if (r == 0) {

@@ -292,7 +292,7 @@ static int rows_entry(const tt_int4_cache* cache, void* k, int64_t k_row, int64_
                       const int32_t* counts, int64_t rows, int64_t tokens, void* stream, const char* what) {
   const int rc = check_cache(cache, rows, what);
   if (rc) return rc;
-  TT_REQUIRE(tokens >= 0 && tokens < (1LL << 30), "%s: bad token count", what);
+  TT_REQUIRE(tokens >= 0 && tokens <= (1 << 26), "%s: at most 2^26 tokens of a row", what);
   TT_REQUIRE(valid_out_dtype(dtype), "%s: dtype must be fp16, bf16 or fp32", what);
   if (rows == 0 || tokens == 0) return TT_OK;
   TT_REQUIRE(k && v && starts, "%s: null pointer", what);

@@ -191,7 +191,7 @@ extern "C" int tt_rotary_rows(const void* q, int64_t q_token, int64_t q_head, co
                               int64_t kv_heads, int64_t head_dim, int64_t rotary, void* q_out, int64_t qo_token,
                               int64_t qo_head, void* k_out, int64_t ko_token, int64_t ko_head, void* stream) {
   const char* what = "rotary_rows";
-  TT_REQUIRE(tokens >= 0 && tokens < (1LL << 31), "%s: bad token count", what);
+  TT_REQUIRE(tokens >= 0 && tokens <= (1 << 22), "%s: at most 2^22 tokens", what);
   TT_REQUIRE(heads > 0 && kv_heads >= 0 && heads <= 65536 && kv_heads <= 65536, "%s: bad head counts", what);
   TT_REQUIRE(head_dim > 0 && head_dim <= 1024 && rotary > 0 && rotary <= head_dim && rotary % 2 == 0,
              "%s: rotary dims must be even and at most head_dim (1024 at most)", what);
