@@ -82,14 +82,13 @@ constexpr uint32_t kNegInf = 0xff800000u;
 __device__ __forceinline__ bool live(float x) { return x > __builtin_bit_cast(float, kNegInf); }
 
 // e^-z for z >= 0 in binary64, as p 2^n: z log2 e = -n + f, p = e^(f ln 2) by its Taylor polynomial
-// (|f ln 2| <= 0.3466: the first term left out is below 2^-57 of it).
+// (|f ln 2| <= 0.3466: the first term left out is below 2^-52 of it).
 __device__ __forceinline__ double exp_neg(double z, int* n) {
   const double y = z * -1.4426950408889634074;
   const double r = __builtin_rint(y);
   const double g = __builtin_fma(r, -0.69314718055994530942, -z);
   const double g2 = __builtin_fma(r, -2.3190468138462996e-17, g);   // the rest of ln 2
-  double p = 1.6059043836821613e-10;                                 // 1/13!
-  p = __builtin_fma(p, g2, 2.08767569878681e-09);
+  double p = 2.08767569878681e-09;                                   // 1/12!
   p = __builtin_fma(p, g2, 2.505210838544172e-08);
   p = __builtin_fma(p, g2, 2.755731922398589e-07);
   p = __builtin_fma(p, g2, 2.7557319223985893e-06);
@@ -106,29 +105,29 @@ __device__ __forceinline__ double exp_neg(double z, int* n) {
   return p;
 }
 
-// What a row's settings and range make of a logit.
+// What a row's settings and range make of a logit.  A greedy row, and one whose largest logit is
+// infinite, is `hard`: only the largest ones weigh.  Elsewhere -inf becomes an infinite z and NaN a NaN,
+// which weigh nothing.
 struct RowScale {
   double top, inv_t, bins_per_z;
-  bool greedy;
+  bool greedy, hard;
   __device__ RowScale(const SampleParams& P, int row, float2 range) {
     const float t = P.temperature ? P.temperature[row] : 1.0f;
     greedy = !(t > 0.0f);
+    hard = greedy || range.x == __builtin_bit_cast(float, 0x7f800000u);
     top = (double)range.x;
     inv_t = greedy ? 0.0 : 1.0 / (double)t;
-    const double far = greedy ? kReach : z_of(range.y);
+    const double far = hard ? kReach : soft_z(range.y);
     // all of the range in bins 0 .. kBins - 2, or what lies below kReach of it
     const double most = far < kReach ? far : kReach;
     bins_per_z = most > 0.0 ? (kBins - 2) / most : 0.0;
   }
+  __device__ double soft_z(float x) const { return (top - (double)x) * inv_t; }
   __device__ double z_of(float x) const {
-    const double d = top - (double)x;
-    if ((double)x == top) return 0.0;   // (infinities among them)
-    return greedy ? __builtin_inf() : d * inv_t;
+    if (hard) return (double)x == top ? 0.0 : __builtin_inf();
+    return soft_z(x);
   }
-  __device__ int bin_of(double z) const {
-    const double b = z == 0.0 ? 0.0 : z * bins_per_z;
-    return b < (double)(kBins - 1) ? (int)b : kBins - 1;
-  }
+  __device__ int bin_of(double z) const { return (int)__builtin_fmin(z * bins_per_z, (double)(kBins - 1)); }
   __device__ double weight_of(double z) const {
     if (!(z < 700.0)) return 0.0;
     int n;
@@ -137,11 +136,10 @@ struct RowScale {
   }
   // in units: 2^52 added leaves the rounded integer in the low bits
   __device__ uint64_t mass_of(double z) const {
-    if (!(z < 31.0)) return 0;
     int n;
     const double p = exp_neg(z, &n);
     const double v = __builtin_amdgcn_ldexp(p, n + 43) + 4503599627370496.0;
-    return __builtin_bit_cast(uint64_t, v) - 0x4330000000000000ull;
+    return z < 31.0 ? __builtin_bit_cast(uint64_t, v) - 0x4330000000000000ull : 0;
   }
 };
 
@@ -254,22 +252,36 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleParams P
   uint32_t far = 0;                     // of the last bin
   __syncthreads();
   while (i < end) {
-    double z[8];
     int b[8];
     uint64_t m[8];
+    if (S.hard) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      z[e] = live(x[e]) ? S.z_of(x[e]) : __builtin_inf();
-      b[e] = S.bin_of(z[e]);
-      m[e] = S.mass_of(z[e]);
-      far += live(x[e]) && b[e] == kBins - 1;
+      for (int e = 0; e < 8; e++) {
+        const bool is_top = (double)x[e] == S.top;
+        b[e] = is_top ? 0 : kBins - 1;
+        m[e] = is_top ? (uint64_t)kUnit : 0;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const double z = S.soft_z(x[e]);
+        b[e] = S.bin_of(z);
+        m[e] = S.mass_of(z);
+      }
+    }
+    if (counts) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (!live(x[e])) continue;
+        if (b[e] < kBins - 1) atomicAdd(&count[b[e]], 1u);
+        else far++;
+      }
     }
     const int next = i + 8 * kBinThreads;
     if (next < end) logits8<T>(P, row, next, x);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       if (m[e]) atomicAdd((unsigned long long*)&mass[b[e]], (unsigned long long)m[e]);
-      if (counts && b[e] < kBins - 1) atomicAdd(&count[b[e]], 1u);
     }
     i = next;
   }
@@ -538,13 +550,24 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams P)
       first = min(first, lo[a]);
       last = max(last, hi[a]);
     }
+  // logits outside [x_lo, x_hi] cannot be in them: the borders in z, with room for their rounding
+  float x_lo = __builtin_bit_cast(float, 0xff7fffffu), x_hi = __builtin_bit_cast(float, 0x7f800000u);
+  if (!S.hard && S.bins_per_z > 0.0) {
+    const double t = 1.0 / (S.bins_per_z * S.inv_t), lo_v = S.top - (last + 1) * t, hi_v = S.top - first * t;
+    const double room = 0x1p-20 * (__builtin_fabs(S.top) + (last + 1) * t);
+    x_lo = fmaxf(x_lo, (float)(lo_v - room));
+    x_hi = (float)(hi_v + room);
+  }
   for (int i0 = c * P.chunk; i0 < end; i0 += kStep) {
     i = i0 + 8 * (int)threadIdx.x;
     if (i0 > c * P.chunk && i < end) logits8<T>(P, row, i, x);
     if (i < end) {
+      uint32_t maybe = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) maybe |= x[e] >= x_lo && x[e] <= x_hi ? 1u << e : 0u;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        if (!live(x[e])) continue;
+        if (!((maybe >> e) & 1u)) continue;
         const int b = S.bin_of(S.z_of(x[e]));
         if (b < first || b > last) continue;
         bool in = false;
