@@ -560,7 +560,8 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams P)
   }
   for (int i0 = c * P.chunk; i0 < end; i0 += kStep) {
     i = i0 + 8 * (int)threadIdx.x;
-    if (i0 > c * P.chunk && i < end) logits8<T>(P, row, i, x);
+    float ahead[8];
+    if (i + kStep < end) logits8<T>(P, row, i + kStep, ahead);
     if (i < end) {
       uint32_t maybe = 0;
 #pragma unroll
@@ -576,9 +577,11 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams P)
         if (in) found[atomicAdd(&n_found, 1u)] = ((uint64_t)key_of(x[e]) << 32) | (uint32_t)~(uint32_t)(i + e);
       }
     }
-    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = ahead[e];
+    lds_barrier();
     const uint32_t n = n_found;
-    __syncthreads();                    // every thread has read it before it counts again
+    lds_barrier();                      // every thread has read it before it counts again
     if (n) {
       if (threadIdx.x == 0) {
         base = atomicAdd(&R.candidates, n);
