@@ -29,7 +29,7 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 constexpr int kTile = 32;          // tokens per step of a wave
 constexpr int kHeadBlock = 16;     // query heads per workgroup
 constexpr int kWaves = 4;
-constexpr int kMostSplits = 128;
+constexpr int kMostSplits = 512;
 // Weights are 2^7 exp(s - m), where m follows the running maximum only when that is more than 2^8 past it:
 // they stay below 2^15.
 constexpr float kPScale = 7.0f;
@@ -446,11 +446,9 @@ __global__ __launch_bounds__(256) void attn4_fold_kernel(Attn4Params P) {
   const float2* ml = P.part_ml + at;
   const f4_t* po = reinterpret_cast<const f4_t*>(P.part_o + at * D);
   // requested before the row's length is known, all inside the scratch: what no workgroup wrote is not used
-  constexpr int PER = kMostSplits / 64, PRE = 4;
-  float2 v[PER];
+  constexpr int PRE = 4;
+  float2 first = ml[min(lane, P.splits - 1)];
   f4_t pre[PRE];
-#pragma unroll
-  for (int k = 0; k < PER; k++) v[k] = ml[min(lane + 64 * k, P.splits - 1)];
 #pragma unroll
   for (int k = 0; k < PRE; k++) pre[k] = po[(int64_t)min(r + k * ROWS, P.splits - 1) * PIECES + piece];
   const Visible vis(P, row);
@@ -458,22 +456,19 @@ __global__ __launch_bounds__(256) void attn4_fold_kernel(Attn4Params P) {
   if (nt <= share) return;
   const int parts = (nt + share - 1) / share;
   const float ninf = __builtin_bit_cast(float, 0xff800000u);
-#pragma unroll
-  for (int k = 0; k < PER; k++)
-    if (lane + 64 * k >= parts) v[k] = make_float2(ninf, 0.0f);
-  float M = ninf;
-#pragma unroll
-  for (int k = 0; k < PER; k++) M = fmaxf(M, v[k].x);
+  if (lane >= parts) first = make_float2(ninf, 0.0f);
+  float M = first.x;
+  for (int k = lane + 64; k < parts; k += 64) M = fmaxf(M, ml[k].x);
 #define TT_LEVEL(X) M = fmaxf(M, xor_partner<X>(M));
   TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8) TT_LEVEL(16) TT_LEVEL(32)
 #undef TT_LEVEL
   const float base = M == ninf ? 0.0f : M;
   float l = 0.0f;
-#pragma unroll
-  for (int k = 0; k < PER; k++) {
-    const float e = __builtin_amdgcn_exp2f(v[k].x - base);
-    l = __builtin_fmaf(v[k].y, e, l);
-    if (threadIdx.x < 64) e_s[lane + 64 * k] = e;
+  for (int k = lane; k < parts; k += 64) {
+    const float2 v = k == lane ? first : ml[k];
+    const float e = __builtin_amdgcn_exp2f(v.x - base);
+    l = __builtin_fmaf(v.y, e, l);
+    if (threadIdx.x < 64) e_s[k] = e;
   }
   l = xor_sum(l, 1, 64);
   __syncthreads();
@@ -481,8 +476,14 @@ __global__ __launch_bounds__(256) void attn4_fold_kernel(Attn4Params P) {
 #pragma unroll
   for (int k = 0; k < PRE; k++)
     if (r + k * ROWS < parts) acc += pre[k] * e_s[r + k * ROWS];
-#pragma unroll 4
-  for (int i = r + PRE * ROWS; i < parts; i += ROWS) acc += po[(int64_t)i * PIECES + piece] * e_s[i];
+  constexpr int MORE = 16;              // (past the end: the last one, weight 0)
+  for (int i = r + PRE * ROWS; i < parts; i += MORE * ROWS) {
+    f4_t more[MORE];
+#pragma unroll
+    for (int k = 0; k < MORE; k++) more[k] = po[(int64_t)min(i + k * ROWS, parts - 1) * PIECES + piece];
+#pragma unroll
+    for (int k = 0; k < MORE; k++) acc += more[k] * (i + k * ROWS < parts ? e_s[i + k * ROWS] : 0.0f);
+  }
   sum[r][piece] = acc;
   __syncthreads();
   if (r == 0) {
@@ -504,11 +505,12 @@ static int64_t most_tiles(int64_t limit, int64_t window, int64_t first) {
 // Workgroups that share a row: few tiles are taken by one, since a second launch has to join several
 // (8 groups of sequence and KV head, head_dim 64: 19 tiles 6.6 us by one and 8.0 shared, 32 tiles 8.3 and
 // 7.8, 64 tiles 13.4 and 7.9), and more of them while there are groups for the chip (256 groups: 16 tiles
-// 6.5 and 10.4, 64 tiles 13.9 and 16.0).  Shared, 512 workgroups and eight tiles each (32768 tokens of 8 x
-// 64: 1024 workgroups 11.7, 512 9.8; four tiles each, 130 tiles, 10 x 128, 4 rows: 15.5 and 14.1).
+// 6.5 and 10.4, 64 tiles 13.9 and 16.0).  Shared, up to 512 workgroups, two for each CU, and eight tiles
+// each: 16384 tokens of 8 x 64, 1024 workgroups 11.7 us, 512 9.8; 52428 tokens of 2 x 10 x 128, 520
+// workgroups, of which some CUs take a third one, 43.0, 500 33.0.
 static int64_t split_count(int64_t groups, int64_t tiles) {
   if (tiles <= 24 || (groups >= 256 && tiles <= 64)) return 1;
-  const int64_t fill = (512 + groups - 1) / groups, most = (tiles + 7) / 8;
+  const int64_t fill = groups < 512 ? 512 / groups : 1, most = (tiles + 7) / 8;
   const int64_t s = fill < most ? fill : most;
   return s < kMostSplits ? s : kMostSplits;
 }
