@@ -135,40 +135,52 @@ struct Tile {
   uint32_t kw[2][KW], ks[2][LG];
   u4_t vw[VJ], vs[VJ], vm;
   static constexpr int NG = D / G;
-  // kc, ksp: this lane's quarter
-  __device__ __forceinline__ void load_k(const uint32_t* kc, const uint16_t* ksp, int t0, int n) {
+  // byte offsets of this lane in a tile, beside the tile's own address, which is the wave's
+  uint32_t k_at, ks_at, v_at, vs_at, vm_at;
+  __device__ __forceinline__ void place(int n, int quad) {
+    const int t = 8 * (n >> 2) + (n & 3);          // its token in the first half; four later in the second
+    k_at = (uint32_t)(t * (D / 2) + quad * (D / 8));
+    ks_at = (uint32_t)(t * (4 * NG) + quad * (D / 4) / G * 4);
+    v_at = (uint32_t)(quad * (4 * D) + 16 * n);
+    vs_at = (uint32_t)((quad * NG + (G == 32 ? n >> 3 : 0)) * 32);
+    // rows past the groups repeat the last one; their products are not used
+    vm_at = (uint32_t)((quad * NG + (n < NG ? n : NG - 1)) * 32 + 16);
+  }
+  __device__ __forceinline__ void load_k(const char* kc, const char* ksp, int t0) {
+    const char* k = kc + (int64_t)t0 * (D / 2);
+    const char* s = ksp + (int64_t)t0 * (4 * NG);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const int64_t t = t0 + 8 * (n >> 2) + 4 * h + (n & 3);
-      const uint32_t* p = kc + t * (D / 8);
+      const char* p = k + (size_t)(k_at + h * (2 * D));
       if constexpr (KW == 2) {
         const uint2 v = *reinterpret_cast<const uint2*>(p);
         kw[h][0] = v.x; kw[h][1] = v.y;
       } else {
 #pragma unroll
         for (int x = 0; x < KW / 4; x++) {
-          const u4_t v = *reinterpret_cast<const u4_t*>(p + 4 * x);
+          const u4_t v = *reinterpret_cast<const u4_t*>(p + 16 * x);
 #pragma unroll
           for (int e = 0; e < 4; e++) kw[h][4 * x + e] = v[e];
         }
       }
+      const char* q = s + (size_t)(ks_at + h * (16 * NG));
       if constexpr (LG == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(ksp + t * (2 * NG));
+        const uint2 v = *reinterpret_cast<const uint2*>(q);
         ks[h][0] = v.x; ks[h][1] = v.y;
       } else {
-        ks[h][0] = *reinterpret_cast<const uint32_t*>(ksp + t * (2 * NG));
+        ks[h][0] = *reinterpret_cast<const uint32_t*>(q);
       }
     }
   }
-  __device__ __forceinline__ void load_v(const uint32_t* vc, const uint16_t* vsp, int t0, int n, int quad) {
-    const int64_t blk = t0 / 8 + quad;
+  __device__ __forceinline__ void load_v(const char* vc, const char* vsp, int t0) {
+    const char* v = vc + (int64_t)t0 * (D / 2);
+    const char* s = vsp + (int64_t)t0 * (4 * NG);
 #pragma unroll
     for (int j = 0; j < VJ; j++) {
-      vw[j] = *reinterpret_cast<const u4_t*>(vc + blk * D + 64 * j + 4 * n);
-      vs[j] = *reinterpret_cast<const u4_t*>(vsp + ((blk * NG + (64 * j + 4 * n) / G) * 2) * 8);
+      vw[j] = *reinterpret_cast<const u4_t*>(v + (size_t)(v_at + j * 256));
+      vs[j] = *reinterpret_cast<const u4_t*>(s + (size_t)(vs_at + 64 * j / G * 32));
     }
-    // rows past the groups repeat the last one; their products are not used
-    vm = *reinterpret_cast<const u4_t*>(vsp + ((blk * NG + (n < NG ? n : NG - 1)) * 2 + 1) * 8);
+    vm = *reinterpret_cast<const u4_t*>(s + (size_t)vm_at);
   }
 };
 
@@ -256,10 +268,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     qm = __builtin_bit_cast(h8_t, r);
   }
 
-  const uint32_t* kc = reinterpret_cast<const uint32_t*>(P.c.k_codes) + row * P.c.kc_seq + kvh * P.c.kc_head + quad * KW;
-  const uint16_t* ks = reinterpret_cast<const uint16_t*>(P.c.k_scales) + row * P.c.ks_seq + kvh * P.c.ks_head + (quad * (D / 4) / G) * 2;
-  const uint32_t* vc = reinterpret_cast<const uint32_t*>(P.c.v_codes) + row * P.c.vc_seq + kvh * P.c.vc_head;
-  const uint16_t* vs = reinterpret_cast<const uint16_t*>(P.c.v_scales) + row * P.c.vs_seq + kvh * P.c.vs_head;
+  const char* kc = reinterpret_cast<const char*>(P.c.k_codes) + 4 * (row * P.c.kc_seq + kvh * P.c.kc_head);
+  const char* ks = reinterpret_cast<const char*>(P.c.k_scales) + 2 * (row * P.c.ks_seq + kvh * P.c.ks_head);
+  const char* vc = reinterpret_cast<const char*>(P.c.v_codes) + 4 * (row * P.c.vc_seq + kvh * P.c.vc_head);
+  const char* vs = reinterpret_cast<const char*>(P.c.v_scales) + 2 * (row * P.c.vs_seq + kvh * P.c.vs_head);
 
   const float ninf = __builtin_bit_cast(float, 0xff800000u);
   f4_t o[VT], om = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -271,6 +283,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   asm volatile("" : "+v"(mask));
 
     Tile<D, G> tile;
+  tile.place(n, quad);
   auto step = [&](int t0, int next) __attribute__((always_inline)) {
     // ---- scores: register e of half h is token t0 + 8 quad + 4 h + e of head n
     f4_t sc[2];
@@ -291,7 +304,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
           sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_codes(tile.kw[h][x], s4, o4, mask), qb[x], sc[h], 0, 0, 0);
       }
     }
-    tile.load_k(kc, ks, next, n);
+    tile.load_k(kc, ks, next);
     float s[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) s[e] = sc[e >> 2][e & 3];
@@ -317,9 +330,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     float top = s[0];
 #pragma unroll
     for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
-    top = col_max(top) * score_scale;
-    if (__builtin_amdgcn_ballot_w64(top > m_run + kSlack) != 0) {
-      const float m_new = fmaxf(m_run, top);
+    // no lane of a column past its maximum by more than the slack: nothing moves
+    if (__builtin_amdgcn_ballot_w64(top * score_scale > m_run + kSlack) != 0) {
+      const float m_new = fmaxf(m_run, col_max(top) * score_scale);
       const float a = m_new == ninf ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       l_run *= a;
 #pragma unroll
@@ -338,7 +351,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
       const uint32_t hw = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(pa, pb));
       const h2 hh = as_h2(hw);
       hi[p] = hw;
-      lo[p] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(pa - (float)hh[0], pb - (float)hh[1]));
+      lo[p] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hh[0], -1.0f, pa), __builtin_fmaf((float)hh[1], -1.0f, pb)));
     }
     const h8_t ph = __builtin_bit_cast(h8_t, hi), pl = __builtin_bit_cast(h8_t, lo);
 
@@ -359,7 +372,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         o[4 * j + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[4 * j + x], 0, 0, 0);
       }
     }
-    tile.load_v(vc, vs, next, n, quad);
+    tile.load_v(vc, vs, next);
   };
 
   // K of the next tile is requested as soon as the scores have taken the present one's, V after the
@@ -367,8 +380,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   int i = first_tile + wave;
   if (i < end_tile) {
     int t0 = vis.tile(i) * kTile;
-    tile.load_k(kc, ks, t0, n);
-    tile.load_v(vc, vs, t0, n, quad);
+    tile.load_k(kc, ks, t0);
+    tile.load_v(vc, vs, t0);
     for (; i < end_tile; i += kWaves) {
       const int next = vis.tile(min(i + kWaves, end_tile - 1)) * kTile;
       step(t0, next);
