@@ -42,13 +42,13 @@ __device__ __forceinline__ double group_step(float hi, float m) {
 
 // (x - m) / s to the nearest code, ties to even.  The quotient is corrected by its residual, which
 // makes it exact where it has few bits (a tie is j + 1/2) and keeps every other off the ties; 1.5 2^52
-// added leaves its nearest integer in the low word.  x is limited to [m, top], top = m + 16 s.
+// added leaves its nearest integer in the low word.  x is limited to [m, top], top = m + 15 s in binary32:
+// no less than the group's maximum, except where s has reached its end and codes past 15 are cut.
 __device__ __forceinline__ uint32_t code_of(float x, float m, float top, double md, double s, double inv) {
   const double d = (double)__builtin_amdgcn_fmed3f(x, m, top) - md;
   const double y0 = d * inv;
   const double y = __builtin_fma(__builtin_fma(-y0, s, d), inv, y0);
-  const uint32_t q = (uint32_t)__builtin_bit_cast(uint64_t, y + 6755399441055744.0);
-  return q < 15u ? q : 15u;
+  return (uint32_t)__builtin_bit_cast(uint64_t, y + 6755399441055744.0);
 }
 
 // Extremes of a group over G / 16 neighbouring lanes, as integers in the order of the values.
@@ -136,15 +136,14 @@ __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
     if (block + 2 < R.end) request(block + 2);
     const int t = 8 * block + token - R.start;
     const bool valid = t >= 0 && t < R.count && block + token / 8 < R.end;
-    // extremes; a NaN, which those leave out, counts as an infinity
-    float lof = x[0], hif = x[0], poison = 0.0f;
+    // extremes; a NaN stays one here and orders past the infinity of its sign
+    float lof = x[0], hif = x[0];
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-      lof = __builtin_fminf(lof, x[e]);
-      hif = __builtin_fmaxf(hif, x[e]);
-      poison = __builtin_fmaf(x[e], 0.0f, poison);
+    for (int e = 1; e < 16; e++) {
+      lof = __builtin_elementwise_minimum(lof, x[e]);
+      hif = __builtin_elementwise_maximum(hif, x[e]);
     }
-    int lo = ordered(lof), hi = poison == poison ? ordered(hif) : 0x7f800000;
+    int lo = ordered(lof), hi = ordered(hif);
     group_extremes<G>(lo, hi);
     const bool finite = hi < 0x7f800000 && lo > ordered(__builtin_bit_cast(float, 0xff800000u));
     const float m = round_f16(__builtin_amdgcn_fmed3f(of_ordered(lo), -65504.0f, 65504.0f));
@@ -153,7 +152,7 @@ __global__ __launch_bounds__(2 * D) void kv_append_int4_kernel(KvRowsParams P) {
     uint2 codes = make_uint2(0, 0);
     if (s > 0.0) {
       const double md = (double)m;
-      const float top = m + 16.0f * sf;
+      const float top = m + 15.0f * sf;
       double inv = __builtin_amdgcn_rcp(s);
       inv = __builtin_fma(__builtin_fma(-s, inv, 1.0), inv, inv);
       inv = __builtin_fma(__builtin_fma(-s, inv, 1.0), inv, inv);
@@ -269,7 +268,7 @@ template <typename T, bool APPEND>
 static int launch_rows(KvRowsParams P, int64_t rows, hipStream_t st, const char* what) {
   // any start inside a block: one block more than the tokens fill
   const int64_t blocks = (P.tokens + 14) / 8;
-  const int64_t fill = blocks * P.c.kv_heads * rows * P.c.head_dim / (256 * 2048);
+  const int64_t fill = blocks * P.c.kv_heads * rows * P.c.head_dim / (256 * (APPEND ? 2048 : 1024));
   P.blocks_per = (int)(fill < 2 ? (APPEND ? 2 : 1) : fill > kMostBlocks ? kMostBlocks : fill & ~1);
   const dim3 grid((unsigned)((blocks + P.blocks_per - 1) / P.blocks_per), (unsigned)P.c.kv_heads, (unsigned)rows);
   const dim3 block((unsigned)(2 * P.c.head_dim));
