@@ -825,7 +825,7 @@ int tt_kv_read_int4(const tt_int4_cache* cache, void* k_out, int64_t k_row, int6
  * t < n = min(max(lengths[r], 0), capacity, max_length) and, with window > 0, t >= n - window or
  * t < first_tokens.  out = sum p v with p the softmax of scale q.k and, where sinks [heads] is
  * given, of the sink's logit, which carries no value.  A row that sees nothing is 0; a row whose q
- * is not finite is NaN.  max_length bounds what the launch is sized for.
+ * is not finite is NaN.  max_length bounds what the launch is sized for.  out may be q.
  * scratch: tt_gqa_attention_int4_scratch_floats of the same arguments (0: none is needed), for one
  * call at a time, 16-byte aligned. */
 int64_t tt_gqa_attention_int4_scratch_floats(const tt_int4_cache* cache, int64_t rows, int64_t heads, int64_t window,
@@ -835,7 +835,7 @@ int tt_gqa_attention_int4(const tt_int4_cache* cache, const void* q, int64_t q_r
                           int64_t max_length, const void* sinks, int sink_dtype, float scale, float* scratch,
                           int64_t scratch_floats, void* out, int64_t out_row, int64_t out_head, void* stream);
 
-/* One token per row of logits [rows, vocab] from uniforms[row] in [0, 1).  Order: logits
+/* One token per row of logits [rows, vocab] (vocab at most 2^20) from uniforms[row] in [0, 1).  Order: logits
  * descending, equal ones (+0 and -0 among them) by index; -inf and NaN are left out.  Weights
  * w = exp((x - max) / temperature); kept: the first top_k of the order, of these the shortest
  * beginning whose weight is at least top_p of theirs, of these the ones with w >= min_p (the first

@@ -247,6 +247,9 @@ def test_attention_split(backend, device, length):
     again = torch.empty_like(q)
     backend.gqa_attention_int4(q, cache, again, n)
     assert torch.equal(out, again)
+    again.copy_(q)
+    backend.gqa_attention_int4(again, cache, again, n)          # in place
+    assert torch.equal(out, again)
     short = length // 3
     backend.gqa_attention_int4(q, cache, out, n, max_length=short)
     _check_attention(cache, q, out, [min(x, short) for x in lengths])
@@ -268,6 +271,17 @@ def test_attention_large_scores_and_late_maximum(backend, device):
     out = torch.empty_like(q)
     backend.gqa_attention_int4(q, cache, out, torch.tensor(lengths, device=device, dtype=torch.int32))
     _check_attention(cache, q, out, lengths)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30])
+def test_attention_softmax_scales(backend, device, scale):
+    """No scale (every visible token weighs the same), a negative one, one that leaves next to nothing."""
+    lengths = [45, 64]
+    cache, g = _filled(backend, device, 2, 2, 96, 64, 32, 6, lengths)
+    q = torch.randn((2, 6, 64), generator=g, device=device).half()
+    out = torch.empty_like(q)
+    backend.gqa_attention_int4(q, cache, out, torch.tensor(lengths, device=device, dtype=torch.int32), scale=scale, window=40)
+    _check_attention(cache, q, out, lengths, 40, scale=scale)
 
 
 @pytest.mark.parametrize("scale", [2.0 ** -16, 60000.0, 2.0 ** 100, 2.0 ** -100])

@@ -99,7 +99,7 @@ def test_cache_shapes():
             c.sequences(a, b)
     t = (c.k_codes, c.k_scales, c.v_codes, c.v_scales)
     for i, bad in ((0, c.k_codes.to(torch.int64)), (1, c.k_scales.float()), (2, c.v_codes[:, :, :-1]), (3, c.v_scales[:, :1]),
-                   (0, c.k_codes[:, :, ::2]), (1, c.k_scales[:, :, :, :1]), (0, c.k_codes[0]), (3, c.v_scales.transpose(3, 4))):
+                   (0, c.k_codes[:, :, ::2]), (0, c.k_codes[:0]), (1, c.k_scales[:, :, :, :1]), (0, c.k_codes[0]), (3, c.v_scales.transpose(3, 4))):
         with pytest.raises(ValueError):
             Int4KvCache(*[bad if i == j else x for j, x in enumerate(t)])
 
@@ -154,6 +154,9 @@ def test_attention_entry_refuses_sizes(be):
         long.desc, one, 0, 0, dt, length, 1, 4, 0, 0, 1 << 16, None, 0, 1.0, scratch, n, one, 0, 0, None)
     assert call(0, None, 0) == -1 and call(0, one, floats - 1) == -1 and call(2, one, floats) == -1
     assert call(0, one, floats, None) == -1
+    for scale in (float("nan"), float("inf")):
+        assert be.lib.tt_gqa_attention_int4(long.desc, one, 0, 0, 0, one, 1, 4, 0, 0, 1 << 16, None, 0, scale, one, floats, one,
+                                            0, 0, None) == -1
     for field, value in (("capacity", 48), ("head_dim", 96), ("group_size", 16), ("k_codes", None), ("kv_heads", 0),
                          ("kc_head", 2), ("vs_seq", 4), ("v_codes", (1 << 20) + 8)):
         d = _lib.Int4Cache.from_buffer_copy(c.desc)

@@ -1661,8 +1661,8 @@ class HipDecodeBackend:
         own included).  With ``window`` > 0 a row sees its last ``window`` tokens and the sequence's
         first ``first_tokens``; ``sinks`` [heads] are logits that join the softmax and carry no value.
         ``scale`` is head_dim ** -0.5 by default.  ``max_length`` (by default the capacity) bounds the
-        lengths, longer ones count as it, and sizes the launch.  A row that sees nothing is 0.  Scratch
-        of long contexts comes from the current stream's allocator with every call."""
+        lengths, longer ones count as it, and sizes the launch.  A row that sees nothing is 0.  ``out`` may
+        be q.  Scratch of long contexts comes from the current stream's allocator with every call."""
         shape, qs, os, dtype = q.shape, q.stride(), out.stride(), q.dtype
         if len(shape) != 3 or out.shape != shape or out.dtype != dtype:
             raise ValueError("gqa_attention_int4 takes q and out [rows, heads, head_dim] of one dtype")
@@ -1700,8 +1700,8 @@ class HipDecodeBackend:
                     temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
                     top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
                     probs: torch.Tensor | None = None) -> torch.Tensor:
-        """One token per row of ``logits`` [rows, vocab] (fp16, bf16 or fp32) from ``uniforms``
-        (float32 [rows], in [0, 1)) to ``tokens`` (int64 [rows]).  Tokens are ordered by logit, equal
+        """One token per row of ``logits`` [rows, vocab] (fp16, bf16 or fp32; vocab at most 2^20) from
+        ``uniforms`` (float32 [rows], in [0, 1)) to ``tokens`` (int64 [rows]).  Tokens are ordered by logit, equal
         ones by index; of exp(logit / temperature) are kept the first ``top_k``, of these the shortest
         beginning that holds ``top_p`` of their weight, of these the ones of at least ``min_p`` times the
         largest; the token is where the cumulative weight passes uniforms times that of the kept.

@@ -4,7 +4,8 @@
 // An angle is position x frequency, formed in binary64 in turns and reduced there (t - rint(t)),
 // since a binary32 product of a position near 10^6 is off by 0.06 radians; sine and cosine of the
 // reduced angle are then taken in binary32.  A workgroup forms the rotary/2 angles of its tokens
-// once, in LDS, for all heads.
+// once, in LDS, for all heads, while the vectors are on their way: what bounds it is memory (8191 tokens
+// of 72 heads of 128, 302 MB: 62 us, 4.9 TB/s; a thread per pair 141).
 #include "tt_abi_internal.h"
 #include "tt_common.h"
 #include "tt_eight.h"

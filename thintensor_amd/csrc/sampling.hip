@@ -11,6 +11,12 @@
 //   4. one workgroup per row: candidates sorted, cuts and target resolved among them.
 // Weights are exp(-z) in units of 2^-43, 64-bit integers: sums have no order, and a total is exact to
 // 2^-43 of the largest weight per token, far below what tells two cumulative sums apart.
+//
+// Four launches: one row of 128256 fp16 logits takes 20.7 us (2.7, 5.6, 7.4 and 5.7 for the steps and the
+// gaps between them), 64 rows of 152064 in binary32 55 us (7.5, 18.8, 18.7, 10.9): the first step at the
+// memory's rate (39 MB, 5.2 TB/s), the second half by the exponentials, the third by the round trips before its
+// candidates are known.  A row that leaves more than kMostCandidates candidates -- thousands of equal
+// logits at a border -- is searched digit by digit by its one workgroup, in about a millisecond.
 #include "tt_abi_internal.h"
 #include "tt_common.h"
 

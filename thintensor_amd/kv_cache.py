@@ -33,6 +33,8 @@ class Int4KvCache:
             raise ValueError("4-bit cache codes must be int32 and scales float16")
         batch, kv_heads, capacity, words = map(int, k_codes.shape)
         head_dim, groups = 8 * words, int(k_scales.shape[3])
+        if batch < 1 or kv_heads < 1:
+            raise ValueError("4-bit cache needs at least one sequence and KV head")
         if head_dim not in (64, 128, 256):
             raise ValueError(f"4-bit cache head_dim must be 64, 128 or 256, got {head_dim}")
         if groups < 1 or head_dim % groups or head_dim // groups not in (32, 64, 128):
