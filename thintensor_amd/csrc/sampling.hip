@@ -16,7 +16,8 @@
 // gaps between them), 64 rows of 152064 in binary32 55 us (7.5, 18.8, 18.7, 10.9): the first step at the
 // memory's rate (39 MB, 5.2 TB/s), the second half by the exponentials, the third by the round trips before its
 // candidates are known.  A row that leaves more than kMostCandidates candidates -- thousands of equal
-// logits at a border -- is searched digit by digit by its one workgroup, in about a millisecond.
+// logits at a border -- is searched digit by digit by its one workgroup (128256 equal logits: 0.17 ms a
+// search, up to three searches).
 #include "tt_abi_internal.h"
 #include "tt_common.h"
 
@@ -665,30 +666,76 @@ struct Found {           // answer of a search
 
 // A candidate list that does not fit: the elements of one interval are searched by the digits of
 // their keys and indexes, over the row itself.  mode 0: the element of rank `rank`; 1: the first
-// whose cumulative weight is at least target; 2: the first whose is more.
+// whose cumulative weight is at least target; 2: the first whose is more.  Digits that all elements
+// share are found first and passed over; once a key is settled its elements weigh the same and are
+// counted.  A thread adds up what falls to one digit in a row before it meets the others in LDS.
 template <typename T>
 __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S, const SamplePlan& L, int a, int mode,
                                uint32_t rank, double target, uint64_t* dm, uint32_t* dn, uint64_t* answer) {
   const int lo = L.lo[a], hi = L.hi[a];
-  uint64_t prefix = 0, mass = L.before[a];
+  auto each = [&](auto f) __attribute__((always_inline)) {   // (key with index, z) of the interval's elements
+    for (int i = 8 * (int)threadIdx.x; i < P.vocab; i += 8 * kFinalThreads) {
+      float x[8];
+      logits8<T>(P, row, i, x);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (!live(x[e])) continue;
+        const double z = S.z_of(x[e]);
+        const int b = S.bin_of(z);
+        if (b >= lo && b <= hi) f(((uint64_t)key_of(x[e]) << 32) | (uint32_t)~(uint32_t)(i + e), z);
+      }
+    }
+  };
+  uint64_t mass = L.before[a];
   uint32_t count = L.rank_before[a];
+  if (threadIdx.x == 0) {
+    answer[0] = ~0ull;
+    answer[1] = 0;
+  }
+  __syncthreads();
+  uint64_t all = ~0ull, any = 0;
+  each([&](uint64_t key, double) {
+    all &= key;
+    any |= key;
+  });
+  atomicAnd((unsigned long long*)&answer[0], (unsigned long long)all);
+  atomicOr((unsigned long long*)&answer[1], (unsigned long long)any);
+  __syncthreads();
+  const uint64_t same = ~(answer[0] ^ answer[1]);   // bits that every key has alike
+  uint64_t prefix = answer[0] & same;               // of these, and of the digits found
+  uint64_t unit = 0;                                // the weight of one element, where the key is settled
   for (int shift = 56; shift >= 0; shift -= 8) {
+    const uint64_t above = shift == 56 ? 0 : ~0ull << (shift + 8);
+    if (((same >> shift) & 255u) == 255u) continue;
+    const bool counted = (same | above) >> 32 == 0xffffffffull;
+    if (counted && unit == 0) unit = S.mass_of(S.z_of(of_key((uint32_t)(prefix >> 32))));
+    __syncthreads();
     for (int b = threadIdx.x; b < 256; b += kFinalThreads) {
       dm[b] = 0;
       dn[b] = 0;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < P.vocab; i += kFinalThreads) {
-      const float x = logit<T>(P, row, i);
-      if (!live(x)) continue;
-      const double z = S.z_of(x);
-      const int b = S.bin_of(z);
-      const uint64_t key = ((uint64_t)key_of(x) << 32) | (uint32_t)~(uint32_t)i;
-      if (b < lo || b > hi || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
-      const int digit = (int)(key >> shift) & 255;
-      atomicAdd(&dn[digit], 1u);
-      atomicAdd((unsigned long long*)&dm[digit], (unsigned long long)S.mass_of(z));
-    }
+    int digit = -1;
+    uint32_t n = 0;
+    uint64_t m = 0;
+    auto flush = [&]() __attribute__((always_inline)) {
+      if (digit < 0) return;
+      atomicAdd(&dn[digit], n);
+      if (!counted) atomicAdd((unsigned long long*)&dm[digit], (unsigned long long)m);
+    };
+    each([&](uint64_t key, double z) {
+      if (((key ^ prefix) & above) != 0) return;
+      const int d = (int)(key >> shift) & 255;
+      if (d != digit) {
+        flush();
+        digit = d;
+        n = 0;
+        m = 0;
+      }
+      n++;
+      if (!counted) m += S.mass_of(z);
+    });
+    flush();
     __syncthreads();
     if (threadIdx.x == 0) {
       int pick = -1;
@@ -699,21 +746,21 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
         pick = b;
         pm = mass;
         pn = count;
-        mass += dm[b];
+        mass += counted ? dn[b] * unit : dm[b];
         count += dn[b];
         if (mode == 0 ? count >= rank : mode == 1 ? (double)mass >= target : (double)mass > target) break;
       }
       answer[0] = pm;
-      answer[1] = ((uint64_t)pn << 32) | (uint32_t)pick;
-      answer[2] = dm[pick < 0 ? 0 : pick];
+      answer[1] = pn;
+      answer[2] = (uint64_t)pick;
     }
     __syncthreads();
     mass = answer[0];
-    count = (uint32_t)(answer[1] >> 32);
-    prefix = (prefix << 8) | (uint32_t)(answer[1] & 255u);
-    if (shift == 0) mass += answer[2];
-    __syncthreads();
+    count = (uint32_t)answer[1];
+    prefix = (prefix & ~(255ull << shift)) | ((answer[2] & 255u) << shift);
   }
+  mass += S.mass_of(S.z_of(of_key((uint32_t)(prefix >> 32))));   // the element itself
+  __syncthreads();                                               // answer may be written again
   return Found{mass, prefix};
 }
 
