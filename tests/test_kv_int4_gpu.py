@@ -366,3 +366,24 @@ def test_attention_past_32_bit_offsets(backend, device):
     ka, va = backend.kv_read_int4(wide, torch.empty_like(k), torch.empty_like(v), starts)
     kb, vb = backend.kv_read_int4(cache, torch.empty_like(k), torch.empty_like(v), starts)
     assert torch.equal(ka, kb) and torch.equal(va, vb)
+
+
+def test_attention_and_read_over_a_shared_sequence(backend, device):
+    """One sequence seen by every row (stride 0): read and attended to as copies of it, never written."""
+    held, g = _filled(backend, device, 1, 2, 288, 128, 64, 77, [288])
+    arrays = (held.k_codes, held.k_scales, held.v_codes, held.v_scales)
+    shared = Int4KvCache(*[t.expand(5, *t.shape[1:]) for t in arrays])
+    copies = Int4KvCache(*[t.repeat(5, *[1] * (t.ndim - 1)) for t in arrays])
+    q = torch.randn((5, 8, 128), generator=g, device=device).half()
+    n = torch.tensor([288, 1, 100, 0, 37], device=device, dtype=torch.int32)
+    outs = [torch.empty_like(q) for _ in range(2)]
+    for cache, out in zip((shared, copies), outs):
+        backend.gqa_attention_int4(q, cache, out, n)
+    assert torch.equal(*outs)
+    starts = torch.tensor([0, 8, 100, 287, 5], device=device, dtype=torch.int32)
+    rows = [[torch.full((5, 9, 2, 128), 3.0, device=device).half() for _ in range(2)] for _ in range(2)]
+    for cache, out in zip((shared, copies), rows):
+        backend.kv_read_int4(cache, *out, starts)
+    assert all(torch.equal(a, b) for a, b in zip(*rows))
+    with pytest.raises(ValueError, match="share"):
+        backend.kv_append_int4(shared, rows[0][0][:, 0], rows[0][1][:, 0], starts)

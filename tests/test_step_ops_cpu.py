@@ -48,7 +48,10 @@ def test_frequencies():
     ratio = (bands / base).numpy()
     assert np.all(ratio[wave < 8192 / 4] == 1.0) and np.allclose(ratio[wave > 8192], 1 / 8)
     for bad in (dict(rotary_dim=63), dict(rotary_dim=0), dict(rotary_dim=64, scaling="other"), dict(rotary_dim=64, factor=0.5),
-                dict(rotary_dim=64, theta=0.0), dict(rotary_dim=64, scaling="bands", low_freq_factor=4.0)):
+                dict(rotary_dim=64, theta=0.0), dict(rotary_dim=64, scaling="bands", low_freq_factor=4.0),
+                dict(rotary_dim=64, factor=math.nan), dict(rotary_dim=64, theta=math.inf),
+                dict(rotary_dim=64, theta=1.0, scaling="yarn"), dict(rotary_dim=64, scaling="yarn", original_positions=0),
+                dict(rotary_dim=64, scaling="yarn", beta_slow=0.0), dict(rotary_dim=64, scaling="yarn", beta_fast=1.0)):
         with pytest.raises(ValueError):
             rotary_frequencies(**bad, device="cpu")
 
@@ -128,6 +131,17 @@ def test_kv_rows_refusals(be, name):
             (ok.transpose(2, 3).contiguous().transpose(2, 3), ok, starts, None), (ok, ok, starts, None)):
         with pytest.raises(ValueError):
             op(c, k, v, s, n)
+
+
+def test_append_refuses_shared_memory(be):
+    """Sequences or heads of stride 0 may be read, not written; calls that write nothing pass."""
+    c, one = _cache(), ctypes.c_void_p(1 << 20)
+    call = lambda d, rows=2, tokens=1: be.lib.tt_kv_append_int4(d, one, 0, 0, 0, one, 0, 0, 0, 0, one, None, rows, tokens, None)  # noqa: E731
+    for field in ("kc_seq", "ks_seq", "vc_seq", "vs_seq", "kc_head", "ks_head", "vc_head", "vs_head"):
+        d = _lib.Int4Cache.from_buffer_copy(c.desc)
+        setattr(d, field, 0)
+        assert call(d) == -1 and b"share" in be.lib.tt_last_error(), field
+        assert call(d, rows=0) == 0 and call(d, tokens=0) == 0
 
 
 def test_attention_refusals(be):

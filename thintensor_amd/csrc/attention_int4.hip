@@ -289,7 +289,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   uint32_t mask = 0x03c003c0u;
   asm volatile("" : "+v"(mask));
 
-    Tile<D, G> tile;
+  Tile<D, G> tile;
   tile.place(n, quad);
   auto step = [&](int t0, int next) __attribute__((always_inline)) {
     // ---- scores: register e of half h is token t0 + 8 quad + 4 h + e of head n

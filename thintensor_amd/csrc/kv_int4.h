@@ -18,7 +18,6 @@ inline int check_cache(const tt_int4_cache* c, int64_t rows, const char* what) {
   TT_REQUIRE(c->kv_heads > 0 && c->kv_heads <= 65535 && c->batch > 0, "%s: bad batch / kv_heads", what);
   TT_REQUIRE(rows >= 0 && rows <= c->batch && rows <= 65535, "%s: %lld rows in a cache of %lld sequences (65535 at most)",
              what, (long long)rows, (long long)c->batch);
-  const int64_t groups = c->head_dim / c->group_size;
   // a lane of the attention reads the scale pairs of head_dim / 4 dims at once
   const int64_t pairs = c->head_dim / 4 > c->group_size ? 2 : 1;
   TT_REQUIRE(aligned(c->k_codes, 16) && aligned(c->v_codes, 16) && aligned(c->v_scales, 16) &&
@@ -28,7 +27,6 @@ inline int check_cache(const tt_int4_cache* c, int64_t rows, const char* what) {
                  c->vs_seq % 8 == 0 && c->vs_head % 8 == 0 && c->ks_seq % (2 * pairs) == 0 &&
                  c->ks_head % (2 * pairs) == 0,
              "%s: cache strides must keep the alignment of sequences and heads", what);
-  (void)groups;
   return TT_OK;
 }
 

@@ -28,8 +28,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str 
     """(inv_freq float64 [rotary_dim / 2] on ``device``, amplitude)."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
-    if theta <= 0 or factor < 1:
-        raise ValueError("rotary theta must be positive and the factor at least 1")
+    if not (0 < theta < math.inf and 1 <= factor < math.inf):
+        raise ValueError("rotary theta must be positive and the factor at least 1, both finite")
     half = rotary_dim // 2
     index = torch.arange(half, dtype=torch.float64)
     freq = theta ** (-2.0 * index / rotary_dim)
@@ -41,6 +41,9 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str 
             raise ValueError("ntk scaling needs at least two frequencies")
         freq = (theta * factor ** (rotary_dim / (rotary_dim - 2.0))) ** (-2.0 * index / rotary_dim)
     elif scaling == "yarn":
+        if theta <= 1 or original_positions < 1 or not 0 < beta_slow < beta_fast:
+            raise ValueError("yarn scaling needs theta above 1, original positions and 0 < beta_slow < beta_fast")
+
         # index at which a frequency turns `turns` times over the original positions
         def at(turns: float) -> float:
             return rotary_dim * math.log(original_positions / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
