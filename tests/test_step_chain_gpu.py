@@ -89,13 +89,50 @@ def test_batch_decoder_refusals(device, model):
     for bad in (([1], [0, 0], u), ([1, 2], [0, 32], u), ([1, 2], [0, 30], u), ([1, 2], [0, 0], u[:, :1]), ([1, 2], [0, 0], u.double())):
         with pytest.raises(ValueError):
             dec.generate(*bad)
-    with pytest.raises(ValueError):
-        _decoder(device, model, 0)
+    for batch in (0, 65):
+        with pytest.raises(ValueError):
+            _decoder(device, model, batch)
     # a request at the capacity's end: further tokens are not stored, nothing else is touched
     dec.prime([3, 4], [31, 5])
     for _ in range(3):
         dec.step()
     assert dec.positions.tolist() == [34, 8]
+
+
+def test_decoders_that_share_a_backend(device, model):
+    """A graph keeps the scratch that it was captured with when a larger batch makes the backend replace
+    it: memory that is handed out afterwards is left alone, and the graph's results stay."""
+    lengths, u = [40, 1, 33], torch.full((4, 3), 0.4, device=device)
+    small = _decoder(device, model, 3)
+    _prior(small, [0, 1, 2], lengths)
+    want = small.generate([5, 17, 900], lengths, u)
+    large = DenseBatchDecoder(small.be, model, 64, 64)
+    large.capture()
+    assert small._graph_scratch.data_ptr() != large._graph_scratch.data_ptr()
+    later = [torch.full((small._graph_scratch.numel(),), 7, device=device, dtype=torch.int64) for _ in range(8)]
+    for _ in range(2):
+        assert small.generate([5, 17, 900], lengths, u) == want
+    assert all(bool((x == 7).all()) for x in later)
+
+
+def test_token_minus_one(device, model):
+    """A request whose logits leave nothing gets token -1; the others get what they would without it."""
+    lengths, u = [40, 1, 33], torch.full((3,), 0.4, device=device)
+    runs = []
+    for spoil in (False, True):
+        dec = _decoder(device, model, 3)
+        _prior(dec, [0, 1, 2], lengths)
+        dec.prime([5, 17, 900], lengths)
+        dec.uniforms.copy_(u)
+        dec.set_sampling(0.9)
+        tokens = []
+        for step in range(3):
+            if spoil and step == 1:
+                dec.tokens[1] = -1
+            dec.step()
+            tokens.append(dec.tokens.tolist())
+        runs.append(tokens)
+    assert [t[::2] for t in runs[0]] == [t[::2] for t in runs[1]]
 
 
 def _chain(be, cache, s):

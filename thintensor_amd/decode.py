@@ -558,14 +558,15 @@ class DenseBatchDecoder:
     model's theta), the append to each layer's cache, attention (optionally a window of ``window``
     tokens and ``first_tokens`` first ones), the lm_head's logits and ``sample_rows``.  Sampling settings
     are per request (:meth:`set_sampling`, greedy at first).  A request that has reached the capacity
-    keeps decoding without storing further tokens; one whose logits leave nothing gets token -1."""
+    keeps decoding without storing further tokens; one whose logits leave nothing gets token -1, after which
+    its own tokens mean nothing and the others' are what they were."""
 
     def __init__(self, backend: HipDecodeBackend, weights: DenseWeights, batch: int, capacity: int, *,
                  group_size: int = 32, window: int = 0, first_tokens: int = 0,
                  rotary: tuple[torch.Tensor, float] | None = None) -> None:
         s = weights.shape
-        if batch < 1 or capacity < 1:
-            raise ValueError("batch and capacity must be at least 1")
+        if not 1 <= batch <= 64 or capacity < 1:
+            raise ValueError("a batch is of 1 to 64 requests (of the batched GEMMs), the capacity at least 1")
         self.be, self.w, self.s, self.batch = backend, weights, s, batch
         dev = weights.embed.device
         self.device, dt = dev, torch.float16
@@ -593,6 +594,7 @@ class DenseBatchDecoder:
         self.logits = empty(int(weights.lm_head.shape[0]))
         self.graph: torch.cuda.CUDAGraph | None = None
         self._graph_stream: torch.cuda.Stream | None = None
+        self._graph_scratch: torch.Tensor | None = None
 
     def set_sampling(self, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0) -> None:
         """Settings of every request: a number for all of them, or one per request."""
@@ -635,11 +637,10 @@ class DenseBatchDecoder:
         self.lengths.add_(1)
 
     def capture(self) -> None:
-        """Record one step into a HIP graph.  Scratch of the operators that keep theirs is reserved
-        first; the others take it from the graph's own pool."""
-        self.be._batched_argmax_scratch(self.batch, int(self.w.lm_head.shape[0]), self.s.hidden)
-        for rows, cols in ((self.s.intermediate, self.s.hidden), (self.s.hidden, self.s.intermediate)):
-            self.be._batched_workspace(self.batch, rows, cols)
+        """Record one step into a HIP graph.  The lm_head's scratch belongs to the backend, which replaces
+        it when a larger batch comes, and is held here for the graph (so graphs of decoders that share a
+        backend replay one at a time); the other operators take theirs from the graph's own pool."""
+        self._graph_scratch = self.be._batched_argmax_scratch(self.batch, int(self.w.lm_head.shape[0]), self.s.hidden)
         torch.cuda.synchronize(self.device)
         self._graph_stream = torch.cuda.Stream(self.device)
         self.graph = torch.cuda.CUDAGraph()
