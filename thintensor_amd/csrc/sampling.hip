@@ -12,12 +12,12 @@
 // Weights are exp(-z) in units of 2^-43, 64-bit integers: sums have no order, and a total is exact to
 // 2^-43 of the largest weight per token, far below what tells two cumulative sums apart.
 //
-// Four launches: one row of 128256 fp16 logits takes 20.7 us (2.7, 5.6, 7.4 and 5.7 for the steps and the
-// gaps between them), 64 rows of 152064 in binary32 55 us (7.5, 18.8, 18.7, 10.9): the first step at the
-// memory's rate (39 MB, 5.2 TB/s), the second half by the exponentials, the third by the round trips before its
-// candidates are known.  A row that leaves more than kMostCandidates candidates -- thousands of equal
-// logits at a border -- is searched digit by digit by its one workgroup (128256 equal logits: 0.17 ms a
-// search, up to three searches).
+// Four launches: one row of 128256 fp16 logits takes 20.3 us (2.7, 5.5, 7.2 and 5.6 for the steps), 64 rows
+// of 152064 in binary32 53 us (7.9, 16.4, 18.4, 10.7): every pass over the 39 MB takes 8 us at the 5 TB/s that
+// the memory gives, the second step adds its round trips and the weights (7 us of vector instructions), the
+// third the round trips before its candidates are known, the last one sorts.  A row that leaves more than
+// kMostCandidates candidates -- thousands of equal logits at a border -- is searched digit by digit by its
+// one workgroup (128256 equal logits: 0.17 ms a search, up to three searches).
 #include "tt_abi_internal.h"
 #include "tt_common.h"
 
@@ -116,7 +116,7 @@ __device__ __forceinline__ double exp_neg(double z, int* n) {
 // infinite, is `hard`: only the largest ones weigh.  Elsewhere -inf becomes an infinite z and NaN a NaN,
 // which weigh nothing.
 struct RowScale {
-  double top, inv_t, bins_per_z;
+  double top, inv_t, y_per_x, bins_per_z;
   bool greedy, hard;
   __device__ RowScale(const SampleParams& P, int row, float2 range) {
     const float t = P.temperature ? P.temperature[row] : 1.0f;
@@ -124,6 +124,7 @@ struct RowScale {
     hard = greedy || range.x == __builtin_bit_cast(float, 0x7f800000u);
     top = (double)range.x;
     inv_t = greedy ? 0.0 : 1.0 / (double)t;
+    y_per_x = inv_t * -1.4426950408889634074;
     const double far = hard ? kReach : soft_z(range.y);
     // all of the range in bins 0 .. kBins - 2, or what lies below kReach of it
     const double most = far < kReach ? far : kReach;
@@ -141,12 +142,29 @@ struct RowScale {
     const double p = exp_neg(z, &n);
     return __builtin_amdgcn_ldexp(p, n);
   }
-  // in units: 2^52 added leaves the rounded integer in the low bits
-  __device__ uint64_t mass_of(double z) const {
-    int n;
-    const double p = exp_neg(z, &n);
-    const double v = __builtin_amdgcn_ldexp(p, n + 43) + 4503599627370496.0;
-    return z < 31.0 ? __builtin_bit_cast(uint64_t, v) - 0x4330000000000000ull : 0;
+  // In units: 2^w, w = 43 - z log2 e, as 2^n p(f) with n the nearest integer and p of degree ten through 1
+  // at f = 0 and at Chebyshev points of -1/2 .. 1/2 (within 2^-50.6 of 2^f; w is off by 2^-48 at most); 2^52
+  // added leaves the rounded integer in the low bits.  What weighs nothing, NaN included, ends as 2^-21.
+  __device__ uint64_t soft_mass(float x) const {
+    const double w = __builtin_fmax(__builtin_fma(top - (double)x, y_per_x, 43.0), -21.0);
+    const double n = __builtin_rint(w), f = w - n;
+    double p = 7.070977866508139e-09;
+    p = __builtin_fma(p, f, 1.0205905413765595e-07);
+    p = __builtin_fma(p, f, 1.3215451623221434e-06);
+    p = __builtin_fma(p, f, 1.5252672924850737e-05);
+    p = __builtin_fma(p, f, 0.00015403530424776529);
+    p = __builtin_fma(p, f, 0.0013333558200794592);
+    p = __builtin_fma(p, f, 0.009618129107618665);
+    p = __builtin_fma(p, f, 0.05550410866465167);
+    p = __builtin_fma(p, f, 0.24022650695910075);
+    p = __builtin_fma(p, f, 0.6931471805599462);
+    p = __builtin_fma(p, f, 1.0);
+    const double v = __builtin_amdgcn_ldexp(p, (int)n) + 4503599627370496.0;
+    return __builtin_bit_cast(uint64_t, v) - 0x4330000000000000ull;
+  }
+  __device__ uint64_t mass_of(float x) const {
+    if (hard) return (double)x == top ? (uint64_t)kUnit : 0;
+    return soft_mass(x);
   }
 };
 
@@ -271,9 +289,8 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleParams P
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const double z = S.soft_z(x[e]);
-        b[e] = S.bin_of(z);
-        m[e] = S.mass_of(z);
+        b[e] = S.bin_of(S.soft_z(x[e]));
+        m[e] = S.soft_mass(x[e]);
       }
     }
     if (counts) {
@@ -412,19 +429,25 @@ struct Settings {
   }
 };
 
+// Steps of a chunk on their way at a time: more take registers that keep four workgroups from a CU (64 rows of
+// 152064: two 18.4 us, three 19.5, four 21.9).
+constexpr int kDeep = 2;
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams P) {
+__global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams P) {
   const int row = blockIdx.y, c = blockIdx.x;
   SampleRow& R = P.rows[row];
   __shared__ uint64_t wave_m[kThreads / 64];
   __shared__ uint32_t wave_n[kThreads / 64];
   __shared__ BinAt at[4 * kCuts];
-  __shared__ uint64_t found[kStep];
+  __shared__ uint64_t found[kMostCandidates];
   __shared__ uint32_t n_found, base;
   const int end = min(P.vocab, (c + 1) * P.chunk);
   int i = c * P.chunk + 8 * (int)threadIdx.x;
-  float x[8];
-  if (i < end) logits8<T>(P, row, i, x);
+  float x[kDeep][8];
+#pragma unroll
+  for (int k = 0; k < kDeep; k++)
+    if (i + k * kStep < end) logits8<T>(P, row, i + k * kStep, x[k]);
   CumBins B;
   B.wave_m = wave_m;
   B.wave_n = wave_n;
@@ -565,41 +588,39 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleParams P)
     x_lo = fmaxf(x_lo, (float)(lo_v - room));
     x_hi = (float)(hi_v + room);
   }
-  for (int i0 = c * P.chunk; i0 < end; i0 += kStep) {
-    i = i0 + 8 * (int)threadIdx.x;
-    float ahead[8];
-    if (i + kStep < end) logits8<T>(P, row, i + kStep, ahead);
-    if (i < end) {
+  for (; i < end; i += kDeep * kStep) {
+#pragma unroll
+    for (int k = 0; k < kDeep; k++) {
+      const int at = i + k * kStep;
+      if (at >= end) break;
       uint32_t maybe = 0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) maybe |= x[e] >= x_lo && x[e] <= x_hi ? 1u << e : 0u;
+      for (int e = 0; e < 8; e++) maybe |= x[k][e] >= x_lo && x[k][e] <= x_hi ? 1u << e : 0u;
+      if (maybe) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        if (!((maybe >> e) & 1u)) continue;
-        const int b = S.bin_of(S.z_of(x[e]));
-        if (b < first || b > last) continue;
-        bool in = false;
+        for (int e = 0; e < 8; e++) {
+          if (!((maybe >> e) & 1u)) continue;
+          const int b = S.bin_of(S.z_of(x[k][e]));
+          if (b < first || b > last) continue;
+          bool in = false;
 #pragma unroll
-        for (int a = 0; a < kCuts; a++) in |= b >= lo[a] && b <= hi[a];
-        if (in) found[atomicAdd(&n_found, 1u)] = ((uint64_t)key_of(x[e]) << 32) | (uint32_t)~(uint32_t)(i + e);
+          for (int a = 0; a < kCuts; a++) in |= b >= lo[a] && b <= hi[a];
+          if (!in) continue;
+          // past the list's end the row is searched another way
+          const uint32_t j = atomicAdd(&n_found, 1u);
+          if (j < (uint32_t)kMostCandidates) found[j] = ((uint64_t)key_of(x[k][e]) << 32) | (uint32_t)~(uint32_t)(at + e);
+        }
       }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = ahead[e];
-    lds_barrier();
-    const uint32_t n = n_found;
-    lds_barrier();                      // every thread has read it before it counts again
-    if (n) {
-      if (threadIdx.x == 0) {
-        base = atomicAdd(&R.candidates, n);
-        n_found = 0;
-      }
-      __syncthreads();
-      for (uint32_t j = threadIdx.x; j < n; j += kThreads)
-        if (base + j < (uint32_t)kMostCandidates) R.list[base + j] = found[j];
-      __syncthreads();
+      if (at + kDeep * kStep < end) logits8<T>(P, row, at + kDeep * kStep, x[k]);
     }
   }
+  __syncthreads();
+  const uint32_t n = n_found;
+  if (n == 0) return;
+  if (threadIdx.x == 0) base = atomicAdd(&R.candidates, n);
+  __syncthreads();
+  for (uint32_t j = threadIdx.x; j < n; j += kThreads)
+    if (base + j < (uint32_t)kMostCandidates) R.list[base + j] = found[j];
 }
 
 // Value of lane ^ M of a 64-bit integer.
@@ -673,16 +694,15 @@ template <typename T>
 __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S, const SamplePlan& L, int a, int mode,
                                uint32_t rank, double target, uint64_t* dm, uint32_t* dn, uint64_t* answer) {
   const int lo = L.lo[a], hi = L.hi[a];
-  auto each = [&](auto f) __attribute__((always_inline)) {   // (key with index, z) of the interval's elements
+  auto each = [&](auto f) __attribute__((always_inline)) {   // (key with index, logit) of the interval's elements
     for (int i = 8 * (int)threadIdx.x; i < P.vocab; i += 8 * kFinalThreads) {
       float x[8];
       logits8<T>(P, row, i, x);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         if (!live(x[e])) continue;
-        const double z = S.z_of(x[e]);
-        const int b = S.bin_of(z);
-        if (b >= lo && b <= hi) f(((uint64_t)key_of(x[e]) << 32) | (uint32_t)~(uint32_t)(i + e), z);
+        const int b = S.bin_of(S.z_of(x[e]));
+        if (b >= lo && b <= hi) f(((uint64_t)key_of(x[e]) << 32) | (uint32_t)~(uint32_t)(i + e), x[e]);
       }
     }
   };
@@ -694,7 +714,7 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
   }
   __syncthreads();
   uint64_t all = ~0ull, any = 0;
-  each([&](uint64_t key, double) {
+  each([&](uint64_t key, float) {
     all &= key;
     any |= key;
   });
@@ -708,7 +728,7 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
     const uint64_t above = shift == 56 ? 0 : ~0ull << (shift + 8);
     if (((same >> shift) & 255u) == 255u) continue;
     const bool counted = (same | above) >> 32 == 0xffffffffull;
-    if (counted && unit == 0) unit = S.mass_of(S.z_of(of_key((uint32_t)(prefix >> 32))));
+    if (counted && unit == 0) unit = S.mass_of(of_key((uint32_t)(prefix >> 32)));
     __syncthreads();
     for (int b = threadIdx.x; b < 256; b += kFinalThreads) {
       dm[b] = 0;
@@ -723,7 +743,7 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
       atomicAdd(&dn[digit], n);
       if (!counted) atomicAdd((unsigned long long*)&dm[digit], (unsigned long long)m);
     };
-    each([&](uint64_t key, double z) {
+    each([&](uint64_t key, float x) {
       if (((key ^ prefix) & above) != 0) return;
       const int d = (int)(key >> shift) & 255;
       if (d != digit) {
@@ -733,7 +753,7 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
         m = 0;
       }
       n++;
-      if (!counted) m += S.mass_of(z);
+      if (!counted) m += S.mass_of(x);
     });
     flush();
     __syncthreads();
@@ -759,7 +779,7 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
     count = (uint32_t)answer[1];
     prefix = (prefix & ~(255ull << shift)) | ((answer[2] & 255u) << shift);
   }
-  mass += S.mass_of(S.z_of(of_key((uint32_t)(prefix >> 32))));   // the element itself
+  mass += S.mass_of(of_key((uint32_t)(prefix >> 32)));   // the element itself
   __syncthreads();                                               // answer may be written again
   return Found{mass, prefix};
 }
@@ -815,9 +835,9 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
       const int i = t * per + k;
       bins[k] = -1;
       if (k < per && i < (int)n) {
-        const double z = S.z_of(of_key((uint32_t)(list[i] >> 32)));
-        bins[k] = S.bin_of(z);
-        sum += S.mass_of(z);
+        const float x = of_key((uint32_t)(list[i] >> 32));
+        bins[k] = S.bin_of(S.z_of(x));
+        sum += S.mass_of(x);
       }
       w[k] = sum;
     }
@@ -934,7 +954,7 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
         if (!live(x)) continue;
         const double z = S.z_of(x);
         const int bz = S.bin_of(z);
-        if (bz >= m_lo && bz <= m_hi && (z == 0.0 || S.weight_of(z) >= C.min_p)) some += S.mass_of(z);
+        if (bz >= m_lo && bz <= m_hi && (z == 0.0 || S.weight_of(z) >= C.min_p)) some += S.mass_of(x);
       }
       __syncthreads();
       if (some) atomicAdd(&kept_m, (unsigned long long)some);
