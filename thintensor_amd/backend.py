@@ -15,7 +15,6 @@ depends only on the tensor shapes.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import Any
@@ -54,12 +53,27 @@ def _stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-_NO_GUARD = contextlib.nullcontext()
+_current_gpu = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _device_of(t: torch.Tensor):
-    """Makes the tensor's GPU the current one, where it is not already."""
-    return _NO_GUARD if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+def _gpu_of(t: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The first tensor's GPU, where every other one has to be."""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("HipDecodeBackend operates on device tensors only")
+    for o in others:
+        if o is not None and o.get_device() != index:
+            raise ValueError(f"tensors on different devices: {t.device} and {o.device}")
+    return index
+
+
+def _on_gpu(index: int, entry, *args) -> int:
+    """entry(*args, stream) with the GPU as the current one, on its current stream."""
+    if index == _current_gpu():
+        return entry(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return entry(*args, _raw_stream(index))
 
 
 def _require_cuda(*tensors: torch.Tensor) -> None:
@@ -1549,16 +1563,6 @@ class HipDecodeBackend:
         return self._argmax_out_idx
 
     # ------------------------------------------------------------ a decode step around its weights (no reference counterpart)
-    @staticmethod
-    def _on_device(t: torch.Tensor, *others: torch.Tensor | None) -> None:
-        """Every tensor on the first one's GPU."""
-        device = t.device
-        if device.type != "cuda":
-            raise ValueError("HipDecodeBackend operates on device tensors only")
-        for o in others:
-            if o is not None and o.device != device:
-                raise ValueError(f"tensors on different devices: {device} and {o.device}")
-
     def rotary_rows(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
                     q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, *,
                     interleaved: bool = False, amplitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor | None]:
@@ -1568,18 +1572,19 @@ class HipDecodeBackend:
         times ``amplitude``; the other dims are copied.  ``inv_freq`` is float64
         (:func:`thintensor_amd.rotary.rotary_frequencies`).  Without outputs in place; an output may be
         its input but not overlap one otherwise."""
-        q_out = q if q_out is None else q_out
+        if q_out is None:
+            q_out = q
         if k is None:
             if k_out is not None:
                 raise ValueError("rotary_rows: k_out without k")
         elif k_out is None:
             k_out = k
-        qs, qos = q.stride(), q_out.stride()
-        if q.ndim != 3 or q_out.shape != q.shape:
+        shape, qs, dtype = q.shape, q.stride(), q.dtype
+        if len(shape) != 3 or q_out is not q and q_out.shape != shape:
             raise ValueError("rotary_rows takes q and its output [tokens, heads, head_dim]")
-        tokens, heads, head_dim = q.shape
-        dtype = q.dtype
-        if q_out.dtype != dtype:
+        tokens, heads, head_dim = shape
+        qos = qs if q_out is q else q_out.stride()
+        if q_out is not q and q_out.dtype != dtype:
             raise ValueError("rotary_rows operands must share a dtype")
         if positions.numel() != tokens or not positions.is_contiguous() or \
                 positions.dtype not in (torch.int32, torch.int64):
@@ -1589,24 +1594,23 @@ class HipDecodeBackend:
         if qs[2] != 1 or qos[2] != 1:
             raise ValueError("rotary_rows operands must be contiguous in their last axis")
         if k is not None:
-            ks, kos, shape = k.stride(), k_out.stride(), k.shape
-            if k.ndim != 3 or shape[0] != tokens or shape[2] != head_dim or k_out.shape != shape:
+            shape, ks = k.shape, k.stride()
+            if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim or k_out is not k and k_out.shape != shape:
                 raise ValueError("rotary_rows takes k and its output [tokens, kv_heads, head_dim]")
-            if k.dtype != dtype or k_out.dtype != dtype:
+            kos = ks if k_out is k else k_out.stride()
+            if k.dtype != dtype or k_out is not k and k_out.dtype != dtype:
                 raise ValueError("rotary_rows operands must share a dtype")
             if ks[2] != 1 or kos[2] != 1:
                 raise ValueError("rotary_rows operands must be contiguous in their last axis")
-            k_args = (k.data_ptr(), ks[0], ks[1])
-            ko_args = (k_out.data_ptr(), kos[0], kos[1])
-            kv_heads = shape[1]
+            k_ptr, ko_ptr, kv_heads = k.data_ptr(), k_out.data_ptr(), shape[1]
         else:
-            k_args, ko_args, kv_heads = (None, 0, 0), (None, 0, 0), 0
-        self._on_device(q, k, positions, inv_freq, q_out, k_out)
-        with _device_of(q):
-            rc = self.lib.tt_rotary_rows(
-                q.data_ptr(), qs[0], qs[1], *k_args, _code(q, "rotary_rows"), positions.data_ptr(),
-                positions.element_size(), inv_freq.data_ptr(), amplitude, int(interleaved), tokens, heads, kv_heads,
-                head_dim, 2 * inv_freq.numel(), q_out.data_ptr(), qos[0], qos[1], *ko_args, _stream(q))
+            ks = kos = (0, 0)
+            k_ptr, ko_ptr, kv_heads = None, None, 0
+        gpu = _gpu_of(q, k, positions, inv_freq, None if q_out is q else q_out, None if k_out is k else k_out)
+        rc = _on_gpu(gpu, self.lib.tt_rotary_rows,
+                     q.data_ptr(), qs[0], qs[1], k_ptr, ks[0], ks[1], _code(q, "rotary_rows"), positions.data_ptr(),
+                     positions.element_size(), inv_freq.data_ptr(), amplitude, 1 if interleaved else 0, tokens, heads, kv_heads,
+                     head_dim, 2 * inv_freq.numel(), q_out.data_ptr(), qos[0], qos[1], ko_ptr, kos[0], kos[1])
         if rc:
             _lib.check(rc, "rotary_rows")
         return q_out, k_out
@@ -1630,11 +1634,9 @@ class HipDecodeBackend:
             raise ValueError(f"{what}: starts must be int32, one per row")
         if counts is not None and (counts.dtype != torch.int32 or counts.numel() != rows or not counts.is_contiguous()):
             raise ValueError(f"{what}: counts must be int32, one per row")
-        self._on_device(k, v, starts, counts, cache.k_codes)
-        with _device_of(k):
-            rc = entry(
-                cache.desc, k.data_ptr(), ks[0], k_token, ks[-2], v.data_ptr(), vs[0], v_token, vs[-2], _code(k, what),
-                starts.data_ptr(), counts.data_ptr() if counts is not None else None, rows, tokens, _stream(k))
+        gpu = _gpu_of(k, v, starts, counts, cache.k_codes)
+        rc = _on_gpu(gpu, entry, cache.desc, k.data_ptr(), ks[0], k_token, ks[-2], v.data_ptr(), vs[0], v_token, vs[-2],
+                     _code(k, what), starts.data_ptr(), counts.data_ptr() if counts is not None else None, rows, tokens)
         if rc:
             _lib.check(rc, what)
 
@@ -1682,16 +1684,16 @@ class HipDecodeBackend:
                 raise ValueError("gqa_attention_int4: sinks must hold one logit per query head")
             sink_ptr, sink_code = sinks.data_ptr(), _code(sinks, "sinks")
         limit = cache.capacity if max_length is None else max_length
-        self._on_device(q, out, lengths, sinks, cache.k_codes)
-        with _device_of(q):
-            need = self.lib.tt_gqa_attention_int4_scratch_floats(cache.desc, rows, heads, window, first_tokens, limit)
-            if need < 0:
-                _lib.check(int(need), "gqa_attention_int4")
-            scratch = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
-            rc = self.lib.tt_gqa_attention_int4(
-                cache.desc, q.data_ptr(), qs[0], qs[1], _code(q, "gqa_attention_int4"), lengths.data_ptr(), rows, heads,
-                window, first_tokens, limit, sink_ptr, sink_code, scale if scale is not None else head_dim ** -0.5,
-                scratch.data_ptr() if need else None, need, out.data_ptr(), os[0], os[1], _stream(q))
+        gpu = _gpu_of(q, out, lengths, sinks, cache.k_codes)
+        need = self.lib.tt_gqa_attention_int4_scratch_floats(cache.desc, rows, heads, window, first_tokens, limit)
+        if need < 0:
+            _lib.check(int(need), "gqa_attention_int4")
+        scratch = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
+        rc = _on_gpu(gpu, self.lib.tt_gqa_attention_int4,
+                     cache.desc, q.data_ptr(), qs[0], qs[1], _code(q, "gqa_attention_int4"), lengths.data_ptr(), rows,
+                     heads, window, first_tokens, limit, sink_ptr, sink_code,
+                     scale if scale is not None else head_dim ** -0.5, scratch.data_ptr() if need else None, need,
+                     out.data_ptr(), os[0], os[1])
         if rc:
             _lib.check(rc, "gqa_attention_int4")
         return out
@@ -1722,13 +1724,12 @@ class HipDecodeBackend:
             if t.dtype != (torch.int32 if name == "top_k" else torch.float32) or t.numel() != rows or not t.is_contiguous():
                 raise ValueError(f"sample_rows: {name} must be contiguous {'int32' if name == 'top_k' else 'float32'}, one per row")
             ptrs.append(t.data_ptr())
-        self._on_device(logits, uniforms, tokens, temperature, top_k, top_p, min_p, probs)
-        with _device_of(logits):
-            need = self.lib.tt_sample_rows_scratch_bytes(rows, vocab)
-            scratch = torch.empty(need, device=logits.device, dtype=torch.uint8)
-            rc = self.lib.tt_sample_rows(
-                logits.data_ptr(), logits.stride(0), _code(logits, "sample_rows"), rows, vocab, *ptrs[:5],
-                scratch.data_ptr(), need, tokens.data_ptr(), ptrs[5], _stream(logits))
+        gpu = _gpu_of(logits, uniforms, tokens, temperature, top_k, top_p, min_p, probs)
+        need = self.lib.tt_sample_rows_scratch_bytes(rows, vocab)
+        scratch = torch.empty(need, device=logits.device, dtype=torch.uint8)
+        rc = _on_gpu(gpu, self.lib.tt_sample_rows,
+                     logits.data_ptr(), logits.stride(0), _code(logits, "sample_rows"), rows, vocab, *ptrs[:5],
+                     scratch.data_ptr(), need, tokens.data_ptr(), ptrs[5])
         if rc:
             _lib.check(rc, "sample_rows")
         return tokens
