@@ -36,13 +36,13 @@ constexpr int kMostCandidates = 4096;   // that the last step sorts in LDS
 constexpr int kFinalThreads = 1024;
 constexpr int kCuts = 4;                // intervals of bins: top-k, top-p, min-p, the target
 
-// What step 3 leaves for step 4: disjoint intervals of bins in increasing order (n of them), the
-// weight and count before each and the weight up to its end; the bins of top-k and min-p.
+// What step 3 leaves for step 4: disjoint intervals of bins in increasing order (n of them, behind them
+// empty ones), the weight and count before each and up to its end; whether top-k divides a bin.
 struct alignas(16) SamplePlan {
   int n;
   int lo[kCuts], hi[kCuts];
   uint64_t before[kCuts], upto[kCuts];
-  uint32_t rank_before[kCuts];
+  uint32_t rank_before[kCuts], rank_upto[kCuts];
   int k_cut;                            // whether top-k divides a bin
   uint32_t k;
   uint64_t k_mass;                      // otherwise: the weight that it keeps
@@ -118,8 +118,7 @@ __device__ __forceinline__ double exp_neg(double z, int* n) {
 struct RowScale {
   double top, inv_t, y_per_x, bins_per_z;
   bool greedy, hard;
-  __device__ RowScale(const SampleParams& P, int row, float2 range) {
-    const float t = P.temperature ? P.temperature[row] : 1.0f;
+  __device__ RowScale(float2 range, float t) {
     greedy = !(t > 0.0f);
     hard = greedy || range.x == __builtin_bit_cast(float, 0x7f800000u);
     top = (double)range.x;
@@ -165,6 +164,28 @@ struct RowScale {
   __device__ uint64_t mass_of(float x) const {
     if (hard) return (double)x == top ? (uint64_t)kUnit : 0;
     return soft_mass(x);
+  }
+};
+
+// A row's settings as they are given: requested together at a kernel's start (one that is not given is read
+// from the uniform numbers, and not used).
+struct RowSettings {
+  float t, p, min_p, u;
+  int32_t k;
+  __device__ RowSettings(const SampleParams& P, int row) {
+    const float a = (P.temperature ? P.temperature : P.uniforms)[row], b = (P.top_p ? P.top_p : P.uniforms)[row];
+    const float c = (P.min_p ? P.min_p : P.uniforms)[row];
+    const int32_t d = (P.top_k ? P.top_k : reinterpret_cast<const int32_t*>(P.uniforms))[row];
+    u = P.uniforms[row];
+    t = P.temperature ? a : 1.0f;
+    p = P.top_p ? b : 1.0f;
+    min_p = P.min_p ? c : 0.0f;
+    k = P.top_k ? d : 0;
+  }
+  // top-k where it cuts the order (a greedy row keeps the first), else 0
+  __device__ uint32_t top_k(bool greedy, int vocab) const {
+    const int32_t n = greedy ? 1 : k;
+    return n > 0 && n < vocab ? (uint32_t)n : 0u;
   }
 };
 
@@ -251,12 +272,6 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleParams P) 
   }
 }
 
-// Whether top-k cuts a row's order (a greedy row keeps the first).
-__device__ __forceinline__ uint32_t row_top_k(const SampleParams& P, int row, bool greedy) {
-  const int32_t k = greedy ? 1 : P.top_k ? P.top_k[row] : 0;
-  return k > 0 && k < P.vocab ? (uint32_t)k : 0u;
-}
-
 template <typename T>
 __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleParams P) {
   const int row = blockIdx.y, c = blockIdx.x;
@@ -267,13 +282,14 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleParams P
   int i = c * P.bin_chunk + 8 * (int)threadIdx.x;
   float x[8];
   if (i < end) logits8<T>(P, row, i, x);
+  const RowSettings G(P, row);
   const float2 range = row_range(P, row);
   for (int b = threadIdx.x; b < kBins / 2; b += kBinThreads) {
     reinterpret_cast<ulonglong2*>(mass)[b] = make_ulonglong2(0, 0);
     reinterpret_cast<uint2*>(count)[b] = make_uint2(0, 0);
   }
-  const RowScale S(P, row, range);
-  const bool counts = row_top_k(P, row, S.greedy) != 0;
+  const RowScale S(range, G.t);
+  const bool counts = G.top_k(S.greedy, P.vocab) != 0;
   uint32_t far = 0;                     // of the last bin
   __syncthreads();
   while (i < end) {
@@ -317,24 +333,61 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleParams P
   }
 }
 
-// A row's cumulative histogram, eight bins per thread, and searches in it.  An answer is a bin with
-// the weight and count before it and up to its end.
-struct BinAt {
-  int bin;
-  uint32_t n0, n1;
-  uint64_t m0, m1;
-};
+// Sum over this lane and the ones before it in the wave: within rows of sixteen lanes, then over the rows.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp0(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+#define TT_LEVEL(CTRL, ROWS) v += dpp0<CTRL, ROWS>(v);
+  TT_LEVEL(0x111, 0xf) TT_LEVEL(0x112, 0xf) TT_LEVEL(0x114, 0xf) TT_LEVEL(0x118, 0xf)   // row_shr 1, 2, 4, 8
+  TT_LEVEL(0x142, 0xa) TT_LEVEL(0x143, 0xc)                                             // row_bcast 15, 31
+#undef TT_LEVEL
+  return v;
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+#define TT_LEVEL(CTRL, ROWS) v += ((uint64_t)dpp0<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | dpp0<CTRL, ROWS>((uint32_t)v);
+  TT_LEVEL(0x111, 0xf) TT_LEVEL(0x112, 0xf) TT_LEVEL(0x114, 0xf) TT_LEVEL(0x118, 0xf)
+  TT_LEVEL(0x142, 0xa) TT_LEVEL(0x143, 0xc)
+#undef TT_LEVEL
+  return v;
+}
 
+// A row's cumulative histogram in LDS, where every wave searches it by itself: a look at the ends of its 64
+// blocks of 32 bins, then one at a block, each a comparison in all lanes.  Blocks lie four banks apart.
 struct CumBins {
+  uint64_t m[kBins + 2 * (kBins / 32)];
+  uint32_t n[kBins + 4 * (kBins / 32)];
+  uint64_t wave_m[kThreads / 64];
+  uint32_t wave_n[kThreads / 64];
+  static __device__ __forceinline__ int at_m(int bin) { return bin + 2 * (bin >> 5); }
+  static __device__ __forceinline__ int at_n(int bin) { return bin + 4 * (bin >> 5); }
+  // weight and count of the bins up to this one
+  __device__ uint64_t mass(int bin) const { return bin < 0 ? 0 : m[at_m(bin)]; }
+  __device__ uint32_t count(int bin) const { return bin < 0 ? 0 : n[at_n(bin)]; }
+  // The first bin with which the weight (count) reaches `want`; the last one if none does.
+  __device__ int find_count(uint32_t want) const {
+    const int lane = threadIdx.x & 63;
+    const int block = __builtin_popcountll(__builtin_amdgcn_ballot_w64(n[at_n(32 * lane + 31)] < want));
+    if (block == kBins / 32) return kBins - 1;
+    return 32 * block + __builtin_popcount((uint32_t)__builtin_amdgcn_ballot_w64(n[at_n(32 * block + (lane & 31))] < want));
+  }
+  __device__ int find_mass(uint64_t want) const {
+    const int lane = threadIdx.x & 63;
+    const int block = __builtin_popcountll(__builtin_amdgcn_ballot_w64(m[at_m(32 * lane + 31)] < want));
+    if (block == kBins / 32) return kBins - 1;
+    return 32 * block + __builtin_popcount((uint32_t)__builtin_amdgcn_ballot_w64(m[at_m(32 * block + (lane & 31))] < want));
+  }
+};
+static_assert(kBins == 64 * 32, "two looks of a wave");
+
+// Eight bins of the histogram per thread.
+struct BinPart {
   static constexpr int PER = kBins / kThreads;
-  uint64_t m[PER + 1], total;           // before each of this thread's bins, and after the last
-  uint32_t n[PER + 1], all;
-  uint64_t* wave_m;
-  uint32_t* wave_n;
+  static_assert(PER == 8 && kThreads % 64 == 0, "a thread's bins lie in one block");
+  uint64_t m[PER];
+  uint32_t n[PER];
   __device__ void load(const SampleRow& R) {
-    const int t = threadIdx.x;
-    const ulonglong2* rm = reinterpret_cast<const ulonglong2*>(R.mass + t * PER);
-    const uint4* rn = reinterpret_cast<const uint4*>(R.count + t * PER);
+    const ulonglong2* rm = reinterpret_cast<const ulonglong2*>(R.mass + threadIdx.x * PER);
+    const uint4* rn = reinterpret_cast<const uint4*>(R.count + threadIdx.x * PER);
 #pragma unroll
     for (int k = 0; k < PER / 2; k++) {
       const ulonglong2 v = rm[k];
@@ -346,87 +399,58 @@ struct CumBins {
       n[4 * k] = v.x; n[4 * k + 1] = v.y; n[4 * k + 2] = v.z; n[4 * k + 3] = v.w;
     }
   }
-  __device__ void sum() {               // one barrier
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    uint64_t ms = 0;
-    uint32_t ns = 0;
+  __device__ void sum(CumBins& C) {     // two barriers
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
 #pragma unroll
-    for (int k = 0; k < PER; k++) {
-      const uint64_t a = m[k];
-      const uint32_t b = n[k];
-      m[k] = ms;
-      n[k] = ns;
-      ms += a;
-      ns += b;
+    for (int k = 1; k < PER; k++) {
+      m[k] += m[k - 1];
+      n[k] += n[k - 1];
     }
-    uint64_t mi = ms;
-    uint32_t ni = ns;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint64_t mo = __shfl_up((unsigned long long)mi, d);
-      const uint32_t no = __shfl_up(ni, d);
-      if (lane >= d) {
-        mi += mo;
-        ni += no;
-      }
-    }
-    if (lane == 63) {
-      wave_m[wave] = mi;
-      wave_n[wave] = ni;
+    const uint64_t mi = wave_scan(m[PER - 1]);
+    const uint32_t ni = wave_scan(n[PER - 1]);
+    if ((t & 63) == 63) {
+      C.wave_m[wave] = mi;
+      C.wave_n[wave] = ni;
     }
     __syncthreads();
-    uint64_t mb = mi - ms;
-    uint32_t nb = ni - ns;
-    total = 0;
-    all = 0;
+    uint64_t mb = mi - m[PER - 1];
+    uint32_t nb = ni - n[PER - 1];
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) {
+    for (int w = 0; w < kThreads / 64 - 1; w++)
       if (w < wave) {
-        mb += wave_m[w];
-        nb += wave_n[w];
+        mb += C.wave_m[w];
+        nb += C.wave_n[w];
       }
-      total += wave_m[w];
-      all += wave_n[w];
-    }
+    ulonglong2* pm = reinterpret_cast<ulonglong2*>(&C.m[CumBins::at_m(t * PER)]);
+    uint4* pn = reinterpret_cast<uint4*>(&C.n[CumBins::at_n(t * PER)]);
 #pragma unroll
-    for (int k = 0; k < PER; k++) {
-      m[k] += mb;
-      n[k] += nb;
-    }
-    m[PER] = mb + ms;
-    n[PER] = nb + ns;
-  }
-  // The thread that holds the answer writes it: before a barrier that the caller makes, into a place
-  // that holds the default.
-  template <typename Cond>              // cond(m0, m1, n0, n1): this bin is the answer
-  __device__ void find(Cond cond, BinAt* out) const {
-    if (!cond(m[0], m[PER], n[0], n[PER])) return;
+    for (int k = 0; k < PER / 2; k++) pm[k] = make_ulonglong2(mb + m[2 * k], mb + m[2 * k + 1]);
 #pragma unroll
-    for (int k = 0; k < PER; k++)
-      if (cond(m[k], m[k + 1], n[k], n[k + 1])) *out = BinAt{(int)threadIdx.x * PER + k, n[k], n[k + 1], m[k], m[k + 1]};
-  }
-  __device__ void get(int bin, BinAt* out) const {
-    if (bin / PER != (int)threadIdx.x) return;
-#pragma unroll
-    for (int k = 0; k < PER; k++)
-      if (bin % PER == k) *out = BinAt{bin, n[k], n[k + 1], m[k], m[k + 1]};
+    for (int k = 0; k < PER / 4; k++) pn[k] = make_uint4(nb + n[4 * k], nb + n[4 * k + 1], nb + n[4 * k + 2], nb + n[4 * k + 3]);
+    __syncthreads();
   }
 };
 
-// A row's settings.
-struct Settings {
+// What the cuts take from a row's settings.
+struct Cuts {
   uint32_t k;                           // 0: none
   double p, min_p, u;
   bool use_p, use_m;
-  __device__ Settings(const SampleParams& P, int row, bool greedy) {
-    k = row_top_k(P, row, greedy);
-    const float tp = P.top_p ? P.top_p[row] : 1.0f, mp = P.min_p ? P.min_p[row] : 0.0f, un = P.uniforms[row];
-    u = un > 0.0f ? (un < 1.0f ? (double)un : 1.0 - 0x1p-24) : 0.0;
-    use_p = tp < 1.0f;
-    p = tp > 0.0f ? (double)tp : 0.0;
-    use_m = mp > 0.0f;
-    min_p = (double)mp;
+  __device__ Cuts(const RowSettings& G, bool greedy, int vocab) {
+    k = G.top_k(greedy, vocab);
+    u = G.u > 0.0f ? (G.u < 1.0f ? (double)G.u : 1.0 - 0x1p-24) : 0.0;
+    use_p = G.p < 1.0f;
+    p = G.p > 0.0f ? (double)G.p : 0.0;
+    use_m = G.min_p > 0.0f;
+    min_p = (double)G.min_p;
   }
+  // The cumulative weight that the last of top-p's share reaches first, and the one that the token does:
+  // integers, so that every step compares alike.  Both are at most `mass` (p and u are 1 - 2^-24 at most).
+  __device__ uint64_t reach(uint64_t mass) const {
+    const double t = p * (double)mass;
+    return t > 1.0 ? (uint64_t)__builtin_ceil(t) : 1;
+  }
+  __device__ uint64_t target(uint64_t mass) const { return (uint64_t)(u * (double)mass) + 1; }
 };
 
 // Steps of a chunk on their way at a time: more take registers that keep four workgroups from a CU (64 rows of
@@ -437,10 +461,11 @@ template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams P) {
   const int row = blockIdx.y, c = blockIdx.x;
   SampleRow& R = P.rows[row];
-  __shared__ uint64_t wave_m[kThreads / 64];
-  __shared__ uint32_t wave_n[kThreads / 64];
-  __shared__ BinAt at[4 * kCuts];
-  __shared__ uint64_t found[kMostCandidates];
+  // the histogram, then the chunk's candidates
+  __shared__ __attribute__((aligned(16))) union {
+    CumBins bins;
+    uint64_t found[kMostCandidates];
+  } U;
   __shared__ uint32_t n_found, base;
   const int end = min(P.vocab, (c + 1) * P.chunk);
   int i = c * P.chunk + 8 * (int)threadIdx.x;
@@ -448,75 +473,49 @@ __global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams
 #pragma unroll
   for (int k = 0; k < kDeep; k++)
     if (i + k * kStep < end) logits8<T>(P, row, i + k * kStep, x[k]);
-  CumBins B;
-  B.wave_m = wave_m;
-  B.wave_n = wave_n;
-  B.load(R);
+  const RowSettings G(P, row);
+  BinPart part;
+  part.load(R);
   const float2 range = row_range(P, row);
   if (!live(range.x)) return;
-  const RowScale S(P, row, range);
-  const Settings C(P, row, S.greedy);
   if (threadIdx.x == 0) n_found = 0;
-  // where nothing answers, the last bin does
-  if (threadIdx.x < 4 * kCuts) at[threadIdx.x].bin = kBins - 1;
-  B.sum();
+  part.sum(U.bins);
+  const CumBins& B = U.bins;
+  const RowScale S(range, G.t);
+  const Cuts C(G, S.greedy, P.vocab);
+  const uint64_t total = B.mass(kBins - 1);
 
   // ---- top-k: the bin of its last one; whole bins and the last bin (no weight) need no resolving
-  uint64_t k_lo = B.total, k_hi = B.total;
+  uint64_t k_lo = total, k_hi = total;
   int k_bin = -1;
-  if (C.k && C.k < B.all) {
-    B.find([&](uint64_t, uint64_t, uint32_t n0, uint32_t n1) { return n0 < C.k && C.k <= n1; }, &at[0]);
-    __syncthreads();
-    const BinAt a = at[0];
-    k_lo = k_hi = a.m1;
-    if (a.n1 != C.k && a.bin != kBins - 1) {
-      k_bin = a.bin;
-      k_lo = a.m0;
+  if (C.k && C.k < B.count(kBins - 1)) {
+    const int b = B.find_count(C.k);
+    k_lo = k_hi = B.mass(b);
+    if (B.count(b) != C.k && b != kBins - 1) {
+      k_bin = b;
+      k_lo = B.mass(b - 1);
     }
   }
   // ---- top-p and min-p, as far as the weight of top-k is known
   uint64_t kept_lo = k_lo, kept_hi = k_hi, m_before = 0;
   int p_lo = -1, p_hi = -2, m_lo = -1, m_hi = -2;
-  if (C.use_p || C.use_m) {
-    const double t_lo = C.p * (double)k_lo, t_hi = C.p * (double)k_hi;
-    auto at_least = [](double t) { return [t](uint64_t m0, uint64_t m1, uint32_t, uint32_t) { return (double)m0 < t && (double)m1 >= t; }; };
-    if (C.use_p) {
-      if (t_lo > 0.0) B.find(at_least(t_lo), &at[1]);
-      else B.get(0, &at[1]);
-      if (t_hi > 0.0) B.find(at_least(t_hi), &at[2]);
-      else B.get(0, &at[2]);
-    }
-    if (C.use_m) {
-      const int b = S.greedy || !(C.min_p < 1.0) ? 0 : S.bin_of(-log(C.min_p));
-      m_lo = max(0, b - 1);
-      m_hi = min(kBins - 1, b + 1);
-      B.get(m_lo, &at[3]);
-      B.get(m_hi, &at[4]);
-    }
-    __syncthreads();
-    if (C.use_p) {
-      p_lo = at[1].bin;
-      p_hi = at[2].bin;
-      if (p_lo < kBins - 1) kept_lo = min(kept_lo, at[1].m0);
-      if (p_hi < kBins - 1) kept_hi = min(kept_hi, at[2].m1);
-    }
-    if (C.use_m) {
-      m_before = at[3].m0;
-      kept_lo = min(kept_lo, at[3].m0);
-      kept_hi = min(kept_hi, at[4].m1);
-    }
+  if (C.use_p) {
+    p_lo = B.find_mass(C.reach(k_lo));
+    p_hi = k_bin < 0 ? p_lo : B.find_mass(C.reach(k_hi));
+    if (p_lo < kBins - 1) kept_lo = min(kept_lo, B.mass(p_lo - 1));
+    if (p_hi < kBins - 1) kept_hi = min(kept_hi, B.mass(p_hi));
   }
-  // ---- the target
-  {
-    const double t_lo = C.u * (double)kept_lo, t_hi = C.u * (double)kept_hi;
-    auto above = [](double t) { return [t](uint64_t m0, uint64_t m1, uint32_t, uint32_t) { return (double)m0 <= t && (double)m1 > t; }; };
-    B.find(above(t_lo), &at[5]);
-    B.find(above(t_hi), &at[6]);
-    __syncthreads();
+  if (C.use_m) {
+    const int b = __builtin_amdgcn_readfirstlane(S.greedy || !(C.min_p < 1.0) ? 0 : S.bin_of(-log(C.min_p)));
+    m_lo = max(0, b - 1);
+    m_hi = min(kBins - 1, b + 1);
+    m_before = B.mass(m_lo - 1);
+    kept_lo = min(kept_lo, m_before);
+    kept_hi = min(kept_hi, B.mass(m_hi));
   }
-  // ---- disjoint intervals in order
-  int lo[kCuts] = {k_bin < 0 ? kBins : k_bin, p_hi < p_lo ? kBins : p_lo, m_hi < m_lo ? kBins : m_lo, at[5].bin};
-  int hi[kCuts] = {k_bin, p_hi, m_hi, at[6].bin};
+  // ---- the target, and disjoint intervals in order
+  int lo[kCuts] = {k_bin < 0 ? kBins : k_bin, p_hi < p_lo ? kBins : p_lo, m_hi < m_lo ? kBins : m_lo, B.find_mass(C.target(kept_lo))};
+  int hi[kCuts] = {k_bin, p_hi, m_hi, B.find_mass(C.target(kept_hi))};
 #pragma unroll
   for (int a = 0; a < kCuts; a++) {
     hi[a] = min(hi[a], kBins - 2);      // the last bin weighs nothing
@@ -542,35 +541,34 @@ __global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams
         lo[a - 1] = kBins;
       }
     }
-  if (c == 0) {                         // the plan, for the last step
+  if (c == 0 && threadIdx.x == 0) {     // the plan, for the last step
+    SamplePlan& L = R.plan;
+    int n = 0;
 #pragma unroll
     for (int a = 0; a < kCuts; a++)
       if (lo[a] < kBins) {
-        B.get(lo[a], &at[2 * kCuts + a]);
-        B.get(hi[a], &at[3 * kCuts + a]);
+        L.lo[n] = lo[a];
+        L.hi[n] = hi[a];
+        L.before[n] = B.mass(lo[a] - 1);
+        L.rank_before[n] = B.count(lo[a] - 1);
+        L.upto[n] = B.mass(hi[a]);
+        L.rank_upto[n] = B.count(hi[a]);
+        n++;
       }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      SamplePlan& L = R.plan;
-      int n = 0;
-#pragma unroll
-      for (int a = 0; a < kCuts; a++)
-        if (lo[a] < kBins) {
-          L.lo[n] = lo[a];
-          L.hi[n] = hi[a];
-          L.before[n] = at[2 * kCuts + a].m0;
-          L.rank_before[n] = at[2 * kCuts + a].n0;
-          L.upto[n] = at[3 * kCuts + a].m1;
-          n++;
-        }
-      L.n = n;
-      L.k_cut = k_bin >= 0;
-      L.k = C.k;
-      L.k_mass = k_hi;
-      L.total = B.total;
-      L.m_before = m_before;
+    L.n = n;
+    for (; n < kCuts; n++) {
+      L.lo[n] = kBins;
+      L.hi[n] = -1;
+      L.before[n] = L.upto[n] = 0;
+      L.rank_before[n] = L.rank_upto[n] = 0;
     }
+    L.k_cut = k_bin >= 0;
+    L.k = C.k;
+    L.k_mass = k_hi;
+    L.total = total;
+    L.m_before = m_before;
   }
+  __syncthreads();                      // the histogram is not read any more
   // ---- this chunk's candidates
   int first = kBins;                    // most logits are past every interval
   int last = -1;
@@ -608,7 +606,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams
           if (!in) continue;
           // past the list's end the row is searched another way
           const uint32_t j = atomicAdd(&n_found, 1u);
-          if (j < (uint32_t)kMostCandidates) found[j] = ((uint64_t)key_of(x[k][e]) << 32) | (uint32_t)~(uint32_t)(at + e);
+          if (j < (uint32_t)kMostCandidates) U.found[j] = ((uint64_t)key_of(x[k][e]) << 32) | (uint32_t)~(uint32_t)(at + e);
         }
       }
       if (at + kDeep * kStep < end) logits8<T>(P, row, at + kDeep * kStep, x[k]);
@@ -620,7 +618,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams
   if (threadIdx.x == 0) base = atomicAdd(&R.candidates, n);
   __syncthreads();
   for (uint32_t j = threadIdx.x; j < n; j += kThreads)
-    if (base + j < (uint32_t)kMostCandidates) R.list[base + j] = found[j];
+    if (base + j < (uint32_t)kMostCandidates) R.list[base + j] = U.found[j];
 }
 
 // Value of lane ^ M of a 64-bit integer.
@@ -686,13 +684,13 @@ struct Found {           // answer of a search
 };
 
 // A candidate list that does not fit: the elements of one interval are searched by the digits of
-// their keys and indexes, over the row itself.  mode 0: the element of rank `rank`; 1: the first
-// whose cumulative weight is at least target; 2: the first whose is more.  Digits that all elements
+// their keys and indexes, over the row itself: the element of rank `rank`, or without one (0) the first whose
+// cumulative weight reaches `want`.  Digits that all elements
 // share are found first and passed over; once a key is settled its elements weigh the same and are
 // counted.  A thread adds up what falls to one digit in a row before it meets the others in LDS.
 template <typename T>
-__device__ Found search_digits(const SampleParams& P, int row, const RowScale& S, const SamplePlan& L, int a, int mode,
-                               uint32_t rank, double target, uint64_t* dm, uint32_t* dn, uint64_t* answer) {
+__device__ Found search_digits(const SampleParams& P, int row, const RowScale& S, const SamplePlan& L, int a,
+                               uint32_t rank, uint64_t want, uint64_t* dm, uint32_t* dn, uint64_t* answer) {
   const int lo = L.lo[a], hi = L.hi[a];
   auto each = [&](auto f) __attribute__((always_inline)) {   // (key with index, logit) of the interval's elements
     for (int i = 8 * (int)threadIdx.x; i < P.vocab; i += 8 * kFinalThreads) {
@@ -768,7 +766,7 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
         pn = count;
         mass += counted ? dn[b] * unit : dm[b];
         count += dn[b];
-        if (mode == 0 ? count >= rank : mode == 1 ? (double)mass >= target : (double)mass > target) break;
+        if (rank ? count >= rank : mass >= want) break;
       }
       answer[0] = pm;
       answer[1] = pn;
@@ -786,17 +784,17 @@ __device__ Found search_digits(const SampleParams& P, int row, const RowScale& S
 
 template <typename T>
 __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParams P) {
-  constexpr int PER = kMostCandidates / kFinalThreads;
-  const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  constexpr int PER = kMostCandidates / kFinalThreads, WAVES = kFinalThreads / 64;
+  const int row = blockIdx.x, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   SampleRow& R = P.rows[row];
-  __shared__ SamplePlan L;
-  __shared__ uint64_t list[kMostCandidates], cum[kMostCandidates];   // cum: weight up to and including
-  __shared__ uint64_t wave_sum[kFinalThreads / 64], answer[4], start_sum[kCuts];
-  __shared__ int start[kCuts];
+  __shared__ uint64_t list[kMostCandidates], digits[256];
+  __shared__ __attribute__((aligned(16))) uint64_t wave_sum[WAVES];
+  __shared__ uint64_t answer[4];
   __shared__ unsigned long long kept_m;
   uint64_t mine = R.list[t];            // (used where the list is that long)
+  const RowSettings G(P, row);
   const uint32_t n = R.candidates;
-  if (t < (int)(sizeof(SamplePlan) / 4)) reinterpret_cast<uint32_t*>(&L)[t] = reinterpret_cast<const uint32_t*>(&R.plan)[t];
+  const SamplePlan L = R.plan;
   const float2 range = row_range(P, row);
   if (!live(range.x)) {
     if (t == 0) {
@@ -805,108 +803,99 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
     }
     return;
   }
-  const RowScale S(P, row, range);
-  const Settings C(P, row, S.greedy);
-  const bool fits = n <= (uint32_t)kMostCandidates;
-  __syncthreads();
-  if (t == 0) kept_m = L.m_before;
+  const RowScale S(range, G.t);
+  const Cuts C(G, S.greedy, P.vocab);
+  if (t == 0) {
+    kept_m = L.m_before;
+    answer[1] = L.total;
+  }
   uint64_t k_mass = L.k_mass, kept, key = 0;
-  if (fits) {
-    // ---- the candidates in order: thread t holds entries t PER' .. in `list`
+  if (n <= (uint32_t)kMostCandidates) {
+    // ---- the candidates in order: thread t holds entries t per .. t per + per - 1
     const bool one = n <= (uint32_t)kFinalThreads;
     const int per = one ? 1 : PER;
     int size = 64;
     while (size < (int)n) size <<= 1;
+    uint64_t entry[PER] = {};
     if (one) {
       if (t >= (int)n) mine = 0;
-      mine = sort_one(mine, size, list);
-      if (t < size) list[t] = mine;
-      __syncthreads();
+      entry[0] = sort_one(mine, size, list);
     } else {
       for (int i = t; i < size; i += kFinalThreads) list[i] = i < (int)n ? R.list[i] : 0;
       __syncthreads();
       sort_many(list, size);
+#pragma unroll
+      for (int k = 0; k < PER; k++) entry[k] = list[t * PER + k];   // (past the size: not used)
     }
-    // ---- their cumulative weights; an interval begins with the weight of all bins before it
+    // ---- their cumulative weights and ranks: of the candidates, plus what lies between their intervals
     uint64_t w[PER], sum = 0;
     int bins[PER];
 #pragma unroll
     for (int k = 0; k < PER; k++) {
-      const int i = t * per + k;
       bins[k] = -1;
-      if (k < per && i < (int)n) {
-        const float x = of_key((uint32_t)(list[i] >> 32));
+      w[k] = 0;
+      if (k < per && t * per + k < (int)n) {
+        const float x = of_key((uint32_t)(entry[k] >> 32));
         bins[k] = S.bin_of(S.z_of(x));
-        sum += S.mass_of(x);
+        w[k] = S.mass_of(x);
       }
-      w[k] = sum;
+      sum += w[k];
     }
-    uint64_t incl = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint64_t o = __shfl_up((unsigned long long)incl, d);
-      if (lane >= d) incl += o;
-    }
-    if (lane == 63) wave_sum[wave] = incl;
+    const uint64_t incl = wave_scan(sum);
+    if ((t & 63) == 63) wave_sum[wave] = incl;
     __syncthreads();
     uint64_t before = incl - sum;
-    for (int v = 0; v < wave; v++) before += wave_sum[v];
-    int own[PER];                       // the interval of each entry
+#pragma unroll
+    for (int v = 0; v < WAVES - 1; v++) before += v < wave ? wave_sum[v] : 0;
+    uint64_t gap[kCuts], inside = 0;
+    uint32_t rank_gap[kCuts], rank_inside = 0;
+#pragma unroll
+    for (int a = 0; a < kCuts; a++) {
+      gap[a] = L.before[a] - inside;
+      rank_gap[a] = L.rank_before[a] - rank_inside;
+      inside += L.upto[a] - L.before[a];
+      rank_inside += L.rank_upto[a] - L.rank_before[a];
+    }
+    uint64_t full[PER];                 // weight up to and including an entry
+    uint32_t rank[PER];
 #pragma unroll
     for (int k = 0; k < PER; k++) {
-      own[k] = -1;
-      const int i = t * per + k;
-      if (bins[k] < 0) continue;
-      for (int a = 0; a < L.n; a++)
-        if (bins[k] >= L.lo[a] && bins[k] <= L.hi[a]) own[k] = a;
-      // the first of its interval: the one before lies in an earlier interval
-      const int prev = i > 0 ? S.bin_of(S.z_of(of_key((uint32_t)(list[i - 1] >> 32)))) : -1;
-      if (prev < L.lo[own[k]]) {
-        start[own[k]] = i;
-        start_sum[own[k]] = before + (k > 0 ? w[k - 1] : 0);
-      }
-    }
-    __syncthreads();
-    uint64_t full[PER];
+      before += w[k];
+      full[k] = before + gap[0];
+      rank[k] = rank_gap[0];
 #pragma unroll
-    for (int k = 0; k < PER; k++) {
-      const int i = t * per + k;
-      full[k] = 0;
-      if (own[k] < 0) continue;
-      full[k] = L.before[own[k]] + (before + w[k] - start_sum[own[k]]);
-      cum[i] = full[k];
+      for (int a = 1; a < kCuts; a++)
+        if (bins[k] >= L.lo[a]) {
+          full[k] = before + gap[a];
+          rank[k] = rank_gap[a];
+        }
+      rank[k] += (uint32_t)(t * per + k) + 1;
     }
-    __syncthreads();
-    auto before_of = [&](int k) {       // the weight before entry k of this thread
-      const int i = t * per + k;
-      return i == start[own[k]] ? L.before[own[k]] : cum[i - 1];
+    // the entry with which the weight reaches `want`
+    auto reaches = [&](int k, uint64_t want) __attribute__((always_inline)) {
+      return bins[k] >= 0 && full[k] >= want && full[k] - w[k] < want;
     };
     // ---- top-k
     if (L.k_cut) {
 #pragma unroll
       for (int k = 0; k < PER; k++)
-        if (own[k] >= 0 && L.rank_before[own[k]] + (uint32_t)(t * per + k - start[own[k]]) + 1 == L.k) answer[0] = full[k];
+        if (bins[k] >= 0 && rank[k] == L.k) answer[0] = full[k];
       __syncthreads();
       k_mass = answer[0];
     }
     kept = k_mass;
     // ---- top-p and min-p
-    const double p_target = C.p * (double)k_mass;
     if (C.use_p) {
-      if (t == 0) answer[1] = L.total;
-      __syncthreads();
+      const uint64_t want = C.reach(k_mass);
 #pragma unroll
       for (int k = 0; k < PER; k++)
-        if (own[k] >= 0 && (double)full[k] >= p_target) {
-          const uint64_t b = before_of(k);
-          if (b == 0 || (double)b < p_target) answer[1] = full[k];
-        }
+        if (reaches(k, want)) answer[1] = full[k];
     }
     if (C.use_m) {
 #pragma unroll
       for (int k = 0; k < PER; k++)
-        if (own[k] >= 0) {
-          const double z = S.z_of(of_key((uint32_t)(list[t * per + k] >> 32)));
+        if (bins[k] >= 0) {
+          const double z = S.z_of(of_key((uint32_t)(entry[k] >> 32)));
           if (z == 0.0 || S.weight_of(z) >= C.min_p) atomicMax(&kept_m, (unsigned long long)full[k]);
         }
     }
@@ -917,32 +906,31 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
       if (C.use_m) kept = min(kept, C.min_p > 1.0 ? (uint64_t)kUnit : (uint64_t)kept_m);
     }
     // ---- the token
-    const double target = C.u * (double)kept;
+    const uint64_t want = C.target(kept);
 #pragma unroll
     for (int k = 0; k < PER; k++)
-      if (own[k] >= 0 && (double)full[k] > target) {
-        const uint64_t b = before_of(k);
-        if (b == 0 || (double)b <= target) answer[2] = list[t * per + k];
-      }
+      if (reaches(k, want)) answer[2] = entry[k];
     __syncthreads();
     key = answer[2];
   } else {
+    const SamplePlan& Q = R.plan;       // (picked from by number)
     // the interval that an answer lies in
-    auto holding = [&](double target, bool above) {
+    auto holding = [&](uint64_t want) {
       int a = 0;
-      while (a + 1 < L.n && !(above ? (double)L.upto[a] > target : (double)L.upto[a] >= target)) a++;
+      while (a + 1 < Q.n && Q.upto[a] < want) a++;
       return a;
     };
     uint32_t* dn = reinterpret_cast<uint32_t*>(list);
+    __syncthreads();
     if (L.k_cut) {
       int a = 0;
-      while (a + 1 < L.n && L.rank_before[a + 1] < L.k) a++;
-      k_mass = search_digits<T>(P, row, S, L, a, 0, L.k, 0.0, cum, dn, answer).mass;
+      while (a + 1 < Q.n && Q.rank_before[a + 1] < Q.k) a++;
+      k_mass = search_digits<T>(P, row, S, Q, a, Q.k, 0, digits, dn, answer).mass;
     }
     kept = k_mass;
     if (C.use_p) {
-      const double target = C.p * (double)k_mass;
-      kept = min(kept, search_digits<T>(P, row, S, L, holding(target, false), 1, 0, target, cum, dn, answer).mass);
+      const uint64_t want = C.reach(k_mass);
+      kept = min(kept, search_digits<T>(P, row, S, Q, holding(want), 0, want, digits, dn, answer).mass);
     }
     if (C.use_m) {
       // every logit from min-p's interval on that passes
@@ -961,8 +949,8 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
       __syncthreads();
       kept = min(kept, C.min_p > 1.0 ? (uint64_t)kUnit : (uint64_t)kept_m);
     }
-    const double target = C.u * (double)kept;
-    key = search_digits<T>(P, row, S, L, holding(target, true), 2, 0, target, cum, dn, answer).key;
+    const uint64_t want = C.target(kept);
+    key = search_digits<T>(P, row, S, Q, holding(want), 0, want, digits, dn, answer).key;
   }
   if (t == 0) {
     P.tokens[row] = (int64_t)(uint32_t)~(uint32_t)key;
