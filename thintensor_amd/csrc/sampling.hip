@@ -221,24 +221,26 @@ __device__ __forceinline__ float2 wave_range(float hi, float lo) {
   return make_float2(hi, lo);
 }
 
-// The row's range from its chunks'; by every wave, all lanes.
-__device__ __forceinline__ float2 row_range(const SampleParams& P, int row) {
-  const float2* r = P.rows[row].range;
-  const float inf = __builtin_bit_cast(float, 0x7f800000u);
+// The row's range from its chunks', by every wave, all lanes: requested first of what a kernel reads, since
+// loads arrive in order.
+struct RowRange {
   float2 v[kMostChunks / 64];
+  __device__ RowRange(const SampleParams& P, int row) {
+    const float2* r = P.rows[row].range;
+    const float inf = __builtin_bit_cast(float, 0x7f800000u);
 #pragma unroll
-  for (int k = 0; k < kMostChunks / 64; k++) {
-    const int c = (threadIdx.x & 63) + 64 * k;
-    v[k] = c < P.chunks ? r[c] : make_float2(-inf, inf);
+    for (int k = 0; k < kMostChunks / 64; k++) {
+      const int c = (threadIdx.x & 63) + 64 * k;
+      v[k] = c < P.chunks ? r[c] : make_float2(-inf, inf);
+    }
   }
-  float hi = -inf, lo = inf;
+  __device__ float2 get() const {
+    float2 w = v[0];
 #pragma unroll
-  for (int k = 0; k < kMostChunks / 64; k++) {
-    hi = fmaxf(hi, v[k].x);
-    lo = fminf(lo, v[k].y);
+    for (int k = 1; k < kMostChunks / 64; k++) w = make_float2(fmaxf(w.x, v[k].x), fminf(w.y, v[k].y));
+    return wave_range(w.x, w.y);
   }
-  return wave_range(hi, lo);
-}
+};
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleParams P) {
@@ -280,15 +282,15 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleParams P
   __shared__ __attribute__((aligned(16))) uint32_t count[kBins];
   const int end = min(P.vocab, (c + 1) * P.bin_chunk);
   int i = c * P.bin_chunk + 8 * (int)threadIdx.x;
+  const RowRange chunks(P, row);
   float x[8];
   if (i < end) logits8<T>(P, row, i, x);
   const RowSettings G(P, row);
-  const float2 range = row_range(P, row);
   for (int b = threadIdx.x; b < kBins / 2; b += kBinThreads) {
     reinterpret_cast<ulonglong2*>(mass)[b] = make_ulonglong2(0, 0);
     reinterpret_cast<uint2*>(count)[b] = make_uint2(0, 0);
   }
-  const RowScale S(range, G.t);
+  const RowScale S(chunks.get(), G.t);
   const bool counts = G.top_k(S.greedy, P.vocab) != 0;
   uint32_t far = 0;                     // of the last bin
   __syncthreads();
@@ -469,14 +471,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams
   __shared__ uint32_t n_found, base;
   const int end = min(P.vocab, (c + 1) * P.chunk);
   int i = c * P.chunk + 8 * (int)threadIdx.x;
+  const RowRange chunks(P, row);
+  BinPart part;
+  part.load(R);
   float x[kDeep][8];
 #pragma unroll
   for (int k = 0; k < kDeep; k++)
     if (i + k * kStep < end) logits8<T>(P, row, i + k * kStep, x[k]);
   const RowSettings G(P, row);
-  BinPart part;
-  part.load(R);
-  const float2 range = row_range(P, row);
+  const float2 range = chunks.get();
   if (!live(range.x)) return;
   if (threadIdx.x == 0) n_found = 0;
   part.sum(U.bins);
@@ -629,8 +632,8 @@ __device__ __forceinline__ uint64_t xor64(uint64_t v) {
   return ((uint64_t)hi << 32) | lo;
 }
 
-// Sorts up to 1024 keys, one per thread, largest first: n is a power of two, 64 at least, and threads
-// past it only meet the barriers.  Bitonic: partners within a wave by lane exchange, others in LDS.
+// Sorts n keys, one per thread, largest first: n is a power of two, 64 to 1024, and the threads past it have
+// left.  Bitonic: partners within a wave by lane exchange, others in LDS.
 __device__ uint64_t sort_one(uint64_t v, int n, uint64_t* buf) {
   const int t = threadIdx.x;
   auto keep = [&](uint64_t mine, uint64_t other, int j, int k) {
@@ -645,18 +648,16 @@ __device__ uint64_t sort_one(uint64_t v, int n, uint64_t* buf) {
     if (from >= 2) v = keep(v, xor64<2>(v), 2, k);
     v = keep(v, xor64<1>(v), 1, k);
   };
-  const bool on = t < n;                // whole waves
-  if (on)
-    for (int k = 2; k <= 64; k <<= 1) within(k, k >> 1);
+  for (int k = 2; k <= 64; k <<= 1) within(k, k >> 1);
   for (int k = 128; k <= n; k <<= 1) {
     for (int j = k >> 1; j >= 64; j >>= 1) {
-      if (on) buf[t] = v;
+      buf[t] = v;
       __syncthreads();
-      const uint64_t o = on ? buf[t ^ j] : 0;
+      const uint64_t o = buf[t ^ j];
       __syncthreads();
-      if (on) v = keep(v, o, j, k);
+      v = keep(v, o, j, k);
     }
-    if (on) within(k, 32);
+    within(k, 32);
   }
   return v;
 }
@@ -791,17 +792,28 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
   __shared__ __attribute__((aligned(16))) uint64_t wave_sum[WAVES];
   __shared__ uint64_t answer[4];
   __shared__ unsigned long long kept_m;
+  const RowRange chunks(P, row);
+  // the plan and the number of candidates, a word per lane
+  constexpr int WORDS = sizeof(SamplePlan) / 4;
+  static_assert(WORDS < 64 && offsetof(SampleRow, candidates) == offsetof(SampleRow, plan) + sizeof(SamplePlan), "one load of a wave");
+  const uint32_t words = reinterpret_cast<const uint32_t*>(&R.plan)[min(t & 63, WORDS)];
   uint64_t mine = R.list[t];            // (used where the list is that long)
   const RowSettings G(P, row);
-  const uint32_t n = R.candidates;
-  const SamplePlan L = R.plan;
-  const float2 range = row_range(P, row);
+  const float2 range = chunks.get();
   if (!live(range.x)) {
     if (t == 0) {
       P.tokens[row] = -1;
       if (P.probs) P.probs[row] = 0.0f;
     }
     return;
+  }
+  const uint32_t n = __builtin_amdgcn_readlane(words, WORDS);
+  SamplePlan L;
+  {
+    uint32_t w[WORDS];
+#pragma unroll
+    for (int k = 0; k < WORDS; k++) w[k] = __builtin_amdgcn_readlane(words, k);
+    __builtin_memcpy(&L, w, sizeof(L));
   }
   const RowScale S(range, G.t);
   const Cuts C(G, S.greedy, P.vocab);
@@ -816,6 +828,7 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
     const int per = one ? 1 : PER;
     int size = 64;
     while (size < (int)n) size <<= 1;
+    if (one && 64 * wave >= size) return;   // (a barrier waits for the waves that are left)
     uint64_t entry[PER] = {};
     if (one) {
       if (t >= (int)n) mine = 0;
