@@ -313,17 +313,23 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleParams P
     }
     if (counts) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        if (!live(x[e])) continue;
-        if (b[e] < kBins - 1) atomicAdd(&count[b[e]], 1u);
-        else far++;
-      }
+      for (int e = 0; e < 8; e++) far += b[e] == kBins - 1 && live(x[e]);
     }
     const int next = i + 8 * kBinThreads;
     if (next < end) logits8<T>(P, row, next, x);
+    // (what is not live lies in the last bin)
+    if (counts) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      if (m[e]) atomicAdd((unsigned long long*)&mass[b[e]], (unsigned long long)m[e]);
+      for (int e = 0; e < 8; e++) {
+        if (b[e] == kBins - 1) continue;
+        atomicAdd(&count[b[e]], 1u);
+        atomicAdd((unsigned long long*)&mass[b[e]], (unsigned long long)m[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (m[e]) atomicAdd((unsigned long long*)&mass[b[e]], (unsigned long long)m[e]);
+      }
     }
     i = next;
   }
@@ -544,32 +550,29 @@ __global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams
         lo[a - 1] = kBins;
       }
     }
-  if (c == 0 && threadIdx.x == 0) {     // the plan, for the last step
+  if (c == 0 && threadIdx.x < kCuts) {  // the plan, for the last step: an interval per lane, empty ones last
     SamplePlan& L = R.plan;
-    int n = 0;
-#pragma unroll
-    for (int a = 0; a < kCuts; a++)
-      if (lo[a] < kBins) {
-        L.lo[n] = lo[a];
-        L.hi[n] = hi[a];
-        L.before[n] = B.mass(lo[a] - 1);
-        L.rank_before[n] = B.count(lo[a] - 1);
-        L.upto[n] = B.mass(hi[a]);
-        L.rank_upto[n] = B.count(hi[a]);
-        n++;
-      }
-    L.n = n;
-    for (; n < kCuts; n++) {
-      L.lo[n] = kBins;
-      L.hi[n] = -1;
-      L.before[n] = L.upto[n] = 0;
-      L.rank_before[n] = L.rank_upto[n] = 0;
+    const int a = (int)threadIdx.x;
+    const int l = a == 0 ? lo[0] : a == 1 ? lo[1] : a == 2 ? lo[2] : lo[3];
+    const int h = a == 0 ? hi[0] : a == 1 ? hi[1] : a == 2 ? hi[2] : hi[3];
+    const bool used = l < kBins;
+    const uint32_t all = (uint32_t)__builtin_amdgcn_ballot_w64(used), below = (1u << a) - 1;
+    const int n = __builtin_popcount(all);
+    const int at = used ? __builtin_popcount(all & below) : n + __builtin_popcount(~all & below);
+    L.lo[at] = l;
+    L.hi[at] = used ? h : -1;
+    L.before[at] = used ? B.mass(l - 1) : 0;
+    L.upto[at] = used ? B.mass(h) : 0;
+    L.rank_before[at] = used ? B.count(l - 1) : 0;
+    L.rank_upto[at] = used ? B.count(h) : 0;
+    if (a == 0) {
+      L.n = n;
+      L.k_cut = k_bin >= 0;
+      L.k = C.k;
+      L.k_mass = k_hi;
+      L.total = total;
+      L.m_before = m_before;
     }
-    L.k_cut = k_bin >= 0;
-    L.k = C.k;
-    L.k_mass = k_hi;
-    L.total = total;
-    L.m_before = m_before;
   }
   __syncthreads();                      // the histogram is not read any more
   // ---- this chunk's candidates
@@ -633,9 +636,10 @@ __device__ __forceinline__ uint64_t xor64(uint64_t v) {
 }
 
 // Sorts n keys, one per thread, largest first: n is a power of two, 64 to 1024, and the threads past it have
-// left.  Bitonic: partners within a wave by lane exchange, others in LDS.
-__device__ uint64_t sort_one(uint64_t v, int n, uint64_t* buf) {
+// left.  Bitonic: partners within a wave by lane exchange, others in LDS, where two halves of `buf` take turns.
+__device__ uint64_t sort_one(uint64_t v, int n, uint64_t* half) {
   const int t = threadIdx.x;
+  uint64_t* buf = half;
   auto keep = [&](uint64_t mine, uint64_t other, int j, int k) {
     const bool larger = ((t & j) == 0) == ((t & k) == 0);   // this thread keeps the larger one
     return (mine < other) == larger ? other : mine;
@@ -652,10 +656,9 @@ __device__ uint64_t sort_one(uint64_t v, int n, uint64_t* buf) {
   for (int k = 128; k <= n; k <<= 1) {
     for (int j = k >> 1; j >= 64; j >>= 1) {
       buf[t] = v;
-      __syncthreads();
-      const uint64_t o = buf[t ^ j];
-      __syncthreads();
-      v = keep(v, o, j, k);
+      lds_barrier();
+      v = keep(v, buf[t ^ j], j, k);
+      buf = buf == half ? half + kFinalThreads : half;
     }
     within(k, 32);
   }
