@@ -23,7 +23,8 @@
 // join: 4.9 TB/s.  A tile of 32 tokens costs a wave about 290 vector instructions, two thirds of them to
 // form operands from codes (shift, and-or and one packed fma for two values), and 28 matrix instructions;
 // the vector units are busy two thirds of the time, the matrix cores a fifth.  Short rows are bound by
-// their round trips: 575 tokens of 8 x 64 6.5 us, of which a launch and one tile are 3.8.
+// their round trips: 575 tokens of 8 x 64 6.0 us (6.1 with the first tile requested after q is used), of which
+// a launch and one tile are 3.8.
 #include "kv_int4.h"
 #include "tt_common.h"
 
@@ -207,13 +208,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   __shared__ __attribute__((aligned(16))) float o_s[kWaves][16][OS];
   __shared__ float m_s[kWaves][16], l_s[kWaves][16];
 
-  const Visible vis(P, row);
-  const int nt = vis.tiles(), share = vis.share(P.splits);
-  const int first_tile = split * share;
-  if (first_tile >= nt && !(nt == 0 && split == 0)) return;
-  const int end_tile = min(first_tile + share, nt);
-
-  // ---- q as f16 operands: element e of step i is dim quad D/4 + 8 i + (e/2) + 4 (e%2)
+  // q is requested before the row's length is known, the first tile before q is used.
+  // Element e of step i is dim quad D/4 + 8 i + (e/2) + 4 (e%2)
   const int hq = h0 + min(n, heads - 1);
   uint32_t qw[KW * 4];                         // pairs of elements as they are stored
   {
@@ -230,6 +226,25 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
       for (int i = 0; i < KW * 4; i++) qw[i] = q[2 * i] | ((uint32_t)q[2 * i + 1] << 16);
     }
   }
+  const Visible vis(P, row);
+  const int nt = vis.tiles(), share = vis.share(P.splits);
+  const int first_tile = split * share;
+  if (first_tile >= nt && !(nt == 0 && split == 0)) return;
+  const int end_tile = min(first_tile + share, nt);
+
+  const char* kc = reinterpret_cast<const char*>(P.c.k_codes) + 4 * (row * P.c.kc_seq + kvh * P.c.kc_head);
+  const char* ks = reinterpret_cast<const char*>(P.c.k_scales) + 2 * (row * P.c.ks_seq + kvh * P.c.ks_head);
+  const char* vc = reinterpret_cast<const char*>(P.c.v_codes) + 4 * (row * P.c.vc_seq + kvh * P.c.vc_head);
+  const char* vs = reinterpret_cast<const char*>(P.c.v_scales) + 2 * (row * P.c.vs_seq + kvh * P.c.vs_head);
+  Tile<D, G> tile;
+  tile.place(n, quad);
+  // (a wave without a tile, of a row without one too, requests one that the cache has: a wait for q behind a
+  // branch would wait for the tile as well)
+  int i = first_tile + wave, t0 = vis.tile(max(min(i, end_tile - 1), 0)) * kTile;
+  tile.load_k(kc, ks, t0);
+  tile.load_v(vc, vs, t0);
+
+  // ---- q as f16 operands
   auto qf = [&](int i) __attribute__((always_inline)) {
     return (i & 1) ? hi_f32<T>(qw[i / 2]) : lo_f32<T>(qw[i / 2]);
   };
@@ -275,11 +290,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     qm = __builtin_bit_cast(h8_t, r);
   }
 
-  const char* kc = reinterpret_cast<const char*>(P.c.k_codes) + 4 * (row * P.c.kc_seq + kvh * P.c.kc_head);
-  const char* ks = reinterpret_cast<const char*>(P.c.k_scales) + 2 * (row * P.c.ks_seq + kvh * P.c.ks_head);
-  const char* vc = reinterpret_cast<const char*>(P.c.v_codes) + 4 * (row * P.c.vc_seq + kvh * P.c.vc_head);
-  const char* vs = reinterpret_cast<const char*>(P.c.v_scales) + 2 * (row * P.c.vs_seq + kvh * P.c.vs_head);
-
   const float ninf = __builtin_bit_cast(float, 0xff800000u);
   f4_t o[VT], om = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -289,8 +299,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   uint32_t mask = 0x03c003c0u;
   asm volatile("" : "+v"(mask));
 
-  Tile<D, G> tile;
-  tile.place(n, quad);
   auto step = [&](int t0, int next) __attribute__((always_inline)) {
     // ---- scores: register e of half h is token t0 + 8 quad + 4 h + e of head n
     f4_t sc[2];
@@ -384,16 +392,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
 
   // K of the next tile is requested as soon as the scores have taken the present one's, V after the
   // products with it (past the end: the last tile once more)
-  int i = first_tile + wave;
-  if (i < end_tile) {
-    int t0 = vis.tile(i) * kTile;
-    tile.load_k(kc, ks, t0);
-    tile.load_v(vc, vs, t0);
-    for (; i < end_tile; i += kWaves) {
-      const int next = vis.tile(min(i + kWaves, end_tile - 1)) * kTile;
-      step(t0, next);
-      t0 = next;
-    }
+  for (; i < end_tile; i += kWaves) {
+    const int next = vis.tile(min(i + kWaves, end_tile - 1)) * kTile;
+    step(t0, next);
+    t0 = next;
   }
 
   // ---- join the waves.  The groups' sums of p m sit in the column's lanes of quads 0 and 1.

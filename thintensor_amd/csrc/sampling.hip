@@ -12,12 +12,12 @@
 // Weights are exp(-z) in units of 2^-43, 64-bit integers: sums have no order, and a total is exact to
 // 2^-43 of the largest weight per token, far below what tells two cumulative sums apart.
 //
-// Four launches: one row of 128256 fp16 logits takes 20.3 us (2.7, 5.5, 7.2 and 5.6 for the steps), 64 rows
-// of 152064 in binary32 53 us (7.9, 16.4, 18.4, 10.7): every pass over the 39 MB takes 8 us at the 5 TB/s that
-// the memory gives, the second step adds its round trips and the weights (7 us of vector instructions), the
-// third the round trips before its candidates are known, the last one sorts.  A row that leaves more than
-// kMostCandidates candidates -- thousands of equal logits at a border -- is searched digit by digit by its
-// one workgroup (128256 equal logits: 0.17 ms a search, up to three searches).
+// Four launches: one row of 128256 fp16 logits takes 16.5 us (2.7, 5.1, 5.6 and 4.1 for the steps: a launch and
+// one round trip to memory are 3 of each), 64 rows of 152064 in binary32 49 us (7.9, 16.2, 16.3, 9.8): every
+// pass over the 39 MB takes 8 us at the 5 TB/s that the memory gives, the weights 8 us of vector instructions
+// beside it, the third step its round trips before the candidates are known, the last one sorts.  A row that
+// leaves more than kMostCandidates candidates -- thousands of equal logits at a border -- is searched digit by
+// digit by its one workgroup (128256 equal logits: 0.17 ms a search, up to three searches).
 #include "tt_abi_internal.h"
 #include "tt_common.h"
 
@@ -28,8 +28,8 @@ constexpr double kReach = 64.0;         // z that the bins reach to at most
 constexpr double kUnit = 8796093022208.0;   // 2^43
 constexpr int kThreads = 256;           // of a chunk's workgroup
 constexpr int kStep = 8 * kThreads;     // logits that it takes at a time
-// of step 2, where fewer workgroups leave fewer bins to add (8 rows of 201088: 256 threads 30.5 us a call,
-// 512 27.5, 1024 27.1; 64 rows of 152064: 62, 61, 68)
+// of step 2, where fewer workgroups leave fewer bins to add (one row of 128256, 8 of 201088, 64 of 152064:
+// 256 threads 17.0, 22.7 and 50.9 us a call, 512 16.5, 22.3 and 49.2, 1024 17.2, 21.7 and 50.1)
 constexpr int kBinThreads = 512;
 constexpr int kMostChunks = 256;
 constexpr int kMostCandidates = 4096;   // that the last step sorts in LDS
@@ -461,8 +461,7 @@ struct Cuts {
   __device__ uint64_t target(uint64_t mass) const { return (uint64_t)(u * (double)mass) + 1; }
 };
 
-// Steps of a chunk on their way at a time: more take registers that keep four workgroups from a CU (64 rows of
-// 152064: two 18.4 us, three 19.5, four 21.9).
+// Steps of a chunk on their way at a time (64 rows of 152064: two 16.5 us, three 16.9, four 17.6).
 constexpr int kDeep = 2;
 
 template <typename T>
