@@ -1710,26 +1710,27 @@ class HipDecodeBackend:
         Settings are per row (float32, ``top_k`` int32) or None; a temperature of 0 is greedy, a top_k
         of 0 keeps all.  ``probs`` (float32 [rows]) takes the token's share of the kept weight.  Logits
         of -inf and NaN are never taken; a row without others gives token -1 and share 0."""
-        if logits.ndim != 2 or logits.stride(1) != 1 or logits.shape[1] == 0:
+        shape, stride = logits.shape, logits.stride()
+        if len(shape) != 2 or stride[1] != 1 or shape[1] == 0:
             raise ValueError("sample_rows takes logits [rows, vocab], contiguous in the vocabulary")
-        rows, vocab = logits.shape
+        rows, vocab = shape
         if tokens.dtype != torch.int64 or tokens.numel() != rows or not tokens.is_contiguous():
             raise ValueError("sample_rows: tokens must be a contiguous int64 tensor, one per row")
-        ptrs = []
-        for name, t in (("uniforms", uniforms), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
-                        ("min_p", min_p), ("probs", probs)):
+
+        def per_row(t: torch.Tensor | None, name: str, dtype: torch.dtype = torch.float32):
             if t is None:
-                ptrs.append(None)
-                continue
-            if t.dtype != (torch.int32 if name == "top_k" else torch.float32) or t.numel() != rows or not t.is_contiguous():
-                raise ValueError(f"sample_rows: {name} must be contiguous {'int32' if name == 'top_k' else 'float32'}, one per row")
-            ptrs.append(t.data_ptr())
+                return None
+            if t.dtype != dtype or t.numel() != rows or not t.is_contiguous():
+                raise ValueError(f"sample_rows: {name} must be contiguous {str(dtype)[6:]}, one per row")
+            return t.data_ptr()
+
         gpu = _gpu_of(logits, uniforms, tokens, temperature, top_k, top_p, min_p, probs)
         need = self.lib.tt_sample_rows_scratch_bytes(rows, vocab)
         scratch = torch.empty(need, device=logits.device, dtype=torch.uint8)
         rc = _on_gpu(gpu, self.lib.tt_sample_rows,
-                     logits.data_ptr(), logits.stride(0), _code(logits, "sample_rows"), rows, vocab, *ptrs[:5],
-                     scratch.data_ptr(), need, tokens.data_ptr(), ptrs[5])
+                     logits.data_ptr(), stride[0], _code(logits, "sample_rows"), rows, vocab, per_row(uniforms, "uniforms"),
+                     per_row(temperature, "temperature"), per_row(top_k, "top_k", torch.int32), per_row(top_p, "top_p"),
+                     per_row(min_p, "min_p"), scratch.data_ptr(), need, tokens.data_ptr(), per_row(probs, "probs"))
         if rc:
             _lib.check(rc, "sample_rows")
         return tokens
