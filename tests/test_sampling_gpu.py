@@ -124,6 +124,18 @@ def test_sample_temperatures_far_from_one(backend, device):
     _check(backend, x * 1e-30, u, torch.tensor([1.0, 1e-28, 1e-30, 1e-32, 1e30, 0.0, 1e-38]), 500, 0.9)
 
 
+@pytest.mark.parametrize("vocab", [30, 3126, 20000])
+@pytest.mark.parametrize("temperature", [1e3, 1e30])
+def test_sample_min_p_at_high_temperatures(backend, device, vocab, temperature):
+    """Weights that are all 1, or nearly: a logit passes min-p by what its weight rounds to, however many
+    bins of the row that is."""
+    x, u, _ = _logits(device, 12, vocab, "f32", vocab)
+    top_k = torch.tensor([0, 7, vocab - 1])[torch.arange(12) % 3]
+    for min_p in (1.0, 1.0 - 2.0 ** -24, 0.999, 0.5, 2.0):
+        _check(backend, x, u, temperature, None, None, min_p)
+        _check(backend, x, u, temperature, top_k, 0.7, min_p)
+
+
 @pytest.mark.parametrize("stride", [0, 1, 3, 8])
 def test_sample_row_strides(backend, device, stride):
     """Rows inside a wider buffer, from an odd first element; many rows at once."""

@@ -452,6 +452,13 @@ struct Cuts {
     use_m = G.min_p > 0.0f;
     min_p = (double)G.min_p;
   }
+  // The bins that min-p's last logit can lie in: around -log(min_p), which its rounding and that of a weight
+  // move by less than 2^-48 -- many bins where the temperature is high.
+  __device__ void min_p_bins(const RowScale& S, int* lo, int* hi) const {
+    const double z = S.greedy || !(min_p < 1.0) ? 0.0 : -log(min_p);
+    *lo = __builtin_amdgcn_readfirstlane(max(0, S.bin_of(__builtin_fmax(z - 0x1p-48, 0.0)) - 1));
+    *hi = __builtin_amdgcn_readfirstlane(min(kBins - 1, S.bin_of(z + 0x1p-48) + 1));
+  }
   // The cumulative weight that the last of top-p's share reaches first, and the one that the token does:
   // integers, so that every step compares alike.  Both are at most `mass` (p and u are 1 - 2^-24 at most).
   __device__ uint64_t reach(uint64_t mass) const {
@@ -514,9 +521,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_gather_kernel(SampleParams
     if (p_hi < kBins - 1) kept_hi = min(kept_hi, B.mass(p_hi));
   }
   if (C.use_m) {
-    const int b = __builtin_amdgcn_readfirstlane(S.greedy || !(C.min_p < 1.0) ? 0 : S.bin_of(-log(C.min_p)));
-    m_lo = max(0, b - 1);
-    m_hi = min(kBins - 1, b + 1);
+    C.min_p_bins(S, &m_lo, &m_hi);
     m_before = B.mass(m_lo - 1);
     kept_lo = min(kept_lo, m_before);
     kept_hi = min(kept_hi, B.mass(m_hi));
@@ -950,8 +955,8 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
     if (C.use_m) {
       // every logit from min-p's interval on that passes
       uint64_t some = 0;
-      const int b = S.greedy || !(C.min_p < 1.0) ? 0 : S.bin_of(-log(C.min_p));
-      const int m_lo = max(0, b - 1), m_hi = min(kBins - 1, b + 1);
+      int m_lo, m_hi;
+      C.min_p_bins(S, &m_lo, &m_hi);
       for (int i = t; i < P.vocab; i += kFinalThreads) {
         const float x = logit<T>(P, row, i);
         if (!live(x)) continue;
