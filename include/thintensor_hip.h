@@ -806,7 +806,8 @@ int64_t tt_int4_cache_size(void); /* sizeof(tt_int4_cache), for bindings */
  * count.  Tokens that would lie before position 0 or past the capacity are left out.  A group's m
  * is its minimum rounded to fp16 (limited to the finite values), s the smallest value of seven
  * significant bits (a multiple of 2^-24, at most 4064) with 15 s >= maximum - m, and codes are
- * (x - m) / s rounded to the nearest, ties to even, limited to 0 .. 15, all as if in exact
+ * (x - m) / s rounded to the nearest, ties to even, limited to 0 .. 15; the differences are those of
+ * binary64 (exact where their operands lie within 2^28 of each other), the rest is as if in exact
  * arithmetic.  A group that holds an infinity or a NaN reads as NaN.  Strides of rows, tokens and
  * heads are free; sequences and heads of the cache must not share memory here.  At most 2^26 tokens of a row. */
 int tt_kv_append_int4(const tt_int4_cache* cache, const void* k, int64_t k_row, int64_t k_token, int64_t k_head,

@@ -8,7 +8,7 @@
 //   * q is scaled by a power of two per head (its largest element to [2^7, 2^8)), which rounds only
 //     what lies 2^-31 below that element; a group's sum of q goes in as three f16 parts;
 //   * p is split into an f16 and the f16 of what that leaves, so a weight is off by 2^-21 of itself or
-//     2^-31 of the largest.
+//     2^-31 of the largest; the two sums of an output are rounded each, by 2^-24 of a group's range.
 // Scores come out as rows = tokens, columns = query heads: a lane holds eight consecutive tokens of
 // one head, which is the operand that the product with V takes, so p never leaves its registers.  The
 // product with V is formed transposed (rows = dims, columns = heads), so that a head's running

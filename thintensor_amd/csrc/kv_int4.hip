@@ -30,8 +30,8 @@ struct KvRowsParams {
   int tokens, vec;         // vec: eight elements of k and v start on 16-byte boundaries
 };
 
-// A group's step, and codes, are decided in binary64, which costs what binary32 does here and where
-// hi - m, x - m and what a code leaves of them are exact.
+// A group's step, and codes, are decided in binary64, which costs what binary32 does here and where hi - m and
+// x - m are exact (their operands within 2^28 of each other, always so for fp16) and decide ties.
 
 // The smallest s of seven significant bits with 15 s >= hi - m; the product with 1/15 only proposes it.
 __device__ __forceinline__ double group_step(float hi, float m) {
