@@ -16,15 +16,18 @@
 // one round trip to memory are 3 of each), 64 rows of 152064 in binary32 49 us (7.9, 16.2, 16.3, 9.8): every
 // pass over the 39 MB takes 8 us at the 5 TB/s that the memory gives, the weights 8 us of vector instructions
 // beside it, the third step its round trips before the candidates are known, the last one sorts.  A row that
-// leaves more than kMostCandidates candidates -- thousands of equal logits at a border -- is searched digit by
-// digit by its one workgroup (128256 equal logits: 0.17 ms a search, up to three searches).
+// leaves more than kMostCandidates candidates -- thousands of equal logits at a border, or 10^6 of nearly equal
+// weight -- is searched digit by digit by its one workgroup (128256 equal logits: 0.17 ms a search, up to
+// three searches).
 #include "tt_abi_internal.h"
 #include "tt_common.h"
 
 namespace tt {
 
-constexpr int kBins = 2048;             // the last one: weights below 2^-43, which count as 0
-constexpr double kReach = 64.0;         // z that the bins reach to at most
+constexpr int kBins = 2048;             // the last one: what lies past kReach
+// z that the bins reach to at most: further ones weigh 2^-44.7, less than half a unit.  (Four rows of 200000, half
+// of them masked by -65504: 48 us, 0.8 ms with bins to 64, which leave more candidates than are sorted.)
+constexpr double kReach = 31.0;
 constexpr double kUnit = 8796093022208.0;   // 2^43
 constexpr int kThreads = 256;           // of a chunk's workgroup
 constexpr int kStep = 8 * kThreads;     // logits that it takes at a time
@@ -453,11 +456,12 @@ struct Cuts {
     min_p = (double)G.min_p;
   }
   // The bins that min-p's last logit can lie in: around -log(min_p), which its rounding and that of a weight
-  // move by less than 2^-48 -- many bins where the temperature is high.
+  // move by less than 2^-48 of it and of 1 -- many bins where the temperature is high.
   __device__ void min_p_bins(const RowScale& S, int* lo, int* hi) const {
     const double z = S.greedy || !(min_p < 1.0) ? 0.0 : -log(min_p);
-    *lo = __builtin_amdgcn_readfirstlane(max(0, S.bin_of(__builtin_fmax(z - 0x1p-48, 0.0)) - 1));
-    *hi = __builtin_amdgcn_readfirstlane(min(kBins - 1, S.bin_of(z + 0x1p-48) + 1));
+    const double room = __builtin_fma(z, 0x1p-48, 0x1p-48);
+    *lo = __builtin_amdgcn_readfirstlane(S.bin_of(__builtin_fmax(z - room, 0.0)));
+    *hi = __builtin_amdgcn_readfirstlane(S.bin_of(z + room));
   }
   // The cumulative weight that the last of top-p's share reaches first, and the one that the token does:
   // integers, so that every step compares alike.  Both are at most `mass` (p and u are 1 - 2^-24 at most).
@@ -669,22 +673,56 @@ __device__ uint64_t sort_one(uint64_t v, int n, uint64_t* half) {
   return v;
 }
 
-// Sorts n (a power of two, at most kMostCandidates) keys in LDS, largest first.
-__device__ void sort_many(uint64_t* a, int n) {
-  for (int k = 2; k <= n; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < n / 2; i += kFinalThreads) {
-        const int l = 2 * i - (i & (j - 1)), r = l + j;
-        const uint64_t x = a[l], y = a[r];
-        const bool desc = (l & k) == 0;
-        if ((x < y) == desc) {
-          a[l] = y;
-          a[r] = x;
-        }
+// More keys: four per thread, n a power of two, 2048 at least, and the threads past it only meet the barriers.
+// Runs of k keys descend where key index & k is 0.
+struct SortKeys {
+  uint64_t v[4];
+  // a pair within the thread: the first keeps the larger one where `down`
+  __device__ __forceinline__ void pair(int i, int j, bool down) {
+    const uint64_t x = v[i], y = v[j];
+    const bool swap = (x < y) == down;
+    v[i] = swap ? y : x;
+    v[j] = swap ? x : y;
+  }
+  __device__ __forceinline__ void keep(int k, uint64_t other, bool larger) { v[k] = (v[k] < other) == larger ? other : v[k]; }
+  template <int M>
+  __device__ __forceinline__ void lanes(bool down) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) keep(k, xor64<M>(v[k]), !(threadIdx.x & M) == down);
+  }
+  __device__ void sort(int n, uint64_t* buf) {
+    const int t = threadIdx.x;
+    pair(0, 1, true);
+    pair(2, 3, false);
+    for (int k = 4; k <= n; k <<= 1) {
+      const bool down = !(t & (k >> 2));
+      for (int j = k >> 3; j >= 64; j >>= 1) {
+        ulonglong2* mine = reinterpret_cast<ulonglong2*>(buf + 4 * t);
+        mine[0] = make_ulonglong2(v[0], v[1]);
+        mine[1] = make_ulonglong2(v[2], v[3]);
+        __syncthreads();
+        const ulonglong2* other = reinterpret_cast<const ulonglong2*>(buf + 4 * (t ^ j));
+        const ulonglong2 a = other[0], b = other[1];
+        __syncthreads();
+        const bool larger = !(t & j) == down;
+        keep(0, a.x, larger);
+        keep(1, a.y, larger);
+        keep(2, b.x, larger);
+        keep(3, b.y, larger);
       }
-      __syncthreads();
+      if (k >= 256) lanes<32>(down);
+      if (k >= 128) lanes<16>(down);
+      if (k >= 64) lanes<8>(down);
+      if (k >= 32) lanes<4>(down);
+      if (k >= 16) lanes<2>(down);
+      if (k >= 8) lanes<1>(down);
+      pair(0, 2, down);
+      pair(1, 3, down);
+      pair(0, 1, down);
+      pair(2, 3, down);
     }
-}
+  }
+};
 
 struct Found {           // answer of a search
   uint64_t mass;         // cumulative weight up to and including the element
@@ -795,7 +833,9 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
   constexpr int PER = kMostCandidates / kFinalThreads, WAVES = kFinalThreads / 64;
   const int row = blockIdx.x, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   SampleRow& R = P.rows[row];
-  __shared__ uint64_t list[kMostCandidates], digits[256];
+  static_assert(PER == 4, "keys of a thread");
+  __shared__ __attribute__((aligned(16))) uint64_t list[kMostCandidates];
+  __shared__ uint64_t digits[256];
   __shared__ __attribute__((aligned(16))) uint64_t wave_sum[WAVES];
   __shared__ uint64_t answer[4];
   __shared__ unsigned long long kept_m;
@@ -841,11 +881,15 @@ __global__ __launch_bounds__(kFinalThreads) void sample_final_kernel(SampleParam
       if (t >= (int)n) mine = 0;
       entry[0] = sort_one(mine, size, list);
     } else {
-      for (int i = t; i < size; i += kFinalThreads) list[i] = i < (int)n ? R.list[i] : 0;
-      __syncthreads();
-      sort_many(list, size);
+      SortKeys keys;
+      const ulonglong2* p = reinterpret_cast<const ulonglong2*>(R.list + PER * t);
+      const ulonglong2 x = p[0], y = p[1];
+      keys.v[0] = x.x; keys.v[1] = x.y; keys.v[2] = y.x; keys.v[3] = y.y;
 #pragma unroll
-      for (int k = 0; k < PER; k++) entry[k] = list[t * PER + k];   // (past the size: not used)
+      for (int k = 0; k < PER; k++) keys.v[k] = PER * t + k < (int)n ? keys.v[k] : 0;
+      keys.sort(size, list);
+#pragma unroll
+      for (int k = 0; k < PER; k++) entry[k] = keys.v[k];
     }
     // ---- their cumulative weights and ranks: of the candidates, plus what lies between their intervals
     uint64_t w[PER], sum = 0;
