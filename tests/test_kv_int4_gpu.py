@@ -233,6 +233,26 @@ def test_attention_windows(backend, device, window, first):
     _check_attention(cache, q, out, lengths, window, first, sinks)
 
 
+@pytest.mark.parametrize("dim,rows,kv_heads,heads", [(64, 64, 8, 24), (128, 64, 8, 8), (256, 70, 4, 16), (128, 33, 1, 48)])
+def test_attention_long_rows_in_large_batches(backend, device, dim, rows, kv_heads, heads):
+    """Batches that fill the chip by themselves: long rows are shared by workgroups, short ones are not, and a
+    row's result does not depend on where it stands."""
+    held, g = _filled(backend, device, 1, kv_heads, 36000, dim, 64, dim + rows, [36000])
+    cache = Int4KvCache(*[t.expand(rows, *t.shape[1:]) for t in (held.k_codes, held.k_scales, held.v_codes, held.v_scales)])
+    some = [36000, 0, 1, 8192, 8193, 16385, 32, 4096, 24577]
+    lengths = [some[b] if b < len(some) else 37 * b for b in range(rows)]
+    q = torch.randn((rows, heads, dim), generator=g, device=device).half()
+    n = torch.tensor(lengths, device=device, dtype=torch.int32)
+    out = torch.full_like(q, 5.0)
+    backend.gqa_attention_int4(q, cache, out, n)
+    for b in (0, 1, 2, 4, 5, 7, rows - 1):
+        _check_attention(held, q[b:b + 1], out[b:b + 1], lengths[b:b + 1])
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(rows)).to(device)
+    mixed = torch.empty_like(q)
+    backend.gqa_attention_int4(q[order].contiguous(), cache, mixed, n[order].contiguous())
+    assert torch.equal(mixed, out[order])
+
+
 @pytest.mark.parametrize("length", [1023, 4097, 20000])
 def test_attention_split(backend, device, length):
     """Lengths that several workgroups share, beside short ones, in one call; a bound on the length."""

@@ -38,6 +38,7 @@ constexpr int kTile = 32;          // tokens per step of a wave
 constexpr int kHeadBlock = 16;     // query heads per workgroup
 constexpr int kWaves = 4;
 constexpr int kMostSplits = 512;
+constexpr int kLongTiles = 256;
 // Weights are 2^7 exp(s - m), where m follows the running maximum only when that is more than 2^8 past it:
 // they stay below 2^15.
 constexpr float kPScale = 7.0f;
@@ -51,6 +52,7 @@ struct Attn4Params {
   const void* sinks;
   int sink_dtype, q_bf16, q_vec;      // q_vec: rows of q start on 16-byte boundaries
   int heads, per_kv, head_blocks, splits;
+  int fill, long_tiles;            // rows that may be long: see Attn4Plan
   int window, first, max_length;
   float scale_log2;                // scale * log2(e)
   float* part_o;                   // [rows, heads, splits, D]
@@ -71,8 +73,11 @@ struct Visible {
   }
   __device__ int tiles() const { return a + e - b; }
   __device__ int tile(int i) const { return i < a ? i : b + i - a; }
-  // workgroups of `splits` that have tiles, and how many each takes
-  __device__ int share(int splits) const { return max(kWaves, (tiles() + splits - 1) / splits); }
+  // the tiles of a workgroup, while there are some
+  __device__ int share(const Attn4Params& P) const {
+    const int t = tiles(), even = max(kWaves, (t + P.splits - 1) / P.splits);
+    return P.long_tiles == 0 ? even : max(even, min(P.long_tiles, (t + P.fill - 1) / P.fill));
+  }
 };
 
 // (__builtin_bit_cast of a vector's element takes element 0: a value of its own, always)
@@ -199,8 +204,15 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   constexpr int VT = D / 16;                   // tiles of 16 dims
   constexpr int VJ = D / 64;
   constexpr int OS = D + 4;                    // LDS row of a head
-  const int row = blockIdx.z, split = blockIdx.x;
-  const int kvh = blockIdx.y / P.head_blocks, hb = blockIdx.y % P.head_blocks;
+  // Splits next to each other, or last, where short rows have no use for most of them: every row's first one
+  // starts before those, and a row's splits are dealt over the CUs (a multiple of 32 apart they would share one).
+  int split = blockIdx.x, group = blockIdx.y, row = blockIdx.z;
+  if (P.long_tiles != 0) {
+    split = blockIdx.z;
+    group = blockIdx.x;
+    row = __builtin_amdgcn_readfirstlane((int)((blockIdx.y + 5u * blockIdx.z) % gridDim.y));
+  }
+  const int kvh = group / P.head_blocks, hb = group % P.head_blocks;
   const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int h0 = kvh * P.per_kv + hb * kHeadBlock;
@@ -227,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     }
   }
   const Visible vis(P, row);
-  const int nt = vis.tiles(), share = vis.share(P.splits);
+  const int nt = vis.tiles(), share = vis.share(P);
   const int first_tile = split * share;
   if (first_tile >= nt && !(nt == 0 && split == 0)) return;
   const int end_tile = min(first_tile + share, nt);
@@ -459,9 +471,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
 // that walked over the splits: 33).
 // Every wave forms all weights (a split per lane); sixteen bytes of a split's o per thread, the splits
 // dealt over the threads' rows and joined in LDS.
-template <int D>
-__global__ __launch_bounds__(256) void attn4_fold_kernel(Attn4Params P) {
-  constexpr int PIECES = D / 4, ROWS = 256 / PIECES;
+// One wave where there are more than 1024 (row, head), which fill the chip by themselves: 4096 without a join
+// 3.9 us, 8.7 with 256 threads.
+template <int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void attn4_fold_kernel(Attn4Params P) {
+  constexpr int PIECES = D / 4, ROWS = THREADS / PIECES;
   const int h = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 63;
   const int piece = threadIdx.x % PIECES, r = threadIdx.x / PIECES;
   __shared__ float e_s[kMostSplits];
@@ -476,7 +490,7 @@ __global__ __launch_bounds__(256) void attn4_fold_kernel(Attn4Params P) {
 #pragma unroll
   for (int k = 0; k < PRE; k++) pre[k] = po[(int64_t)min(r + k * ROWS, P.splits - 1) * PIECES + piece];
   const Visible vis(P, row);
-  const int nt = vis.tiles(), share = vis.share(P.splits);
+  const int nt = vis.tiles(), share = vis.share(P);
   if (nt <= share) return;
   const int parts = (nt + share - 1) / share;
   const float ninf = __builtin_bit_cast(float, 0xff800000u);
@@ -526,22 +540,32 @@ static int64_t most_tiles(int64_t limit, int64_t window, int64_t first) {
   return some < all ? some : all;
 }
 
+struct Attn4Plan {
+  int64_t limit, window, first, head_blocks, splits;
+  int64_t fill, long_tiles;   // 0, or what bounds a workgroup's tiles beside `splits`: see split_rows
+};
+
 // Workgroups that share a row: few tiles are taken by one, since a second launch has to join several
 // (8 groups of sequence and KV head, head_dim 64: 19 tiles 6.6 us by one and 8.0 shared, 32 tiles 8.3 and
 // 7.8, 64 tiles 13.4 and 7.9), and more of them while there are groups for the chip (256 groups: 16 tiles
 // 6.5 and 10.4, 64 tiles 13.9 and 16.0).  Shared, up to 512 workgroups, two for each CU, and eight tiles
 // each: 16384 tokens of 8 x 64, 1024 workgroups 11.7 us, 512 9.8; 52428 tokens of 2 x 10 x 128, 520
 // workgroups, of which some CUs take a third one, 43.0, 500 33.0.
-static int64_t split_count(int64_t groups, int64_t tiles) {
-  if (tiles <= 24 || (groups >= 256 && tiles <= 64)) return 1;
-  const int64_t fill = groups < 512 ? 512 / groups : 1, most = (tiles + 7) / 8;
-  const int64_t s = fill < most ? fill : most;
-  return s < kMostSplits ? s : kMostSplits;
+// Lengths are not known here.  So that one long row among short ones is not left to a few workgroups, none takes
+// more than kLongTiles tiles; of the splits that this adds a row uses what the chip has room for, or its length
+// needs (64 rows of 8 KV heads x 128, capacity 65536: one row of 65536 among 500s 94 us, 383 without; all of 500
+// 18.5 and 13.6, of 16384 228 and 215, lengths up to 16384 138 and 149; of 512 tiles 113, 17.2, 226 and 154).
+static void split_rows(int64_t groups, int64_t tiles, Attn4Plan* p) {
+  p->splits = 1;
+  p->long_tiles = 0;
+  p->fill = groups < 512 ? 512 / groups : 1;
+  if (tiles <= 24 || (groups >= 256 && tiles <= 64)) return;
+  const int64_t most = (tiles + 7) / 8, s = p->fill < most ? p->fill : most;
+  const int64_t for_long = (tiles + kLongTiles - 1) / kLongTiles;
+  p->splits = s > for_long ? s : for_long;
+  if (p->splits > s) p->long_tiles = kLongTiles;
+  if (p->splits > kMostSplits) p->splits = kMostSplits;
 }
-
-struct Attn4Plan {
-  int64_t limit, window, first, head_blocks, splits;
-};
 
 static Attn4Plan plan(const tt_int4_cache* c, int64_t rows, int64_t heads, int64_t window, int64_t first, int64_t max_length) {
   Attn4Plan p;
@@ -549,18 +573,21 @@ static Attn4Plan plan(const tt_int4_cache* c, int64_t rows, int64_t heads, int64
   p.window = window > p.limit ? 0 : (window > 0 ? window : 0);
   p.first = p.window == 0 ? 0 : (first < p.limit ? first : p.limit);
   p.head_blocks = (heads / c->kv_heads + kHeadBlock - 1) / kHeadBlock;
-  p.splits = split_count(rows * c->kv_heads * p.head_blocks, most_tiles(p.limit, p.window, p.first));
+  split_rows(rows * c->kv_heads * p.head_blocks, most_tiles(p.limit, p.window, p.first), &p);
   return p;
 }
 
 template <int D, int G>
 static int launch_attn4(const Attn4Params& P, int64_t rows, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)P.splits, (unsigned)(P.c.kv_heads * P.head_blocks), (unsigned)rows);
+  const unsigned groups = (unsigned)(P.c.kv_heads * P.head_blocks);
+  const dim3 grid = P.long_tiles ? dim3(groups, (unsigned)rows, (unsigned)P.splits) : dim3((unsigned)P.splits, groups, (unsigned)rows);
   if (P.q_bf16) hipLaunchKernelGGL((attn4_kernel<bf16_t, D, G>), grid, dim3(64 * kWaves), 0, st, P);
   else hipLaunchKernelGGL((attn4_kernel<f16_t, D, G>), grid, dim3(64 * kWaves), 0, st, P);
   const int rc = check_launch(what);
   if (rc || P.splits == 1) return rc;
-  hipLaunchKernelGGL((attn4_fold_kernel<D>), dim3((unsigned)P.heads, (unsigned)rows), dim3(256), 0, st, P);
+  const dim3 pairs((unsigned)P.heads, (unsigned)rows);
+  if (P.heads * rows > 1024) hipLaunchKernelGGL((attn4_fold_kernel<D, 64>), pairs, dim3(64), 0, st, P);
+  else hipLaunchKernelGGL((attn4_fold_kernel<D, 256>), pairs, dim3(256), 0, st, P);
   return check_launch(what);
 }
 
@@ -609,7 +636,7 @@ extern "C" int tt_gqa_attention_int4(const tt_int4_cache* cache, const void* q, 
   P.lengths = lengths;
   P.sinks = sinks; P.sink_dtype = sink_dtype;
   P.heads = (int)heads; P.per_kv = (int)(heads / cache->kv_heads);
-  P.head_blocks = (int)p.head_blocks; P.splits = (int)p.splits;
+  P.head_blocks = (int)p.head_blocks; P.splits = (int)p.splits; P.fill = (int)p.fill; P.long_tiles = (int)p.long_tiles;
   P.window = (int)p.window; P.first = (int)p.first; P.max_length = (int)p.limit;
   P.scale_log2 = (float)((double)scale * 1.4426950408889634);
   P.part_o = scratch;
