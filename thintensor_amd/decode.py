@@ -651,6 +651,8 @@ class DenseBatchDecoder:
         """The requests' next input tokens and the positions that these take."""
         if len(tokens) != self.batch or len(positions) != self.batch:
             raise ValueError("one start token and position per request")
+        if not all(0 <= t < int(self.w.embed.shape[0]) for t in tokens):
+            raise ValueError("start token outside the vocabulary")
         if not all(0 <= p < self.capacity for p in positions):
             raise ValueError("position outside the KV cache")
         self.tokens.copy_(torch.tensor(tokens, dtype=torch.int64))
