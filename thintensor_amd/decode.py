@@ -27,6 +27,8 @@ Differences from the reference, by design:
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -558,8 +560,8 @@ class DenseBatchDecoder:
     model's theta), the append to each layer's cache, attention (optionally a window of ``window``
     tokens and ``first_tokens`` first ones), the lm_head's logits and ``sample_rows``.  Sampling settings
     are per request (:meth:`set_sampling`, greedy at first).  A request that has reached the capacity
-    keeps decoding without storing further tokens; one whose logits leave nothing gets token -1, after which
-    its own tokens mean nothing and the others' are what they were."""
+    keeps decoding without storing further tokens; one whose logits leave nothing gets token -1 and stays
+    there until it is primed again, the others' tokens are what they were."""
 
     def __init__(self, backend: HipDecodeBackend, weights: DenseWeights, batch: int, capacity: int, *,
                  group_size: int = 32, window: int = 0, first_tokens: int = 0,
@@ -611,6 +613,8 @@ class DenseBatchDecoder:
         be, w, s, B = self.be, self.w, self.s, self.batch
         heads = self.q.view(B, s.heads, s.head_dim)
         k, v = self.k.view(B, s.kv_heads, s.head_dim), self.v.view(B, s.kv_heads, s.head_dim)
+        # the embedding writes nothing for token -1, whose row then is NaN: no logits, token -1 again
+        self.embedded.fill_(math.nan)
         for b in range(B):
             be.embedding(w.embed, self.tokens[b], self.embedded[b])
         left, right = self.embedded, self.zeros
