@@ -770,8 +770,9 @@ int tt_archive_close(tt_archive* archive);
 /* Rotates q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (kv_heads may be 0)
  * to their positions: for i < rotary/2, t = positions[token] inv_freq[i], the pair (a, b) of
  * dims (i, i + rotary/2) -- (2i, 2i + 1) with `interleaved` -- becomes amplitude times
- * (a cos t - b sin t, b cos t + a sin t); dims past `rotary` are copied.  Outputs may be the
- * inputs themselves, but not overlap them otherwise.  inv_freq is binary64 (radians per
+ * (a cos t - b sin t, b cos t + a sin t); dims past `rotary` are copied.  An output may be its
+ * input; otherwise outputs share no memory with the inputs, with each other or, between tokens
+ * and heads, with themselves, which is refused.  inv_freq is binary64 (radians per
  * position): t is formed and reduced in binary64, the rotation in binary32, rounded once.
  * Strides of tokens and heads are free, the last axis is contiguous.  positions are int32 or
  * int64 (position_bytes 4 or 8), negative ones included.  At most 2^22 tokens. */

@@ -1571,7 +1571,8 @@ class HipDecodeBackend:
         (i, i + half), or (2i, 2i + 1) with ``interleaved``, by position * inv_freq[i] radians and
         times ``amplitude``; the other dims are copied.  ``inv_freq`` is float64
         (:func:`thintensor_amd.rotary.rotary_frequencies`).  Without outputs in place; an output may be
-        its input but not overlap one otherwise."""
+        its input, but shares no memory with one otherwise, nor with the other output or (as an
+        expanded tensor does) with itself."""
         if q_out is None:
             q_out = q
         if k is None:

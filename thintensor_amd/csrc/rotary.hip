@@ -9,6 +9,7 @@
 #include "tt_abi_internal.h"
 #include "tt_common.h"
 #include "tt_eight.h"
+#include "tt_regions.h"
 
 namespace tt {
 
@@ -207,6 +208,16 @@ extern "C" int tt_rotary_rows(const void* q, int64_t q_token, int64_t q_head, co
   P.heads[0] = (int)heads; P.heads[1] = (int)kv_heads;
   P.positions = positions; P.inv_freq = inv_freq; P.amplitude = amplitude;
   P.tokens = tokens; P.head_dim = (int)head_dim; P.rotary = (int)rotary;
+  // an output has one writer for each place, and nobody else's input there
+  const int64_t element = dtype == TT_F32 ? 4 : 2;
+  const Region in[2] = {{q, element, head_dim, {{tokens, q_token}, {heads, q_head}}},
+                        {k, element, head_dim, {{tokens, k_token}, {kv_heads, k_head}}}};
+  const Region made[2] = {{q_out, element, head_dim, {{tokens, qo_token}, {heads, qo_head}}},
+                          {k_out, element, head_dim, {{tokens, ko_token}, {kv_heads, ko_head}}}};
+  TT_REQUIRE(made[0].once() && made[1].once() && apart(made[0], made[1]), "%s: tokens and heads that are written must not share memory", what);
+  for (int w = 0; w < 2; w++)
+    TT_REQUIRE((made[w].same(in[w]) || apart(made[w], in[w])) && apart(made[w], in[1 - w]),
+               "%s: an output may be its input, but share no memory with one otherwise", what);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == TT_F16) return launch_rotary<f16_t>(P, interleaved != 0, st);
   if (dtype == TT_BF16) return launch_rotary<bf16_t>(P, interleaved != 0, st);
