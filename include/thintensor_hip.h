@@ -810,7 +810,8 @@ int64_t tt_int4_cache_size(void); /* sizeof(tt_int4_cache), for bindings */
  * (x - m) / s rounded to the nearest, ties to even, limited to 0 .. 15; the differences are those of
  * binary64 (exact where their operands lie within 2^28 of each other), the rest is as if in exact
  * arithmetic.  A group that holds an infinity or a NaN reads as NaN.  Strides of rows, tokens and
- * heads are free; sequences and heads of the cache must not share memory here.  At most 2^26 tokens of a row. */
+ * heads are free; sequences, heads and arrays of the cache must not share memory here, which is refused.
+ * At most 2^26 tokens of a row. */
 int tt_kv_append_int4(const tt_int4_cache* cache, const void* k, int64_t k_row, int64_t k_token, int64_t k_head,
                       const void* v, int64_t v_row, int64_t v_token, int64_t v_head, int dtype,
                       const int32_t* starts, const int32_t* counts, int64_t rows, int64_t tokens, void* stream);

@@ -116,3 +116,26 @@ def test_rotary_refuses_shared_memory(be, change):
     point = lambda n, x: ctypes.c_void_p(x) if n in ("q", "k", "pos", "f", "qo", "ko") else x  # noqa: E731
     rc = be.lib.tt_rotary_rows(*[point(n, args[n]) for n in "q qt qh k kt kh dt pos pb f a i t h kv d r qo qot qoh ko kot koh st".split()])
     assert rc == -1 and b"memory" in be.lib.tt_last_error(), be.lib.tt_last_error()
+
+
+def _desc(rows=3, kv_heads=2, capacity=64, head_dim=64, group=32, **change):
+    """Arrays far from each other, sequences and heads one after the other."""
+    words, pairs = capacity * head_dim // 8, capacity * head_dim // group * 2
+    d = _lib.Int4Cache(*[_AT + (i << 20) for i in range(4)], kv_heads * words, words, kv_heads * pairs, pairs, kv_heads * words,
+                       words, kv_heads * pairs, pairs, rows, kv_heads, capacity, head_dim, group)
+    for n, x in change.items():
+        setattr(d, n, x)
+    return d
+
+
+_WORDS, _PAIRS = 64 * 8, 64 * 2 * 2            # of a sequence and head of _desc(): int32 and fp16 elements
+
+
+@pytest.mark.parametrize("change", [
+    dict(kc_head=_WORDS - 4), dict(vc_head=_WORDS - 4), dict(ks_head=_PAIRS - 8), dict(vs_head=_PAIRS - 8),
+    dict(kc_seq=_WORDS), dict(vs_seq=_PAIRS), dict(kc_seq=0, kv_heads=1), dict(v_codes=_AT),
+    dict(v_codes=_AT + 4 * 3 * 2 * _WORDS - 16), dict(k_scales=_AT + (3 << 20) + 2 * _PAIRS)])
+def test_append_refuses_memory_that_meets(be, change):
+    one = ctypes.c_void_p(1 << 30)
+    rc = be.lib.tt_kv_append_int4(_desc(**change), one, 128, 0, 64, one, 128, 0, 64, 0, one, None, 3, 1, None)
+    assert rc == -1 and b"share" in be.lib.tt_last_error(), be.lib.tt_last_error()

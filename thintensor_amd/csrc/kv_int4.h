@@ -3,6 +3,7 @@
 #pragma once
 
 #include "tt_abi_internal.h"
+#include "tt_regions.h"
 
 namespace tt {
 
@@ -29,5 +30,24 @@ inline int check_cache(const tt_int4_cache* c, int64_t rows, const char* what) {
              "%s: cache strides must keep the alignment of sequences and heads", what);
   return TT_OK;
 }
+
+// What sequences 0 .. rows - 1 of a cache take up: codes and scales of K, of V.
+struct CacheRegions {
+  Region of[4];
+  CacheRegions(const tt_int4_cache* c, int64_t rows)
+      : of{{c->k_codes, 4, c->capacity * c->head_dim / 8, {{rows, c->kc_seq}, {c->kv_heads, c->kc_head}}},
+           {c->k_scales, 2, c->capacity * c->head_dim / c->group_size * 2, {{rows, c->ks_seq}, {c->kv_heads, c->ks_head}}},
+           {c->v_codes, 4, c->capacity * c->head_dim / 8, {{rows, c->vc_seq}, {c->kv_heads, c->vc_head}}},
+           {c->v_scales, 2, c->capacity * c->head_dim / c->group_size * 2, {{rows, c->vs_seq}, {c->kv_heads, c->vs_head}}}} {}
+  // every byte of one sequence, head and array alone
+  bool once() const {
+    for (int i = 0; i < 4; i++) {
+      if (!of[i].once()) return false;
+      for (int j = 0; j < i; j++)
+        if (!apart(of[i], of[j])) return false;
+    }
+    return true;
+  }
+};
 
 }  // namespace tt

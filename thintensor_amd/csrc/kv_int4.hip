@@ -304,12 +304,8 @@ static int rows_entry(const tt_int4_cache* cache, void* k, int64_t k_row, int64_
   TT_REQUIRE(valid_out_dtype(dtype), "%s: dtype must be fp16, bf16 or fp32", what);
   if (rows == 0 || tokens == 0) return TT_OK;
   TT_REQUIRE(k && v && starts, "%s: null pointer", what);
-  if (APPEND) {   // a word of the cache has one writer (reading sequences that share their tokens is fine)
-    const auto own = [](int64_t n, int64_t a, int64_t b, int64_t c, int64_t d) { return n == 1 || (a != 0 && b != 0 && c != 0 && d != 0); };
-    TT_REQUIRE(own(rows, cache->kc_seq, cache->ks_seq, cache->vc_seq, cache->vs_seq) &&
-                   own(cache->kv_heads, cache->kc_head, cache->ks_head, cache->vc_head, cache->vs_head),
-               "%s: sequences and heads that are written must not share memory", what);
-  }
+  if (APPEND)   // a word of the cache has one writer (reading sequences that share their tokens is fine)
+    TT_REQUIRE(CacheRegions(cache, rows).once(), "%s: sequences, heads and arrays that are written must not share memory", what);
   KvRowsParams P{};
   P.c = *cache;
   P.x[0] = k; P.x[1] = v;
