@@ -818,7 +818,8 @@ int tt_kv_append_int4(const tt_int4_cache* cache, const void* k, int64_t k_row, 
 
 /* The inverse: tokens starts[row] .. of rows 0 .. rows - 1 as code s + m (rounded to binary32, then
  * to the output type) to k_out and v_out, laid out as tt_kv_append_int4 takes them.  Tokens outside
- * 0 .. capacity - 1 or past counts[row] are left as they were. */
+ * 0 .. capacity - 1 or past counts[row] are left as they were.  Outputs that share memory with
+ * themselves (between rows, tokens or heads), each other or the cache are refused. */
 int tt_kv_read_int4(const tt_int4_cache* cache, void* k_out, int64_t k_row, int64_t k_token, int64_t k_head, void* v_out,
                     int64_t v_row, int64_t v_token, int64_t v_head, int dtype, const int32_t* starts,
                     const int32_t* counts, int64_t rows, int64_t tokens, void* stream);

@@ -139,3 +139,17 @@ def test_append_refuses_memory_that_meets(be, change):
     one = ctypes.c_void_p(1 << 30)
     rc = be.lib.tt_kv_append_int4(_desc(**change), one, 128, 0, 64, one, 128, 0, 64, 0, one, None, 3, 1, None)
     assert rc == -1 and b"share" in be.lib.tt_last_error(), be.lib.tt_last_error()
+
+
+@pytest.mark.parametrize("change", [
+    dict(k_token=0), dict(k_head=0), dict(k_row=0), dict(v_row=4 * 128), dict(v_head=32), dict(v_token=64),
+    dict(v=1 << 30), dict(v=(1 << 30) + 2 * 64), dict(k=_AT + (2 << 20)), dict(v=_AT + (1 << 20) + 2 * _PAIRS), dict(k=_AT - 4)])
+def test_read_refuses_outputs_that_meet(be, change):
+    """Three rows of five tokens, two heads of 64 dims, elements of two bytes."""
+    a = dict(k=1 << 30, k_row=640, k_token=128, k_head=64, v=1 << 31, v_row=640, v_token=128, v_head=64)
+    a.update(change)
+    if "v" in change and change["v"] == (1 << 30) + 128:        # v's heads among k's
+        a.update(k_token=256, k_row=5 * 256, v_token=256, v_row=5 * 256, k_head=64)
+    rc = be.lib.tt_kv_read_int4(_desc(), ctypes.c_void_p(a["k"]), a["k_row"], a["k_token"], a["k_head"], ctypes.c_void_p(a["v"]),
+                                a["v_row"], a["v_token"], a["v_head"], 0, ctypes.c_void_p(64), None, 3, 5, None)
+    assert rc == -1 and b"share" in be.lib.tt_last_error(), be.lib.tt_last_error()

@@ -1652,7 +1652,8 @@ class HipDecodeBackend:
     def kv_read_int4(self, cache: Int4KvCache, k_out: torch.Tensor, v_out: torch.Tensor, starts: torch.Tensor,
                      counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The inverse of :meth:`kv_append_int4`: the values that the cache holds, to outputs laid out
-        as its inputs.  Tokens outside the cache or past ``counts`` are left as they were."""
+        as its inputs.  Tokens outside the cache or past ``counts`` are left as they were.  Outputs share
+        no memory with themselves (as expanded tensors do), each other or the cache."""
         self._kv_rows(self.lib.tt_kv_read_int4, "kv_read_int4", cache, k_out, v_out, starts, counts)
         return k_out, v_out
 

@@ -48,6 +48,7 @@ struct CacheRegions {
     }
     return true;
   }
+  bool apart_from(const Region& r) const { return apart(of[0], r) && apart(of[1], r) && apart(of[2], r) && apart(of[3], r); }
 };
 
 }  // namespace tt

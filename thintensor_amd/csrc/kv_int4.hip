@@ -304,8 +304,16 @@ static int rows_entry(const tt_int4_cache* cache, void* k, int64_t k_row, int64_
   TT_REQUIRE(valid_out_dtype(dtype), "%s: dtype must be fp16, bf16 or fp32", what);
   if (rows == 0 || tokens == 0) return TT_OK;
   TT_REQUIRE(k && v && starts, "%s: null pointer", what);
-  if (APPEND)   // a word of the cache has one writer (reading sequences that share their tokens is fine)
-    TT_REQUIRE(CacheRegions(cache, rows).once(), "%s: sequences, heads and arrays that are written must not share memory", what);
+  const CacheRegions held(cache, rows);
+  if (APPEND) {   // a word of the cache has one writer (reading sequences that share their tokens is fine)
+    TT_REQUIRE(held.once(), "%s: sequences, heads and arrays that are written must not share memory", what);
+  } else {
+    const int64_t element = dtype == TT_F32 ? 4 : 2;
+    const Region ko(k, element, cache->head_dim, {{rows, k_row}, {tokens, k_token}, {cache->kv_heads, k_head}});
+    const Region vo(v, element, cache->head_dim, {{rows, v_row}, {tokens, v_token}, {cache->kv_heads, v_head}});
+    TT_REQUIRE(ko.once() && vo.once() && apart(ko, vo) && held.apart_from(ko) && held.apart_from(vo),
+               "%s: outputs must not share memory with themselves, each other or the cache", what);
+  }
   KvRowsParams P{};
   P.c = *cache;
   P.x[0] = k; P.x[1] = v;
