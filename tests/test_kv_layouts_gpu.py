@@ -36,3 +36,22 @@ def test_read_into_parts_of_one_buffer(backend, device):
         backend.kv_read_int4(cache, k, v, starts)
         assert torch.equal(k, want[0]) and torch.equal(v, want[1])
         assert not torch.any(whole == 7)
+
+
+def test_attention_beside_its_queries(backend, device):
+    """Outputs among the queries' rows, head by head, and heads as the slowest axis; queries of stride 0."""
+    cache, g = _held(backend, device, 3, 2, 64, 64)
+    n = torch.tensor([64, 5, 40], device=device, dtype=torch.int32)
+    q = torch.randn((3, 4, 64), generator=g, device=device).half()
+    want = backend.gqa_attention_int4(q, cache, torch.empty_like(q), n)
+    for shape, parts in (((3, 4, 2, 64), lambda b: (b[:, :, 0], b[:, :, 1])), ((3, 2, 4, 64), lambda b: (b[:, 0], b[:, 1])),
+                         ((4, 2, 3, 64), lambda b: (b[:, 0].transpose(0, 1), b[:, 1].transpose(0, 1)))):
+        a, out = parts(torch.zeros(shape, device=device).half())
+        a.copy_(q)
+        backend.gqa_attention_int4(a, cache, out, n)
+        assert torch.equal(out, want) and torch.equal(a, q)
+    one = q[:1].expand(3, 4, 64)
+    out = backend.gqa_attention_int4(one, cache, torch.empty_like(q), n)
+    assert torch.equal(out, backend.gqa_attention_int4(one.contiguous(), cache, torch.empty_like(q), n))
+    with pytest.raises(ValueError, match="share"):
+        backend.gqa_attention_int4(q, cache, torch.empty((1, 4, 64), device=device).half().expand(3, 4, 64), n)

@@ -153,3 +153,15 @@ def test_read_refuses_outputs_that_meet(be, change):
     rc = be.lib.tt_kv_read_int4(_desc(), ctypes.c_void_p(a["k"]), a["k_row"], a["k_token"], a["k_head"], ctypes.c_void_p(a["v"]),
                                 a["v_row"], a["v_token"], a["v_head"], 0, ctypes.c_void_p(64), None, 3, 5, None)
     assert rc == -1 and b"share" in be.lib.tt_last_error(), be.lib.tt_last_error()
+
+
+@pytest.mark.parametrize("change", [
+    dict(out_row=0), dict(out_head=0), dict(out_head=60), dict(out_row=200), dict(out=1 << 30, out_row=512),
+    dict(out=(1 << 30) + 2 * 64), dict(out=(1 << 30) - 2), dict(out=_AT + (2 << 20)), dict(q_row=0, out=1 << 30, out_row=0)])
+def test_attention_refuses_outputs_that_meet(be, change):
+    """Three rows of four heads of 64 dims."""
+    a = dict(q=1 << 30, q_row=256, q_head=64, out=1 << 31, out_row=256, out_head=64)
+    a.update(change)
+    rc = be.lib.tt_gqa_attention_int4(_desc(), ctypes.c_void_p(a["q"]), a["q_row"], a["q_head"], 0, ctypes.c_void_p(64), 3, 4, 0, 0, 64,
+                                      None, 0, 1.0, None, 0, ctypes.c_void_p(a["out"]), a["out_row"], a["out_head"], None)
+    assert rc == -1 and b"share" in be.lib.tt_last_error(), be.lib.tt_last_error()

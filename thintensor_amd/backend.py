@@ -1666,7 +1666,7 @@ class HipDecodeBackend:
         first ``first_tokens``; ``sinks`` [heads] are logits that join the softmax and carry no value.
         ``scale`` is head_dim ** -0.5 by default.  ``max_length`` (by default the capacity) bounds the
         lengths, longer ones count as it, and sizes the launch.  A row that sees nothing is 0.  ``out`` may
-        be q.  Scratch of long contexts comes from the current stream's allocator with every call."""
+        be q; otherwise it shares no memory with q, the cache or itself.  Scratch of long contexts comes from the current stream's allocator with every call."""
         shape, qs, os, dtype = q.shape, q.stride(), out.stride(), q.dtype
         if len(shape) != 3 or out.shape != shape or out.dtype != dtype:
             raise ValueError("gqa_attention_int4 takes q and out [rows, heads, head_dim] of one dtype")

@@ -626,6 +626,11 @@ extern "C" int tt_gqa_attention_int4(const tt_int4_cache* cache, const void* q, 
   TT_REQUIRE(scale - scale == 0.0f, "%s: scale must be finite", what);
   if (rows == 0) return TT_OK;
   TT_REQUIRE(q && out && lengths, "%s: null pointer", what);
+  // every output has one writer; in place each workgroup reads its own heads of q before it writes them
+  const Region qr(q, 2, cache->head_dim, {{rows, q_row}, {heads, q_head}});
+  const Region made(out, 2, cache->head_dim, {{rows, out_row}, {heads, out_head}});
+  TT_REQUIRE(made.once() && (made.same(qr) || apart(made, qr)) && CacheRegions(cache, rows).apart_from(made),
+             "%s: out may be q, but must not share memory with itself, the cache or q otherwise", what);
   const Attn4Plan p = plan(cache, rows, heads, window, first_tokens, max_length);
   TT_REQUIRE(p.splits == 1 || (scratch && aligned(scratch, 16) && scratch_floats >= rows * heads * p.splits * (cache->head_dim + 2)),
              "%s: scratch too small or not 16-byte aligned", what);
