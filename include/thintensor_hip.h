@@ -790,7 +790,8 @@ int tt_rotary_rows(const void* q, int64_t q_token, int64_t q_head, const void* k
  *            nibble t/2 + 4 (t % 2) of the dim's word
  *   v_scales fp16   [batch, kv_heads, capacity/8, groups, 2, 8]   (s of eight tokens, m of eight)
  * Strides of sequences and heads are free, the inner axes contiguous; codes and v_scales start on
- * 16-byte boundaries in every sequence and head, k_scales on 4 times groups / 8 bytes (4 at least).
+ * 16-byte boundaries in every sequence and head, k_scales on 8 bytes with head_dim 256 and group_size
+ * 32, on 4 otherwise.
  * head_dim 64, 128 or 256; capacity a multiple of 32.  s has at most seven significant bits, so
  * that code s is exact in fp16. */
 typedef struct {

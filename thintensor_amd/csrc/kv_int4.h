@@ -21,13 +21,14 @@ inline int check_cache(const tt_int4_cache* c, int64_t rows, const char* what) {
              what, (long long)rows, (long long)c->batch);
   // a lane of the attention reads the scale pairs of head_dim / 4 dims at once
   const int64_t pairs = c->head_dim / 4 > c->group_size ? 2 : 1;
-  TT_REQUIRE(aligned(c->k_codes, 16) && aligned(c->v_codes, 16) && aligned(c->v_scales, 16) &&
-                 aligned(c->k_scales, 4 * (uintptr_t)pairs),
-             "%s: cache arrays must be 16-byte aligned", what);
+  TT_REQUIRE(aligned(c->k_codes, 16) && aligned(c->v_codes, 16) && aligned(c->v_scales, 16),
+             "%s: cache codes and v_scales must be 16-byte aligned", what);
+  TT_REQUIRE(aligned(c->k_scales, 4 * (uintptr_t)pairs), "%s: cache k_scales must be %d-byte aligned", what, (int)(4 * pairs));
   TT_REQUIRE(c->kc_seq % 4 == 0 && c->kc_head % 4 == 0 && c->vc_seq % 4 == 0 && c->vc_head % 4 == 0 &&
-                 c->vs_seq % 8 == 0 && c->vs_head % 8 == 0 && c->ks_seq % (2 * pairs) == 0 &&
-                 c->ks_head % (2 * pairs) == 0,
-             "%s: cache strides must keep the alignment of sequences and heads", what);
+                 c->vs_seq % 8 == 0 && c->vs_head % 8 == 0,
+             "%s: cache strides must keep codes and v_scales of sequences and heads 16-byte aligned", what);
+  TT_REQUIRE(c->ks_seq % (2 * pairs) == 0 && c->ks_head % (2 * pairs) == 0,
+             "%s: cache strides must keep k_scales of sequences and heads %d-byte aligned", what, (int)(4 * pairs));
   return TT_OK;
 }
 
