@@ -8,7 +8,8 @@ position.  For contexts longer than a model was trained on, the published scalin
   frequency by the factor and leaves the highest;
 * ``"yarn"``: frequencies that turn more than ``beta_fast`` times over ``original_positions`` are kept,
   those that turn less than ``beta_slow`` times are divided by the factor, with a linear ramp over the
-  index between; vectors grow by 0.1 ln(factor) + 1;
+  index between, whose ends are rounded outwards to whole indices unless ``truncate`` is false (as in
+  gpt-oss's settings); vectors grow by 0.1 ln(factor) + 1;
 * ``"bands"``: by wavelength: kept below original_positions / ``high_freq_factor``, divided by the
   factor above original_positions / ``low_freq_factor``, blended linearly in original_positions /
   wavelength between.
@@ -23,7 +24,7 @@ import torch
 
 def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
                        original_positions: int = 8192, beta_fast: float = 32.0, beta_slow: float = 1.0,
-                       low_freq_factor: float = 1.0, high_freq_factor: float = 4.0,
+                       truncate: bool = True, low_freq_factor: float = 1.0, high_freq_factor: float = 4.0,
                        device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
     """(inv_freq float64 [rotary_dim / 2] on ``device``, amplitude)."""
     if rotary_dim < 2 or rotary_dim % 2:
@@ -48,7 +49,10 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str 
         def at(turns: float) -> float:
             return rotary_dim * math.log(original_positions / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
 
-        low, high = max(math.floor(at(beta_fast)), 0), min(math.ceil(at(beta_slow)), rotary_dim - 1)
+        low, high = at(beta_fast), at(beta_slow)
+        if truncate:
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
         ramp = ((index - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
         freq = freq * (1.0 - ramp) + freq / factor * ramp
         amplitude = 0.1 * math.log(factor) + 1.0
