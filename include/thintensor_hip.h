@@ -832,8 +832,8 @@ int tt_kv_read_int4(const tt_int4_cache* cache, void* k_out, int64_t k_row, int6
  * given, of the sink's logit, which carries no value.  A row that sees nothing is 0; a row whose q
  * is not finite is NaN.  max_length bounds what the launch is sized for.  out may be q; otherwise it
  * shares no memory with q, the cache or (between rows or heads) itself, which is refused.
- * scratch: tt_gqa_attention_int4_scratch_floats of the same arguments (0: none is needed), for one
- * call at a time, 16-byte aligned. */
+ * scratch: tt_gqa_attention_int4_scratch_floats of the same arguments with the same GPU current (0: none
+ * is needed), for one call at a time, 16-byte aligned. */
 int64_t tt_gqa_attention_int4_scratch_floats(const tt_int4_cache* cache, int64_t rows, int64_t heads, int64_t window,
                                              int64_t first_tokens, int64_t max_length);
 int tt_gqa_attention_int4(const tt_int4_cache* cache, const void* q, int64_t q_row, int64_t q_head, int dtype,

@@ -76,6 +76,14 @@ def _on_gpu(index: int, entry, *args) -> int:
         return entry(*args, _raw_stream(index))
 
 
+def _planned(index: int, entry, *args) -> int:
+    """entry(*args), a size that goes by the GPU, with that one as the current one."""
+    if index == _current_gpu():
+        return entry(*args)
+    with torch.cuda.device(index):
+        return entry(*args)
+
+
 def _require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
@@ -1687,7 +1695,7 @@ class HipDecodeBackend:
             sink_ptr, sink_code = sinks.data_ptr(), _code(sinks, "sinks")
         limit = cache.capacity if max_length is None else max_length
         gpu = _gpu_of(q, out, lengths, sinks, cache.k_codes)
-        need = self.lib.tt_gqa_attention_int4_scratch_floats(cache.desc, rows, heads, window, first_tokens, limit)
+        need = _planned(gpu, self.lib.tt_gqa_attention_int4_scratch_floats, cache.desc, rows, heads, window, first_tokens, limit)
         if need < 0:
             _lib.check(int(need), "gqa_attention_int4")
         scratch = torch.empty(need, device=q.device, dtype=torch.float32) if need else None

@@ -471,7 +471,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
 // that walked over the splits: 33).
 // Every wave forms all weights (a split per lane); sixteen bytes of a split's o per thread, the splits
 // dealt over the threads' rows and joined in LDS.
-// One wave where there are more than 1024 (row, head), which fill the chip by themselves: 4096 without a join
+// One wave where there are more than four (row, head) for each CU, which fill the chip by themselves: 4096 without a join
 // 3.9 us, 8.7 with 256 threads.
 template <int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void attn4_fold_kernel(Attn4Params P) {
@@ -547,8 +547,8 @@ struct Attn4Plan {
 
 // Workgroups that share a row: few tiles are taken by one, since a second launch has to join several
 // (8 groups of sequence and KV head, head_dim 64: 19 tiles 6.6 us by one and 8.0 shared, 32 tiles 8.3 and
-// 7.8, 64 tiles 13.4 and 7.9), and more of them while there are groups for the chip (256 groups: 16 tiles
-// 6.5 and 10.4, 64 tiles 13.9 and 16.0).  Shared, up to 512 workgroups, two for each CU, and eight tiles
+// 7.8, 64 tiles 13.4 and 7.9), and more of them while there are groups for the chip (256 groups, one for each CU:
+// 16 tiles 6.5 and 10.4, 64 tiles 13.9 and 16.0).  Shared, up to two workgroups for each CU, 512, and eight tiles
 // each: 16384 tokens of 8 x 64, 1024 workgroups 11.7 us, 512 9.8; 52428 tokens of 2 x 10 x 128, 520
 // workgroups, of which some CUs take a third one, 43.0, 500 33.0.
 // Lengths are not known here.  So that one long row among short ones is not left to a few workgroups, none takes
@@ -556,10 +556,11 @@ struct Attn4Plan {
 // needs (64 rows of 8 KV heads x 128, capacity 65536: one row of 65536 among 500s 94 us, 383 without; all of 500
 // 18.5 and 13.6, of 16384 228 and 215, lengths up to 16384 138 and 149; of 512 tiles 113, 17.2, 226 and 154).
 static void split_rows(int64_t groups, int64_t tiles, Attn4Plan* p) {
+  const int64_t cus = device_cus();
   p->splits = 1;
   p->long_tiles = 0;
-  p->fill = groups < 512 ? 512 / groups : 1;
-  if (tiles <= 24 || (groups >= 256 && tiles <= 64)) return;
+  p->fill = groups < 2 * cus ? 2 * cus / groups : 1;
+  if (tiles <= 24 || (groups >= cus && tiles <= 64)) return;
   const int64_t most = (tiles + 7) / 8, s = p->fill < most ? p->fill : most;
   const int64_t for_long = (tiles + kLongTiles - 1) / kLongTiles;
   p->splits = s > for_long ? s : for_long;
@@ -586,7 +587,7 @@ static int launch_attn4(const Attn4Params& P, int64_t rows, hipStream_t st, cons
   const int rc = check_launch(what);
   if (rc || P.splits == 1) return rc;
   const dim3 pairs((unsigned)P.heads, (unsigned)rows);
-  if (P.heads * rows > 1024) hipLaunchKernelGGL((attn4_fold_kernel<D, 64>), pairs, dim3(64), 0, st, P);
+  if (P.heads * rows > 4 * device_cus()) hipLaunchKernelGGL((attn4_fold_kernel<D, 64>), pairs, dim3(64), 0, st, P);
   else hipLaunchKernelGGL((attn4_fold_kernel<D, 256>), pairs, dim3(256), 0, st, P);
   return check_launch(what);
 }

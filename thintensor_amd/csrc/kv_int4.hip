@@ -277,7 +277,7 @@ static int launch_rows(KvRowsParams P, int64_t rows, hipStream_t st, const char*
   // Blocks of a workgroup: as many as leave the chip its fill of workgroups, up to eight (packing is
   // indifferent to half or twice as many; reading 8193 tokens of 10 x 128: 16.6 us with half as many, 14.3,
   // 15.0 with twice as many; one block each at 16384 of 8 x 128: 35 us against 20).
-  const int64_t fill = blocks * P.c.kv_heads * rows * P.c.head_dim / (256 * (APPEND ? 2048 : 1024));
+  const int64_t fill = blocks * P.c.kv_heads * rows * P.c.head_dim / (device_cus() * (APPEND ? 2048 : 1024));
   P.blocks_per = (int)(fill < 2 ? (APPEND ? 2 : 1) : fill > kMostBlocks ? kMostBlocks : fill & ~1);
   const dim3 grid((unsigned)((blocks + P.blocks_per - 1) / P.blocks_per), (unsigned)P.c.kv_heads, (unsigned)rows);
   const dim3 block((unsigned)(2 * P.c.head_dim));

@@ -164,7 +164,7 @@ static int launch_rotary(const RotaryParams& P, bool interleaved, hipStream_t st
     // second turn, 67.8 us, 320 without one 65.6; 61.8, 4.9 TB/s, since turned and copied pieces share a
     // store).  Several tokens together where a token has few (4096 tokens of 3 heads of 64: 5.0 us with
     // one token per workgroup, 4.0 with eight).
-    const bool many = P.tokens * pieces > 4 * 65536;
+    const bool many = P.tokens * pieces > (int64_t)kAhead * 256 * device_cus();
     int64_t per = (many ? 1024 : P.tokens >= 1024 ? 256 : 0) / pieces;
     per = per < 1 ? 1 : per > 8 ? 8 : per;
     int64_t threads = (per * pieces + (many ? kAhead : 1) - 1) / (many ? kAhead : 1);

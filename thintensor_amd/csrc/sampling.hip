@@ -1073,8 +1073,9 @@ extern "C" int tt_sample_rows(const void* logits, int64_t row_stride, int dtype,
     *chunk = (int)(per * step);
     *chunks = (int)((steps + per - 1) / per);
   };
-  cut(kStep, 1024, &P.chunks, &P.chunk);
-  cut(8 * kBinThreads, 512, &P.bin_chunks, &P.bin_chunk);
+  const int64_t cus = device_cus();
+  cut(kStep, 4 * cus, &P.chunks, &P.chunk);
+  cut(8 * kBinThreads, 2 * cus, &P.bin_chunks, &P.bin_chunk);
   P.tokens = tokens; P.probs = probs;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == TT_F16) return launch_sample<f16_t>(P, rows, st);
