@@ -19,10 +19,10 @@
 // (m, l, o) for a second kernel.  (Sixteen waves in a workgroup, to keep longer rows in one launch, were
 // slower everywhere: 1024 tokens of 8 x 64 8.3 us against 8.3 with four, 575 tokens 7.1 against 6.5.)
 //
-// 131072 and 98304 tokens of 8 KV heads x 128 with 64 query heads (250 MB) take 50.7 us and 4.8 for the
-// join: 4.9 TB/s.  A tile of 32 tokens costs a wave about 290 vector instructions, two thirds of them to
+// 131072 and 98304 tokens of 8 KV heads x 128 with 64 query heads (250 MB) take 48 to 51 us and 4.7 for the
+// join: 4.9 to 5.2 TB/s.  A tile of 32 tokens costs a wave about 290 vector instructions, two thirds of them to
 // form operands from codes (shift, and-or and one packed fma for two values), and 28 matrix instructions;
-// the vector units are busy two thirds of the time, the matrix cores a fifth.  Short rows are bound by
+// the vector units are busy 74% of the time, the matrix cores 25%.  Short rows are bound by
 // their round trips: 575 tokens of 8 x 64 6.0 us (6.1 with the first tile requested after q is used), of which
 // a launch and one tile are 3.8.
 #include "kv_int4.h"

@@ -6,11 +6,11 @@
 // of its threads pack K, half V, two blocks at a time; a thread holds sixteen dims of one token, and a
 // group's extremes are exact under any order, taken over its 2, 4 or 8 lanes.
 //
-// Packing 16384 tokens of 8 KV heads x 128 (85 MB with what is written) takes 24 us, 3.5 TB/s: vector
-// instructions, 18 a value, hold 60% of the time, the rest are round trips to memory.  (One block per
+// Packing 16384 tokens of 8 KV heads x 128 (85 MB with what is written) takes 24 us, 3.5 TB/s (28 where the inputs
+// come from memory): vector instructions, 18 a value, hold 60% of the time, the rest are round trips to memory.  (One block per
 // workgroup and eight dims per thread: 38; several blocks and codes decided in binary64 without branches:
-// 30, eight dims, 24, sixteen.)  Reading them back takes 20 us, 4.2 TB/s, of which four fifths are
-// written; with one block requested at a time 23, with heads as the fastest grid axis 22.
+// 30, eight dims, 24, sixteen.)  Reading them back takes 16.6 us, 5.1 TB/s, of which four fifths are
+// written (an earlier form took 20, with one block requested at a time 23, with heads as the fastest grid axis 22).
 #include "kv_int4.h"
 #include "tt_common.h"
 #include "tt_eight.h"

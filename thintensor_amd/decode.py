@@ -561,8 +561,8 @@ class DenseBatchDecoder:
     cache, attention (optionally a window of ``window`` tokens and ``first_tokens`` first ones, planned for the
     capacity), the lm_head's logits and ``sample_rows``.  Sampling settings are per request
     (:meth:`set_sampling`, greedy at first).  The model's head also leaves its argmax in ``greedy``.  A step of
-    the 1B model takes 0.94 ms for one request, 1.37 for 8 and 2.31 for 64 in a graph (some 500 tokens each,
-    capacity 1024), 1.70, 1.69 and 2.41 launched one by one.  A request that has reached the capacity
+    the 1B model takes 0.94 ms for one request, 1.37 for 8 and 2.36 for 64 in a graph (500 tokens each, capacity
+    1024), 1.67, 1.67 and 2.39 launched one by one.  A request that has reached the capacity
     keeps decoding without storing further tokens; one whose logits leave nothing gets token -1 and stays
     there until it is primed again, the others' tokens are what they were."""
 
