@@ -829,9 +829,11 @@ int tt_kv_read_int4(const tt_int4_cache* cache, void* k_out, int64_t k_row, int6
  * [rows, heads, head_dim], heads a multiple of the cache's kv_heads.  Row r sees token t where
  * t < n = min(max(lengths[r], 0), capacity, max_length) and, with window > 0, t >= n - window or
  * t < first_tokens.  out = sum p v with p the softmax of scale q.k and, where sinks [heads] is
- * given, of the sink's logit, which carries no value.  A row that sees nothing is 0; a row whose q
- * is not finite is NaN.  max_length bounds what the launch is sized for.  out may be q; otherwise it
- * shares no memory with q, the cache or (between rows or heads) itself, which is refused.
+ * given, of the sink's logit, which carries no value.  A row that sees nothing is 0.  A head is NaN where its q
+ * is not finite, where one of its scores (binary32, in units of ln 2) passes the largest value, and
+ * where all of them pass the smallest one and no sink takes the weight.  max_length bounds what the
+ * launch is sized for.  out may be q; otherwise it shares no memory with q, the cache or (between rows
+ * or heads) itself, which is refused.
  * scratch: tt_gqa_attention_int4_scratch_floats of the same arguments with the same GPU current (0: none
  * is needed), for one call at a time, 16-byte aligned. */
 int64_t tt_gqa_attention_int4_scratch_floats(const tt_int4_cache* cache, int64_t rows, int64_t heads, int64_t window,

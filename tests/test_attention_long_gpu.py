@@ -86,3 +86,29 @@ def test_long_rows(backend, device, dtype, dim, rows, kv_heads, heads, capacity)
     mixed = torch.empty_like(q)
     backend.gqa_attention_int4(q[order].contiguous(), _shared(cache, rows), mixed, n[order].contiguous(), scale=scale)
     assert torch.equal(mixed, out[order])
+
+
+@pytest.mark.parametrize("scale", [1e38, 3e38])
+@pytest.mark.parametrize("tokens", [50, 4000])
+def test_scores_past_binary32(backend, device, scale, tokens):
+    """A score past the largest value makes its head NaN, scores all past the smallest one do without a
+    sink; a head of scores 0 is the mean of V where the scale itself is in range, whatever the others are."""
+    cache = Int4KvCache.allocate(1, 1, tokens + 32, 64, 32, device)
+    g = torch.Generator(device=device).manual_seed(tokens)
+    k = torch.rand((1, tokens, 1, 64), generator=g, device=device) + 1
+    v = torch.randn((1, tokens, 1, 64), generator=g, device=device)
+    backend.kv_append_int4(cache, k, v, torch.zeros(1, device=device, dtype=torch.int32))
+    q = torch.ones((1, 3, 64), device=device).half()
+    q[0, 1] = -1.0
+    q[0, 2] = 0.0
+    n = torch.tensor([tokens], device=device, dtype=torch.int32)
+    out = backend.gqa_attention_int4(q, cache, torch.empty_like(q), n, scale=scale)
+    sinks = torch.zeros(3, device=device)
+    beside = backend.gqa_attention_int4(q, cache, torch.empty_like(q), n, scale=scale, sinks=sinks)
+    assert torch.isnan(out[0, :2]).all() and torch.isnan(beside[0, 0]).all()
+    if scale < 2e38:
+        assert torch.count_nonzero(beside[0, 1]) == 0
+        mean = backend.kv_read_int4(cache, torch.empty_like(k), torch.empty_like(v), torch.zeros(1, device=device, dtype=torch.int32))[1]
+        mean = mean.double().sum((0, 1, 2))
+        assert torch.all((out[0, 2].double() - mean / tokens).abs() <= 2.0 ** -10 * (mean / tokens).abs() + 2.0 ** -18)
+        assert torch.all((beside[0, 2].double() - mean / (tokens + 1)).abs() <= 2.0 ** -10 * (mean / (tokens + 1)).abs() + 2.0 ** -18)
