@@ -860,6 +860,81 @@ int tt_sample_rows(const void* logits, int64_t row_stride, int dtype, int64_t ro
                    const float* min_p, void* scratch, int64_t scratch_bytes, int64_t* tokens, float* probs,
                    void* stream);
 
+/* ---------------------------------------------------------------- a paged KV cache
+ * 16-bit keys and values in pages that requests own through a table: appending with the
+ * rotation on the way, attention of single tokens, a few, or chunks of prompts, behind a
+ * shared prefix or over selected pages.  The reference pages its flat cache on the host
+ * (gpu_runtime.py:8817-8965); it has no kernel over pages. */
+
+/* dtype TT_F16 or TT_BF16.  k_pages, v_pages [pages, kv_heads, page_size, head_dim] with free strides
+ * (elements) of pages, heads and tokens, the last axis contiguous; every vector starts on a 16-byte
+ * boundary.  k_bounds (or NULL) [pages, kv_heads, 2, head_dim], the last two axes contiguous: of
+ * every dim the least and the greatest key of the page.  page_size 16, 32, 64, 128 or 256; head_dim
+ * 64, 128 or 256.  Token t of a row lies in page table[row, t / page_size], slot t % page_size. */
+typedef struct {
+  void *k_pages, *v_pages, *k_bounds;
+  int64_t k_page, k_head, k_token, v_page, v_head, v_token, b_page, b_head;
+  int64_t pages, kv_heads, page_size, head_dim, dtype;
+} tt_paged_cache;
+
+int64_t tt_paged_cache_size(void); /* sizeof(tt_paged_cache), for bindings */
+
+/* Tokens cu_tokens[r] .. cu_tokens[r + 1] - 1 (cu_tokens int32 [rows + 1], not decreasing; NULL: tokens / rows
+ * each, which must divide) of q [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim] belong to row r
+ * and have the positions starts[r], starts[r] + 1, ...  q and k are rotated to them as tt_rotary_rows does
+ * (rotary = 0: not at all; the same rounding), q to q_out, k and v to their places in the row's pages.
+ * k_bounds is kept where the cache has it: a page whose slot 0 is written begins anew, others widen.  A
+ * token without a place (a negative position, one past the table, an entry of the table that is no page)
+ * stores no key and value.  Tokens behind the last row are left alone; so is what the cache holds elsewhere.
+ * Rows of one call must not write the same slot, nor a page between them where bounds are kept: which one stays
+ * is not defined.  heads may be 0 (q and q_out unused).
+ * q_out may be q; it shares no memory with k, v, the cache or itself otherwise, which is refused, and
+ * neither does the cache with itself, q, k or v.  At most 2^22 tokens. */
+int tt_rotary_append_paged(const tt_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head, const void* k,
+                           int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                           const int32_t* table, int64_t table_row, int64_t table_pages, const int32_t* starts,
+                           const int32_t* cu_tokens, int64_t rows, int64_t tokens, int64_t heads, const double* inv_freq,
+                           int64_t rotary, int interleaved, float amplitude, void* q_out, int64_t qo_token,
+                           int64_t qo_head, void* stream);
+
+/* Attention of the last tokens of each row over its pages.  q and out [tokens, heads, head_dim] in the cache's
+ * dtype, heads a multiple of kv_heads, row r's queries as tt_rotary_append_paged takes them: query i of
+ * n_r sees the tokens t < e = N - (n_r - 1 - i), N = min(max(lengths[r], 0), max_length, table_pages page_size),
+ * and with window > 0 only t >= e - window.  out = sum p v with p the softmax of scale q.k and, where sinks
+ * [heads] is given, of the sink's logit, which carries no value; a query that sees nothing is 0.  Queries behind
+ * the last row are left as they were.  A query that sees a token whose table entry is no page is NaN.
+ * shared_pages: the first ones of every row's table are the same pages (row 0's entries are used): they are read
+ * once for all rows, and rows end where their lengths say, inside them too.
+ * selected (or NULL) int32 [rows, kv_heads, selected_count], one query a row, no shared pages: only the tokens
+ * of these pages (places in the table, each once) are seen; negative entries and those past the length are skipped.
+ * out may be q; otherwise it shares no memory with q, the cache or itself, which is refused.  max_length
+ * (at least 1) bounds what the launch is sized for.  scratch: tt_gqa_attention_paged_scratch_floats of the same
+ * arguments with the same GPU current (0: none is needed), for one call at a time, 16-byte aligned. */
+int64_t tt_gqa_attention_paged_scratch_floats(const tt_paged_cache* cache, int64_t table_pages, int ragged, int64_t rows,
+                                              int64_t tokens, int64_t heads, int64_t window, int64_t shared_pages,
+                                              int64_t selected_count, int64_t max_length);
+int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head,
+                           const int32_t* table, int64_t table_row, int64_t table_pages, const int32_t* lengths,
+                           const int32_t* cu_tokens, int64_t rows, int64_t tokens, int64_t heads, int64_t window,
+                           int64_t shared_pages, const int32_t* selected, int64_t selected_count, int64_t max_length,
+                           const void* sinks, int sink_dtype, float scale, float* scratch, int64_t scratch_floats,
+                           void* out, int64_t out_token, int64_t out_head, void* stream);
+
+/* The pages that tt_gqa_attention_paged may read for one query per row, q [rows, heads, head_dim]: for every KV
+ * head, the first first_pages and the last last_pages of the row's pages ((N - 1) / page_size + 1 of them), and of
+ * the others those of the greatest score, selected_count (at least first_pages + last_pages, at most 4096) in all,
+ * in ascending order to selected int32 [rows, kv_heads, selected_count], -1 behind them.  A page's score is the
+ * greatest product that a key within its k_bounds can have with one of the KV head's queries,
+ *   max over its heads of sum_d max(q_d low_d, q_d high_d),
+ * summed in binary64 and rounded to binary32; of equal scores the lower page is taken, NaN counts as the greatest,
+ * and so does the score of a table entry that is no page.  scratch: tt_select_pages_scratch_floats, for one call
+ * at a time. */
+int64_t tt_select_pages_scratch_floats(const tt_paged_cache* cache, int64_t table_pages, int64_t rows, int64_t max_length);
+int tt_select_pages(const tt_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head, const int32_t* table,
+                    int64_t table_row, int64_t table_pages, const int32_t* lengths, int64_t rows, int64_t heads,
+                    int64_t first_pages, int64_t last_pages, int64_t max_length, float* scratch, int64_t scratch_floats,
+                    int32_t* selected, int64_t selected_count, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -86,6 +86,18 @@ class Int4Cache(ctypes.Structure):
 
 _CP = ctypes.POINTER(Int4Cache)
 
+
+class PagedCache(ctypes.Structure):
+    """tt_paged_cache: pointers, strides (elements) and sizes of a paged 16-bit KV cache."""
+    _fields_ = [
+        ("k_pages", _P), ("v_pages", _P), ("k_bounds", _P),
+        ("k_page", _L), ("k_head", _L), ("k_token", _L), ("v_page", _L), ("v_head", _L), ("v_token", _L),
+        ("b_page", _L), ("b_head", _L), ("pages", _L), ("kv_heads", _L), ("page_size", _L), ("head_dim", _L), ("dtype", _L),
+    ]
+
+
+_GP = ctypes.POINTER(PagedCache)
+
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES: dict[str, list] = {
     "tt_version": [],
@@ -171,6 +183,14 @@ SIGNATURES: dict[str, list] = {
     "tt_kv_read_int4": [_CP, _P, _L, _L, _L, _P, _L, _L, _L, _I, _P, _P, _L, _L, _P],
     "tt_gqa_attention_int4_scratch_floats": [_CP, _L, _L, _L, _L, _L],
     "tt_gqa_attention_int4": [_CP, _P, _L, _L, _I, _P, _L, _L, _L, _L, _L, _P, _I, _F, _P, _L, _P, _L, _L, _P],
+    "tt_paged_cache_size": [],
+    "tt_rotary_append_paged": [_GP, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _L, _L, _L, _P, _L, _I, _F, _P,
+                               _L, _L, _P],
+    "tt_gqa_attention_paged_scratch_floats": [_GP, _L, _I, _L, _L, _L, _L, _L, _L, _L],
+    "tt_gqa_attention_paged": [_GP, _P, _L, _L, _P, _L, _L, _P, _P, _L, _L, _L, _L, _L, _P, _L, _L, _P, _I, _F, _P, _L, _P,
+                               _L, _L, _P],
+    "tt_select_pages_scratch_floats": [_GP, _L, _L, _L],
+    "tt_select_pages": [_GP, _P, _L, _L, _P, _L, _L, _P, _L, _L, _L, _L, _L, _P, _L, _P, _L, _P],
     "tt_sample_rows_scratch_bytes": [_L, _L],
     "tt_sample_rows": [_P, _L, _I, _L, _L, _P, _P, _P, _P, _P, _P, _L, _P, _P, _P],
     "tt_archive_open": [ctypes.c_char_p, ctypes.POINTER(_P)],
@@ -186,6 +206,8 @@ SIGNATURES: dict[str, list] = {
 _RESTYPES = {"tt_last_error": ctypes.c_char_p, "tt_matvec_argmax_partials": ctypes.c_int64,
              "tt_batched_workspace_floats": ctypes.c_int64, "tt_int4_cache_size": ctypes.c_int64,
              "tt_gqa_attention_int4_scratch_floats": ctypes.c_int64, "tt_sample_rows_scratch_bytes": ctypes.c_int64,
+             "tt_paged_cache_size": ctypes.c_int64, "tt_gqa_attention_paged_scratch_floats": ctypes.c_int64,
+             "tt_select_pages_scratch_floats": ctypes.c_int64,
              "tt_norm_router_workspace_bytes": ctypes.c_int64,
              "tt_stream_read_waves": ctypes.c_int64,
              "tt_matvec_argmax_batched_partials": ctypes.c_int64, "tt_archive_find": ctypes.c_int64,
@@ -235,6 +257,9 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         if lib.tt_int4_cache_size() != ctypes.sizeof(Int4Cache):
             raise KernelLibraryError(f"4-bit cache descriptor mismatch: library {lib.tt_int4_cache_size()} bytes, binding "
                                      f"{ctypes.sizeof(Int4Cache)}")
+        if lib.tt_paged_cache_size() != ctypes.sizeof(PagedCache):
+            raise KernelLibraryError(f"paged cache descriptor mismatch: library {lib.tt_paged_cache_size()} bytes, binding "
+                                     f"{ctypes.sizeof(PagedCache)}")
         _lib = lib
         return lib
 

@@ -23,6 +23,7 @@ import torch
 
 from . import _lib
 from .kv_cache import Int4KvCache
+from .paged_cache import PagedKvCache
 
 _DTYPE_CODE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
@@ -1707,6 +1708,170 @@ class HipDecodeBackend:
         if rc:
             _lib.check(rc, "gqa_attention_int4")
         return out
+
+    @staticmethod
+    def _paged_rows(what: str, page_table: torch.Tensor, per_row: torch.Tensor, name: str, cu_tokens: torch.Tensor | None,
+                    tokens: int) -> int:
+        """Checks the table, its rows' int32 values and their tokens; the number of rows."""
+        rows = page_table.shape[0] if page_table.ndim == 2 else -1
+        if rows < 0 or page_table.dtype != torch.int32 or (rows and (page_table.shape[1] < 1 or page_table.stride(1) != 1)):
+            raise ValueError(f"{what}: page_table must be int32 [rows, pages], contiguous in its last axis")
+        if per_row.dtype != torch.int32 or per_row.numel() != rows or not per_row.is_contiguous():
+            raise ValueError(f"{what}: {name} must be int32, one per row")
+        if cu_tokens is not None:
+            if cu_tokens.dtype != torch.int32 or cu_tokens.numel() != rows + 1 or not cu_tokens.is_contiguous():
+                raise ValueError(f"{what}: cu_tokens must be int32, one more than rows")
+        elif tokens and (rows == 0 or tokens % rows):
+            raise ValueError(f"{what}: {tokens} tokens do not divide over {rows} rows (cu_tokens says whose they are)")
+        return rows
+
+    def rotary_append_paged(self, cache: PagedKvCache, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                            page_table: torch.Tensor, starts: torch.Tensor, inv_freq: torch.Tensor | None,
+                            q_out: torch.Tensor | None = None, *, cu_tokens: torch.Tensor | None = None,
+                            interleaved: bool = False, amplitude: float = 1.0) -> torch.Tensor | None:
+        """Rotate q [tokens, heads, head_dim] (to ``q_out``, or in place) and k to their positions, as
+        :meth:`rotary_rows` does, and store k and v [tokens, kv_heads, head_dim] in ``cache``, all of its
+        type.  Tokens ``cu_tokens[r]`` to ``cu_tokens[r + 1]`` (int32 [rows + 1]; by default as many for every row)
+        are row r's, at positions ``starts[r]`` (int32 [rows]) and on; position p lies in page
+        ``page_table[r, p // page_size]`` (int32 [rows, pages]).  ``inv_freq`` None rotates nothing; q may be None.
+        Page bounds, where the cache keeps them, follow: a page whose first slot is written begins anew.  Tokens
+        without a place store nothing, those behind the last row are left alone.  Rows of one call must not write
+        the same slot, or pages of each other where bounds are kept.  ``q_out`` may be q, but shares no memory
+        otherwise, nor does the cache with q, k and v.  Returns the rotated q."""
+        what = "rotary_append_paged"
+        shape, ks, vs, dtype = k.shape, k.stride(), v.stride(), cache.dtype
+        if len(shape) != 3 or v.shape != shape or shape[1] != cache.kv_heads or shape[2] != cache.head_dim:
+            raise ValueError(f"{what} takes k and v [tokens, {cache.kv_heads}, {cache.head_dim}] for this cache")
+        if k.dtype != dtype or v.dtype != dtype:
+            raise ValueError(f"{what} operands must have the cache's dtype {dtype}")
+        if ks[2] != 1 or vs[2] != 1:
+            raise ValueError(f"{what} operands must be contiguous in their last axis")
+        tokens, head_dim = shape[0], shape[2]
+        if q is None:
+            if q_out is not None:
+                raise ValueError(f"{what}: q_out without q")
+            heads, qs, qos, q_ptr, qo_ptr = 0, (0, 0), (0, 0), None, None
+        else:
+            if q_out is None:
+                q_out = q
+            qs, qos, heads = q.stride(), q_out.stride(), q.shape[1] if q.ndim == 3 else 0
+            if heads < 1 or tuple(q.shape) != (tokens, heads, head_dim) or q_out.shape != q.shape:
+                raise ValueError(f"{what} takes q and its output [tokens, heads, {head_dim}]")
+            if q.dtype != dtype or q_out.dtype != dtype:
+                raise ValueError(f"{what} operands must have the cache's dtype {dtype}")
+            if qs[2] != 1 or qos[2] != 1:
+                raise ValueError(f"{what} operands must be contiguous in their last axis")
+            q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
+        rows = self._paged_rows(what, page_table, starts, "starts", cu_tokens, tokens)
+        rotary = 0
+        if inv_freq is not None:
+            if inv_freq.dtype != torch.float64 or inv_freq.ndim != 1 or not inv_freq.is_contiguous():
+                raise ValueError(f"{what} frequencies must be a contiguous float64 vector")
+            rotary = 2 * inv_freq.numel()
+        gpu = _gpu_of(k, v, q, q_out, page_table, starts, inv_freq, cu_tokens, cache.k_pages)
+        rc = _on_gpu(gpu, self.lib.tt_rotary_append_paged,
+                     cache.desc, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                     page_table.data_ptr(), page_table.stride(0), page_table.shape[1], starts.data_ptr(),
+                     cu_tokens.data_ptr() if cu_tokens is not None else None, rows, tokens, heads,
+                     inv_freq.data_ptr() if rotary else None, rotary, 1 if interleaved else 0, amplitude, qo_ptr,
+                     qos[0], qos[1])
+        if rc:
+            _lib.check(rc, what)
+        return q_out
+
+    def gqa_attention_paged(self, q: torch.Tensor, cache: PagedKvCache, page_table: torch.Tensor, lengths: torch.Tensor,
+                            out: torch.Tensor, *, cu_tokens: torch.Tensor | None = None, shared_pages: int = 0,
+                            selected: torch.Tensor | None = None, window: int = 0, sinks: torch.Tensor | None = None,
+                            scale: float | None = None, max_length: int | None = None) -> torch.Tensor:
+        """Causal attention of the last tokens of each row over its pages: q and out [tokens, heads,
+        head_dim] of the cache's type, ``lengths`` int32 [rows] the tokens that a row holds, its queries included;
+        tokens belong to rows as in :meth:`rotary_append_paged`.  With ``window`` > 0 a query sees the last
+        ``window`` tokens up to its own.  ``sinks`` [heads] are logits that join the softmax and carry no value;
+        ``scale`` is head_dim ** -0.5 by default.  A query that sees nothing is 0, one that needs an entry of the table
+        that is no page NaN; queries behind the last row are left as they were.
+        ``shared_pages``: so many first entries of the table are the same in every row (row 0's are read), and
+        these pages are read and multiplied once for the whole batch.  ``selected`` (int32 [rows, kv_heads, count],
+        from :meth:`select_pages`; one query per row): only these pages are read.  ``max_length`` (by default
+        what the table holds) bounds the lengths, longer ones count as it, and sizes the launch.  ``out`` may be q;
+        otherwise it shares no memory with q, the cache or itself.  Scratch comes from the current stream's
+        allocator with every call."""
+        what = "gqa_attention_paged"
+        shape, qs, os, dtype = q.shape, q.stride(), out.stride(), cache.dtype
+        if len(shape) != 3 or out.shape != shape or q.dtype != dtype or out.dtype != dtype:
+            raise ValueError(f"{what} takes q and out [tokens, heads, head_dim] of the cache's dtype {dtype}")
+        tokens, heads, head_dim = shape
+        if head_dim != cache.head_dim or heads == 0 or heads % cache.kv_heads:
+            raise ValueError(f"{what}: q {tuple(shape)} does not fit a cache of {cache.kv_heads} KV heads of {cache.head_dim}")
+        if qs[2] != 1 or os[2] != 1:
+            raise ValueError(f"{what}: q and out must be contiguous in their last axis")
+        rows = self._paged_rows(what, page_table, lengths, "lengths", cu_tokens, tokens)
+        table_pages = page_table.shape[1]
+        count, sel_ptr, sink_ptr, sink_code = 0, None, None, _lib.F32
+        if selected is not None:
+            if selected.dtype != torch.int32 or selected.ndim != 3 or tuple(selected.shape[:2]) != (rows, cache.kv_heads) or \
+                    selected.shape[2] < 1 or not selected.is_contiguous():
+                raise ValueError(f"{what}: selected must be contiguous int32 [rows, kv_heads, count]")
+            if tokens != rows or cu_tokens is not None or shared_pages:
+                raise ValueError(f"{what}: selected pages are for one query per row, without shared pages")
+            count, sel_ptr = selected.shape[2], selected.data_ptr()
+        if sinks is not None:
+            if sinks.numel() != heads or not sinks.is_contiguous():
+                raise ValueError(f"{what}: sinks must hold one logit per query head")
+            sink_ptr, sink_code = sinks.data_ptr(), _code(sinks, "sinks")
+        limit = table_pages * cache.page_size if max_length is None else max_length
+        gpu = _gpu_of(q, out, page_table, lengths, cu_tokens, selected, sinks, cache.k_pages)
+        need = _planned(gpu, self.lib.tt_gqa_attention_paged_scratch_floats, cache.desc, table_pages,
+                        1 if cu_tokens is not None else 0, rows, tokens, heads, window, shared_pages, count, limit)
+        if need < 0:
+            _lib.check(int(need), what)
+        scratch = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
+        rc = _on_gpu(gpu, self.lib.tt_gqa_attention_paged,
+                     cache.desc, q.data_ptr(), qs[0], qs[1], page_table.data_ptr(), page_table.stride(0), table_pages,
+                     lengths.data_ptr(), cu_tokens.data_ptr() if cu_tokens is not None else None, rows, tokens, heads,
+                     window, shared_pages, sel_ptr, count, limit, sink_ptr, sink_code,
+                     scale if scale is not None else head_dim ** -0.5, scratch.data_ptr() if need else None, need,
+                     out.data_ptr(), os[0], os[1])
+        if rc:
+            _lib.check(rc, what)
+        return out
+
+    def select_pages(self, q: torch.Tensor, cache: PagedKvCache, page_table: torch.Tensor, lengths: torch.Tensor,
+                     selected: torch.Tensor, *, first_pages: int = 1, last_pages: int = 2,
+                     max_length: int | None = None) -> torch.Tensor:
+        """The pages that :meth:`gqa_attention_paged` then reads for one query per row, q [rows, heads,
+        head_dim]: for every KV head the row's first ``first_pages`` and last ``last_pages`` pages, and of the others those
+        with the greatest score, as many as ``selected`` (int32 [rows, kv_heads, count]) takes, in ascending order, -1
+        behind them.  A page's score is the greatest product that a key within the cache's ``k_bounds`` of that page can
+        have with one of the KV head's queries, summed in float64 and rounded to float32; of equal ones the lower page is
+        taken.  ``max_length`` as in :meth:`gqa_attention_paged`."""
+        what = "select_pages"
+        shape, qs = q.shape, q.stride()
+        if len(shape) != 3 or q.dtype != cache.dtype or qs[2] != 1:
+            raise ValueError(f"{what} takes q [rows, heads, head_dim] of the cache's dtype {cache.dtype}")
+        rows, heads, head_dim = shape
+        if head_dim != cache.head_dim or heads == 0 or heads % cache.kv_heads:
+            raise ValueError(f"{what}: q {tuple(shape)} does not fit a cache of {cache.kv_heads} KV heads of {cache.head_dim}")
+        if cache.k_bounds is None:
+            raise ValueError(f"{what}: the cache keeps no k_bounds")
+        if self._paged_rows(what, page_table, lengths, "lengths", None, rows) != rows:
+            raise ValueError(f"{what} takes one query per row of the table")
+        if selected.dtype != torch.int32 or selected.ndim != 3 or tuple(selected.shape[:2]) != (rows, cache.kv_heads) or \
+                not selected.is_contiguous():
+            raise ValueError(f"{what}: selected must be contiguous int32 [rows, kv_heads, count]")
+        table_pages = page_table.shape[1]
+        limit = table_pages * cache.page_size if max_length is None else max_length
+        gpu = _gpu_of(q, page_table, lengths, selected, cache.k_pages)
+        need = self.lib.tt_select_pages_scratch_floats(cache.desc, table_pages, rows, limit)
+        if need < 0:
+            _lib.check(int(need), what)
+        scratch = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
+        rc = _on_gpu(gpu, self.lib.tt_select_pages,
+                     cache.desc, q.data_ptr(), qs[0], qs[1], page_table.data_ptr(), page_table.stride(0), table_pages,
+                     lengths.data_ptr(), rows, heads, first_pages, last_pages, limit,
+                     scratch.data_ptr() if need else None, need, selected.data_ptr(), selected.shape[2])
+        if rc:
+            _lib.check(rc, what)
+        return selected
 
     def sample_rows(self, logits: torch.Tensor, uniforms: torch.Tensor, tokens: torch.Tensor, *,
                     temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
