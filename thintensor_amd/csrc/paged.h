@@ -19,10 +19,10 @@ inline int check_paged(const tt_paged_cache* c, const char* what) {
   TT_REQUIRE(aligned(c->k_pages, 16) && aligned(c->v_pages, 16) && aligned(c->k_bounds, 16) &&
                  ((c->k_page | c->k_head | c->k_token | c->v_page | c->v_head | c->v_token | c->b_page | c->b_head) & 7) == 0,
              "%s: every vector of the cache must start on a 16-byte boundary", what);
-  // a lane's places inside a page and head are 32-bit byte offsets
+  // a lane's places inside a page and head are unsigned 32-bit byte offsets
   const int64_t most = (1LL << 31) / 2 / c->page_size;
-  TT_REQUIRE(c->k_token > -most && c->k_token < most && c->v_token > -most && c->v_token < most,
-             "%s: tokens of a page must lie within 2 GiB of each other", what);
+  TT_REQUIRE(c->k_token >= 0 && c->k_token < most && c->v_token >= 0 && c->v_token < most,
+             "%s: tokens of a page must lie in order within 2 GiB", what);
   return TT_OK;
 }
 

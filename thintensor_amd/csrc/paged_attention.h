@@ -1,0 +1,220 @@
+// Attention over the paged cache: what its kernels share.
+//
+// A launch serves one job: the rows' own pages (every row's queries against the tokens that the row
+// does not share), or the shared pages (all rows' queries against them, from row 0's table).  Either
+// way the queries of a KV head are columns: column c is query head c % per_kv of the job's token
+// c / per_kv, sees the tokens lo <= t < hi, and a row's keys meet all its columns at once.
+#pragma once
+
+#include "paged.h"
+#include "tt_common.h"
+
+namespace tt {
+
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef float f16v_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+
+// Weights are 2^7 exp(s - m), where m follows the running maximum only when that is more than 2^8 past it: they
+// stay below 2^15, and the smallest step of fp16 is 2^-31 of the largest.
+constexpr float kPScale = 7.0f;
+constexpr float kSlack = 8.0f;
+constexpr int kMostParts = 1024;       // parts of a query that the join takes
+
+struct PagedParams {
+  tt_paged_cache c;
+  const void* q;
+  int64_t q_token, q_head;
+  const int32_t* table;
+  int64_t table_row;
+  int table_pages, page_shift;
+  const int32_t* lengths;
+  RowTokens of;
+  const int32_t* selected;
+  int selected_count;
+  int heads, per_kv, window, shared, max_length;     // shared: tokens
+  int q_vec;                                         // vectors of q start on 16-byte boundaries
+  float scale_log2;                                  // scale * log2(e)
+  const void* sinks;
+  int sink_dtype;
+  void* out;
+  int64_t out_token, out_head;
+  // what parts of a query's tokens leave: weighted sums [tokens, heads, parts, D], (maximum, sum) of their weights
+  float* part_o;
+  float2* part_ml;
+  int parts;
+  // the launch: which job, its first part, tiles of a workgroup, column tiles of a row and in all
+  int shared_job, part0, share, row_tiles, tiles;
+};
+
+template <typename T> struct Bits16;
+template <> struct Bits16<f16_t> {
+  static constexpr uint32_t kExp = 0x7c00, kOne = 0x3c00, k128 = 0x5800, k16384 = 0x7400;
+  // (weights come from an exponential: there is no product or sum before the conversion to fold into it)
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, h2));
+  }
+  static __device__ __forceinline__ f4_t mfma16(u4_t a, u4_t b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f16v_t mfma32(u4_t a, u4_t b, f16v_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+  }
+};
+template <> struct Bits16<bf16_t> {
+  static constexpr uint32_t kExp = 0x7f80, kOne = 0x3f80, k128 = 0x4300, k16384 = 0x4680;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, b2_t));
+  }
+  static __device__ __forceinline__ f4_t mfma16(u4_t a, u4_t b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f16v_t mfma32(u4_t a, u4_t b, f16v_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+  }
+};
+
+__device__ __forceinline__ float sink_log2(const PagedParams& P, int h) {
+  const float v = P.sink_dtype == TT_F32    ? reinterpret_cast<const float*>(P.sinks)[h]
+                  : P.sink_dtype == TT_BF16 ? to_f32(reinterpret_cast<const bf16_t*>(P.sinks)[h])
+                                            : to_f32(reinterpret_cast<const f16_t*>(P.sinks)[h]);
+  return v * 0x1.715476p+0f;
+}
+
+// What a query head's sums become: o scale[0], where m is the maximum that o and l carry.  A query that saw
+// nothing has no weight and is 0.
+__device__ __forceinline__ float finish_scale(const PagedParams& P, int h, float m, float l) {
+  if (l == 0.0f) return 0.0f;
+  if (P.sinks) {
+    const float sk = sink_log2(P, h), top = fmaxf(m, sk), e = __builtin_amdgcn_exp2f(m - top);
+    return e / (l * e + __builtin_amdgcn_exp2f(sk - top + kPScale));
+  }
+  return 1.0f / l;
+}
+
+// The row of one of the call's tokens (rows when it is behind the last one), its place in the row and the row's count:
+// for single lanes, by halving.
+__device__ __forceinline__ int row_of(const RowTokens& of, int token, int* place, int* count) {
+  if (of.cu == nullptr) {
+    const int r = token / of.each;
+    *place = token - r * of.each;
+    *count = of.each;
+    return r;
+  }
+  int a = 0, b = of.rows;                // the last row that begins at or before the token
+  while (b - a > 1) {
+    const int mid = (a + b) >> 1;
+    if (of.begin(mid) <= token) a = mid;
+    else b = mid;
+  }
+  int first;
+  *count = of.count(a, &first);
+  *place = token - first;
+  return *place >= 0 && *place < *count ? a : of.rows;
+}
+
+// What column c of a job sees: [lo, hi).
+struct Seen {
+  int lo, hi;
+};
+__device__ __forceinline__ Seen seen_of(const PagedParams& P, int n, int place, int count) {
+  Seen s;
+  s.hi = n - (count - 1 - place);
+  s.lo = P.window > 0 ? max(0, s.hi - P.window) : 0;
+  if (P.shared_job) s.hi = min(s.hi, P.shared);
+  else s.lo = max(s.lo, P.shared);
+  return s;
+}
+__device__ __forceinline__ int row_length(const PagedParams& P, int row) { return min(max(P.lengths[row], 0), P.max_length); }
+
+// Sixteen tokens of a KV head that begin at a multiple of sixteen: one page holds them.
+struct Place {
+  const char *k, *v;
+  int t;             // their first token; past every length where a selection has none
+  bool bad;          // no page
+};
+__device__ __forceinline__ Place place_of(const PagedParams& P, const int32_t* table, const int32_t* sel, int kvh, int u) {
+  Place p;
+  int logical = u >> P.page_shift;
+  const int slot = u & ((1 << P.page_shift) - 1);
+  if (sel) logical = logical < P.selected_count ? sel[logical] : -1;
+  const bool none = logical < 0 || logical >= P.table_pages;
+  const int at = none ? 0 : logical;
+  const int32_t id = table[at];
+  p.bad = id < 0 || id >= P.c.pages;
+  const int64_t page = p.bad ? 0 : id;
+  p.t = none ? 0x7fffff00 : (at << P.page_shift) + slot;
+  p.k = reinterpret_cast<const char*>(P.c.k_pages) + 2 * (page * P.c.k_page + kvh * P.c.k_head + slot * P.c.k_token);
+  p.v = reinterpret_cast<const char*>(P.c.v_pages) + 2 * (page * P.c.v_page + kvh * P.c.v_head + slot * P.c.v_token);
+  return p;
+}
+
+// Orders this wave's LDS accesses for its other lanes: a wave's LDS operations execute in order, the
+// compiler has to keep them so.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// Four rows of sixteen 16-bit values in LDS, transposed: of each sixteen lanes, lane 4 r + x gives the address of
+// row r's values 4 x ..  and lane i gets value i of the four rows.
+__device__ __forceinline__ u2_t lds_transposed(const char* p) {
+  typedef __attribute__((address_space(3))) s4_t* Lds;
+  return __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p));
+}
+
+template <typename T> __device__ __forceinline__ bool any_not_finite(u4_t v) {
+  bool r = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t e = v[i] & (0x10001u * Bits16<T>::kExp);
+    r |= (e & 0xffffu) == Bits16<T>::kExp || (e >> 16) == Bits16<T>::kExp;
+  }
+  return r;
+}
+
+// Values of tokens that some columns of a tile see and others do not: a weight of 0 would turn an infinite or
+// NaN value into NaN for those that do not see it.  Such values are taken out (`clean`), and where they lie
+// goes to a second operand: 1 for infinity, 128 for minus infinity, 16384 for NaN, of which a product with ones
+// for what a column sees counts no more than 32.
+template <typename T>
+__device__ __forceinline__ void take_odd(u4_t v, u4_t& clean, u4_t& odd) {
+  using B = Bits16<T>;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    uint32_t c = 0, n = 0;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      const uint32_t x = (v[i] >> h) & 0xffffu;
+      const bool is_odd = (x & B::kExp) == B::kExp, frac = (x & 0x7fffu) != B::kExp;
+      c |= (is_odd ? 0u : x) << h;
+      n |= (!is_odd ? 0u : frac ? B::k16384 : x >> 15 ? B::k128 : B::kOne) << h;
+    }
+    clean[i] = c;
+    odd[i] = n;
+  }
+}
+// o with what such values among a column's tokens make of it
+__device__ __forceinline__ float with_odd(float o, float count) {
+  const bool neg = count >= 128.0f, pos = __builtin_amdgcn_fractf(count * 0.0078125f) > 0.0f;
+  if (count >= 16384.0f || (pos && neg)) return __builtin_bit_cast(float, 0x7fc00000u);
+  if (pos) return o + __builtin_bit_cast(float, 0x7f800000u);
+  if (neg) return o + __builtin_bit_cast(float, 0xff800000u);
+  return o;
+}
+
+// paged_few.hip: up to few_columns() columns of a row and KV head; paged_many.hip: any number
+constexpr int few_columns(int64_t head_dim) { return head_dim == 64 ? 64 : head_dim == 128 ? 32 : 16; }
+int launch_paged_few(const PagedParams& P, int blocks16, int rows, int splits, hipStream_t st, const char* what);
+int launch_paged_many(const PagedParams& P, int splits, hipStream_t st, const char* what);
+inline int many_tile_tokens(int64_t head_dim) { return head_dim == 256 ? 32 : 64; }
+constexpr int kManyColumns = 128;
+
+}  // namespace tt

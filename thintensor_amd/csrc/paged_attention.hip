@@ -1,117 +1,170 @@
-// Attention over the paged cache.
-#include "paged.h"
-#include "tt_common.h"
+// Attention over the paged cache: the plan of a call, its checks, and the join of its parts.
+#include "paged_attention.h"
 
 namespace tt {
 
-struct PagedParams {
-  tt_paged_cache c;
-  const void* q;
-  int64_t q_token, q_head;
-  const int32_t* table;
-  int64_t table_row;
-  int table_pages, page_shift;
-  const int32_t* lengths;
-  RowTokens of;
-  const int32_t* selected;
-  int selected_count;
-  int heads, per_kv, window, shared, max_length;     // shared: tokens
-  float scale_log2;                                  // scale * log2(e)
-  const void* sinks;
-  int sink_dtype;
-  void* out;
-  int64_t out_token, out_head;
-};
-
-__device__ __forceinline__ float sink_log2(const PagedParams& P, int h) {
-  const float v = P.sink_dtype == TT_F32    ? reinterpret_cast<const float*>(P.sinks)[h]
-                  : P.sink_dtype == TT_BF16 ? to_f32(reinterpret_cast<const bf16_t*>(P.sinks)[h])
-                                            : to_f32(reinterpret_cast<const f16_t*>(P.sinks)[h]);
-  return v * 0x1.715476p+0f;
+// Joins the parts of one (token, head).  Every wave forms all weights; sixteen bytes of a part's sum per
+// thread, the parts dealt over the threads' rows and joined in LDS.  A part without weight is not read.
+template <typename T, int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedParams P) {
+  constexpr int PIECES = D / 4, ROWS = THREADS / PIECES;
+  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63;
+  const int piece = threadIdx.x % PIECES, r = threadIdx.x / PIECES;
+  __shared__ float e_s[kMostParts];
+  __shared__ __attribute__((aligned(16))) f4_t sum[ROWS][PIECES];
+  const int64_t at = ((int64_t)token * P.heads + head) * P.parts;
+  const float2* ml = P.part_ml + at;
+  const f4_t* po = reinterpret_cast<const f4_t*>(P.part_o + at * D);
+  if (P.of.cu) {                                       // tokens behind the last row are left as they were
+    const int row = P.of.find(token, 1, 1, 0);
+    int first;
+    const int n = P.of.count(row, &first);
+    if (token < first || token >= first + n) return;
+  }
+  const float ninf = __builtin_bit_cast(float, 0xff800000u);
+  float M = ninf;
+  for (int k = lane; k < P.parts; k += 64) M = fmaxf(M, ml[k].x);
+#define TT_LEVEL(X) M = fmaxf(M, xor_partner<X>(M));
+  TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8) TT_LEVEL(16) TT_LEVEL(32)
+#undef TT_LEVEL
+  const float base = M == ninf ? 0.0f : M;
+  float l = 0.0f;
+  for (int k = lane; k < P.parts; k += 64) {
+    const float2 v = ml[k];
+    const float e = v.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(v.x - base);
+    l = __builtin_fmaf(v.y, e, l);
+    if (threadIdx.x < 64) e_s[k] = v.y == 0.0f ? -1.0f : e;
+  }
+  l = xor_sum(l, 1, 64);
+  __syncthreads();
+  f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int MORE = 8;
+  for (int i = r; i < P.parts; i += MORE * ROWS) {
+    f4_t more[MORE];
+    float e[MORE];
+#pragma unroll
+    for (int k = 0; k < MORE; k++) {
+      const int p = i + k * ROWS;
+      e[k] = p < P.parts ? e_s[p] : -1.0f;
+      if (!(e[k] < 0.0f)) more[k] = po[(int64_t)p * PIECES + piece];
+    }
+#pragma unroll
+    for (int k = 0; k < MORE; k++)
+      if (!(e[k] < 0.0f)) acc += more[k] * e[k];
+  }
+  sum[r][piece] = acc;
+  __syncthreads();
+  if (r != 0) return;
+#pragma unroll
+  for (int k = 1; k < ROWS; k++) acc += sum[k][piece];
+  const float f = finish_scale(P, head, M, l);
+  T* out = reinterpret_cast<T*>(P.out) + token * P.out_token + head * P.out_head + 4 * piece;
+#pragma unroll
+  for (int x = 0; x < 4; x++) store<T>(out + x, l == 0.0f ? 0.0f : acc[x] * f);
 }
 
-// One workgroup takes one query head of one token, 256 tokens of its context at a time.
+template <typename T, int D>
+static int launch_join(const PagedParams& P, hipStream_t st, const char* what) {
+  const dim3 grid((unsigned)P.of.tokens, (unsigned)P.heads);
+  if ((int64_t)P.heads * P.of.tokens > 4 * device_cus()) hipLaunchKernelGGL((paged_join_kernel<T, D, 64>), grid, dim3(64), 0, st, P);
+  else hipLaunchKernelGGL((paged_join_kernel<T, D, 256>), grid, dim3(256), 0, st, P);
+  return check_launch(what);
+}
 template <typename T>
-__global__ __launch_bounds__(256) void paged_simple_kernel(PagedParams P) {
-  const int token = blockIdx.x, head = blockIdx.y, dim = (int)P.c.head_dim, page = 1 << P.page_shift;
-  __shared__ float q_s[256], p_s[256], red[4];
-  __shared__ int id_s[256];
-  const int row = P.of.cu ? P.of.find(token, 1, 1, 0) : token / P.of.each;
-  int first;
-  const int n_row = P.of.count(row, &first);
-  if (token < first || token >= first + n_row) return;
-  const int n = min(max(P.lengths[row], 0), P.max_length);
-  const int hi = n - (n_row - 1 - (token - first)), lo = P.window > 0 ? max(0, hi - P.window) : 0;
-  const int kvh = head / P.per_kv, tid = threadIdx.x;
-  const T* q = reinterpret_cast<const T*>(P.q) + token * P.q_token + head * P.q_head;
-  if (tid < dim) q_s[tid] = to_f32(q[tid]);
-  __syncthreads();
-  const float ninf = __builtin_bit_cast(float, 0xff800000u);
-  float m = ninf, l = 0.0f, o = 0.0f;
-  bool any = false;
-  const int end = P.selected ? P.selected_count << P.page_shift : max(hi, 0);
-  for (int u0 = P.selected ? 0 : lo; u0 < end; u0 += 256) {
-    const int u = u0 + tid;
-    int t = -1, id = -1;
-    if (u < end) {
-      const int logical = P.selected ? P.selected[((int64_t)row * P.c.kv_heads + kvh) * P.selected_count + (u >> P.page_shift)]
-                                     : u >> P.page_shift;
-      if (logical >= 0 && logical < P.table_pages) {
-        t = (logical << P.page_shift) + (u & (page - 1));
-        const int32_t* tab = t < P.shared ? P.table : P.table + row * P.table_row;
-        id = tab[logical];
-      }
-    }
-    const bool seen = t >= lo && t < hi;
-    float s = ninf;
-    if (seen) {
-      if (id >= 0 && id < P.c.pages) {
-        const T* k = reinterpret_cast<const T*>(P.c.k_pages) + (int64_t)id * P.c.k_page + kvh * P.c.k_head + (t & (page - 1)) * P.c.k_token;
-        float dot = 0.0f;
-        for (int d = 0; d < dim; d++) dot = __builtin_fmaf(q_s[d], to_f32(k[d]), dot);
-        s = dot * P.scale_log2;
-      } else {
-        s = __builtin_bit_cast(float, 0x7fc00000u);
-        id = 0;
-      }
-    }
-    any = __syncthreads_or(seen) || any;
-    float top = s;
-#define TT_LEVEL(X) top = fmaxf(top, xor_partner<X>(top));
-    TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8) TT_LEVEL(16) TT_LEVEL(32)
-#undef TT_LEVEL
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float m_new = fmaxf(m, top), base = m_new == ninf ? 0.0f : m_new;
-    const float a = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(s - base);
-    m = m_new;
-    __syncthreads();
-    p_s[tid] = p;
-    id_s[tid] = seen ? id : -1;
-    l = l * a + block_sum256(p, red);
-    if (tid < dim) {
-      o *= a;
-      for (int i = 0; i < 256; i++) {
-        if (id_s[i] < 0) continue;
-        const int slot = (u0 + i) & (page - 1);
-        o = __builtin_fmaf(p_s[i], to_f32(reinterpret_cast<const T*>(P.c.v_pages)[(int64_t)id_s[i] * P.c.v_page + kvh * P.c.v_head + slot * P.c.v_token + tid]), o);
-      }
-    }
-    __syncthreads();
-  }
-  if (tid >= dim) return;
-  T* out = reinterpret_cast<T*>(P.out) + token * P.out_token + head * P.out_head + tid;
-  float r = 0.0f;
-  if (any) {
-    if (P.sinks) {
-      const float sk = sink_log2(P, head), top = fmaxf(m, sk), e = __builtin_amdgcn_exp2f(m - top);
-      r = o * e / (l * e + __builtin_amdgcn_exp2f(sk - top));
+static int launch_join(const PagedParams& P, hipStream_t st, const char* what) {
+  if (P.c.head_dim == 64) return launch_join<T, 64>(P, st, what);
+  if (P.c.head_dim == 128) return launch_join<T, 128>(P, st, what);
+  return launch_join<T, 256>(P, st, what);
+}
+
+// One of a call's launches.
+struct PagedJob {
+  bool many;
+  int blocks16, row_tiles, rows;        // few: columns of a workgroup in sixteens, workgroups of a row, rows
+  int64_t tiles;                        // many: column tiles
+  int splits, share;
+};
+
+struct PagedPlan {
+  int64_t limit, shared, window;        // tokens
+  PagedJob own, prefix;
+  int parts;
+};
+
+// Workgroups that share a row's tokens, for `groups` of them that each may take up to `tiles` tiles of 32.
+static void split_few(int64_t groups, int64_t tiles, bool parts, PagedJob* j) {
+  const int64_t cus = device_cus();
+  j->splits = 1;
+  j->share = (int)tiles;
+  if (!parts && (tiles <= 24 || (groups >= cus && tiles <= 64))) return;
+  const int64_t want = groups >= cus / 2 ? 12 * cus : 2 * cus;
+  int64_t share = (tiles * groups + want - 1) / want;
+  if (share < 8) share = 8;
+  if (share < (tiles + 511) / 512) share = (tiles + 511) / 512;
+  j->share = (int)share;
+  j->splits = (int)((tiles + share - 1) / share);
+  if (j->splits < 1) j->splits = 1;
+}
+
+static void split_many(int64_t groups, int64_t tiles, PagedJob* j) {
+  const int64_t most = tiles / 4, fill = 2 * device_cus() / (groups > 0 ? groups : 1);
+  int64_t s = most < fill ? most : fill;
+  s = s < 1 ? 1 : s > 256 ? 256 : s;
+  j->splits = (int)s;
+  j->share = 1;
+}
+
+static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged, int64_t rows, int64_t tokens, int64_t heads,
+                      int64_t window, int64_t shared_pages, int64_t selected_count, int64_t max_length) {
+  PagedPlan p{};
+  const int64_t holds = table_pages * c->page_size, G = heads / c->kv_heads;
+  p.limit = max_length < holds ? max_length : holds;
+  p.window = window < p.limit ? window : 0;
+  p.shared = rows > 1 ? shared_pages * c->page_size : 0;
+  const int64_t each = ragged ? 0 : tokens / rows;
+  const int tt = many_tile_tokens(c->head_dim);
+  if (p.shared > 0) {
+    const int64_t cols = tokens * G, reach = p.shared < p.limit ? p.shared : p.limit;
+    p.prefix.many = cols > few_columns(c->head_dim);
+    if (p.prefix.many) {
+      p.prefix.tiles = (cols + kManyColumns - 1) / kManyColumns;
+      split_many(p.prefix.tiles * c->kv_heads, (reach + tt - 1) / tt, &p.prefix);
     } else {
-      r = o / l;
+      p.prefix.blocks16 = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
+      p.prefix.row_tiles = p.prefix.rows = 1;
+      split_few(c->kv_heads, (reach + 31) / 32, true, &p.prefix);
     }
   }
-  store<T>(out, r);
+  // tokens of its own that a row's queries may see
+  int64_t reach = p.limit > p.shared ? p.limit - p.shared : 0;
+  if (p.window > 0 && p.window + (ragged ? tokens : each) < reach) reach = p.window + (ragged ? tokens : each);
+  if (selected_count > 0) reach = selected_count * c->page_size;
+  p.own.many = ragged || each * G > few_columns(c->head_dim);
+  if (p.own.many) {
+    p.own.row_tiles = (int)((each * G + kManyColumns - 1) / kManyColumns);
+    p.own.tiles = ragged ? tokens * G / kManyColumns + rows : rows * p.own.row_tiles;
+    split_many(p.own.tiles * c->kv_heads, (reach + tt - 1) / tt + 1, &p.own);
+  } else {
+    p.own.blocks16 = each * G <= 16 ? 1 : each * G <= 32 ? 2 : 4;
+    p.own.row_tiles = 1;
+    p.own.rows = (int)rows;
+    split_few(rows * c->kv_heads, (reach + 31) / 32 + (p.window > 0 ? 1 : 0), p.shared > 0, &p.own);
+  }
+  p.parts = p.own.splits + (p.shared > 0 ? p.prefix.splits : 0);
+  return p;
+}
+
+static int64_t scratch_floats_of(const PagedPlan& p, const tt_paged_cache* c, int64_t tokens, int64_t heads) {
+  return p.parts == 1 ? 0 : tokens * heads * p.parts * (c->head_dim + 2);
+}
+
+static int launch_job(PagedParams P, const PagedJob& j, bool shared, int part0, hipStream_t st, const char* what) {
+  P.shared_job = shared;
+  P.part0 = part0;
+  P.share = j.share;
+  P.row_tiles = j.row_tiles;
+  P.tiles = (int)j.tiles;
+  return j.many ? launch_paged_many(P, j.splits, st, what) : launch_paged_few(P, j.blocks16, j.rows, j.splits, st, what);
 }
 
 static int check_attention(const tt_paged_cache* c, int64_t table_pages, bool ragged, int64_t rows, int64_t tokens,
@@ -122,6 +175,7 @@ static int check_attention(const tt_paged_cache* c, int64_t table_pages, bool ra
   TT_REQUIRE(heads > 0, "%s: heads must be a multiple of kv_heads", what);
   TT_REQUIRE(window >= 0 && max_length > 0, "%s: window must not be negative, max_length at least 1", what);
   TT_REQUIRE(shared_pages >= 0 && shared_pages <= table_pages, "%s: shared_pages outside the table", what);
+  TT_REQUIRE((tokens * heads) / kManyColumns + (ragged ? rows * c->kv_heads : 0) < (1 << 23), "%s: too many queries for one call", what);
   TT_REQUIRE(selected_count >= 0 && selected_count <= 65536 && (selected_count == 0 || (!ragged && tokens == rows && shared_pages == 0)),
              "%s: selected pages (65536 at most) are for one query per row, without shared pages", what);
   return TT_OK;
@@ -137,7 +191,9 @@ extern "C" int64_t tt_gqa_attention_paged_scratch_floats(const tt_paged_cache* c
   const int rc = check_attention(cache, table_pages, ragged != 0, rows, tokens, heads, window, shared_pages, selected_count,
                                  max_length, "gqa_attention_paged");
   if (rc) return rc;
-  return 0;
+  if (rows == 0 || tokens == 0) return 0;
+  const PagedPlan p = plan(cache, table_pages, ragged != 0, rows, tokens, heads, window, shared_pages, selected_count, max_length);
+  return scratch_floats_of(p, cache, tokens, heads);
 }
 
 extern "C" int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head,
@@ -160,7 +216,9 @@ extern "C" int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q
   const Region made(out, 2, cache->head_dim, {{tokens, out_token}, {heads, out_head}});
   TT_REQUIRE(made.once() && (made.same(qr) || apart(made, qr)) && PagedRegions(cache).apart_from(made),
              "%s: out may be q, but must not share memory with itself, the cache or q otherwise", what);
-  (void)scratch; (void)scratch_floats;
+  const PagedPlan p = plan(cache, table_pages, cu_tokens != nullptr, rows, tokens, heads, window, shared_pages, selected_count, max_length);
+  const int64_t need = scratch_floats_of(p, cache, tokens, heads);
+  TT_REQUIRE(need == 0 || (scratch && aligned(scratch, 16) && scratch_floats >= need), "%s: scratch too small or not 16-byte aligned", what);
   PagedParams P{};
   P.c = *cache;
   P.q = q; P.q_token = q_token; P.q_head = q_head;
@@ -170,16 +228,18 @@ extern "C" int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q
   P.of = RowTokens{cu_tokens, (int)rows, (int)tokens, cu_tokens ? 0 : (int)(tokens / rows)};
   P.selected = selected; P.selected_count = (int)selected_count;
   P.heads = (int)heads; P.per_kv = (int)(heads / cache->kv_heads);
-  const int64_t holds = table_pages * cache->page_size;
-  P.max_length = (int)(max_length < holds ? max_length : holds);
-  P.window = (int)(window < holds ? window : 0);
-  P.shared = (int)(shared_pages * cache->page_size);
+  P.max_length = (int)p.limit; P.window = (int)p.window; P.shared = (int)p.shared;
+  P.q_vec = aligned(q, 16) && ((q_token | q_head) & 7) == 0;
   P.scale_log2 = (float)((double)scale * 1.4426950408889634);
   P.sinks = sinks; P.sink_dtype = sink_dtype;
   P.out = out; P.out_token = out_token; P.out_head = out_head;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)tokens, (unsigned)heads);
-  if (cache->dtype == TT_F16) hipLaunchKernelGGL((paged_simple_kernel<f16_t>), grid, dim3(256), 0, st, P);
-  else hipLaunchKernelGGL((paged_simple_kernel<bf16_t>), grid, dim3(256), 0, st, P);
-  return check_launch(what);
+  P.parts = p.parts;
+  P.part_o = scratch;
+  P.part_ml = reinterpret_cast<float2*>(scratch + tokens * heads * p.parts * cache->head_dim);
+  int err = TT_OK;
+  if (p.shared > 0) err = launch_job(P, p.prefix, true, p.own.splits, st, what);
+  if (err == TT_OK) err = launch_job(P, p.own, false, 0, st, what);
+  if (err != TT_OK || p.parts == 1) return err;
+  return cache->dtype == TT_F16 ? launch_join<f16_t>(P, st, what) : launch_join<bf16_t>(P, st, what);
 }

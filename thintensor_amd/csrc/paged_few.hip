@@ -1,0 +1,345 @@
+// Paged attention for few columns (a row's queries of one KV head: single tokens, drafts; or a small
+// batch against its shared pages): one wave takes 32 tokens at a time for 16 NB columns, the waves of a
+// workgroup take turns and are joined in LDS, a long row is split over workgroups.
+//
+// What bounds it is memory: a tile's K and V are read once, 4 D bytes a token.
+//   * scores are rows = tokens, columns = query heads (v_mfma_f32_16x16x32, K straight from memory as
+//     the first operand); a lane then holds 4 + 4 tokens of one column, which is the second operand of the product
+//     with V, so weights stay in registers;
+//   * V comes in whole rows, goes through the wave's own LDS and is read back transposed
+//     (ds_read_b64_tr_b16: four tokens of a dim to a lane), rows 32 bytes further apart than they are
+//     long, so that the sixteen rows of a read take all banks alike; no barrier;
+//   * K of the next tile is requested once the scores hold the present one's, V once LDS does;
+//   * a weight is rounded once to the 16-bit type, half a step, and its sum adds the rounded ones, so that
+//     what weights have in common cancels in the quotient; the rest averages out to about what the store's own
+//     rounding costs.  (A second part of a weight would be exact to 2^-17, but its product with an infinite value
+//     is NaN.)
+#include "paged_attention.h"
+
+namespace tt {
+
+constexpr int kTile = 32;
+constexpr int kWaves = 4;
+
+__device__ __forceinline__ int over_columns_max(int v) {
+#define TT_LEVEL(X) v = max(v, __builtin_bit_cast(int, xor_partner<X>(__builtin_bit_cast(float, v))));
+  TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8)
+#undef TT_LEVEL
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ float col_max(float v) {   // over the four lanes of a column
+  v = fmaxf(v, xor_partner<16>(v));
+  return fmaxf(v, xor_partner<32>(v));
+}
+
+// MIXED: a tile's tokens may be seen by some columns and not by others.
+template <typename T, int D, int NB, bool MIXED>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D * NB == 256 ? 2 : 3)))
+void paged_few_kernel(PagedParams P) {
+  using B = Bits16<T>;
+  constexpr int KI = D / 32, VT = D / 16;
+  constexpr int PC = D / 8, VR = 64 / PC, VK = 32 / VR;   // pieces of a V row, rows of a request, requests
+  constexpr int VS = 2 * D + 32;                          // LDS bytes of a V row
+  constexpr int OS = D + 4;                               // floats of a column when the waves are joined
+  static_assert(kWaves * 16 * OS * 4 <= kWaves * kTile * VS, "the join fits where V was");
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * kTile * VS];
+  __shared__ float m_s[kWaves][16], l_s[kWaves][16];
+  const int kvh = blockIdx.x / P.row_tiles, cb = blockIdx.x % P.row_tiles, row = blockIdx.y, split = blockIdx.z;
+  const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int G = P.per_kv;
+  const int first = P.shared_job ? 0 : row * P.of.each, count = P.shared_job ? P.of.tokens : P.of.each;
+  const int c0 = cb * 16 * NB, cols = min(16 * NB, count * G - c0);
+
+  // ---- columns: q is requested before anything else
+  int token[NB], head[NB];
+  u4_t qb[NB][KI];
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    const int c = c0 + min(16 * b + n, cols - 1);
+    const int i = c / G;
+    token[b] = first + i;
+    head[b] = kvh * G + c - i * G;
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(P.q) + token[b] * P.q_token + head[b] * P.q_head + 8 * quad;
+    if (P.q_vec) {
+#pragma unroll
+      for (int k = 0; k < KI; k++) qb[b][k] = *reinterpret_cast<const u4_t*>(q + 32 * k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < KI; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) qb[b][k][e] = q[32 * k + 2 * e] | ((uint32_t)q[32 * k + 2 * e + 1] << 16);
+    }
+  }
+  Seen see[NB];
+  int hi_most = 0, hi_least, lo_least, lo_most;             // over the columns
+  if (P.shared_job) {
+    int hl = 0x7fffffff, ll = 0x7fffffff, lm = 0;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      int place, each;
+      const int r = row_of(P.of, token[b], &place, &each);
+      see[b] = r < P.of.rows ? seen_of(P, row_length(P, r), place, each) : Seen{0, 0};
+      see[b].hi = max(see[b].hi, 0);
+      hi_most = max(hi_most, see[b].hi); hl = min(hl, see[b].hi);
+      ll = min(ll, see[b].lo); lm = max(lm, see[b].lo);
+    }
+    hi_most = over_columns_max(hi_most);
+    lo_most = over_columns_max(lm);
+    hi_least = -over_columns_max(-hl);
+    lo_least = -over_columns_max(-ll);
+  } else {
+    const int len = row_length(P, row);
+#pragma unroll
+    for (int b = 0; b < NB; b++) see[b] = seen_of(P, len, token[b] - first, count);
+    const Seen a = seen_of(P, len, c0 / G, count), z = seen_of(P, len, (c0 + cols - 1) / G, count);
+    hi_most = max(z.hi, 0); hi_least = a.hi; lo_least = a.lo; lo_most = z.lo;
+  }
+  const int32_t* table = P.table + (P.shared_job ? 0 : row * P.table_row);
+  const int32_t* sel = P.selected ? P.selected + ((int64_t)row * P.c.kv_heads + kvh) * P.selected_count : nullptr;
+  int tile0 = lo_least / kTile, tile1 = (hi_most + kTile - 1) / kTile;
+  if (sel) {
+    tile0 = 0;
+    tile1 = ((P.selected_count << P.page_shift) + kTile - 1) / kTile;
+    if (hi_most == 0) tile1 = 0;
+  }
+  tile0 += split * P.share;
+  tile1 = min(tile1, tile0 + P.share);
+  const bool only = P.parts == 1;
+  if (tile0 >= tile1) {
+    if (!only) {                                             // nothing here: no weight
+      for (int c = threadIdx.x; c < cols; c += 64 * kWaves) {
+        const int i = (c0 + c) / G;
+        P.part_ml[((int64_t)(first + i) * P.heads + kvh * G + (c0 + c - i * G)) * P.parts + P.part0 + split] =
+            make_float2(__builtin_bit_cast(float, 0xff800000u), 0.0f);
+      }
+      return;
+    }
+    tile1 = tile0;
+  }
+
+  // ---- tiles
+  const uint32_t k_at = (uint32_t)n * (uint32_t)(2 * P.c.k_token) + 16 * quad, v_step = (uint32_t)(2 * P.c.v_token);
+  const int v_row = lane / PC, v_piece = lane % PC;
+  u4_t kr[2][KI], vr[VK];
+  auto load_k = [&](const Place (&p)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int k = 0; k < KI; k++) kr[h][k] = *reinterpret_cast<const u4_t*>(p[h].k + (size_t)(k_at + 64 * k));
+  };
+  auto load_v = [&](const Place (&p)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < VK; k++) {
+      const int h = k * VR / 16;
+      vr[k] = *reinterpret_cast<const u4_t*>(p[h].v + (size_t)((uint32_t)(k * VR - 16 * h + v_row) * v_step + 16 * v_piece));
+    }
+  };
+  const int last = tile1 - 1;
+  auto place = [&](int i, Place (&p)[2]) __attribute__((always_inline)) {
+    const int j = max(min(i, last), 0);
+    p[0] = place_of(P, table, sel, kvh, kTile * j);
+    p[1] = place_of(P, table, sel, kvh, kTile * j + 16);
+  };
+  int i = tile0 + wave;
+  Place now[2], next[2];
+  place(i, now);
+  if (tile0 < tile1) {
+    load_k(now);
+    load_v(now);
+  }
+  place(i + kWaves, next);
+
+  // the sign of the scale goes to q, so that the largest product is the largest score
+  const float score_scale = fmaxf(__builtin_fabsf(P.scale_log2), 0x1p-126f);
+  if (P.scale_log2 < 0.0f) {
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int k = 0; k < KI; k++) qb[b][k] ^= 0x80008000u;
+  }
+  const float ninf = __builtin_bit_cast(float, 0xff800000u);
+  f4_t o[NB][VT];
+  float m_run[NB], l_run[NB];
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+#pragma unroll
+    for (int x = 0; x < VT; x++) o[b][x] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
+    m_run[b] = ninf;
+    l_run[b] = 0.0f;
+  }
+  char* const mine = lds + wave * (kTile * VS);
+  char* const put = mine + v_row * VS + 16 * v_piece;
+  const char* const get = mine + (4 * quad + (n >> 2)) * VS + 8 * (n & 3);
+
+  for (; i < tile1; i += kWaves) {
+    f4_t sc[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        sc[b][h] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KI; k++) sc[b][h] = B::mfma16(kr[h][k], qb[b][k], sc[b][h]);
+      }
+    load_k(next);
+    const int t0 = now[0].t, t1 = now[1].t;
+    const bool whole = t0 >= lo_most && t0 + 16 <= hi_least && t1 >= lo_most && t1 + 16 <= hi_least && !now[0].bad && !now[1].bad;
+    bool odd = false;
+    if (!whole) {
+      // tokens out of every column's sight: no value (what lies there may be NaN)
+#pragma unroll
+      for (int k = 0; k < VK; k++) {
+        const int h = k * VR / 16, t = (h ? t1 : t0) + k * VR - 16 * h + v_row;
+        if (t < lo_least || t >= hi_most) vr[k] = (u4_t){0u, 0u, 0u, 0u};
+        if (MIXED) odd |= any_not_finite<T>(vr[k]);
+      }
+      odd = MIXED && __builtin_amdgcn_ballot_w64(odd) != 0;
+    }
+    wave_lds_order();
+#pragma unroll
+    for (int k = 0; k < VK; k++) *reinterpret_cast<u4_t*>(put + k * VR * VS) = vr[k];
+    wave_lds_order();
+    load_v(next);
+    const bool bad0 = now[0].bad, bad1 = now[1].bad;
+    now[0] = next[0];
+    now[1] = next[1];
+    place(i + 2 * kWaves, next);
+
+    u4_t pw[NB], vis[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      float s[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) s[e] = sc[b][e >> 2][e & 3];
+      if (!whole) {
+        uint32_t ones[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int t = (e < 4 ? t0 : t1) + 4 * quad + (e & 3);
+          const bool in = t >= see[b].lo && t < see[b].hi;
+          if (e < 4 ? bad0 : bad1) s[e] = __builtin_bit_cast(float, 0x7fc00000u);
+          if (!in) s[e] = ninf;
+          ones[e >> 1] |= in ? (uint32_t)B::kOne << (16 * (e & 1)) : 0u;
+        }
+        vis[b] = (u4_t){ones[0], ones[1], ones[2], ones[3]};
+      }
+      float top = s[0];
+#pragma unroll
+      for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
+      // no lane of a column past its maximum by more than the slack: nothing moves
+      if (__builtin_amdgcn_ballot_w64(top * score_scale > m_run[b] + kSlack) != 0) {
+        const float m_new = fmaxf(m_run[b], col_max(top) * score_scale);
+        const float a = m_new == ninf ? 1.0f : __builtin_amdgcn_exp2f(m_run[b] - m_new);
+        l_run[b] *= a;
+#pragma unroll
+        for (int x = 0; x < VT; x++) o[b][x] *= a;
+        m_run[b] = m_new;
+      }
+      const float base = kPScale - (m_run[b] == ninf ? 0.0f : m_run[b]);
+#pragma unroll
+      for (int p = 0; p < 4; p++) {
+        const float pa = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * p], score_scale, base));
+        const float pb = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * p + 1], score_scale, base));
+        const uint32_t w = B::pack(pa, pb);
+        l_run[b] += lo_f32<T>(w) + hi_f32<T>(w);
+        pw[b][p] = w;
+      }
+    }
+    auto values = [&](int x) __attribute__((always_inline)) {
+      const u2_t va = lds_transposed(get + 32 * x), vb = lds_transposed(get + 16 * VS + 32 * x);
+      return (u4_t){va[0], va[1], vb[0], vb[1]};
+    };
+    if (!MIXED || !odd) {
+#pragma unroll
+      for (int x = 0; x < VT; x++) {
+        const u4_t v = values(x);
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[b][x] = B::mfma16(v, pw[b], o[b][x]);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < VT; x++) {
+        __builtin_amdgcn_sched_barrier(0);     // one at a time: rare, and should cost no registers
+        u4_t clean, code;
+        take_odd<T>(values(x), clean, code);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+          o[b][x] = B::mfma16(clean, pw[b], o[b][x]);
+          const f4_t count = B::mfma16(code, vis[b], (f4_t){0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[b][x][r] = with_odd(o[b][x][r], count[r]);
+        }
+      }
+    }
+  }
+
+  // ---- the waves are joined, sixteen columns at a time
+  float* const o_s = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    const float l_col = bfly<32>(bfly<16>(l_run[b]));
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < VT; x++) *reinterpret_cast<f4_t*>(o_s + (wave * 16 + n) * OS + 16 * x + 4 * quad) = o[b][x];
+    if (quad == 0) {
+      m_s[wave][n] = m_run[b];
+      l_s[wave][n] = l_col;
+    }
+    __syncthreads();
+    const int here = min(16, cols - 16 * b);
+    for (int u = threadIdx.x; u < here * (D / 4); u += 64 * kWaves) {
+      const int cc = u / (D / 4), d = 4 * (u % (D / 4));
+      const int c = c0 + 16 * b + cc, at = c / G;
+      float M = m_s[0][cc];
+#pragma unroll
+      for (int w = 1; w < kWaves; w++) M = fmaxf(M, m_s[w][cc]);
+      const float base = M == ninf ? 0.0f : M;
+      f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      float l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        const float e = __builtin_amdgcn_exp2f(m_s[w][cc] - base);
+        acc += *reinterpret_cast<const f4_t*>(o_s + (w * 16 + cc) * OS + d) * e;
+        l = __builtin_fmaf(l_s[w][cc], e, l);
+      }
+      const int tok = first + at, hd = kvh * G + c - at * G;
+      if (only) {
+        const float f = finish_scale(P, hd, M, l);
+        T* out = reinterpret_cast<T*>(P.out) + tok * P.out_token + hd * P.out_head + d;
+#pragma unroll
+        for (int r = 0; r < 4; r++) store<T>(out + r, l == 0.0f ? 0.0f : acc[r] * f);
+      } else {
+        const int64_t part = ((int64_t)tok * P.heads + hd) * P.parts + P.part0 + split;
+        *reinterpret_cast<f4_t*>(P.part_o + part * D + d) = acc;
+        if (d == 0) P.part_ml[part] = make_float2(M, l);
+      }
+    }
+  }
+}
+
+template <typename T, int D, int NB>
+static int launch_blocks(const PagedParams& P, int rows, int splits, hipStream_t st, const char* what) {
+  const dim3 grid((unsigned)(P.c.kv_heads * P.row_tiles), (unsigned)rows, (unsigned)splits), block(64 * kWaves);
+  if (P.shared_job || P.of.each > 1) hipLaunchKernelGGL((paged_few_kernel<T, D, NB, true>), grid, block, 0, st, P);
+  else hipLaunchKernelGGL((paged_few_kernel<T, D, NB, false>), grid, block, 0, st, P);
+  return check_launch(what);
+}
+
+template <typename T>
+static int launch_type(const PagedParams& P, int blocks16, int rows, int splits, hipStream_t st, const char* what) {
+  if (P.c.head_dim == 64)
+    return blocks16 == 1   ? launch_blocks<T, 64, 1>(P, rows, splits, st, what)
+           : blocks16 == 2 ? launch_blocks<T, 64, 2>(P, rows, splits, st, what)
+                           : launch_blocks<T, 64, 4>(P, rows, splits, st, what);
+  if (P.c.head_dim == 128)
+    return blocks16 == 1 ? launch_blocks<T, 128, 1>(P, rows, splits, st, what) : launch_blocks<T, 128, 2>(P, rows, splits, st, what);
+  return launch_blocks<T, 256, 1>(P, rows, splits, st, what);
+}
+
+int launch_paged_few(const PagedParams& P, int blocks16, int rows, int splits, hipStream_t st, const char* what) {
+  return P.c.dtype == TT_F16 ? launch_type<f16_t>(P, blocks16, rows, splits, st, what)
+                             : launch_type<bf16_t>(P, blocks16, rows, splits, st, what);
+}
+
+}  // namespace tt
