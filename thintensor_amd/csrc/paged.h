@@ -81,4 +81,25 @@ struct RowTokens {
   }
 };
 
+// The row of one of the call's tokens (rows when it is behind the last one), its place in the row and the row's count:
+// for single lanes, by halving.
+__device__ __forceinline__ int row_of(const RowTokens& of, int token, int* place, int* count) {
+  if (of.cu == nullptr) {
+    const int r = token / of.each;
+    *place = token - r * of.each;
+    *count = of.each;
+    return r;
+  }
+  int a = 0, b = of.rows;                // the last row that begins at or before the token
+  while (b - a > 1) {
+    const int mid = (a + b) >> 1;
+    if (of.begin(mid) <= token) a = mid;
+    else b = mid;
+  }
+  int first;
+  *count = of.count(a, &first);
+  *place = token - first;
+  return *place >= 0 && *place < *count ? a : of.rows;
+}
+
 }  // namespace tt

@@ -1,6 +1,12 @@
-// Appending to the paged cache with the rotation on the way.
+// Appending to the paged cache with the rotation on the way (angles and rotation as in rotary.hip).
+//
+// What bounds it is memory: every value is read and written once.  One launch holds two kinds of workgroups.
+// Those of keys and values take the tokens of one row that fall into one page, for some KV heads: a page's bounds
+// then have one writer, which keeps the extremes of its places in registers and joins them in LDS, and no atomics
+// are needed.  Those of queries take a few tokens with all their heads.
 #include "paged.h"
 #include "tt_common.h"
+#include "tt_eight.h"
 
 namespace tt {
 
@@ -17,29 +23,271 @@ struct AppendParams {
   int heads, rotary, interleaved;
   const double* inv_freq;
   float amplitude;
+  int runs, head_groups, group_heads;      // workgroups of keys and values: runs x groups of KV heads
+  int q_tokens;                            // tokens of a workgroup of queries
 };
 
-// One workgroup takes the tokens of one row that fall into one page.
+// The tokens of one row that fall into one page: tokens first + from .. of the call, slot slot0 of the page on.
+struct Run {
+  int64_t first, start, logical;           // the row's first token and its position; the page's place in the table
+  int from, to;
+  int32_t id;                              // the page, or -1
+};
+__device__ __forceinline__ Run run_of(const AppendParams& P, int x) {
+  Run r;
+  const int page = (int)P.c.page_size;
+  const int row = __builtin_amdgcn_readfirstlane(P.of.cu ? P.of.find(x, 1, page, 2) : 0);
+  int row_u = row, unit;
+  if (P.of.cu == nullptr) {
+    const int units = P.of.each / page + 2;
+    row_u = x / units;
+    unit = x - row_u * units;
+  }
+  int first;
+  const int n = P.of.count(row_u, &first);
+  if (P.of.cu) unit = x - (first / page + 2 * row_u);
+  r.first = first;
+  r.start = P.starts[row_u];
+  r.logical = (r.start >> __builtin_ctz(page)) + unit;      // floor, of negative positions too
+  const int64_t a = r.logical * page - r.start, b = a + page;
+  r.from = (int)(a > 0 ? (a < n ? a : n) : 0);
+  r.to = (int)(b < n ? b : n);
+  r.id = r.logical >= 0 && r.logical < P.table_pages ? P.table[row_u * P.table_row + r.logical] : -1;
+  if (r.id >= P.c.pages || r.id < 0) r.id = -1;
+  return r;
+}
+
+// cos and sin times the amplitude of `n` tokens' angles, to turn[token][half] and turn[token][half + ...].
+template <typename F>
+__device__ __forceinline__ void form_turns(const AppendParams& P, float* turn, int n, F&& position) {
+  const int half = P.rotary >> 1;
+  for (int v = threadIdx.x; v < n * half; v += 256) {
+    const int tk = v / half, i = v - tk * half;
+    const double t = (double)position(tk) * P.inv_freq[i] * 0.15915494309189533577;
+    float s, c;
+    sincospif(2.0f * (float)(t - __builtin_rint(t)), &s, &c);
+    turn[tk * P.rotary + i] = c * P.amplitude;
+    turn[tk * P.rotary + half + i] = s * P.amplitude;
+  }
+}
+
+// A place of a head: eight pairs of the half layout (two pieces of eight dims), four of the interleaved one (one
+// piece), or a piece to copy.
+template <typename T, bool INTERLEAVED> struct Turned {
+  static constexpr int NP = INTERLEAVED ? 1 : 2;
+  Eight<T> a, b;
+  __device__ __forceinline__ void load(const T* x, int d0, int d1, bool copy) {
+    a.load(x + d0);
+    if (NP == 2 && !copy) b.load(x + d1);
+  }
+  __device__ __forceinline__ void turn(const float* cs, int half, int u) {
+    float ra[8], rb[8];
+    if (INTERLEAVED) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float c = cs[4 * u + e], s = cs[half + 4 * u + e], x = a.get(2 * e), y = a.get(2 * e + 1);
+        ra[2 * e] = x * c - y * s;
+        ra[2 * e + 1] = y * c + x * s;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float c = cs[8 * u + e], s = cs[half + 8 * u + e], x = a.get(e), y = b.get(e);
+        ra[e] = x * c - y * s;
+        rb[e] = y * c + x * s;
+      }
+      b.set(rb);
+    }
+    a.set(ra);
+  }
+  __device__ __forceinline__ void store(T* o, int d0, int d1, bool copy) const {
+    if (NP == 2 && !copy) b.store(o + d1);
+    a.store(o + d0);
+  }
+};
+
+constexpr int kAhead = 4;                  // requested together, so that loads do not wait behind stores
+constexpr int kTurnFloats = 8192;          // of LDS: tokens whose angles are formed at once, times rotary
+
+// Rows whose vectors start on 16-byte boundaries and whose parts come in whole pieces of eight dims.
+template <typename T, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
+  __shared__ __attribute__((aligned(16))) float turn_s[kTurnFloats];
+  constexpr int NP = INTERLEAVED ? 1 : 2;
+  const int dim = (int)P.c.head_dim, half = P.rotary >> 1, tid = threadIdx.x;
+  const int turns = P.rotary / (8 * NP), units = turns + (dim - P.rotary) / 8;
+  const int rows = 256 / units, r0 = tid / units, u = tid - r0 * units;
+  const bool copy = u >= turns;
+  const int d0 = copy ? P.rotary + 8 * (u - turns) : 8 * u, d1 = copy ? d0 : d0 + half;
+  typedef Turned<T, INTERLEAVED> Piece;
+  const int kv_groups = P.runs * P.head_groups;
+
+  if ((int)blockIdx.x >= kv_groups) {
+    // ---- queries
+    const int t0 = ((int)blockIdx.x - kv_groups) * P.q_tokens, tokens = min(P.q_tokens, P.of.tokens - t0);
+    const int total = r0 < rows ? tokens * P.heads : 0;
+    Piece x[kAhead];
+    auto at = [&](int r, int* tk, int* h) __attribute__((always_inline)) {
+      *tk = r / P.heads;
+      *h = r - *tk * P.heads;
+    };
+    auto load = [&](int r) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < kAhead; k++) {
+        int tk, h;
+        at(min(r + k * rows, max(total - 1, 0)), &tk, &h);
+        x[k].load(reinterpret_cast<const T*>(P.q) + (int64_t)(t0 + tk) * P.q_token + h * P.q_head, d0, d1, copy);
+      }
+    };
+    load(r0);
+    __shared__ int64_t pos_s[64];
+    __shared__ int in_row[64];
+    if (tid < tokens) {
+      int place, count;
+      const int r = row_of(P.of, t0 + tid, &place, &count);
+      in_row[tid] = r < P.of.rows;
+      pos_s[tid] = r < P.of.rows ? (int64_t)P.starts[r] + place : 0;
+    }
+    __syncthreads();
+    form_turns(P, turn_s, tokens, [&](int tk) { return pos_s[tk]; });
+    __syncthreads();
+    for (int r = r0; r < total; r += kAhead * rows) {
+      if (r != r0) load(r);
+#pragma unroll
+      for (int k = 0; k < kAhead; k++) {
+        if (r + k * rows >= total) break;
+        int tk, h;
+        at(r + k * rows, &tk, &h);
+        if (!in_row[tk]) continue;
+        if (!copy) x[k].turn(turn_s + tk * P.rotary, half, u);
+        x[k].store(reinterpret_cast<T*>(P.q_out) + (int64_t)(t0 + tk) * P.o_token + h * P.o_head, d0, d1, copy);
+      }
+    }
+    return;
+  }
+
+  // ---- keys and values
+  const Run run = run_of(P, blockIdx.x / P.head_groups);
+  if (run.from >= run.to || run.id < 0) return;
+  const int kvh0 = (blockIdx.x % P.head_groups) * P.group_heads, heads = min(P.group_heads, (int)P.c.kv_heads - kvh0);
+  const int n = run.to - run.from, slot0 = (int)(run.start + run.from - run.logical * P.c.page_size);
+  const int64_t token0 = run.first + run.from;
+  const T* k = reinterpret_cast<const T*>(P.k) + token0 * P.k_token + kvh0 * P.k_head;
+  const T* v = reinterpret_cast<const T*>(P.v) + token0 * P.v_token + kvh0 * P.v_head;
+  T* kp = reinterpret_cast<T*>(P.c.k_pages) + (int64_t)run.id * P.c.k_page + kvh0 * P.c.k_head + (int64_t)slot0 * P.c.k_token;
+  T* vp = reinterpret_cast<T*>(P.c.v_pages) + (int64_t)run.id * P.c.v_page + kvh0 * P.c.v_head + (int64_t)slot0 * P.c.v_token;
+
+  // a thread keeps one place of one head and walks over the tokens
+  const int lanes = rows / heads, tk0 = r0 / heads, head = r0 - tk0 * heads;
+  const bool works = tk0 < lanes;
+  float lo[8 * NP], hi[8 * NP];
+#pragma unroll
+  for (int e = 0; e < 8 * NP; e++) {
+    lo[e] = __builtin_bit_cast(float, 0x7f800000u);
+    hi[e] = __builtin_bit_cast(float, 0xff800000u);
+  }
+  const int chunk = P.rotary > 0 ? min(n, kTurnFloats / P.rotary) : n;
+  for (int c0 = 0; c0 < n; c0 += chunk) {
+    const int end = min(c0 + chunk, n);
+    Piece x[kAhead];
+    auto load = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kAhead; i++)
+        x[i].load(k + (int64_t)min(t + i * lanes, end - 1) * P.k_token + head * P.k_head, d0, d1, copy);
+    };
+    if (works) load(c0 + tk0);
+    if (c0 > 0) __syncthreads();
+    form_turns(P, turn_s, end - c0, [&](int tk) { return run.start + run.from + c0 + tk; });
+    __syncthreads();
+    if (works)
+      for (int t = c0 + tk0; t < end; t += kAhead * lanes) {
+        if (t != c0 + tk0) load(t);
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+          const int tt = t + i * lanes;
+          if (tt >= end) break;
+          if (!copy) x[i].turn(turn_s + (tt - c0) * P.rotary, half, u);
+          x[i].store(kp + (int64_t)tt * P.c.k_token + head * P.c.k_head, d0, d1, copy);
+          if (P.c.k_bounds) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {                     // of the keys as they are stored; NaN stays
+              lo[e] = __builtin_elementwise_minimum(lo[e], x[i].a.get(e));
+              hi[e] = __builtin_elementwise_maximum(hi[e], x[i].a.get(e));
+              if (NP == 2 && !copy) {
+                lo[8 * (NP - 1) + e] = __builtin_elementwise_minimum(lo[8 * (NP - 1) + e], x[i].b.get(e));
+                hi[8 * (NP - 1) + e] = __builtin_elementwise_maximum(hi[8 * (NP - 1) + e], x[i].b.get(e));
+              }
+            }
+          }
+        }
+      }
+  }
+  {
+    const int pieces = dim / 8, per = heads * pieces;
+    const int total = n * per;
+    for (int i = tid; i < total; i += kAhead * 256) {
+      Eight<T> y[kAhead];
+      auto at = [&](int j, int* tk, int* h) __attribute__((always_inline)) {
+        *tk = j / per;
+        *h = (j - *tk * per) / pieces;
+        return 8 * (j % pieces);
+      };
+#pragma unroll
+      for (int a = 0; a < kAhead; a++) {
+        int tk, h;
+        const int d = at(min(i + a * 256, total - 1), &tk, &h);
+        y[a].load(v + (int64_t)tk * P.v_token + h * P.v_head + d);
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; a++) {
+        if (i + a * 256 >= total) break;
+        int tk, h;
+        const int d = at(i + a * 256, &tk, &h);
+        y[a].store(vp + (int64_t)tk * P.c.v_token + h * P.c.v_head + d);
+      }
+    }
+  }
+  if (P.c.k_bounds == nullptr) return;
+  // ---- a dim's extremes over the token lanes: first those of low, then those of high, in the angles' LDS
+  T* bp = reinterpret_cast<T*>(P.c.k_bounds) + (int64_t)run.id * P.c.b_page + kvh0 * P.c.b_head;
+  const bool anew = slot0 == 0;
+#pragma unroll
+  for (int side = 0; side < 2; side++) {
+    __syncthreads();
+    if (works)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        float* const to = turn_s + (tk0 * heads + head) * dim;
+        to[d0 + e] = side ? hi[e] : lo[e];
+        if (NP == 2 && !copy) to[d1 + e] = side ? hi[8 * (NP - 1) + e] : lo[8 * (NP - 1) + e];
+      }
+    __syncthreads();
+    for (int i = tid; i < heads * dim; i += 256) {
+      const int h = i / dim, d = i - h * dim;
+      T* const b = bp + h * P.c.b_head + side * dim + d;
+      float r = anew ? turn_s[i] : to_f32(*b);
+      for (int t = 0; t < lanes; t++) {
+        const float y = turn_s[t * heads * dim + i];
+        r = side ? __builtin_elementwise_maximum(r, y) : __builtin_elementwise_minimum(r, y);
+      }
+      store<T>(b, r);
+    }
+  }
+}
+
+// Any strides, alignment and rotary dims: a thread per pair or copied dim, one token after another.
 template <typename T>
 __global__ __launch_bounds__(256) void append_kernel(AppendParams P) {
   __shared__ float2 turn[128];
-  const int page = (int)P.c.page_size, dim = (int)P.c.head_dim, kvh = (int)P.c.kv_heads, half = P.rotary >> 1;
-  const int row = P.of.find(blockIdx.x, 1, page, 2);
-  int first;
-  const int n = P.of.count(row, &first);
-  const int64_t start = P.starts[row];
-  const int64_t unit = (int64_t)blockIdx.x - (first / page + 2 * row);
-  // floor(start / page), negative positions too
-  const int64_t logical = (start >> __builtin_ctz(page)) + unit;
-  const int from = (int)max((int64_t)0, logical * page - start), to = (int)min((int64_t)n, (logical + 1) * page - start);
-  if (from >= to) return;
-  const int32_t id = logical >= 0 && logical < P.table_pages ? P.table[row * P.table_row + logical] : -1;
-  const bool place = id >= 0 && id < P.c.pages;
-  T* kp = reinterpret_cast<T*>(P.c.k_pages) + (int64_t)id * P.c.k_page;
-  T* vp = reinterpret_cast<T*>(P.c.v_pages) + (int64_t)id * P.c.v_page;
-  for (int i = from; i < to; i++) {
-    const int64_t token = first + i, pos = start + i;
-    const int slot = (int)(pos - logical * page);
+  const int dim = (int)P.c.head_dim, kvh = (int)P.c.kv_heads, half = P.rotary >> 1;
+  const Run run = run_of(P, blockIdx.x);
+  const bool place = run.id >= 0;
+  const int slot0 = (int)(run.start + run.from - run.logical * P.c.page_size);
+  T* kp = reinterpret_cast<T*>(P.c.k_pages) + (int64_t)run.id * P.c.k_page;
+  T* vp = reinterpret_cast<T*>(P.c.v_pages) + (int64_t)run.id * P.c.v_page;
+  for (int i = run.from; i < run.to; i++) {
+    const int64_t token = run.first + i, pos = run.start + i;
+    const int slot = slot0 + i - run.from;
     __syncthreads();
     for (int e = threadIdx.x; e < half; e += 256) {
       const double t = (double)pos * P.inv_freq[e] * 0.15915494309189533577;
@@ -73,23 +321,55 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams P) {
         vp[h * P.c.v_head + slot * P.c.v_token + d] = reinterpret_cast<const T*>(P.v)[token * P.v_token + h * P.v_head + d];
       }
   }
-  if (!place || P.c.k_bounds == nullptr) return;
+  if (!place || P.c.k_bounds == nullptr || run.from >= run.to) return;
   __syncthreads();
-  T* bp = reinterpret_cast<T*>(P.c.k_bounds) + (int64_t)id * P.c.b_page;
-  const int slot0 = (int)(start + from - logical * page);
+  T* bp = reinterpret_cast<T*>(P.c.k_bounds) + (int64_t)run.id * P.c.b_page;
   for (int u = threadIdx.x; u < kvh * dim; u += 256) {
     const int h = u / dim, d = u - h * dim;
     T* b = bp + h * P.c.b_head + d;
     const T* x = kp + h * P.c.k_head + d;
-    float lo = slot0 == 0 ? to_f32(x[0]) : to_f32(b[0]), hi = slot0 == 0 ? lo : to_f32(b[dim]);
-    for (int s = slot0; s < slot0 + to - from; s++) {
+    float lo = to_f32(slot0 == 0 ? x[0] : b[0]), hi = to_f32(slot0 == 0 ? x[0] : b[dim]);
+    for (int s = slot0; s < slot0 + run.to - run.from; s++) {
       const float y = to_f32(x[s * P.c.k_token]);
-      lo = y < lo || y != y ? y : lo;
-      hi = y > hi || y != y ? y : hi;
+      lo = __builtin_elementwise_minimum(lo, y);
+      hi = __builtin_elementwise_maximum(hi, y);
     }
     store<T>(b, lo);
     store<T>(b + dim, hi);
   }
+}
+
+template <typename T>
+static int launch_append(AppendParams& P, int64_t rows, int64_t tokens, hipStream_t st, const char* what) {
+  const int64_t page = P.c.page_size, kvh = P.c.kv_heads;
+  P.runs = (int)(P.of.cu ? tokens / page + 2 * rows : rows * (P.of.each / page + 2));
+  bool vec = P.rotary % (P.interleaved ? 8 : 16) == 0 && aligned(P.k, 16) && aligned(P.v, 16) &&
+             ((P.k_token | P.k_head | P.v_token | P.v_head) & 7) == 0;
+  if (P.heads > 0) vec = vec && aligned(P.q, 16) && aligned(P.q_out, 16) && ((P.q_token | P.q_head | P.o_token | P.o_head) & 7) == 0;
+  if (!vec) {
+    hipLaunchKernelGGL((append_kernel<T>), dim3((unsigned)P.runs), dim3(256), 0, st, P);
+    return check_launch(what);
+  }
+  const int64_t units = (P.interleaved ? P.rotary / 8 : P.rotary / 16) + (P.c.head_dim - P.rotary) / 8, in_flight = 256 / units;
+  // KV heads of a workgroup: as many as have places among its threads, fewer where runs are long and few
+  int64_t heads = kvh < in_flight ? kvh : in_flight;
+  while (heads > 1 && tokens >= 8 * rows && P.runs * ((kvh + heads - 1) / heads) < 4 * device_cus()) heads = (heads + 1) / 2;
+  P.group_heads = (int)heads;
+  P.head_groups = (int)((kvh + heads - 1) / heads);
+  // tokens of a workgroup of queries: kAhead places for each thread
+  int64_t q_tokens = 1;
+  if (P.heads > 0) {
+    q_tokens = kAhead * in_flight / P.heads;
+    if (tokens / (q_tokens > 0 ? q_tokens : 1) < 2 * device_cus()) q_tokens = 1;
+    const int64_t most = P.rotary > 0 && kTurnFloats / P.rotary < 64 ? kTurnFloats / P.rotary : 64;
+    q_tokens = q_tokens < 1 ? 1 : q_tokens > most ? most : q_tokens;
+  }
+  P.q_tokens = (int)q_tokens;
+  const int64_t blocks = (int64_t)P.runs * P.head_groups + (P.heads > 0 ? (tokens + q_tokens - 1) / q_tokens : 0);
+  TT_REQUIRE(blocks < (1 << 24), "%s: too many tokens and heads for one call", what);
+  if (P.interleaved) hipLaunchKernelGGL((append_vec_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, P);
+  else hipLaunchKernelGGL((append_vec_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, P);
+  return check_launch(what);
 }
 
 }  // namespace tt
@@ -129,9 +409,6 @@ extern "C" int tt_rotary_append_paged(const tt_paged_cache* cache, const void* q
   P.of = RowTokens{cu_tokens, (int)rows, (int)tokens, cu_tokens ? 0 : (int)(tokens / rows)};
   P.heads = (int)heads; P.rotary = (int)rotary; P.interleaved = interleaved != 0;
   P.inv_freq = inv_freq; P.amplitude = amplitude;
-  const dim3 grid((unsigned)(tokens / cache->page_size + 2 * rows));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache->dtype == TT_F16) hipLaunchKernelGGL((append_kernel<f16_t>), grid, dim3(256), 0, st, P);
-  else hipLaunchKernelGGL((append_kernel<bf16_t>), grid, dim3(256), 0, st, P);
-  return check_launch(what);
+  return cache->dtype == TT_F16 ? launch_append<f16_t>(P, rows, tokens, st, what) : launch_append<bf16_t>(P, rows, tokens, st, what);
 }

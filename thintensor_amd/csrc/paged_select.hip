@@ -1,6 +1,5 @@
 // Selecting the pages that a query reads by the bounds of their keys.
-#include "paged.h"
-#include "tt_common.h"
+#include "paged_attention.h"
 
 namespace tt {
 
@@ -13,8 +12,8 @@ struct SelectParams {
   int table_pages, page_shift;
   const int32_t* lengths;
   int max_length, per_kv, first, last, count;
-  float* scores;
-  int64_t scores_row;          // of one (row, KV head)
+  uint32_t* keys;              // scores as integers in their order
+  int64_t keys_row;            // of one (row, KV head)
   int32_t* selected;
 };
 
@@ -30,66 +29,267 @@ __device__ __forceinline__ uint32_t score_key(float s) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-template <typename T>
+// Scores.  A workgroup takes 64 pages of a row and KV head, whose bounds it brings to LDS in whole rows; a lane then
+// has a page and a wave a quarter of the dims.  max(q low, q high) = q (high + low) / 2 + |q| (high - low) / 2, two
+// binary64 fmas with what LDS holds of half the queries, the same for all lanes; both are exact but for the addition.
+// With bounds or queries that are not finite the equation fails, and such lanes form their sums once more by the
+// definition.  What bounds it is memory where there are many pages, 4 D bytes each, and the reads of the queries.  (8 x 10 x 2048 pages of 128, four
+// heads each: lanes that read their own pages' bounds in turns of sixteen bytes, 43 us, since every line came to the CU
+// four times over; queries through scalar registers, 103; two pages a lane, with room for one workgroup in LDS, 47; now
+// 26, its bytes 17.)
+template <typename T, int D, int GH>
 __global__ __launch_bounds__(256) void page_score_kernel(SelectParams P) {
-  const int row = blockIdx.z, kvh = blockIdx.y, dim = (int)P.c.head_dim;
-  const int p = blockIdx.x * 256 + threadIdx.x;
-  if (p >= row_pages(P, row)) return;
-  const int32_t id = P.table[row * P.table_row + p];
-  float best = __builtin_bit_cast(float, 0x7fc00000u);
-  if (id >= 0 && id < P.c.pages) {
-    const T* b = reinterpret_cast<const T*>(P.c.k_bounds) + (int64_t)id * P.c.b_page + kvh * P.c.b_head;
-    best = __builtin_bit_cast(float, 0xff800000u);
-    for (int g = 0; g < P.per_kv; g++) {
-      const T* q = reinterpret_cast<const T*>(P.q) + row * P.q_token + (kvh * P.per_kv + g) * P.q_head;
-      double sum = 0.0;
-      for (int d = 0; d < dim; d++) {
-        const double x = (double)to_f32(q[d]), lo = x * (double)to_f32(b[d]), hi = x * (double)to_f32(b[dim + d]);
-        sum += lo > hi || lo != lo ? lo : hi;
-      }
-      const float s = (float)sum;
-      best = s > best || s != s ? s : best;
+  constexpr int QD = D / 4, PIECES = QD / 8;
+  constexpr int RP = D / 4, RR = 256 / RP, NR = 64 / RR;      // pieces of a page's bounds, pages of a request, requests
+  constexpr int BS = 4 * D + 16;                                   // LDS bytes of a page: reads of a column take all banks alike
+  typedef double d2_t __attribute__((ext_vector_type(2)));
+  __shared__ __attribute__((aligned(16))) char b_s[64 * BS];
+  __shared__ __attribute__((aligned(16))) double q_s[D][GH];       // halves
+  __shared__ double part_s[4][GH][64];
+  __shared__ int odd_q;
+  const int row = blockIdx.z, kvh = blockIdx.y, p0 = blockIdx.x * 64;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int pages = row_pages(P, row);
+  if (p0 >= pages) return;
+  auto page_of = [&](int p) __attribute__((always_inline)) {
+    const int32_t id = P.table[row * P.table_row + min(p, pages - 1)];
+    return id < 0 || id >= P.c.pages ? -1 : id;
+  };
+  {
+    const int l_row = threadIdx.x / RP, l_piece = threadIdx.x % RP;
+    const char* base = reinterpret_cast<const char*>(P.c.k_bounds) + 2 * kvh * P.c.b_head + 16 * l_piece;
+    constexpr int AT_ONCE = NR < 8 ? NR : 8;
+#pragma unroll
+    for (int r0 = 0; r0 < NR; r0 += AT_ONCE) {
+      u4_t v[AT_ONCE];
+#pragma unroll
+      for (int r = 0; r < AT_ONCE; r++)
+        v[r] = *reinterpret_cast<const u4_t*>(base + 2 * (int64_t)max(page_of(p0 + (r0 + r) * RR + l_row), 0) * P.c.b_page);
+#pragma unroll
+      for (int r = 0; r < AT_ONCE; r++) *reinterpret_cast<u4_t*>(b_s + ((r0 + r) * RR + l_row) * BS + 16 * l_piece) = v[r];
     }
   }
-  P.scores[((int64_t)row * P.c.kv_heads + kvh) * P.scores_row + p] = best;
+  const char* const mine = b_s + lane * BS + 2 * wave * QD;
+  uint32_t best = 0;
+  for (int h0 = 0; h0 < P.per_kv; h0 += GH) {
+    __syncthreads();
+    if (threadIdx.x == 0) odd_q = 0;
+    __syncthreads();
+    for (int u = threadIdx.x; u < GH * D; u += 256) {      // heads past the last repeat it, which changes no maximum
+      const int h = min(h0 + u / D, P.per_kv - 1), d = u % D;
+      const float x = to_f32(reinterpret_cast<const T*>(P.q)[row * P.q_token + (kvh * P.per_kv + h) * P.q_head + d]);
+      if (!(__builtin_fabsf(x) < __builtin_bit_cast(float, 0x7f800000u))) odd_q = 1;
+      q_s[d][u / D] = 0.5 * (double)x;
+    }
+    __syncthreads();
+    double sum[GH];
+#pragma unroll
+    for (int h = 0; h < GH; h++) sum[h] = 0.0;
+    bool odd = false;
+#pragma unroll 1
+    for (int x = 0; x < PIECES; x++) {
+      const u4_t lo = *reinterpret_cast<const u4_t*>(mine + 16 * x), hi = *reinterpret_cast<const u4_t*>(mine + 2 * D + 16 * x);
+      odd |= any_not_finite<T>(lo) || any_not_finite<T>(hi);
+      const double* q = q_s[wave * QD + 8 * x];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const double a = (double)((e & 1) ? hi_f32<T>(lo[e >> 1]) : lo_f32<T>(lo[e >> 1]));
+        const double b = (double)((e & 1) ? hi_f32<T>(hi[e >> 1]) : lo_f32<T>(hi[e >> 1]));
+#pragma unroll
+        for (int h = 0; h < GH; h += 2) {
+          const d2_t qq = *reinterpret_cast<const d2_t*>(q + GH * e + h);
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+            sum[h + i] = __builtin_fma(__builtin_fabs(qq[i]), b - a, __builtin_fma(qq[i], b + a, sum[h + i]));
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < GH; h++) part_s[wave][h][lane] = sum[h];
+    if (odd || odd_q != 0) {
+      const T* at = reinterpret_cast<const T*>(mine);
+#pragma unroll 1
+      for (int h = 0; h < GH; h++) {
+        double t = 0.0;
+#pragma unroll 1
+        for (int d = 0; d < QD; d++) {
+          const double q = 2.0 * q_s[wave * QD + d][h], x = q * (double)to_f32(at[d]), y = q * (double)to_f32(at[D + d]);
+          t += x > y || x != x ? x : y;
+        }
+        part_s[wave][h][lane] = t;
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+#pragma unroll
+      for (int h = 0; h < GH; h++) {
+        const int at = threadIdx.x;
+        const uint32_t k = score_key((float)((part_s[0][h][at] + part_s[1][h][at]) + (part_s[2][h][at] + part_s[3][h][at])));
+        best = k > best ? k : best;
+      }
+    }
+  }
+  const int p = p0 + threadIdx.x;
+  if (threadIdx.x < 64 && p < pages)
+    P.keys[((int64_t)row * P.c.kv_heads + kvh) * P.keys_row + p] = page_of(p) < 0 ? 0xffffffffu : best;
 }
 
-// A page is kept where fewer than the free places go to better ones.
-__global__ __launch_bounds__(256) void page_pick_kernel(SelectParams P) {
-  const int row = blockIdx.y, kvh = blockIdx.x;
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
+#define TT_STEP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
+  TT_STEP(0x111, 0xF) TT_STEP(0x112, 0xF) TT_STEP(0x114, 0xF) TT_STEP(0x118, 0xF)     // within rows of 16
+#undef TT_STEP
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);      // row 0's sum to row 1, row 2's to row 3
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);      // the first half's to the second
+  return v;
+}
+
+// The least kept score is found digit by digit: digits of eight bits of key - least key, from the highest that is set
+// anywhere, so that the first one already spreads; histograms in LDS, one for each digit, searched by every wave for
+// itself, so that a digit takes one barrier.  Then every thread counts what is kept of its run of pages, and the runs
+// are written one after another.  Keys stay in registers up to HELD a thread.  What bounds it is the chain of
+// barriers and round trips.
+template <int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void page_pick_kernel(SelectParams P) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ __attribute__((aligned(16))) uint32_t hist[4][256];
+  __shared__ uint32_t ends[2][WAVES], counts[2][WAVES];
+  const int row = blockIdx.y, kvh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t at = (int64_t)row * P.c.kv_heads + kvh;
-  const float* s = P.scores + at * P.scores_row;
+  const uint32_t* keys = P.keys + at * P.keys_row;
   int32_t* out = P.selected + at * P.count;
   const int pages = row_pages(P, row), first = min(P.first, pages), last = max(first, pages - P.last);
-  const int places = P.count - (first + pages - last);
-  __shared__ int base, part[4];
-  if (threadIdx.x == 0) base = 0;
-  for (int p0 = 0; p0 < pages; p0 += 256) {
-    const int p = p0 + threadIdx.x;
-    bool keep = p < pages && (p < first || p >= last);
-    if (p < pages && !keep) {
-      const uint32_t mine = score_key(s[p]);
-      int better = 0;
-      for (int o = first; o < last; o++) {
-        const uint32_t k = score_key(s[o]);
-        better += k > mine || (k == mine && o < p);
+  const int places = P.count - (first + pages - last), per = (pages + THREADS - 1) / THREADS;
+  const int p0 = min(tid * per, pages), p1 = min(p0 + per, pages);
+  uint32_t held[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; k++) held[k] = pages > 0 ? keys[min(p0 + k, pages - 1)] : 0;
+  for (int i = tid; i < 4 * 256; i += THREADS) (&hist[0][0])[i] = 0;
+  auto each = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < HELD; k++)
+      if (p0 + k < p1) f(p0 + k, held[k]);
+    for (int p = p0 + HELD; p < p1; p++) f(p, keys[p]);
+  };
+  // kept: the forced ones, keys past `least`, and the first `want` of those that equal it
+  uint32_t least = 0;
+  int want = 0;
+  if (places >= last - first) {
+    want = last - first;                     // everything: equal ones are all that are not greater
+    least = 0xffffffffu;
+  } else if (places > 0) {
+    uint32_t lo = 0xffffffffu, hi = 0;
+    each([&](int p, uint32_t k) {
+      if (p >= first && p < last) {
+        lo = min(lo, k);
+        hi = max(hi, k);
       }
-      keep = better < places;
+    });
+    lo = ~(uint32_t)(wave_max_u64(~lo));
+    hi = (uint32_t)wave_max_u64(hi);
+    if (lane == 0) {
+      ends[0][wave] = lo;
+      ends[1][wave] = hi;
     }
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(keep);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane == 0) part[wave] = __popcll(mask);
     __syncthreads();
-    int put = base;
-    for (int w = 0; w < wave; w++) put += part[w];
-    put += __popcll(mask & ((1ull << lane) - 1));
-    if (keep) out[put] = p;
-    __syncthreads();
-    if (threadIdx.x == 0) base += part[0] + part[1] + part[2] + part[3];
-    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+      lo = min(lo, ends[0][w]);
+      hi = max(hi, ends[1][w]);
+    }
+    uint32_t prefix = 0, mask = 0;
+    int shift = hi > lo ? max(0, 24 - __builtin_clz(hi - lo)) : 0;
+    want = places;
+#pragma unroll 1
+    for (int step = 0; step < 4; step++) {
+      uint32_t* const h = hist[step];
+      each([&](int p, uint32_t k) {
+        const uint32_t x = k - lo;
+        if (p >= first && p < last && (x & mask) == prefix) atomicAdd(&h[(x >> shift) & 255], 1u);
+      });
+      __syncthreads();
+      // lane l holds the four bins from 252 - 4 l on, so that sums over the lanes run from the top
+      const u4_t bins = *reinterpret_cast<const u4_t*>(h + 252 - 4 * lane);
+      const uint32_t four = bins[0] + bins[1] + bins[2] + bins[3];
+      const uint32_t upto = lanes_before(four), above = upto - four;
+      const uint64_t reached = __builtin_amdgcn_ballot_w64(upto >= (uint32_t)want);
+      const int where = __builtin_ctzll(reached);
+      uint32_t digit = 0, over = above;
+      bool done = false;
+#pragma unroll
+      for (int i = 3; i >= 0; i--) {
+        if (!done && over + bins[i] >= (uint32_t)want) {
+          digit = 252 - 4 * lane + i;
+          done = true;
+        }
+        if (!done) over += bins[i];
+      }
+      digit = __builtin_amdgcn_readlane(digit, where);
+      over = __builtin_amdgcn_readlane(over, where);
+      prefix |= digit << shift;
+      mask |= 255u << shift;
+      want -= (int)over;
+      if (shift == 0) break;
+      // the next eight bits; the last digit may repeat some of those before
+      shift = max(0, shift - 8);
+    }
+    least = prefix + lo;
+  } else {
+    least = 0xffffffffu;
+  }
+  auto kind = [&](int p, uint32_t k) __attribute__((always_inline)) {      // 2: kept, 1: if among the first
+    if (p < first || p >= last) return 2;
+    if (places >= last - first) return 2;
+    return places <= 0 ? 0 : k > least ? 2 : k == least ? 1 : 0;
+  };
+  uint32_t greater = 0, equal = 0;
+  each([&](int p, uint32_t k) {
+    const int c = kind(p, k);
+    greater += c == 2;
+    equal += c == 1;
+  });
+  const uint32_t g = lanes_before(greater), e = lanes_before(equal);
+  if (lane == 63) {
+    counts[0][wave] = g;
+    counts[1][wave] = e;
   }
   __syncthreads();
-  for (int i = base + threadIdx.x; i < P.count; i += 256) out[i] = -1;
+  uint32_t put = g - greater, eq = e - equal, kept = 0, ties = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) {
+    const uint32_t a = counts[0][w], b = counts[1][w];
+    if (w < wave) {
+      put += a;
+      eq += b;
+    }
+    kept += a;
+    ties += b;
+  }
+  put += min(eq, (uint32_t)want);
+  each([&](int p, uint32_t k) {
+    const int c = kind(p, k);
+    const bool keep = c == 2 || (c == 1 && eq < (uint32_t)want);
+    eq += c == 1;
+    if (keep) out[put++] = p;
+  });
+  for (int i = (int)(kept + min(ties, (uint32_t)want)) + tid; i < P.count; i += THREADS) out[i] = -1;
+}
+
+template <typename T, int D, int GH>
+static void launch_score(const SelectParams& P, int64_t most, int64_t rows, hipStream_t st) {
+  const dim3 grid((unsigned)((most + 63) / 64), (unsigned)P.c.kv_heads, (unsigned)rows);
+  hipLaunchKernelGGL((page_score_kernel<T, D, GH>), grid, dim3(256), 0, st, P);
+}
+template <typename T, int D>
+static void launch_score(const SelectParams& P, int64_t most, int64_t rows, hipStream_t st) {
+  if (P.per_kv <= 4) launch_score<T, D, 4>(P, most, rows, st);
+  else launch_score<T, D, 8>(P, most, rows, st);
+}
+template <typename T>
+static void launch_score(const SelectParams& P, int64_t most, int64_t rows, hipStream_t st) {
+  if (P.c.head_dim == 64) launch_score<T, 64>(P, most, rows, st);
+  else if (P.c.head_dim == 128) launch_score<T, 128>(P, most, rows, st);
+  else launch_score<T, 256>(P, most, rows, st);
 }
 
 static int check_select(const tt_paged_cache* c, int64_t table_pages, int64_t rows, int64_t heads, int64_t max_length,
@@ -140,13 +340,14 @@ extern "C" int tt_select_pages(const tt_paged_cache* cache, const void* q, int64
   P.max_length = (int)(max_length < table_pages * cache->page_size ? max_length : table_pages * cache->page_size);
   P.per_kv = (int)(heads / cache->kv_heads); P.first = (int)first_pages; P.last = (int)last_pages;
   P.count = (int)selected_count;
-  P.scores = scratch; P.scores_row = most; P.selected = selected;
+  P.keys = reinterpret_cast<uint32_t*>(scratch); P.keys_row = most; P.selected = selected;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)((most + 255) / 256), (unsigned)cache->kv_heads, (unsigned)rows);
-  if (cache->dtype == TT_F16) hipLaunchKernelGGL((page_score_kernel<f16_t>), grid, dim3(256), 0, st, P);
-  else hipLaunchKernelGGL((page_score_kernel<bf16_t>), grid, dim3(256), 0, st, P);
+  if (cache->dtype == TT_F16) launch_score<f16_t>(P, most, rows, st);
+  else launch_score<bf16_t>(P, most, rows, st);
   const int err = check_launch(what);
   if (err) return err;
-  hipLaunchKernelGGL(page_pick_kernel, dim3((unsigned)cache->kv_heads, (unsigned)rows), dim3(256), 0, st, P);
+  const dim3 pairs((unsigned)cache->kv_heads, (unsigned)rows);
+  if (most <= 256 * 8) hipLaunchKernelGGL((page_pick_kernel<256, 8>), pairs, dim3(256), 0, st, P);
+  else hipLaunchKernelGGL((page_pick_kernel<1024, 8>), pairs, dim3(1024), 0, st, P);
   return check_launch(what);
 }
