@@ -39,7 +39,7 @@ struct PagedParams {
   const int32_t* selected;
   int selected_count;
   int heads, per_kv, window, shared, max_length;     // shared: tokens
-  int q_vec;                                         // vectors of q start on 16-byte boundaries
+  int q_vec, out_vec;                                // vectors of q start on 16-byte boundaries, of out on 8-byte ones
   float scale_log2;                                  // scale * log2(e)
   const void* sinks;
   int sink_dtype;
@@ -55,10 +55,13 @@ struct PagedParams {
 
 template <typename T> struct Bits16;
 template <> struct Bits16<f16_t> {
-  static constexpr uint32_t kExp = 0x7c00, kOne = 0x3c00, k128 = 0x5800, k16384 = 0x7400;
+  static constexpr uint32_t kExp = 0x7c00;
   // (weights come from an exponential: there is no product or sum before the conversion to fold into it)
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, h2));
+  }
+  static __device__ __forceinline__ float add_pair(uint32_t w, float c) {      // c + both halves
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), (h2){(_Float16)1.0f, (_Float16)1.0f}, c, false);
   }
   static __device__ __forceinline__ f4_t mfma16(u4_t a, u4_t b, f4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
@@ -68,9 +71,12 @@ template <> struct Bits16<f16_t> {
   }
 };
 template <> struct Bits16<bf16_t> {
-  static constexpr uint32_t kExp = 0x7f80, kOne = 0x3f80, k128 = 0x4300, k16384 = 0x4680;
+  static constexpr uint32_t kExp = 0x7f80;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, b2_t));
+  }
+  static __device__ __forceinline__ float add_pair(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2_t, w), (b2_t){(__bf16)1.0f, (__bf16)1.0f}, c, false);
   }
   static __device__ __forceinline__ f4_t mfma16(u4_t a, u4_t b, f4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
@@ -85,6 +91,15 @@ __device__ __forceinline__ float sink_log2(const PagedParams& P, int h) {
                   : P.sink_dtype == TT_BF16 ? to_f32(reinterpret_cast<const bf16_t*>(P.sinks)[h])
                                             : to_f32(reinterpret_cast<const f16_t*>(P.sinks)[h]);
   return v * 0x1.715476p+0f;
+}
+
+template <typename T> __device__ __forceinline__ void store_four(T* p, f4_t v, int vec) {
+  if (vec) {
+    *reinterpret_cast<u2_t*>(p) = (u2_t){bits16<T>(v[0]) | (bits16<T>(v[1]) << 16), bits16<T>(v[2]) | (bits16<T>(v[3]) << 16)};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) store<T>(p + e, v[e]);
+  }
 }
 
 // What a query head's sums become: o scale[0], where m is the maximum that o and l carry.  A query that saw
@@ -159,35 +174,45 @@ template <typename T> __device__ __forceinline__ bool any_not_finite(u4_t v) {
   return r;
 }
 
-// Values of tokens that some columns of a tile see and others do not: a weight of 0 would turn an infinite or
-// NaN value into NaN for those that do not see it.  Such values are taken out (`clean`), and where they lie
-// goes to a second operand: 1 for infinity, 128 for minus infinity, 16384 for NaN, of which a product with ones
-// for what a column sees counts no more than 32.
-template <typename T>
-__device__ __forceinline__ void take_odd(u4_t v, u4_t& clean, u4_t& odd) {
-  using B = Bits16<T>;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    uint32_t c = 0, n = 0;
-#pragma unroll
-    for (int h = 0; h < 32; h += 16) {
-      const uint32_t x = (v[i] >> h) & 0xffffu;
-      const bool is_odd = (x & B::kExp) == B::kExp, frac = (x & 0x7fffu) != B::kExp;
-      c |= (is_odd ? 0u : x) << h;
-      n |= (!is_odd ? 0u : frac ? B::k16384 : x >> 15 ? B::k128 : B::kOne) << h;
+// Values of tokens that some columns of a tile see and others do not: a weight of 0 would turn an infinite or NaN
+// value into NaN for those that do not see it.  Such values are taken out of the tile, and what they make of the columns
+// that see them is noted in LDS, two bits for each column and dim: 1 infinity, 2 minus infinity, 3 NaN.  So is, for
+// all dims, that a column sees a token which lies in no page.
+struct Marks {
+  uint32_t* bits;                // [columns][words]: sixteen dims a word
+  const Seen* see;               // [columns]
+  int columns, words;
+  __device__ __forceinline__ void no_page(int t, int tokens) const {      // of tokens t .. t + tokens - 1
+#pragma unroll 1
+    for (int c = 0; c < columns; c++) {
+      const Seen s = see[c];
+      if (s.lo < t + tokens && s.hi > t && s.hi > s.lo)
+#pragma unroll 1
+        for (int w = 0; w < words; w++) atomicOr(&bits[c * words + w], 0xffffffffu);
     }
-    clean[i] = c;
-    odd[i] = n;
   }
-}
-// o with what such values among a column's tokens make of it
-__device__ __forceinline__ float with_odd(float o, float count) {
-  const bool neg = count >= 128.0f, pos = __builtin_amdgcn_fractf(count * 0.0078125f) > 0.0f;
-  if (count >= 16384.0f || (pos && neg)) return __builtin_bit_cast(float, 0x7fc00000u);
-  if (pos) return o + __builtin_bit_cast(float, 0x7f800000u);
-  if (neg) return o + __builtin_bit_cast(float, 0xff800000u);
-  return o;
-}
+  // eight values of token t from dim d on, in LDS
+  template <typename T> __device__ __forceinline__ void take_odd(uint16_t* v, int t, int d) const {
+    using B = Bits16<T>;
+#pragma unroll 1
+    for (int e = 0; e < 8; e++) {
+      const uint32_t x = v[e];
+      if ((x & B::kExp) != B::kExp) continue;
+      v[e] = 0;
+      const uint32_t kind = (x & 0x7fffu) != B::kExp ? 3u : x >> 15 ? 2u : 1u;
+#pragma unroll 1
+      for (int c = 0; c < columns; c++) {
+        const Seen s = see[c];
+        if (t >= s.lo && t < s.hi) atomicOr(&bits[c * words + (d + e) / 16], kind << (2 * ((d + e) % 16)));
+      }
+    }
+  }
+  __device__ __forceinline__ float marked(float o, int c, int d) const {
+    const uint32_t kind = (bits[c * words + d / 16] >> (2 * (d % 16))) & 3u;
+    const float inf = __builtin_bit_cast(float, 0x7f800000u);
+    return kind == 0 ? o : kind == 1 ? o + inf : kind == 2 ? o - inf : __builtin_bit_cast(float, 0x7fc00000u);
+  }
+};
 
 // paged_few.hip: up to few_columns() columns of a row and KV head; paged_many.hip: any number
 constexpr int few_columns(int64_t head_dim) { return head_dim == 64 ? 64 : head_dim == 128 ? 32 : 16; }

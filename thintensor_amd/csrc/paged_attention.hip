@@ -58,9 +58,8 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedParams P) {
 #pragma unroll
   for (int k = 1; k < ROWS; k++) acc += sum[k][piece];
   const float f = finish_scale(P, head, M, l);
-  T* out = reinterpret_cast<T*>(P.out) + token * P.out_token + head * P.out_head + 4 * piece;
-#pragma unroll
-  for (int x = 0; x < 4; x++) store<T>(out + x, l == 0.0f ? 0.0f : acc[x] * f);
+  if (l == 0.0f) acc = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
+  store_four<T>(reinterpret_cast<T*>(P.out) + token * P.out_token + head * P.out_head + 4 * piece, acc * f, P.out_vec);
 }
 
 template <typename T, int D>
@@ -230,6 +229,7 @@ extern "C" int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q
   P.heads = (int)heads; P.per_kv = (int)(heads / cache->kv_heads);
   P.max_length = (int)p.limit; P.window = (int)p.window; P.shared = (int)p.shared;
   P.q_vec = aligned(q, 16) && ((q_token | q_head) & 7) == 0;
+  P.out_vec = aligned(out, 8) && ((out_token | out_head) & 3) == 0;
   P.scale_log2 = (float)((double)scale * 1.4426950408889634);
   P.sinks = sinks; P.sink_dtype = sink_dtype;
   P.out = out; P.out_token = out_token; P.out_head = out_head;

@@ -44,6 +44,9 @@ void paged_few_kernel(PagedParams P) {
   static_assert(kWaves * 16 * OS * 4 <= kWaves * kTile * VS, "the join fits where V was");
   __shared__ __attribute__((aligned(16))) char lds[kWaves * kTile * VS];
   __shared__ float m_s[kWaves][16], l_s[kWaves][16];
+  __shared__ Seen see_s[MIXED ? 16 * NB : 1];
+  __shared__ uint32_t marks_s[16 * NB * (D / 16)];
+  __shared__ int marked;
   const int kvh = blockIdx.x / P.row_tiles, cb = blockIdx.x % P.row_tiles, row = blockIdx.y, split = blockIdx.z;
   const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -118,6 +121,16 @@ void paged_few_kernel(PagedParams P) {
     tile1 = tile0;
   }
 
+  // ---- marks
+  for (int i = threadIdx.x; i < 16 * NB * (D / 16); i += 64 * kWaves) marks_s[i] = 0;
+  if (threadIdx.x == 0) marked = 0;
+  if (MIXED && wave == 0 && quad == 0) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) see_s[16 * b + n] = see[b];
+  }
+  __syncthreads();
+  const Marks marks{marks_s, see_s, cols, D / 16};
+
   // ---- tiles
   const uint32_t k_at = (uint32_t)n * (uint32_t)(2 * P.c.k_token) + 16 * quad, v_step = (uint32_t)(2 * P.c.v_token);
   const int v_row = lane / PC, v_piece = lane % PC;
@@ -184,7 +197,17 @@ void paged_few_kernel(PagedParams P) {
       }
     load_k(next);
     const int t0 = now[0].t, t1 = now[1].t;
-    const bool whole = t0 >= lo_most && t0 + 16 <= hi_least && t1 >= lo_most && t1 + 16 <= hi_least && !now[0].bad && !now[1].bad;
+    const bool whole = t0 >= lo_most && t0 + 16 <= hi_least && t1 >= lo_most && t1 + 16 <= hi_least;
+    if (now[0].bad || now[1].bad) {                          // a column that sees a token in no page is NaN
+      if constexpr (MIXED) {
+        if (now[0].bad) marks.no_page(t0, 16);
+        if (now[1].bad) marks.no_page(t1, 16);
+        marked = 1;
+      } else if ((now[0].bad && t0 < hi_most && t0 + 16 > lo_least) || (now[1].bad && t1 < hi_most && t1 + 16 > lo_least)) {
+        for (int w = lane; w < 16 * NB * (D / 16); w += 64) marks_s[w] = 0xffffffffu;
+        marked = 1;
+      }
+    }
     bool odd = false;
     if (!whole) {
       // tokens out of every column's sight: no value (what lies there may be NaN)
@@ -194,35 +217,38 @@ void paged_few_kernel(PagedParams P) {
         if (t < lo_least || t >= hi_most) vr[k] = (u4_t){0u, 0u, 0u, 0u};
         if (MIXED) odd |= any_not_finite<T>(vr[k]);
       }
-      odd = MIXED && __builtin_amdgcn_ballot_w64(odd) != 0;
     }
     wave_lds_order();
 #pragma unroll
     for (int k = 0; k < VK; k++) *reinterpret_cast<u4_t*>(put + k * VR * VS) = vr[k];
+    if constexpr (MIXED) {
+      if (odd) {
+        marked = 1;
+#pragma unroll 1
+        for (int k = 0; k < VK; k++) {
+          const int h = k * VR / 16;
+          marks.take_odd<T>(reinterpret_cast<uint16_t*>(put + k * VR * VS), (h ? t1 : t0) + k * VR - 16 * h + v_row, 8 * v_piece);
+        }
+      }
+    }
     wave_lds_order();
     load_v(next);
-    const bool bad0 = now[0].bad, bad1 = now[1].bad;
     now[0] = next[0];
     now[1] = next[1];
     place(i + 2 * kWaves, next);
 
-    u4_t pw[NB], vis[NB];
+    u4_t pw[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
       float s[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) s[e] = sc[b][e >> 2][e & 3];
       if (!whole) {
-        uint32_t ones[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const int t = (e < 4 ? t0 : t1) + 4 * quad + (e & 3);
-          const bool in = t >= see[b].lo && t < see[b].hi;
-          if (e < 4 ? bad0 : bad1) s[e] = __builtin_bit_cast(float, 0x7fc00000u);
-          if (!in) s[e] = ninf;
-          ones[e >> 1] |= in ? (uint32_t)B::kOne << (16 * (e & 1)) : 0u;
+          if (t < see[b].lo || t >= see[b].hi) s[e] = ninf;
         }
-        vis[b] = (u4_t){ones[0], ones[1], ones[2], ones[3]};
       }
       float top = s[0];
 #pragma unroll
@@ -246,31 +272,11 @@ void paged_few_kernel(PagedParams P) {
         pw[b][p] = w;
       }
     }
-    auto values = [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < VT; x++) {
       const u2_t va = lds_transposed(get + 32 * x), vb = lds_transposed(get + 16 * VS + 32 * x);
-      return (u4_t){va[0], va[1], vb[0], vb[1]};
-    };
-    if (!MIXED || !odd) {
 #pragma unroll
-      for (int x = 0; x < VT; x++) {
-        const u4_t v = values(x);
-#pragma unroll
-        for (int b = 0; b < NB; b++) o[b][x] = B::mfma16(v, pw[b], o[b][x]);
-      }
-    } else {
-#pragma unroll
-      for (int x = 0; x < VT; x++) {
-        __builtin_amdgcn_sched_barrier(0);     // one at a time: rare, and should cost no registers
-        u4_t clean, code;
-        take_odd<T>(values(x), clean, code);
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-          o[b][x] = B::mfma16(clean, pw[b], o[b][x]);
-          const f4_t count = B::mfma16(code, vis[b], (f4_t){0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-          for (int r = 0; r < 4; r++) o[b][x][r] = with_odd(o[b][x][r], count[r]);
-        }
-      }
+      for (int b = 0; b < NB; b++) o[b][x] = B::mfma16((u4_t){va[0], va[1], vb[0], vb[1]}, pw[b], o[b][x]);
     }
   }
 
@@ -304,11 +310,14 @@ void paged_few_kernel(PagedParams P) {
         l = __builtin_fmaf(l_s[w][cc], e, l);
       }
       const int tok = first + at, hd = kvh * G + c - at * G;
+      if (l == 0.0f) acc = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
+      if (marked) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[r] = marks.marked(acc[r], 16 * b + cc, d + r);
+      }
       if (only) {
         const float f = finish_scale(P, hd, M, l);
-        T* out = reinterpret_cast<T*>(P.out) + tok * P.out_token + hd * P.out_head + d;
-#pragma unroll
-        for (int r = 0; r < 4; r++) store<T>(out + r, l == 0.0f ? 0.0f : acc[r] * f);
+        store_four<T>(reinterpret_cast<T*>(P.out) + tok * P.out_token + hd * P.out_head + d, acc * f, P.out_vec);
       } else {
         const int64_t part = ((int64_t)tok * P.heads + hd) * P.parts + P.part0 + split;
         *reinterpret_cast<f4_t*>(P.part_o + part * D + d) = acc;

@@ -85,6 +85,13 @@ void paged_many_kernel(PagedParams P, int splits) {
   };
   const int hi_most = most(see.hi), hi_least = -most(-see.hi), lo_most = most(see.lo), lo_least = -most(-see.lo);
   __shared__ int reach[4][kWaves];
+  __shared__ Seen see_s[kManyColumns];
+  __shared__ uint32_t marks_s[kManyColumns * (D / 16)];
+  __shared__ int marked;
+  for (int i = threadIdx.x; i < kManyColumns * (D / 16); i += 64 * kWaves) marks_s[i] = 0;
+  if (threadIdx.x == 0) marked = 0;
+  if (half == 0) see_s[32 * wave + n] = see;
+  const Marks marks{marks_s, see_s, cols, D / 16};
   if (lane == 0) {
     reach[0][wave] = -lo_least;
     reach[1][wave] = hi_most;
@@ -109,61 +116,62 @@ void paged_many_kernel(PagedParams P, int splits) {
     return;
   }
 
+  // A wave brings 64 / PC rows of every request, which lie in one page, so that where they are is the wave's.
   const int32_t* table = P.table + (P.shared_job ? 0 : row * P.table_row);
-  const int l_row = threadIdx.x / PC, l_piece = threadIdx.x % PC;
-  const int page_mask = (1 << P.page_shift) - 1;
+  const int l_piece = lane % PC, w_row = lane / PC, l_row = wave * (64 / PC) + w_row;
   const uint32_t k_step = (uint32_t)(2 * P.c.k_token), v_step = (uint32_t)(2 * P.c.v_token);
-  const char* const kbase = reinterpret_cast<const char*>(P.c.k_pages) + 2 * kvh * P.c.k_head + 16 * l_piece;
-  const char* const vbase = reinterpret_cast<const char*>(P.c.v_pages) + 2 * kvh * P.c.v_head + 16 * l_piece;
+  const uint32_t k_at = (uint32_t)w_row * k_step + 16 * l_piece, v_at = (uint32_t)w_row * v_step + 16 * l_piece;
+  const int page_mask = (1 << P.page_shift) - 1;
+  const char* const kbase = reinterpret_cast<const char*>(P.c.k_pages) + 2 * kvh * P.c.k_head;
+  const char* const vbase = reinterpret_cast<const char*>(P.c.v_pages) + 2 * kvh * P.c.v_head;
   u4_t kr[NK], vr[NK];
   int ids[NK];
   auto look = [&](int tile) __attribute__((always_inline)) {      // the pages of a tile's rows
 #pragma unroll
     for (int k = 0; k < NK; k++) {
-      const int t = min(tile, tile1 - 1) * TT + k * RR + l_row;
-      ids[k] = table[min(max(t >> P.page_shift, 0), P.table_pages - 1)];
+      const int t = min(tile, tile1 - 1) * TT + k * RR + wave * (64 / PC);
+      ids[k] = table[min(t >> P.page_shift, P.table_pages - 1)];
     }
   };
-  uint64_t bad_now = 0;                    // whether a row of the loaded tile is in no page
   auto load = [&](int tile) __attribute__((always_inline)) {
-    bool bad = false;
 #pragma unroll
     for (int k = 0; k < NK; k++) {
-      const uint32_t slot = (uint32_t)((min(tile, tile1 - 1) * TT + k * RR + l_row) & page_mask);
-      const bool b = (uint32_t)ids[k] >= (uint32_t)P.c.pages;
-      const int64_t id = b ? 0 : ids[k];
-      bad |= b;
-      kr[k] = *reinterpret_cast<const u4_t*>(kbase + 2 * id * P.c.k_page + (size_t)(slot * k_step));
-      vr[k] = *reinterpret_cast<const u4_t*>(vbase + 2 * id * P.c.v_page + (size_t)(slot * v_step));
+      const int t = min(tile, tile1 - 1) * TT + k * RR + wave * (64 / PC);
+      const bool bad = (uint32_t)ids[k] >= (uint32_t)P.c.pages;
+      if (bad && tile < tile1) {           // (rare, and more than one lane may say so)
+        marks.no_page(t, 64 / PC);
+        marked = 1;
+      }
+      const int64_t id = bad ? 0 : ids[k];
+      const int64_t slot = t & page_mask;
+      kr[k] = *reinterpret_cast<const u4_t*>(kbase + 2 * id * P.c.k_page + slot * k_step + (size_t)k_at);
+      vr[k] = *reinterpret_cast<const u4_t*>(vbase + 2 * id * P.c.v_page + slot * v_step + (size_t)v_at);
     }
-    return bad;
   };
-  // Of a buffer: a row in no page, a value that is not finite.  Once set they stay: later tiles then are
-  // looked at more closely than they need.
-  __shared__ int flags[2][2];
-  if (threadIdx.x < 4) flags[threadIdx.x >> 1][threadIdx.x & 1] = 0;
-  __syncthreads();
-  // rows outside of every column's sight hold no value; what a partly seen tile holds is looked at
-  auto stage = [&](int tile, int buf, bool bad) __attribute__((always_inline)) {
+  // rows outside of every column's sight hold no value; what some columns see and others do not is looked at
+  auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
     char* const k_s = lds + buf * BUF + l_row * KS + 16 * l_piece;
     char* const v_s = lds + buf * BUF + TT * KS + l_row * VS + 16 * l_piece;
     const int t0 = tile * TT;
+    bool odd = false;
     if (t0 < part_lo || t0 + TT > part_hi) {
-      bool odd = false;
 #pragma unroll
       for (int k = 0; k < NK; k++) {
         const int t = t0 + k * RR + l_row;
         if (t < all_lo || t >= all_hi) vr[k] = (u4_t){0u, 0u, 0u, 0u};
         odd |= any_not_finite<T>(vr[k]);
       }
-      if (odd) flags[buf][1] = 1;
     }
 #pragma unroll
     for (int k = 0; k < NK; k++) {
       *reinterpret_cast<u4_t*>(k_s + k * RR * KS) = kr[k];
       *reinterpret_cast<u4_t*>(v_s + k * RR * VS) = vr[k];
     }
-    if (bad) flags[buf][0] = 1;
+    if (odd) {
+      marked = 1;
+#pragma unroll 1
+      for (int k = 0; k < NK; k++) marks.take_odd<T>(reinterpret_cast<uint16_t*>(v_s + k * RR * VS), t0 + k * RR + l_row, 8 * l_piece);
+    }
   };
 
   const float score_scale = fmaxf(__builtin_fabsf(P.scale_log2), 0x1p-126f);
@@ -180,22 +188,20 @@ void paged_many_kernel(PagedParams P, int splits) {
   const uint32_t k_get = (uint32_t)(n * KS + 16 * half);
   const uint32_t v_get = (uint32_t)(TT * KS + (4 * half + ((lane & 15) >> 2)) * VS + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
 
-  bool bad_next = false;
   if (tile0 < tile1) {
     look(tile0);
-    bool bad = load(tile0);
+    load(tile0);
     look(tile0 + 1);
-    stage(tile0, 0, bad);
-    bad_next = load(tile0 + 1);
+    stage(tile0, 0);
+    load(tile0 + 1);
     look(tile0 + 2);
   }
   lds_barrier();
   for (int tile = tile0; tile < tile1; tile++) {
     const int buf = (tile - tile0) & 1, t0 = tile * TT;
-    const bool bad = flags[buf][0] != 0, odd_tile = flags[buf][1] != 0;
     if (tile + 1 < tile1) {
-      stage(tile + 1, buf ^ 1, bad_next);
-      bad_next = load(tile + 2);
+      stage(tile + 1, buf ^ 1);
+      load(tile + 2);
       look(tile + 3);
     }
     const char* const buf_s = lds + buf * BUF;
@@ -209,15 +215,12 @@ void paged_many_kernel(PagedParams P, int splits) {
         for (int k = 0; k < KI; k++)
           s[j] = B::mfma32(*reinterpret_cast<const u4_t*>(buf_s + k_get + j * 32 * KS + 32 * k), qb[k], s[j]);
       }
-      const bool whole = t0 >= lo_most && t0 + TT <= hi_least && !bad;
-      if (!whole) {
+      if (t0 < lo_most || t0 + TT > hi_least) {
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
           for (int r = 0; r < 16; r++) {
             const int t = t0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (bad && (uint32_t)table[min(t >> P.page_shift, P.table_pages - 1)] >= (uint32_t)P.c.pages)
-              s[j][r] = __builtin_bit_cast(float, 0x7fc00000u);
             if (t < see.lo || t >= see.hi) s[j][r] = ninf;
           }
       }
@@ -235,7 +238,7 @@ void paged_many_kernel(PagedParams P, int splits) {
         m_run = m_new;
       }
       const float base = kPScale - (m_run == ninf ? 0.0f : m_run);
-      const bool odd = odd_tile && !whole;
+      float sum = 0.0f;                    // (of a tile: the pair's addition may cut where it should round)
 #pragma unroll
       for (int j = 0; j < J; j++)
 #pragma unroll
@@ -246,64 +249,41 @@ void paged_many_kernel(PagedParams P, int splits) {
             const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][8 * k + 2 * e], score_scale, base));
             const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][8 * k + 2 * e + 1], score_scale, base));
             p[e] = B::pack(a, b);
-            l_run += lo_f32<T>(p[e]) + hi_f32<T>(p[e]);
+            sum = B::add_pair(p[e], sum);
           }
           const char* const v_s = buf_s + v_get + (32 * j + 16 * k) * VS;
-          if (!odd) {
 #pragma unroll
-            for (int v = 0; v < VT; v++) {
-              const u2_t lo = lds_transposed(v_s + 64 * v), hi = lds_transposed(v_s + 8 * VS + 64 * v);
-              o[v] = B::mfma32((u4_t){lo[0], lo[1], hi[0], hi[1]}, p, o[v]);
-            }
-          } else {
-            u4_t vis;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              vis[e] = 0;
-#pragma unroll
-              for (int h = 0; h < 2; h++) {
-                const int r = 8 * k + 2 * e + h, t = t0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
-                if (t >= see.lo && t < see.hi) vis[e] |= (uint32_t)B::kOne << (16 * h);
-              }
-            }
-#pragma unroll
-            for (int v = 0; v < VT; v++) {
-              const u2_t lo = lds_transposed(v_s + 64 * v), hi = lds_transposed(v_s + 8 * VS + 64 * v);
-              __builtin_amdgcn_sched_barrier(0);     // one at a time: rare, and should cost no registers
-              u4_t clean, code;
-              take_odd<T>((u4_t){lo[0], lo[1], hi[0], hi[1]}, clean, code);
-              o[v] = B::mfma32(clean, p, o[v]);
-              f16v_t count;
-#pragma unroll
-              for (int r = 0; r < 16; r++) count[r] = 0.0f;
-              count = B::mfma32(code, vis, count);
-#pragma unroll
-              for (int r = 0; r < 16; r++) o[v][r] = with_odd(o[v][r], count[r]);
-            }
+          for (int v = 0; v < VT; v++) {
+            const u2_t lo = lds_transposed(v_s + 64 * v), hi = lds_transposed(v_s + 8 * VS + 64 * v);
+            o[v] = B::mfma32((u4_t){lo[0], lo[1], hi[0], hi[1]}, p, o[v]);
           }
         }
+      l_run += sum;
     }
     lds_barrier();
   }
 
   const float l = bfly<32>(l_run);
   if (!mine) return;
-  if (only) {
-    const float f = finish_scale(P, head, m_run, l);
-    T* out = reinterpret_cast<T*>(P.out) + token * P.out_token + head * P.out_head;
+  const bool any_marks = marked != 0;
+  const float f = only ? finish_scale(P, head, m_run, l) : 1.0f;
+  T* out = reinterpret_cast<T*>(P.out) + token * P.out_token + head * P.out_head;
+  float* po = P.part_o + part * D;
+  if (!only && half == 0) P.part_ml[part] = make_float2(m_run, l);
 #pragma unroll
-    for (int v = 0; v < VT; v++)
+  for (int v = 0; v < VT; v++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) store<T>(out + 32 * v + 8 * (r >> 2) + 4 * half + (r & 3), l == 0.0f ? 0.0f : o[v][r] * f);
-  } else {
-    float* po = P.part_o + part * D;
+    for (int r = 0; r < 4; r++) {
+      const int d = 32 * v + 8 * r + 4 * half;
+      f4_t y;
 #pragma unroll
-    for (int v = 0; v < VT; v++)
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-        *reinterpret_cast<f4_t*>(po + 32 * v + 8 * r + 4 * half) = (f4_t){o[v][4 * r], o[v][4 * r + 1], o[v][4 * r + 2], o[v][4 * r + 3]};
-    if (half == 0) P.part_ml[part] = make_float2(m_run, l);
-  }
+      for (int e = 0; e < 4; e++) {
+        y[e] = l == 0.0f ? 0.0f : o[v][4 * r + e] * f;
+        if (any_marks) y[e] = marks.marked(y[e], 32 * wave + n, d + e);
+      }
+      if (only) store_four<T>(out + d, y, P.out_vec);
+      else *reinterpret_cast<f4_t*>(po + d) = y;
+    }
 }
 
 template <typename T>
