@@ -3,6 +3,7 @@
 #pragma once
 
 #include "tt_abi_internal.h"
+#include "tt_common.h"
 #include "tt_regions.h"
 
 namespace tt {
@@ -51,6 +52,16 @@ struct PagedRegions {
   }
   bool apart_from(const Region& r) const { return apart(of[0], r) && apart(of[1], r) && apart(of[2], r); }
 };
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
+#define TT_STEP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
+  TT_STEP(0x111, 0xF) TT_STEP(0x112, 0xF) TT_STEP(0x114, 0xF) TT_STEP(0x118, 0xF)     // within rows of 16
+#undef TT_STEP
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);      // row 0's sum to row 1, row 2's to row 3
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);      // the first half's to the second
+  return v;
+}
 
 // Which of the call's tokens are a row's: cu int32 [rows + 1], or `each` tokens for every row.  Values of cu
 // outside 0 .. tokens count as the nearest inside, so that nothing lies outside the operands.

@@ -50,15 +50,14 @@ struct PagedParams {
   float2* part_ml;
   int parts;
   // the launch: which job, its first part, tiles of a workgroup, column tiles of a row and in all
-  int shared_job, part0, share, row_tiles, tiles;
+  int shared_job, part0, share, row_tiles, tiles, ordered;
 };
 
 template <typename T> struct Bits16;
 template <> struct Bits16<f16_t> {
   static constexpr uint32_t kExp = 0x7c00;
-  // (weights come from an exponential: there is no product or sum before the conversion to fold into it)
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, h2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){pin_f32(a), pin_f32(b)}, h2));
   }
   static __device__ __forceinline__ float add_pair(uint32_t w, float c) {      // c + both halves
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), (h2){(_Float16)1.0f, (_Float16)1.0f}, c, false);
@@ -94,11 +93,12 @@ __device__ __forceinline__ float sink_log2(const PagedParams& P, int h) {
 }
 
 template <typename T> __device__ __forceinline__ void store_four(T* p, f4_t v, int vec) {
+  const u2_t w = {Bits16<T>::pack(v[0], v[1]), Bits16<T>::pack(v[2], v[3])};
   if (vec) {
-    *reinterpret_cast<u2_t*>(p) = (u2_t){bits16<T>(v[0]) | (bits16<T>(v[1]) << 16), bits16<T>(v[2]) | (bits16<T>(v[3]) << 16)};
+    *reinterpret_cast<u2_t*>(p) = w;
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; e++) store<T>(p + e, v[e]);
+    for (int e = 0; e < 4; e++) p[e].bits = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
   }
 }
 

@@ -163,6 +163,8 @@ static int launch_job(PagedParams P, const PagedJob& j, bool shared, int part0, 
   P.share = j.share;
   P.row_tiles = j.row_tiles;
   P.tiles = (int)j.tiles;
+  // in order of their length where they do not all run at once
+  P.ordered = j.many && !shared && P.window == 0 && P.of.rows <= 64 && j.tiles * P.c.kv_heads * j.splits > 2 * device_cus();
   return j.many ? launch_paged_many(P, j.splits, st, what) : launch_paged_few(P, j.blocks16, j.rows, j.splits, st, what);
 }
 

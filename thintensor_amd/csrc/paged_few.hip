@@ -84,8 +84,10 @@ void paged_few_kernel(PagedParams P) {
       const int r = row_of(P.of, token[b], &place, &each);
       see[b] = r < P.of.rows ? seen_of(P, row_length(P, r), place, each) : Seen{0, 0};
       see[b].hi = max(see[b].hi, 0);
-      hi_most = max(hi_most, see[b].hi); hl = min(hl, see[b].hi);
-      ll = min(ll, see[b].lo); lm = max(lm, see[b].lo);
+      if (see[b].hi > see[b].lo) {         // (one that sees nothing may compute what it will, it ends without weight)
+        hi_most = max(hi_most, see[b].hi); hl = min(hl, see[b].hi);
+        ll = min(ll, see[b].lo); lm = max(lm, see[b].lo);
+      }
     }
     hi_most = over_columns_max(hi_most);
     lo_most = over_columns_max(lm);
@@ -284,7 +286,7 @@ void paged_few_kernel(PagedParams P) {
   float* const o_s = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int b = 0; b < NB; b++) {
-    const float l_col = bfly<32>(bfly<16>(l_run[b]));
+    const float l_col = see[b].hi <= see[b].lo ? 0.0f : bfly<32>(bfly<16>(l_run[b]));
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < VT; x++) *reinterpret_cast<f4_t*>(o_s + (wave * 16 + n) * OS + 16 * x + 4 * quad) = o[b][x];

@@ -15,6 +15,39 @@ namespace tt {
 
 constexpr int kWaves = 4;
 
+// The column tile with the x-th most tokens to see (of up to 64 rows, one for each lane; of equal ones the lower row's),
+// so that no long one begins when the others end.  Tile j of a row with n of them sees about b + j + 1 times 128 / per_kv
+// tokens; how many tiles see h or more is a sum over the rows, and h is found by halving.
+__device__ __forceinline__ bool longest(const PagedParams& P, int x, int* row, int* tile) {
+  const int lane = threadIdx.x & 63, r = min(lane, P.of.rows - 1);
+  int first, n = P.of.count(r, &first);
+  const int b = (int)(((int64_t)max(row_length(P, r) - n, 0) * P.per_kv) / kManyColumns);
+  n = lane < P.of.rows ? (int)(((int64_t)n * P.per_kv + kManyColumns - 1) / kManyColumns) : 0;
+  auto at_least = [&](int h) __attribute__((always_inline)) {
+    return (int)__builtin_amdgcn_readlane((int)lanes_before((uint32_t)min(max(b + n - h + 1, 0), n)), 63);
+  };
+  if (x >= at_least(0)) return false;
+  int lo = 0, hi = 0x40000000;                 // at_least(lo) > x, at_least(hi) <= x
+  {
+    int most = n > 0 ? b + n + 1 : 1;
+#define TT_LEVEL(X) most = max(most, __builtin_bit_cast(int, xor_partner<X>(__builtin_bit_cast(float, most))));
+    TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8) TT_LEVEL(16) TT_LEVEL(32)
+#undef TT_LEVEL
+    hi = __builtin_amdgcn_readfirstlane(most);
+  }
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (at_least(mid) > x) lo = mid;
+    else hi = mid;
+  }
+  uint64_t equal = __builtin_amdgcn_ballot_w64(lo - 1 - b >= 0 && lo - 1 - b < n);
+  for (int skip = x - at_least(lo + 1); skip > 0; skip--) equal &= equal - 1;
+  if (equal == 0) return false;
+  *row = __builtin_ctzll(equal);
+  *tile = lo - 1 - __builtin_amdgcn_readlane(b, *row);
+  return true;
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
 void paged_many_kernel(PagedParams P, int splits) {
@@ -25,14 +58,31 @@ void paged_many_kernel(PagedParams P, int splits) {
   constexpr int KS = 2 * D + 16, VS = 2 * D + 32, BUF = TT * (KS + VS);
   __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
 
-  const int kvhs = (int)P.c.kv_heads, kvh = blockIdx.x % kvhs;
-  const int rest = blockIdx.x / kvhs, split = rest % splits, x = P.tiles - 1 - rest / splits;   // long rows' ends first
+  // Workgroups go to the eight XCDs in turn.  Of kvhs = 8 F + R heads an XCD takes F by itself, so that their K and V come
+  // to its L2 alone, and an eighth of the tiles of the others; eight tiles of all heads follow the eight before.
+  const int kvhs = (int)P.c.kv_heads, xcd = blockIdx.x & 7, turn = blockIdx.x >> 3, full = kvhs >> 3;
+  const int eight = turn / kvhs, i = turn - eight * kvhs;
+  int kvh, rest = 8 * eight;
+  if (i < 8 * full) {
+    kvh = xcd * full + i % full;
+    rest += i / full;
+  } else {
+    kvh = i;
+    rest += (xcd + i) & 7;
+  }
+  const int split = rest % splits, x_first = rest / splits, x = P.tiles - 1 - x_first;
+  if (x < 0) return;
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int G = P.per_kv;
   int row = 0, first = 0, count = P.of.tokens, c0 = x * kManyColumns;
   if (!P.shared_job) {
-    if (P.of.cu) {
+    if (P.ordered) {
+      int tile;
+      if (!longest(P, x_first, &row, &tile)) return;
+      count = P.of.count(row, &first);
+      c0 = tile * kManyColumns;
+    } else if (P.of.cu) {
       row = P.of.find(x, G, kManyColumns, 1);
       count = P.of.count(row, &first);
       c0 = (x - (int)((int64_t)first * G / kManyColumns) - row) * kManyColumns;
@@ -83,14 +133,22 @@ void paged_many_kernel(PagedParams P, int splits) {
 #undef TT_LEVEL
     return __builtin_amdgcn_readfirstlane(v);
   };
-  const int hi_most = most(see.hi), hi_least = -most(-see.hi), lo_most = most(see.lo), lo_least = -most(-see.lo);
+  // (a column that sees nothing may compute what it will, it ends without weight)
+  constexpr int kFar = 0x7fffffff;
+  const bool blind = see.hi <= see.lo;
+  const int hi_most = most(blind ? 0 : see.hi), hi_least = -most(blind ? -kFar : -see.hi);
+  const int lo_most = most(blind ? 0 : see.lo), lo_least = -most(blind ? -kFar : -see.lo);
   __shared__ int reach[4][kWaves];
   __shared__ Seen see_s[kManyColumns];
+  __shared__ uint32_t which_s[kManyColumns];         // a column's token past the first one's, its head in the KV head
   __shared__ uint32_t marks_s[kManyColumns * (D / 16)];
   __shared__ int marked;
   for (int i = threadIdx.x; i < kManyColumns * (D / 16); i += 64 * kWaves) marks_s[i] = 0;
   if (threadIdx.x == 0) marked = 0;
-  if (half == 0) see_s[32 * wave + n] = see;
+  if (half == 0) {
+    see_s[32 * wave + n] = see;
+    which_s[32 * wave + n] = ((uint32_t)(at - c0 / G) << 16) | (uint32_t)(c - at * G);
+  }
   const Marks marks{marks_s, see_s, cols, D / 16};
   if (lane == 0) {
     reach[0][wave] = -lo_least;
@@ -263,32 +321,47 @@ void paged_many_kernel(PagedParams P, int splits) {
     lds_barrier();
   }
 
-  const float l = bfly<32>(l_run);
-  if (!mine) return;
-  const bool any_marks = marked != 0;
+  // ---- through LDS, so that whole vectors are written: 128 dims of the wave's columns at a time
+  const float l = blind ? 0.0f : bfly<32>(l_run);
   const float f = only ? finish_scale(P, head, m_run, l) : 1.0f;
-  T* out = reinterpret_cast<T*>(P.out) + token * P.out_token + head * P.out_head;
-  float* po = P.part_o + part * D;
-  if (!only && half == 0) P.part_ml[part] = make_float2(m_run, l);
+  if (!only && mine && half == 0) P.part_ml[part] = make_float2(m_run, l);
+  const bool any_marks = marked != 0;
+  constexpr int DD = D < 128 ? D : 128, OS = DD + 4, LANES = DD / 4, COLS = 64 / LANES;
+  static_assert(kWaves * 32 * OS * 4 <= 2 * BUF, "the wave's sums fit where tiles were");
+  float* const o_s = reinterpret_cast<float*>(lds) + wave * 32 * OS;
+  const int wave_cols = min(32, cols - 32 * wave), y_col = lane / LANES, y_dim = 4 * (lane % LANES);
 #pragma unroll
-  for (int v = 0; v < VT; v++)
+  for (int v0 = 0; v0 < VT; v0 += DD / 32) {
+    wave_lds_order();
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int d = 32 * v + 8 * r + 4 * half;
-      f4_t y;
+    for (int v = 0; v < DD / 32; v++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        y[e] = l == 0.0f ? 0.0f : o[v][4 * r + e] * f;
-        if (any_marks) y[e] = marks.marked(y[e], 32 * wave + n, d + e);
+      for (int r = 0; r < 4; r++) {
+        f4_t y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = l == 0.0f ? 0.0f : o[v0 + v][4 * r + e] * f;
+        *reinterpret_cast<f4_t*>(o_s + n * OS + 32 * v + 8 * r + 4 * half) = y;
       }
-      if (only) store_four<T>(out + d, y, P.out_vec);
-      else *reinterpret_cast<f4_t*>(po + d) = y;
+    wave_lds_order();
+#pragma unroll 4
+    for (int i = y_col; i < wave_cols; i += COLS) {
+      f4_t y = *reinterpret_cast<const f4_t*>(o_s + i * OS + y_dim);
+      const int d = 32 * v0 + y_dim;
+      if (any_marks) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = marks.marked(y[e], 32 * wave + i, d + e);
+      }
+      const uint32_t which = which_s[32 * wave + i];
+      const int tok = first + c0 / G + (int)(which >> 16), hd = kvh * G + (int)(which & 0xffffu);
+      if (only) store_four<T>(reinterpret_cast<T*>(P.out) + tok * P.out_token + hd * P.out_head + d, y, P.out_vec);
+      else *reinterpret_cast<f4_t*>(P.part_o + (((int64_t)tok * P.heads + hd) * P.parts + P.part0 + split) * D + d) = y;
     }
+  }
 }
 
 template <typename T>
 static int launch_type(const PagedParams& P, int splits, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)(P.c.kv_heads * P.tiles * splits)), block(64 * kWaves);
+  const dim3 grid((unsigned)(P.c.kv_heads * 8 * ((P.tiles * splits + 7) / 8))), block(64 * kWaves);
   if (P.c.head_dim == 64) hipLaunchKernelGGL((paged_many_kernel<T, 64>), grid, block, 0, st, P, splits);
   else if (P.c.head_dim == 128) hipLaunchKernelGGL((paged_many_kernel<T, 128>), grid, block, 0, st, P, splits);
   else hipLaunchKernelGGL((paged_many_kernel<T, 256>), grid, block, 0, st, P, splits);

@@ -134,16 +134,6 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectParams P) {
     P.keys[((int64_t)row * P.c.kv_heads + kvh) * P.keys_row + p] = page_of(p) < 0 ? 0xffffffffu : best;
 }
 
-// Sum over the lanes up to this one.
-__device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
-#define TT_STEP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
-  TT_STEP(0x111, 0xF) TT_STEP(0x112, 0xF) TT_STEP(0x114, 0xF) TT_STEP(0x118, 0xF)     // within rows of 16
-#undef TT_STEP
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);      // row 0's sum to row 1, row 2's to row 3
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);      // the first half's to the second
-  return v;
-}
-
 // The least kept score is found digit by digit: digits of eight bits of key - least key, from the highest that is set
 // anywhere, so that the first one already spreads; histograms in LDS, one for each digit, searched by every wave for
 // itself, so that a digit takes one barrier.  Then every thread counts what is kept of its run of pages, and the runs
