@@ -50,7 +50,7 @@ struct PagedParams {
   float2* part_ml;
   int parts;
   // the launch: which job, its first part, tiles of a workgroup, column tiles of a row and in all
-  int shared_job, part0, share, row_tiles, tiles, ordered;
+  int shared_job, part0, share, row_tiles, tiles, ordered, wide;
 };
 
 template <typename T> struct Bits16;

@@ -81,7 +81,7 @@ struct PagedJob {
   bool many;
   int blocks16, row_tiles, rows;        // few: columns of a workgroup in sixteens, workgroups of a row, rows
   int64_t tiles;                        // many: column tiles
-  int splits, share;
+  int splits, share, wide;
 };
 
 struct PagedPlan {
@@ -90,12 +90,17 @@ struct PagedPlan {
   int parts;
 };
 
-// Workgroups that share a row's tokens, for `groups` of them that each may take up to `tiles` tiles of 32.
+// Workgroups that share a row's tokens, for `groups` of them that each may take up to `tiles` tiles of 32.  A
+// workgroup alone saves the join (3.7 us in a row of calls).  With a CU for each, eight waves instead of four have more on
+// its way (one row of 8 KV heads in a graph, us: x 64, 256 tokens 5.1 and 5.4, 512 7.0 and 6.1, 768 9.0 and 7.4, shared 8.6;
+// x 128, 256 tokens 6.9 and 6.6, 512 9.6 and 7.8, 768 12.3 and 9.6, shared 10.0).
 static void split_few(int64_t groups, int64_t tiles, bool parts, PagedJob* j) {
   const int64_t cus = device_cus();
   j->splits = 1;
   j->share = (int)tiles;
+  j->wide = !parts && groups <= cus && tiles > 8;
   if (!parts && (tiles <= 24 || (groups >= cus && tiles <= 64))) return;
+  j->wide = 0;
   const int64_t want = groups >= cus / 2 ? 12 * cus : 2 * cus;
   int64_t share = (tiles * groups + want - 1) / want;
   if (share < 8) share = 8;
@@ -163,6 +168,7 @@ static int launch_job(PagedParams P, const PagedJob& j, bool shared, int part0, 
   P.share = j.share;
   P.row_tiles = j.row_tiles;
   P.tiles = (int)j.tiles;
+  P.wide = j.wide;
   // in order of their length where they do not all run at once
   P.ordered = j.many && !shared && P.window == 0 && P.of.rows <= 64 && j.tiles * P.c.kv_heads * j.splits > 2 * device_cus();
   return j.many ? launch_paged_many(P, j.splits, st, what) : launch_paged_few(P, j.blocks16, j.rows, j.splits, st, what);

@@ -19,7 +19,6 @@
 namespace tt {
 
 constexpr int kTile = 32;
-constexpr int kWaves = 4;
 
 __device__ __forceinline__ int over_columns_max(int v) {
 #define TT_LEVEL(X) v = max(v, __builtin_bit_cast(int, xor_partner<X>(__builtin_bit_cast(float, v))));
@@ -33,17 +32,17 @@ __device__ __forceinline__ float col_max(float v) {   // over the four lanes of 
 }
 
 // MIXED: a tile's tokens may be seen by some columns and not by others.
-template <typename T, int D, int NB, bool MIXED>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D * NB == 256 ? 2 : 3)))
+template <typename T, int D, int NB, bool MIXED, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D * NB == 256 || WAVES == 8 ? 2 : 3)))
 void paged_few_kernel(PagedParams P) {
   using B = Bits16<T>;
   constexpr int KI = D / 32, VT = D / 16;
   constexpr int PC = D / 8, VR = 64 / PC, VK = 32 / VR;   // pieces of a V row, rows of a request, requests
-  constexpr int VS = 2 * D + 32;                          // LDS bytes of a V row
+  constexpr int KS = 2 * D + 16, VS = 2 * D + 32;         // LDS bytes of a row of K, of V
   constexpr int OS = D + 4;                               // floats of a column when the waves are joined
-  static_assert(kWaves * 16 * OS * 4 <= kWaves * kTile * VS, "the join fits where V was");
-  __shared__ __attribute__((aligned(16))) char lds[kWaves * kTile * VS];
-  __shared__ float m_s[kWaves][16], l_s[kWaves][16];
+  static_assert(WAVES * 16 * OS * 4 <= WAVES * kTile * VS, "the join fits where V was");
+  __shared__ __attribute__((aligned(16))) char lds[WAVES * kTile * VS];
+  __shared__ float m_s[WAVES][16], l_s[WAVES][16];
   __shared__ Seen see_s[MIXED ? 16 * NB : 1];
   __shared__ uint32_t marks_s[16 * NB * (D / 16)];
   __shared__ int marked;
@@ -53,14 +52,16 @@ void paged_few_kernel(PagedParams P) {
   const int G = P.per_kv;
   const int first = P.shared_job ? 0 : row * P.of.each, count = P.shared_job ? P.of.tokens : P.of.each;
   const int c0 = cb * 16 * NB, cols = min(16 * NB, count * G - c0);
+  const int32_t* table = P.table + (P.shared_job ? 0 : row * P.table_row);
+  const int32_t* sel = P.selected ? P.selected + ((int64_t)row * P.c.kv_heads + kvh) * P.selected_count : nullptr;
 
-  // ---- columns: q is requested before anything else
+  // ---- q, and the first tile where it does not depend on the row's length, are requested before anything else
   int token[NB], head[NB];
   u4_t qb[NB][KI];
 #pragma unroll
   for (int b = 0; b < NB; b++) {
     const int c = c0 + min(16 * b + n, cols - 1);
-    const int i = c / G;
+    const int i = MIXED ? c / G : 0;
     token[b] = first + i;
     head[b] = kvh * G + c - i * G;
     const uint16_t* q = reinterpret_cast<const uint16_t*>(P.q) + token[b] * P.q_token + head[b] * P.q_head + 8 * quad;
@@ -74,9 +75,41 @@ void paged_few_kernel(PagedParams P) {
         for (int e = 0; e < 4; e++) qb[b][k][e] = q[32 * k + 2 * e] | ((uint32_t)q[32 * k + 2 * e + 1] << 16);
     }
   }
+  const uint32_t k_step = (uint32_t)(2 * P.c.k_token), v_step = (uint32_t)(2 * P.c.v_token);
+  const int v_row = lane / PC, v_piece = lane % PC;
+  u4_t kr[VK], vr[VK];
+  auto load_k = [&](const Place (&p)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < VK; k++) {
+      const int h = k * VR / 16;
+      kr[k] = *reinterpret_cast<const u4_t*>(p[h].k + (size_t)((uint32_t)(k * VR - 16 * h + v_row) * k_step + 16 * v_piece));
+    }
+  };
+  auto load_v = [&](const Place (&p)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < VK; k++) {
+      const int h = k * VR / 16;
+      vr[k] = *reinterpret_cast<const u4_t*>(p[h].v + (size_t)((uint32_t)(k * VR - 16 * h + v_row) * v_step + 16 * v_piece));
+    }
+  };
+  auto place = [&](int j, Place (&p)[2]) __attribute__((always_inline)) {
+    p[0] = place_of(P, table, sel, kvh, kTile * j);
+    p[1] = place_of(P, table, sel, kvh, kTile * j + 16);
+  };
+  // (a place past the table is one in page 0 that nobody sees; a row's first split has a tile unless the row is empty)
+  int tile0 = sel || P.shared_job ? 0 : P.shared / kTile;
+  const bool early = split == 0 && (P.window == 0 || sel);
+  Place now[2], next[2];
+  if (early) {
+    place(tile0 + wave, now);
+    load_k(now);
+    load_v(now);
+    place(tile0 + wave + WAVES, next);
+  }
+
   Seen see[NB];
   int hi_most = 0, hi_least, lo_least, lo_most;             // over the columns
-  if (P.shared_job) {
+  if (MIXED && P.shared_job) {
     int hl = 0x7fffffff, ll = 0x7fffffff, lm = 0;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
@@ -95,25 +128,21 @@ void paged_few_kernel(PagedParams P) {
     lo_least = -over_columns_max(-ll);
   } else {
     const int len = row_length(P, row);
+    const int z0 = MIXED ? c0 / G : 0, z1 = MIXED ? (c0 + cols - 1) / G : 0;
 #pragma unroll
     for (int b = 0; b < NB; b++) see[b] = seen_of(P, len, token[b] - first, count);
-    const Seen a = seen_of(P, len, c0 / G, count), z = seen_of(P, len, (c0 + cols - 1) / G, count);
+    const Seen a = seen_of(P, len, z0, count), z = seen_of(P, len, z1, count);
     hi_most = max(z.hi, 0); hi_least = a.hi; lo_least = a.lo; lo_most = z.lo;
   }
-  const int32_t* table = P.table + (P.shared_job ? 0 : row * P.table_row);
-  const int32_t* sel = P.selected ? P.selected + ((int64_t)row * P.c.kv_heads + kvh) * P.selected_count : nullptr;
-  int tile0 = lo_least / kTile, tile1 = (hi_most + kTile - 1) / kTile;
-  if (sel) {
-    tile0 = 0;
-    tile1 = ((P.selected_count << P.page_shift) + kTile - 1) / kTile;
-    if (hi_most == 0) tile1 = 0;
-  }
+  int tile1 = (hi_most + kTile - 1) / kTile;
+  if (sel) tile1 = hi_most == 0 ? 0 : ((P.selected_count << P.page_shift) + kTile - 1) / kTile;
+  else tile0 = lo_least / kTile;
   tile0 += split * P.share;
   tile1 = min(tile1, tile0 + P.share);
   const bool only = P.parts == 1;
   if (tile0 >= tile1) {
     if (!only) {                                             // nothing here: no weight
-      for (int c = threadIdx.x; c < cols; c += 64 * kWaves) {
+      for (int c = threadIdx.x; c < cols; c += 64 * WAVES) {
         const int i = (c0 + c) / G;
         P.part_ml[((int64_t)(first + i) * P.heads + kvh * G + (c0 + c - i * G)) * P.parts + P.part0 + split] =
             make_float2(__builtin_bit_cast(float, 0xff800000u), 0.0f);
@@ -122,48 +151,23 @@ void paged_few_kernel(PagedParams P) {
     }
     tile1 = tile0;
   }
+  int i = tile0 + wave;
+  if (!early && tile0 < tile1) {
+    place(min(i, tile1 - 1), now);
+    load_k(now);
+    load_v(now);
+    place(i + WAVES, next);
+  }
 
   // ---- marks
-  for (int i = threadIdx.x; i < 16 * NB * (D / 16); i += 64 * kWaves) marks_s[i] = 0;
+  for (int i = threadIdx.x; i < 16 * NB * (D / 16); i += 64 * WAVES) marks_s[i] = 0;
   if (threadIdx.x == 0) marked = 0;
   if (MIXED && wave == 0 && quad == 0) {
 #pragma unroll
     for (int b = 0; b < NB; b++) see_s[16 * b + n] = see[b];
   }
-  __syncthreads();
+  lds_barrier();
   const Marks marks{marks_s, see_s, cols, D / 16};
-
-  // ---- tiles
-  const uint32_t k_at = (uint32_t)n * (uint32_t)(2 * P.c.k_token) + 16 * quad, v_step = (uint32_t)(2 * P.c.v_token);
-  const int v_row = lane / PC, v_piece = lane % PC;
-  u4_t kr[2][KI], vr[VK];
-  auto load_k = [&](const Place (&p)[2]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int k = 0; k < KI; k++) kr[h][k] = *reinterpret_cast<const u4_t*>(p[h].k + (size_t)(k_at + 64 * k));
-  };
-  auto load_v = [&](const Place (&p)[2]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < VK; k++) {
-      const int h = k * VR / 16;
-      vr[k] = *reinterpret_cast<const u4_t*>(p[h].v + (size_t)((uint32_t)(k * VR - 16 * h + v_row) * v_step + 16 * v_piece));
-    }
-  };
-  const int last = tile1 - 1;
-  auto place = [&](int i, Place (&p)[2]) __attribute__((always_inline)) {
-    const int j = max(min(i, last), 0);
-    p[0] = place_of(P, table, sel, kvh, kTile * j);
-    p[1] = place_of(P, table, sel, kvh, kTile * j + 16);
-  };
-  int i = tile0 + wave;
-  Place now[2], next[2];
-  place(i, now);
-  if (tile0 < tile1) {
-    load_k(now);
-    load_v(now);
-  }
-  place(i + kWaves, next);
 
   // the sign of the scale goes to q, so that the largest product is the largest score
   const float score_scale = fmaxf(__builtin_fabsf(P.scale_log2), 0x1p-126f);
@@ -184,20 +188,29 @@ void paged_few_kernel(PagedParams P) {
     l_run[b] = 0.0f;
   }
   char* const mine = lds + wave * (kTile * VS);
+  char* const k_put = mine + v_row * KS + 16 * v_piece;
+  const char* const k_get = mine + n * KS + 16 * quad;
   char* const put = mine + v_row * VS + 16 * v_piece;
   const char* const get = mine + (4 * quad + (n >> 2)) * VS + 8 * (n & 3);
 
-  for (; i < tile1; i += kWaves) {
+  for (; i < tile1; i += WAVES) {
     f4_t sc[NB][2];
+    wave_lds_order();
 #pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        sc[b][h] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < KI; k++) sc[b][h] = B::mfma16(kr[h][k], qb[b][k], sc[b][h]);
-      }
+    for (int k = 0; k < VK; k++) *reinterpret_cast<u4_t*>(k_put + k * VR * KS) = kr[k];
     load_k(next);
+    wave_lds_order();
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+      for (int b = 0; b < NB; b++) sc[b][h] = (f4_t){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < KI; k++) {
+        const u4_t key = *reinterpret_cast<const u4_t*>(k_get + 16 * h * KS + 64 * k);
+#pragma unroll
+        for (int b = 0; b < NB; b++) sc[b][h] = B::mfma16(key, qb[b][k], sc[b][h]);
+      }
+    }
     const int t0 = now[0].t, t1 = now[1].t;
     const bool whole = t0 >= lo_most && t0 + 16 <= hi_least && t1 >= lo_most && t1 + 16 <= hi_least;
     if (now[0].bad || now[1].bad) {                          // a column that sees a token in no page is NaN
@@ -237,7 +250,7 @@ void paged_few_kernel(PagedParams P) {
     load_v(next);
     now[0] = next[0];
     now[1] = next[1];
-    place(i + 2 * kWaves, next);
+    if (i + 2 * WAVES < tile1) place(i + 2 * WAVES, next);
 
     u4_t pw[NB];
 #pragma unroll
@@ -296,17 +309,17 @@ void paged_few_kernel(PagedParams P) {
     }
     __syncthreads();
     const int here = min(16, cols - 16 * b);
-    for (int u = threadIdx.x; u < here * (D / 4); u += 64 * kWaves) {
+    for (int u = threadIdx.x; u < here * (D / 4); u += 64 * WAVES) {
       const int cc = u / (D / 4), d = 4 * (u % (D / 4));
       const int c = c0 + 16 * b + cc, at = c / G;
       float M = m_s[0][cc];
 #pragma unroll
-      for (int w = 1; w < kWaves; w++) M = fmaxf(M, m_s[w][cc]);
+      for (int w = 1; w < WAVES; w++) M = fmaxf(M, m_s[w][cc]);
       const float base = M == ninf ? 0.0f : M;
       f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
       float l = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWaves; w++) {
+      for (int w = 0; w < WAVES; w++) {
         const float e = __builtin_amdgcn_exp2f(m_s[w][cc] - base);
         acc += *reinterpret_cast<const f4_t*>(o_s + (w * 16 + cc) * OS + d) * e;
         l = __builtin_fmaf(l_s[w][cc], e, l);
@@ -331,9 +344,16 @@ void paged_few_kernel(PagedParams P) {
 
 template <typename T, int D, int NB>
 static int launch_blocks(const PagedParams& P, int rows, int splits, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)(P.c.kv_heads * P.row_tiles), (unsigned)rows, (unsigned)splits), block(64 * kWaves);
-  if (P.shared_job || P.of.each > 1) hipLaunchKernelGGL((paged_few_kernel<T, D, NB, true>), grid, block, 0, st, P);
-  else hipLaunchKernelGGL((paged_few_kernel<T, D, NB, false>), grid, block, 0, st, P);
+  const dim3 grid((unsigned)(P.c.kv_heads * P.row_tiles), (unsigned)rows, (unsigned)splits);
+  const bool mixed = P.shared_job || P.of.each > 1;
+  if constexpr (NB == 1 && D < 256) {
+    if (P.wide && !mixed) {
+      hipLaunchKernelGGL((paged_few_kernel<T, D, NB, false, 8>), grid, dim3(64 * 8), 0, st, P);
+      return check_launch(what);
+    }
+  }
+  if (mixed) hipLaunchKernelGGL((paged_few_kernel<T, D, NB, true, 4>), grid, dim3(64 * 4), 0, st, P);
+  else hipLaunchKernelGGL((paged_few_kernel<T, D, NB, false, 4>), grid, dim3(64 * 4), 0, st, P);
   return check_launch(what);
 }
 
