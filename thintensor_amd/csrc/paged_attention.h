@@ -219,6 +219,6 @@ constexpr int few_columns(int64_t head_dim) { return head_dim == 64 ? 64 : head_
 int launch_paged_few(const PagedParams& P, int blocks16, int rows, int splits, hipStream_t st, const char* what);
 int launch_paged_many(const PagedParams& P, int splits, hipStream_t st, const char* what);
 inline int many_tile_tokens(int64_t head_dim) { return head_dim == 256 ? 32 : 64; }
-constexpr int kManyColumns = 128;
+constexpr int many_columns(int64_t head_dim) { return head_dim == 256 ? 256 : 128; }
 
 }  // namespace tt

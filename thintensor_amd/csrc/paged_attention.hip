@@ -126,12 +126,12 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
   p.window = window < p.limit ? window : 0;
   p.shared = rows > 1 ? shared_pages * c->page_size : 0;
   const int64_t each = ragged ? 0 : tokens / rows;
-  const int tt = many_tile_tokens(c->head_dim);
+  const int tt = many_tile_tokens(c->head_dim), mc = many_columns(c->head_dim);
   if (p.shared > 0) {
     const int64_t cols = tokens * G, reach = p.shared < p.limit ? p.shared : p.limit;
     p.prefix.many = cols > few_columns(c->head_dim);
     if (p.prefix.many) {
-      p.prefix.tiles = (cols + kManyColumns - 1) / kManyColumns;
+      p.prefix.tiles = (cols + mc - 1) / mc;
       split_many(p.prefix.tiles * c->kv_heads, (reach + tt - 1) / tt, &p.prefix);
     } else {
       p.prefix.blocks16 = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
@@ -145,8 +145,8 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
   if (selected_count > 0) reach = selected_count * c->page_size;
   p.own.many = ragged || each * G > few_columns(c->head_dim);
   if (p.own.many) {
-    p.own.row_tiles = (int)((each * G + kManyColumns - 1) / kManyColumns);
-    p.own.tiles = ragged ? tokens * G / kManyColumns + rows : rows * p.own.row_tiles;
+    p.own.row_tiles = (int)((each * G + mc - 1) / mc);
+    p.own.tiles = ragged ? tokens * G / mc + rows : rows * p.own.row_tiles;
     split_many(p.own.tiles * c->kv_heads, (reach + tt - 1) / tt + 1, &p.own);
   } else {
     p.own.blocks16 = each * G <= 16 ? 1 : each * G <= 32 ? 2 : 4;
@@ -182,7 +182,7 @@ static int check_attention(const tt_paged_cache* c, int64_t table_pages, bool ra
   TT_REQUIRE(heads > 0, "%s: heads must be a multiple of kv_heads", what);
   TT_REQUIRE(window >= 0 && max_length > 0, "%s: window must not be negative, max_length at least 1", what);
   TT_REQUIRE(shared_pages >= 0 && shared_pages <= table_pages, "%s: shared_pages outside the table", what);
-  TT_REQUIRE((tokens * heads) / kManyColumns + (ragged ? rows * c->kv_heads : 0) < (1 << 23), "%s: too many queries for one call", what);
+  TT_REQUIRE((tokens * heads) / 128 + (ragged ? rows * c->kv_heads : 0) < (1 << 23), "%s: too many queries for one call", what);
   TT_REQUIRE(selected_count >= 0 && selected_count <= 65536 && (selected_count == 0 || (!ragged && tokens == rows && shared_pages == 0)),
              "%s: selected pages (65536 at most) are for one query per row, without shared pages", what);
   return TT_OK;

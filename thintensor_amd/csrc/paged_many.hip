@@ -13,16 +13,15 @@
 
 namespace tt {
 
-constexpr int kWaves = 4;
-
 // The column tile with the x-th most tokens to see (of up to 64 rows, one for each lane; of equal ones the lower row's),
 // so that no long one begins when the others end.  Tile j of a row with n of them sees about b + j + 1 times 128 / per_kv
 // tokens; how many tiles see h or more is a sum over the rows, and h is found by halving.
+template <int COLUMNS>
 __device__ __forceinline__ bool longest(const PagedParams& P, int x, int* row, int* tile) {
   const int lane = threadIdx.x & 63, r = min(lane, P.of.rows - 1);
   int first, n = P.of.count(r, &first);
-  const int b = (int)(((int64_t)max(row_length(P, r) - n, 0) * P.per_kv) / kManyColumns);
-  n = lane < P.of.rows ? (int)(((int64_t)n * P.per_kv + kManyColumns - 1) / kManyColumns) : 0;
+  const int b = (int)(((int64_t)max(row_length(P, r) - n, 0) * P.per_kv) / COLUMNS);
+  n = lane < P.of.rows ? (int)(((int64_t)n * P.per_kv + COLUMNS - 1) / COLUMNS) : 0;
   auto at_least = [&](int h) __attribute__((always_inline)) {
     return (int)__builtin_amdgcn_readlane((int)lanes_before((uint32_t)min(max(b + n - h + 1, 0), n)), 63);
   };
@@ -48,13 +47,14 @@ __device__ __forceinline__ bool longest(const PagedParams& P, int x, int* row, i
   return true;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_many_kernel(PagedParams P, int splits) {
   using B = Bits16<T>;
+  constexpr int COLUMNS = 32 * WAVES;
   constexpr int TT = D == 256 ? 32 : 64, J = TT / 32;
   constexpr int KI = D / 16, VT = D / 32;
-  constexpr int PC = D / 8, RR = 64 * kWaves / PC, NK = TT / RR;      // pieces of a row, rows of a request, requests
+  constexpr int PC = D / 8, RR = 64 * WAVES / PC, NK = TT / RR;      // pieces of a row, rows of a request, requests
   constexpr int KS = 2 * D + 16, VS = 2 * D + 32, BUF = TT * (KS + VS);
   __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
 
@@ -75,29 +75,29 @@ void paged_many_kernel(PagedParams P, int splits) {
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int G = P.per_kv;
-  int row = 0, first = 0, count = P.of.tokens, c0 = x * kManyColumns;
+  int row = 0, first = 0, count = P.of.tokens, c0 = x * COLUMNS;
   if (!P.shared_job) {
     if (P.ordered) {
       int tile;
-      if (!longest(P, x_first, &row, &tile)) return;
+      if (!longest<COLUMNS>(P, x_first, &row, &tile)) return;
       count = P.of.count(row, &first);
-      c0 = tile * kManyColumns;
+      c0 = tile * COLUMNS;
     } else if (P.of.cu) {
-      row = P.of.find(x, G, kManyColumns, 1);
+      row = P.of.find(x, G, COLUMNS, 1);
       count = P.of.count(row, &first);
-      c0 = (x - (int)((int64_t)first * G / kManyColumns) - row) * kManyColumns;
+      c0 = (x - (int)((int64_t)first * G / COLUMNS) - row) * COLUMNS;
     } else {
       row = x / P.row_tiles;
       count = P.of.each;
       first = row * count;
-      c0 = (x - row * P.row_tiles) * kManyColumns;
+      c0 = (x - row * P.row_tiles) * COLUMNS;
     }
     row = __builtin_amdgcn_readfirstlane(row);
     first = __builtin_amdgcn_readfirstlane(first);
     count = __builtin_amdgcn_readfirstlane(count);
     c0 = __builtin_amdgcn_readfirstlane(c0);
   }
-  const int cols = min(kManyColumns, count * G - c0);
+  const int cols = min(COLUMNS, count * G - c0);
   if (cols <= 0 || c0 < 0) return;
 
   // ---- columns
@@ -138,12 +138,12 @@ void paged_many_kernel(PagedParams P, int splits) {
   const bool blind = see.hi <= see.lo;
   const int hi_most = most(blind ? 0 : see.hi), hi_least = -most(blind ? -kFar : -see.hi);
   const int lo_most = most(blind ? 0 : see.lo), lo_least = -most(blind ? -kFar : -see.lo);
-  __shared__ int reach[4][kWaves];
-  __shared__ Seen see_s[kManyColumns];
-  __shared__ uint32_t which_s[kManyColumns];         // a column's token past the first one's, its head in the KV head
-  __shared__ uint32_t marks_s[kManyColumns * (D / 16)];
+  __shared__ int reach[4][WAVES];
+  __shared__ Seen see_s[COLUMNS];
+  __shared__ uint32_t which_s[COLUMNS];         // a column's token past the first one's, its head in the KV head
+  __shared__ uint32_t marks_s[COLUMNS * (D / 16)];
   __shared__ int marked;
-  for (int i = threadIdx.x; i < kManyColumns * (D / 16); i += 64 * kWaves) marks_s[i] = 0;
+  for (int i = threadIdx.x; i < COLUMNS * (D / 16); i += 64 * WAVES) marks_s[i] = 0;
   if (threadIdx.x == 0) marked = 0;
   if (half == 0) {
     see_s[32 * wave + n] = see;
@@ -157,7 +157,12 @@ void paged_many_kernel(PagedParams P, int splits) {
     reach[3][wave] = -hi_least;
   }
   __syncthreads();
-  auto of_all = [&](int i) __attribute__((always_inline)) { return max(max(reach[i][0], reach[i][1]), max(reach[i][2], reach[i][3])); };
+  auto of_all = [&](int i) __attribute__((always_inline)) {
+    int v = reach[i][0];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) v = max(v, reach[i][w]);
+    return v;
+  };
   const int all_lo = -of_all(0), all_hi = of_all(1), part_lo = of_all(2), part_hi = -of_all(3);
   int tile0 = __builtin_amdgcn_readfirstlane(all_lo / TT), tile1 = __builtin_amdgcn_readfirstlane((all_hi + TT - 1) / TT);
   if (splits > 1) {
@@ -321,13 +326,13 @@ void paged_many_kernel(PagedParams P, int splits) {
     lds_barrier();
   }
 
-  // ---- through LDS, so that whole vectors are written: 128 dims of the wave's columns at a time
+  // ---- through LDS, so that whole vectors are written: up to 128 dims of the wave's columns at a time
   const float l = blind ? 0.0f : bfly<32>(l_run);
   const float f = only ? finish_scale(P, head, m_run, l) : 1.0f;
   if (!only && mine && half == 0) P.part_ml[part] = make_float2(m_run, l);
   const bool any_marks = marked != 0;
-  constexpr int DD = D < 128 ? D : 128, OS = DD + 4, LANES = DD / 4, COLS = 64 / LANES;
-  static_assert(kWaves * 32 * OS * 4 <= 2 * BUF, "the wave's sums fit where tiles were");
+  constexpr int DD = D == 256 ? 32 : D, OS = DD + 4, LANES = DD / 4, COLS = 64 / LANES;
+  static_assert(WAVES * 32 * OS * 4 <= 2 * BUF, "the wave's sums fit where tiles were");
   float* const o_s = reinterpret_cast<float*>(lds) + wave * 32 * OS;
   const int wave_cols = min(32, cols - 32 * wave), y_col = lane / LANES, y_dim = 4 * (lane % LANES);
 #pragma unroll
@@ -361,10 +366,10 @@ void paged_many_kernel(PagedParams P, int splits) {
 
 template <typename T>
 static int launch_type(const PagedParams& P, int splits, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)(P.c.kv_heads * 8 * ((P.tiles * splits + 7) / 8))), block(64 * kWaves);
-  if (P.c.head_dim == 64) hipLaunchKernelGGL((paged_many_kernel<T, 64>), grid, block, 0, st, P, splits);
-  else if (P.c.head_dim == 128) hipLaunchKernelGGL((paged_many_kernel<T, 128>), grid, block, 0, st, P, splits);
-  else hipLaunchKernelGGL((paged_many_kernel<T, 256>), grid, block, 0, st, P, splits);
+  const dim3 grid((unsigned)(P.c.kv_heads * 8 * ((P.tiles * splits + 7) / 8)));
+  if (P.c.head_dim == 64) hipLaunchKernelGGL((paged_many_kernel<T, 64, 4>), grid, dim3(64 * 4), 0, st, P, splits);
+  else if (P.c.head_dim == 128) hipLaunchKernelGGL((paged_many_kernel<T, 128, 4>), grid, dim3(64 * 4), 0, st, P, splits);
+  else hipLaunchKernelGGL((paged_many_kernel<T, 256, 8>), grid, dim3(64 * 8), 0, st, P, splits);
   return check_launch(what);
 }
 
