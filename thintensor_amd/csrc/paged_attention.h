@@ -217,8 +217,7 @@ struct Marks {
 // paged_few.hip: up to few_columns() columns of a row and KV head; paged_many.hip: any number
 constexpr int few_columns(int64_t head_dim) { return head_dim == 64 ? 64 : head_dim == 128 ? 32 : 16; }
 int launch_paged_few(const PagedParams& P, int blocks16, int rows, int splits, hipStream_t st, const char* what);
-int launch_paged_many(const PagedParams& P, int splits, hipStream_t st, const char* what);
+int launch_paged_many(const PagedParams& P, int waves, int splits, hipStream_t st, const char* what);
 inline int many_tile_tokens(int64_t head_dim) { return head_dim == 256 ? 32 : 64; }
-constexpr int many_columns(int64_t head_dim) { return head_dim == 256 ? 256 : 128; }
 
 }  // namespace tt

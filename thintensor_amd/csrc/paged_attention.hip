@@ -79,6 +79,7 @@ static int launch_join(const PagedParams& P, hipStream_t st, const char* what) {
 // One of a call's launches.
 struct PagedJob {
   bool many;
+  int waves;                            // many: of a workgroup, 32 columns each
   int blocks16, row_tiles, rows;        // few: columns of a workgroup in sixteens, workgroups of a row, rows
   int64_t tiles;                        // many: column tiles
   int splits, share, wide;
@@ -110,8 +111,16 @@ static void split_few(int64_t groups, int64_t tiles, bool parts, PagedJob* j) {
   if (j->splits < 1) j->splits = 1;
 }
 
-static void split_many(int64_t groups, int64_t tiles, PagedJob* j) {
-  const int64_t most = tiles / 4, fill = 2 * device_cus() / (groups > 0 ? groups : 1);
+// Waves of a workgroup for rows of `cols` columns, 32 each: eight share what comes to LDS further (4096 queries behind
+// 16384 tokens, 64 / 8 heads: x 128 2212 us with four, 2075 with eight, x 64 1271 and 1217; 512 rows of heads behind 32768
+// shared tokens 143 and 140; x 256, with registers for one wave of a SIMD or two, 1957 and 1109 us for 2048 behind 8192).
+static int many_waves(int64_t head_dim, int64_t cols) { return head_dim == 256 || cols > 128 ? 8 : 4; }
+
+// Workgroups of them that a CU holds (registers, LDS).
+static int many_per_cu(int64_t head_dim, int waves) { return waves == 8 ? (head_dim == 64 ? 2 : 1) : (head_dim == 64 ? 3 : 2); }
+
+static void split_many(int64_t groups, int64_t tiles, int per_cu, PagedJob* j) {
+  const int64_t most = tiles / 4, fill = per_cu * device_cus() / (groups > 0 ? groups : 1);
   int64_t s = most < fill ? most : fill;
   s = s < 1 ? 1 : s > 256 ? 256 : s;
   j->splits = (int)s;
@@ -126,13 +135,15 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
   p.window = window < p.limit ? window : 0;
   p.shared = rows > 1 ? shared_pages * c->page_size : 0;
   const int64_t each = ragged ? 0 : tokens / rows;
-  const int tt = many_tile_tokens(c->head_dim), mc = many_columns(c->head_dim);
+  const int tt = many_tile_tokens(c->head_dim);
   if (p.shared > 0) {
     const int64_t cols = tokens * G, reach = p.shared < p.limit ? p.shared : p.limit;
     p.prefix.many = cols > few_columns(c->head_dim);
     if (p.prefix.many) {
+      p.prefix.waves = many_waves(c->head_dim, cols);
+      const int mc = 32 * p.prefix.waves;
       p.prefix.tiles = (cols + mc - 1) / mc;
-      split_many(p.prefix.tiles * c->kv_heads, (reach + tt - 1) / tt, &p.prefix);
+      split_many(p.prefix.tiles * c->kv_heads, (reach + tt - 1) / tt, many_per_cu(c->head_dim, p.prefix.waves), &p.prefix);
     } else {
       p.prefix.blocks16 = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
       p.prefix.row_tiles = p.prefix.rows = 1;
@@ -145,9 +156,11 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
   if (selected_count > 0) reach = selected_count * c->page_size;
   p.own.many = ragged || each * G > few_columns(c->head_dim);
   if (p.own.many) {
+    p.own.waves = many_waves(c->head_dim, ragged ? tokens * G / rows : each * G);
+    const int mc = 32 * p.own.waves;
     p.own.row_tiles = (int)((each * G + mc - 1) / mc);
     p.own.tiles = ragged ? tokens * G / mc + rows : rows * p.own.row_tiles;
-    split_many(p.own.tiles * c->kv_heads, (reach + tt - 1) / tt + 1, &p.own);
+    split_many(p.own.tiles * c->kv_heads, (reach + tt - 1) / tt + 1, many_per_cu(c->head_dim, p.own.waves), &p.own);
   } else {
     p.own.blocks16 = each * G <= 16 ? 1 : each * G <= 32 ? 2 : 4;
     p.own.row_tiles = 1;
@@ -170,8 +183,8 @@ static int launch_job(PagedParams P, const PagedJob& j, bool shared, int part0, 
   P.tiles = (int)j.tiles;
   P.wide = j.wide;
   // in order of their length where they do not all run at once
-  P.ordered = j.many && !shared && P.window == 0 && P.of.rows <= 64 && j.tiles * P.c.kv_heads * j.splits > 2 * device_cus();
-  return j.many ? launch_paged_many(P, j.splits, st, what) : launch_paged_few(P, j.blocks16, j.rows, j.splits, st, what);
+  P.ordered = j.many && !shared && P.window == 0 && P.of.rows <= 64 && j.tiles * P.c.kv_heads * j.splits > many_per_cu(P.c.head_dim, j.waves) * device_cus();
+  return j.many ? launch_paged_many(P, j.waves, j.splits, st, what) : launch_paged_few(P, j.blocks16, j.rows, j.splits, st, what);
 }
 
 static int check_attention(const tt_paged_cache* c, int64_t table_pages, bool ragged, int64_t rows, int64_t tokens,

@@ -13,14 +13,14 @@
 
 namespace tt {
 
-// The column tile with the x-th most tokens to see (of up to 64 rows, one for each lane; of equal ones the lower row's),
+// The column tile with the x-th most tokens to see (of up to 64 rows, `count` and `len` of one in each lane; of equal ones the lower row's),
 // so that no long one begins when the others end.  Tile j of a row with n of them sees about b + j + 1 times 128 / per_kv
 // tokens; how many tiles see h or more is a sum over the rows, and h is found by halving.
 template <int COLUMNS>
-__device__ __forceinline__ bool longest(const PagedParams& P, int x, int* row, int* tile) {
-  const int lane = threadIdx.x & 63, r = min(lane, P.of.rows - 1);
-  int first, n = P.of.count(r, &first);
-  const int b = (int)(((int64_t)max(row_length(P, r) - n, 0) * P.per_kv) / COLUMNS);
+__device__ __forceinline__ bool longest(const PagedParams& P, int x, int count, int len, int* row, int* tile) {
+  const int lane = threadIdx.x & 63;
+  int n = count;
+  const int b = (int)(((int64_t)max(len - n, 0) * P.per_kv) / COLUMNS);
   n = lane < P.of.rows ? (int)(((int64_t)n * P.per_kv + COLUMNS - 1) / COLUMNS) : 0;
   auto at_least = [&](int h) __attribute__((always_inline)) {
     return (int)__builtin_amdgcn_readlane((int)lanes_before((uint32_t)min(max(b + n - h + 1, 0), n)), 63);
@@ -48,7 +48,7 @@ __device__ __forceinline__ bool longest(const PagedParams& P, int x, int* row, i
 }
 
 template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D == 64 ? (WAVES == 8 ? 4 : 3) : 2)))
 void paged_many_kernel(PagedParams P, int splits) {
   using B = Bits16<T>;
   constexpr int COLUMNS = 32 * WAVES;
@@ -75,26 +75,41 @@ void paged_many_kernel(PagedParams P, int splits) {
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int G = P.per_kv;
-  int row = 0, first = 0, count = P.of.tokens, c0 = x * COLUMNS;
+  int row = 0, first = 0, count = P.of.tokens, len = 0, c0 = x * COLUMNS;
   if (!P.shared_job) {
-    if (P.ordered) {
+    if (P.of.rows <= 64 && (P.ordered || P.of.cu)) {       // a row for each lane, what is known of it in one request
+      const int r = min(lane, P.of.rows - 1);
+      int r_first;
+      const int r_count = P.of.count(r, &r_first), r_len = row_length(P, r);
       int tile;
-      if (!longest<COLUMNS>(P, x_first, &row, &tile)) return;
-      count = P.of.count(row, &first);
+      if (P.ordered) {
+        if (!longest<COLUMNS>(P, x_first, r_count, r_len, &row, &tile)) return;
+      } else {
+        const int before = (int)((int64_t)r_first * G / COLUMNS) + r;
+        row = max(0, __popcll(__builtin_amdgcn_ballot_w64(lane < P.of.rows && before <= x)) - 1);
+        tile = x - __builtin_amdgcn_readlane(before, row);
+      }
+      first = __builtin_amdgcn_readlane(r_first, row);
+      count = __builtin_amdgcn_readlane(r_count, row);
+      len = __builtin_amdgcn_readlane(r_len, row);
       c0 = tile * COLUMNS;
-    } else if (P.of.cu) {
-      row = P.of.find(x, G, COLUMNS, 1);
-      count = P.of.count(row, &first);
-      c0 = (x - (int)((int64_t)first * G / COLUMNS) - row) * COLUMNS;
     } else {
-      row = x / P.row_tiles;
-      count = P.of.each;
-      first = row * count;
-      c0 = (x - row * P.row_tiles) * COLUMNS;
+      if (P.of.cu) {
+        row = P.of.find(x, G, COLUMNS, 1);
+        count = P.of.count(row, &first);
+        c0 = (x - (int)((int64_t)first * G / COLUMNS) - row) * COLUMNS;
+      } else {
+        row = x / P.row_tiles;
+        count = P.of.each;
+        first = row * count;
+        c0 = (x - row * P.row_tiles) * COLUMNS;
+      }
+      len = row_length(P, row);
     }
     row = __builtin_amdgcn_readfirstlane(row);
     first = __builtin_amdgcn_readfirstlane(first);
     count = __builtin_amdgcn_readfirstlane(count);
+    len = __builtin_amdgcn_readfirstlane(len);
     c0 = __builtin_amdgcn_readfirstlane(c0);
   }
   const int cols = min(COLUMNS, count * G - c0);
@@ -123,7 +138,7 @@ void paged_many_kernel(PagedParams P, int splits) {
     const int r = row_of(P.of, token, &place, &each);
     see = r < P.of.rows ? seen_of(P, row_length(P, r), place, each) : Seen{0, 0};
   } else {
-    see = seen_of(P, row_length(P, row), at, count);
+    see = seen_of(P, len, at, count);
   }
   see.hi = max(see.hi, 0);
   // of this wave's columns, and of all of them
@@ -262,14 +277,10 @@ void paged_many_kernel(PagedParams P, int splits) {
   lds_barrier();
   for (int tile = tile0; tile < tile1; tile++) {
     const int buf = (tile - tile0) & 1, t0 = tile * TT;
-    if (tile + 1 < tile1) {
-      stage(tile + 1, buf ^ 1);
-      load(tile + 2);
-      look(tile + 3);
-    }
     const char* const buf_s = lds + buf * BUF;
-    if (t0 < hi_most && t0 + TT > lo_least) {
-      f16v_t s[J];
+    const bool seen = t0 < hi_most && t0 + TT > lo_least;
+    f16v_t s[J];
+    if (seen) {
 #pragma unroll
       for (int j = 0; j < J; j++) {
 #pragma unroll
@@ -278,13 +289,22 @@ void paged_many_kernel(PagedParams P, int splits) {
         for (int k = 0; k < KI; k++)
           s[j] = B::mfma32(*reinterpret_cast<const u4_t*>(buf_s + k_get + j * 32 * KS + 32 * k), qb[k], s[j]);
       }
+    }
+    // the next tile goes to LDS while the matrix cores work
+    if (tile + 1 < tile1) {
+      stage(tile + 1, buf ^ 1);
+      load(tile + 2);
+      look(tile + 3);
+    }
+    if (seen) {
       if (t0 < lo_most || t0 + TT > hi_least) {
+        const int t_lane = t0 + 4 * half - see.lo;
+        const uint32_t width = (uint32_t)max(see.hi - see.lo, 0);
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
           for (int r = 0; r < 16; r++) {
-            const int t = t0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (t < see.lo || t >= see.hi) s[j][r] = ninf;
+            if ((uint32_t)(t_lane + 32 * j + 8 * (r >> 2) + (r & 3)) >= width) s[j][r] = ninf;
           }
       }
       float top = s[0][0];
@@ -331,7 +351,7 @@ void paged_many_kernel(PagedParams P, int splits) {
   const float f = only ? finish_scale(P, head, m_run, l) : 1.0f;
   if (!only && mine && half == 0) P.part_ml[part] = make_float2(m_run, l);
   const bool any_marks = marked != 0;
-  constexpr int DD = D == 256 ? 32 : D, OS = DD + 4, LANES = DD / 4, COLS = 64 / LANES;
+  constexpr int DD = WAVES == 8 ? 32 : D, OS = DD + 4, LANES = DD / 4, COLS = 64 / LANES;
   static_assert(WAVES * 32 * OS * 4 <= 2 * BUF, "the wave's sums fit where tiles were");
   float* const o_s = reinterpret_cast<float*>(lds) + wave * 32 * OS;
   const int wave_cols = min(32, cols - 32 * wave), y_col = lane / LANES, y_dim = 4 * (lane % LANES);
@@ -364,17 +384,28 @@ void paged_many_kernel(PagedParams P, int splits) {
   }
 }
 
-template <typename T>
-static int launch_type(const PagedParams& P, int splits, hipStream_t st, const char* what) {
+template <typename T, int D>
+static int launch_dim(const PagedParams& P, int waves, int splits, hipStream_t st, const char* what) {
   const dim3 grid((unsigned)(P.c.kv_heads * 8 * ((P.tiles * splits + 7) / 8)));
-  if (P.c.head_dim == 64) hipLaunchKernelGGL((paged_many_kernel<T, 64, 4>), grid, dim3(64 * 4), 0, st, P, splits);
-  else if (P.c.head_dim == 128) hipLaunchKernelGGL((paged_many_kernel<T, 128, 4>), grid, dim3(64 * 4), 0, st, P, splits);
-  else hipLaunchKernelGGL((paged_many_kernel<T, 256, 8>), grid, dim3(64 * 8), 0, st, P, splits);
+  if constexpr (D < 256) {
+    if (waves == 4) {
+      hipLaunchKernelGGL((paged_many_kernel<T, D, 4>), grid, dim3(64 * 4), 0, st, P, splits);
+      return check_launch(what);
+    }
+  }
+  hipLaunchKernelGGL((paged_many_kernel<T, D, 8>), grid, dim3(64 * 8), 0, st, P, splits);
   return check_launch(what);
 }
 
-int launch_paged_many(const PagedParams& P, int splits, hipStream_t st, const char* what) {
-  return P.c.dtype == TT_F16 ? launch_type<f16_t>(P, splits, st, what) : launch_type<bf16_t>(P, splits, st, what);
+template <typename T>
+static int launch_type(const PagedParams& P, int waves, int splits, hipStream_t st, const char* what) {
+  if (P.c.head_dim == 64) return launch_dim<T, 64>(P, waves, splits, st, what);
+  if (P.c.head_dim == 128) return launch_dim<T, 128>(P, waves, splits, st, what);
+  return launch_dim<T, 256>(P, waves, splits, st, what);
+}
+
+int launch_paged_many(const PagedParams& P, int waves, int splits, hipStream_t st, const char* what) {
+  return P.c.dtype == TT_F16 ? launch_type<f16_t>(P, waves, splits, st, what) : launch_type<bf16_t>(P, waves, splits, st, what);
 }
 
 }  // namespace tt
