@@ -127,25 +127,60 @@ __device__ __forceinline__ Seen seen_of(const PagedParams& P, int n, int place, 
 }
 __device__ __forceinline__ int row_length(const PagedParams& P, int row) { return min(max(P.lengths[row], 0), P.max_length); }
 
+// The pages of a row, or of a selection of them: entry e of the table (of the selection) in lane e - base, of 64 and
+// the 64 after them, so that looking one up is a move between registers.  (Scalar loads of the table would be waited for
+// with every read of LDS.)
+struct PageLanes {
+  const int32_t* table;
+  const int32_t* sel;
+  int pages, count, valid;       // of the table, of the selection; of the cache
+  int base, id[2], logical[2];
+  __device__ __forceinline__ void load(int slot, int from) {
+    const int e = from + (int)(threadIdx.x & 63);
+    if (sel) {
+      const int l = sel[min(e, count - 1)];
+      const bool ok = e < count && l >= 0 && l < pages;
+      logical[slot] = ok ? l : -1;
+      id[slot] = table[ok ? l : 0];
+    } else {
+      id[slot] = table[min(e, pages - 1)];
+    }
+  }
+  __device__ __forceinline__ void start(int entry) {
+    base = entry;
+    load(0, base);
+    load(1, base + 64);
+  }
+  __device__ __forceinline__ void reach(int entry) {         // entries from this one on (at most 127 past base)
+    if (entry - base >= 64) {
+      base += 64;
+      id[0] = id[1];
+      logical[0] = logical[1];
+      load(1, base + 64);
+    }
+  }
+  __device__ __forceinline__ int pick(const int (&v)[2], int entry) const {
+    const int at = entry - base;
+    return at < 64 ? __builtin_amdgcn_readlane(v[0], at) : __builtin_amdgcn_readlane(v[1], at - 64);
+  }
+};
+
 // Sixteen tokens of a KV head that begin at a multiple of sixteen: one page holds them.
 struct Place {
   const char *k, *v;
-  int t;             // their first token; past every length where a selection has none
+  int t;             // their first token; past every length where there is none
   bool bad;          // no page
 };
-__device__ __forceinline__ Place place_of(const PagedParams& P, const int32_t* table, const int32_t* sel, int kvh, int u) {
+__device__ __forceinline__ Place place_of(const PagedParams& P, const PageLanes& L, const char* k, const char* v, int u) {
   Place p;
-  int logical = u >> P.page_shift;
-  const int slot = u & ((1 << P.page_shift) - 1);
-  if (sel) logical = logical < P.selected_count ? sel[logical] : -1;
-  const bool none = logical < 0 || logical >= P.table_pages;
-  const int at = none ? 0 : logical;
-  const int32_t id = table[at];
-  p.bad = id < 0 || id >= P.c.pages;
+  const int entry = u >> P.page_shift, slot = u & ((1 << P.page_shift) - 1);
+  const int logical = L.sel ? L.pick(L.logical, entry) : entry;
+  const int32_t id = L.pick(L.id, entry);
+  p.bad = (uint32_t)id >= (uint32_t)L.valid;
   const int64_t page = p.bad ? 0 : id;
-  p.t = none ? 0x7fffff00 : (at << P.page_shift) + slot;
-  p.k = reinterpret_cast<const char*>(P.c.k_pages) + 2 * (page * P.c.k_page + kvh * P.c.k_head + slot * P.c.k_token);
-  p.v = reinterpret_cast<const char*>(P.c.v_pages) + 2 * (page * P.c.v_page + kvh * P.c.v_head + slot * P.c.v_token);
+  p.t = (uint32_t)logical >= (uint32_t)L.pages ? 0x7fffff00 : (logical << P.page_shift) + slot;
+  p.k = k + 2 * (page * P.c.k_page + slot * P.c.k_token);
+  p.v = v + 2 * (page * P.c.v_page + slot * P.c.v_token);
   return p;
 }
 

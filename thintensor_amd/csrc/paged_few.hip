@@ -92,15 +92,20 @@ void paged_few_kernel(PagedParams P) {
       vr[k] = *reinterpret_cast<const u4_t*>(p[h].v + (size_t)((uint32_t)(k * VR - 16 * h + v_row) * v_step + 16 * v_piece));
     }
   };
+  PageLanes lanes{table, sel, P.table_pages, P.selected_count, (int)P.c.pages, 0, {0, 0}, {0, 0}};
+  const char* const kbase = reinterpret_cast<const char*>(P.c.k_pages) + 2 * kvh * P.c.k_head;
+  const char* const vbase = reinterpret_cast<const char*>(P.c.v_pages) + 2 * kvh * P.c.v_head;
   auto place = [&](int j, Place (&p)[2]) __attribute__((always_inline)) {
-    p[0] = place_of(P, table, sel, kvh, kTile * j);
-    p[1] = place_of(P, table, sel, kvh, kTile * j + 16);
+    lanes.reach((kTile * j) >> P.page_shift);
+    p[0] = place_of(P, lanes, kbase, vbase, kTile * j);
+    p[1] = place_of(P, lanes, kbase, vbase, kTile * j + 16);
   };
   // (a place past the table is one in page 0 that nobody sees; a row's first split has a tile unless the row is empty)
   int tile0 = sel || P.shared_job ? 0 : P.shared / kTile;
   const bool early = split == 0 && (P.window == 0 || sel);
   Place now[2], next[2];
   if (early) {
+    lanes.start((kTile * (tile0 + wave)) >> P.page_shift);
     place(tile0 + wave, now);
     load_k(now);
     load_v(now);
@@ -153,7 +158,8 @@ void paged_few_kernel(PagedParams P) {
   }
   int i = tile0 + wave;
   if (!early && tile0 < tile1) {
-    place(min(i, tile1 - 1), now);
+    lanes.start((kTile * i) >> P.page_shift);
+    place(i, now);
     load_k(now);
     load_v(now);
     place(i + WAVES, next);

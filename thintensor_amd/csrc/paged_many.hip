@@ -203,24 +203,19 @@ void paged_many_kernel(PagedParams P, int splits) {
   const char* const kbase = reinterpret_cast<const char*>(P.c.k_pages) + 2 * kvh * P.c.k_head;
   const char* const vbase = reinterpret_cast<const char*>(P.c.v_pages) + 2 * kvh * P.c.v_head;
   u4_t kr[NK], vr[NK];
-  int ids[NK];
-  auto look = [&](int tile) __attribute__((always_inline)) {      // the pages of a tile's rows
-#pragma unroll
-    for (int k = 0; k < NK; k++) {
-      const int t = min(tile, tile1 - 1) * TT + k * RR + wave * (64 / PC);
-      ids[k] = table[min(t >> P.page_shift, P.table_pages - 1)];
-    }
-  };
+  PageLanes lanes{table, nullptr, P.table_pages, 0, (int)P.c.pages, 0, {0, 0}, {0, 0}};
   auto load = [&](int tile) __attribute__((always_inline)) {
+    lanes.reach((min(tile, tile1 - 1) * TT) >> P.page_shift);
 #pragma unroll
     for (int k = 0; k < NK; k++) {
       const int t = min(tile, tile1 - 1) * TT + k * RR + wave * (64 / PC);
-      const bool bad = (uint32_t)ids[k] >= (uint32_t)P.c.pages;
+      const int page = lanes.pick(lanes.id, t >> P.page_shift);
+      const bool bad = (uint32_t)page >= (uint32_t)P.c.pages;
       if (bad && tile < tile1) {           // (rare, and more than one lane may say so)
         marks.no_page(t, 64 / PC);
         marked = 1;
       }
-      const int64_t id = bad ? 0 : ids[k];
+      const int64_t id = bad ? 0 : page;
       const int64_t slot = t & page_mask;
       kr[k] = *reinterpret_cast<const u4_t*>(kbase + 2 * id * P.c.k_page + slot * k_step + (size_t)k_at);
       vr[k] = *reinterpret_cast<const u4_t*>(vbase + 2 * id * P.c.v_page + slot * v_step + (size_t)v_at);
@@ -267,12 +262,10 @@ void paged_many_kernel(PagedParams P, int splits) {
   const uint32_t v_get = (uint32_t)(TT * KS + (4 * half + ((lane & 15) >> 2)) * VS + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
 
   if (tile0 < tile1) {
-    look(tile0);
+    lanes.start((tile0 * TT) >> P.page_shift);
     load(tile0);
-    look(tile0 + 1);
     stage(tile0, 0);
     load(tile0 + 1);
-    look(tile0 + 2);
   }
   lds_barrier();
   for (int tile = tile0; tile < tile1; tile++) {
@@ -294,7 +287,6 @@ void paged_many_kernel(PagedParams P, int splits) {
     if (tile + 1 < tile1) {
       stage(tile + 1, buf ^ 1);
       load(tile + 2);
-      look(tile + 3);
     }
     if (seen) {
       if (t0 < lo_most || t0 + TT > hi_least) {
