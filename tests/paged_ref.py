@@ -68,8 +68,9 @@ def attention(q, k_pages, v_pages, table, lengths, counts, page, *, window=0, si
 def attention_bound(want, mag, reach, seen, peak, dtype):
     """Scores: D exact products added in binary32 and one scaling, (D + 24) 2^-24 of the largest sum of
     |q| |k| scale; the exponential 2^-20 with the rounding of its argument.  Both count twice, above and below the
-    line.  Weights: rounded once to the cache's 16-bit type before the product with V (where many queries
-    share the work), half a step, finfo.eps / 2 of sum p |v|; where that type is fp16 at least half of its smallest step,
+    line.  Weights: rounded once to the cache's 16-bit type, p' = p (1 + d) with |d| <= e = finfo.eps / 2, for the
+    product with V and for their own sum alike: sum p' v / sum p' - out = (sum p d v - out sum p d) / sum p', no more
+    than e (sum p |v| / sum p + |out|) / (1 - e); where that type is fp16 at least half of its smallest step,
     2^-25 of the largest weight for each token (weights are scaled so that the largest is no less than 1), times the
     largest |v|.
     Sums over the tokens seen: every token adds at most one rounding in each of two sums, 2^-24 of them, and a few
@@ -78,7 +79,8 @@ def attention_bound(want, mag, reach, seen, peak, dtype):
     d = want.shape[-1]
     rel = 2 * ((d + 24) * 2.0 ** -24 * reach + 2.0 ** -20) + (2 * seen[:, None, None] + 64) * 2.0 ** -24 + info.eps / 2
     small = seen[:, None, None] * 2.0 ** -25 * peak if dtype == torch.float16 else 0.0
-    return rel * mag + small + info.eps / 2 * np.abs(want) * (1 + 2.0 ** -8) + info.tiny * info.eps
+    rel, out = rel * (1 + 2.0 ** -7), info.eps * np.abs(want) * (1 + 2.0 ** -7)     # 1 / (1 - e); weights' sum and the store
+    return rel * mag + small + out + info.tiny * info.eps
 
 
 def scores(q, bounds, table_row, pages_of_row):

@@ -36,23 +36,36 @@ struct Run {
 __device__ __forceinline__ Run run_of(const AppendParams& P, int x) {
   Run r;
   const int page = (int)P.c.page_size;
-  const int row = __builtin_amdgcn_readfirstlane(P.of.cu ? P.of.find(x, 1, page, 2) : 0);
-  int row_u = row, unit;
-  if (P.of.cu == nullptr) {
-    const int units = P.of.each / page + 2;
-    row_u = x / units;
-    unit = x - row_u * units;
+  int row, unit, first, n;
+  if (P.of.cu && P.of.rows <= 64) {        // a row for each lane, what is known of it in one request
+    const int lane = threadIdx.x & 63, mine = min(lane, P.of.rows - 1);
+    int my_first;
+    const int my_n = P.of.count(mine, &my_first), my_start = P.starts[mine];
+    const int before = my_first / page + 2 * mine;
+    row = max(0, __popcll(__builtin_amdgcn_ballot_w64(lane < P.of.rows && before <= x)) - 1);
+    unit = x - __builtin_amdgcn_readlane(before, row);
+    first = __builtin_amdgcn_readlane(my_first, row);
+    n = __builtin_amdgcn_readlane(my_n, row);
+    r.start = __builtin_amdgcn_readlane(my_start, row);
+  } else {
+    if (P.of.cu) {
+      row = __builtin_amdgcn_readfirstlane(P.of.find(x, 1, page, 2));
+      n = P.of.count(row, &first);
+      unit = x - (first / page + 2 * row);
+    } else {
+      const int units = P.of.each / page + 2;
+      row = x / units;
+      unit = x - row * units;
+      n = P.of.count(row, &first);
+    }
+    r.start = P.starts[row];
   }
-  int first;
-  const int n = P.of.count(row_u, &first);
-  if (P.of.cu) unit = x - (first / page + 2 * row_u);
   r.first = first;
-  r.start = P.starts[row_u];
   r.logical = (r.start >> __builtin_ctz(page)) + unit;      // floor, of negative positions too
   const int64_t a = r.logical * page - r.start, b = a + page;
   r.from = (int)(a > 0 ? (a < n ? a : n) : 0);
   r.to = (int)(b < n ? b : n);
-  r.id = r.logical >= 0 && r.logical < P.table_pages ? P.table[row_u * P.table_row + r.logical] : -1;
+  r.id = r.logical >= 0 && r.logical < P.table_pages ? P.table[row * P.table_row + r.logical] : -1;
   if (r.id >= P.c.pages || r.id < 0) r.id = -1;
   return r;
 }
@@ -142,15 +155,23 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
     load(r0);
     __shared__ int64_t pos_s[64];
     __shared__ int in_row[64];
-    if (tid < tokens) {
-      int place, count;
-      const int r = row_of(P.of, t0 + tid, &place, &count);
-      in_row[tid] = r < P.of.rows;
-      pos_s[tid] = r < P.of.rows ? (int64_t)P.starts[r] + place : 0;
+    __shared__ int cu_s[257], start_s[256];
+    const bool by_lds = P.of.cu && P.of.rows <= 256;
+    if (by_lds) {                          // the rows' bounds and positions in one request, halved in LDS
+      for (int i = tid; i <= P.of.rows; i += 256) cu_s[i] = P.of.begin(i);
+      if (tid < P.of.rows) start_s[tid] = P.starts[tid];
+      lds_barrier();
     }
-    __syncthreads();
+    if (tid < tokens) {
+      int place, count, start = 0;
+      const int r = by_lds ? row_of(RowTokens{cu_s, P.of.rows, P.of.tokens, 0}, t0 + tid, &place, &count) : row_of(P.of, t0 + tid, &place, &count);
+      if (r < P.of.rows) start = by_lds ? start_s[r] : P.starts[r];
+      in_row[tid] = r < P.of.rows;
+      pos_s[tid] = r < P.of.rows ? (int64_t)start + place : 0;
+    }
+    lds_barrier();
     form_turns(P, turn_s, tokens, [&](int tk) { return pos_s[tk]; });
-    __syncthreads();
+    lds_barrier();
     for (int r = r0; r < total; r += kAhead * rows) {
       if (r != r0) load(r);
 #pragma unroll
@@ -196,9 +217,9 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
         x[i].load(k + (int64_t)min(t + i * lanes, end - 1) * P.k_token + head * P.k_head, d0, d1, copy);
     };
     if (works) load(c0 + tk0);
-    if (c0 > 0) __syncthreads();
+    if (c0 > 0) lds_barrier();
     form_turns(P, turn_s, end - c0, [&](int tk) { return run.start + run.from + c0 + tk; });
-    __syncthreads();
+    lds_barrier();
     if (works)
       for (int t = c0 + tk0; t < end; t += kAhead * lanes) {
         if (t != c0 + tk0) load(t);

@@ -165,7 +165,8 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
     p.own.blocks16 = each * G <= 16 ? 1 : each * G <= 32 ? 2 : 4;
     p.own.row_tiles = 1;
     p.own.rows = (int)rows;
-    split_few(rows * c->kv_heads, (reach + 31) / 32 + (p.window > 0 ? 1 : 0), p.shared > 0, &p.own);
+    // (one tile more where they may begin inside one)
+    split_few(rows * c->kv_heads, (reach + 31) / 32 + (p.window > 0 || p.shared % 32 != 0 ? 1 : 0), false, &p.own);
   }
   p.parts = p.own.splits + (p.shared > 0 ? p.prefix.splits : 0);
   return p;

@@ -50,11 +50,12 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectParams P) {
   const int row = blockIdx.z, kvh = blockIdx.y, p0 = blockIdx.x * 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int pages = row_pages(P, row);
-  if (p0 >= pages) return;
+  // (entries past the row's pages may be anything, what they lead to is not used)
   auto page_of = [&](int p) __attribute__((always_inline)) {
-    const int32_t id = P.table[row * P.table_row + min(p, pages - 1)];
+    const int32_t id = P.table[row * P.table_row + min(p, P.table_pages - 1)];
     return id < 0 || id >= P.c.pages ? -1 : id;
   };
+  if (p0 > 0 && p0 >= pages) return;       // the first ones do not wait for the length
   {
     const int l_row = threadIdx.x / RP, l_piece = threadIdx.x % RP;
     const char* base = reinterpret_cast<const char*>(P.c.k_bounds) + 2 * kvh * P.c.b_head + 16 * l_piece;
@@ -149,11 +150,13 @@ __global__ __launch_bounds__(THREADS) void page_pick_kernel(SelectParams P) {
   const uint32_t* keys = P.keys + at * P.keys_row;
   int32_t* out = P.selected + at * P.count;
   const int pages = row_pages(P, row), first = min(P.first, pages), last = max(first, pages - P.last);
-  const int places = P.count - (first + pages - last), per = (pages + THREADS - 1) / THREADS;
-  const int p0 = min(tid * per, pages), p1 = min(p0 + per, pages);
+  const int places = P.count - (first + pages - last);
+  // runs of pages by the most there may be, so that keys are requested before the row's length is known (what lies past
+  // its pages is not used)
+  const int per = ((int)P.keys_row + THREADS - 1) / THREADS, p0 = tid * per, p1 = min(p0 + per, pages);
   uint32_t held[HELD];
 #pragma unroll
-  for (int k = 0; k < HELD; k++) held[k] = pages > 0 ? keys[min(p0 + k, pages - 1)] : 0;
+  for (int k = 0; k < HELD; k++) held[k] = keys[min(p0 + k, (int)P.keys_row - 1)];
   for (int i = tid; i < 4 * 256; i += THREADS) (&hist[0][0])[i] = 0;
   auto each = [&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
