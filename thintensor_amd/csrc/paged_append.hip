@@ -8,6 +8,8 @@
 #include "tt_common.h"
 #include "tt_eight.h"
 
+#include <type_traits>
+
 namespace tt {
 
 struct AppendParams {
@@ -119,8 +121,16 @@ template <typename T, bool INTERLEAVED> struct Turned {
   }
 };
 
+// f(0) .. f(N - 1), each with its own code: indexes of registers have to be known
+template <int N, typename F> __device__ __forceinline__ void each_of(F&& f) {
+  if constexpr (N > 0) {
+    each_of<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+
 constexpr int kAhead = 4;                  // requested together, so that loads do not wait behind stores
-constexpr int kTurnFloats = 8192;          // of LDS: tokens whose angles are formed at once, times rotary
+constexpr int kTurnFloats = 4096;          // of LDS: tokens whose angles are formed at once, times rotary
 
 // Rows whose vectors start on 16-byte boundaries and whose parts come in whole pieces of eight dims.
 template <typename T, bool INTERLEAVED>
@@ -174,15 +184,15 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
     lds_barrier();
     for (int r = r0; r < total; r += kAhead * rows) {
       if (r != r0) load(r);
-#pragma unroll
-      for (int k = 0; k < kAhead; k++) {
-        if (r + k * rows >= total) break;
+      each_of<kAhead>([&](auto index) __attribute__((always_inline)) {
+        constexpr int k = index;
+        if (r + k * rows >= total) return;
         int tk, h;
         at(r + k * rows, &tk, &h);
-        if (!in_row[tk]) continue;
+        if (!in_row[tk]) return;
         if (!copy) x[k].turn(turn_s + tk * P.rotary, half, u);
         x[k].store(reinterpret_cast<T*>(P.q_out) + (int64_t)(t0 + tk) * P.o_token + h * P.o_head, d0, d1, copy);
-      }
+      });
     }
     return;
   }
@@ -207,6 +217,25 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
     lo[e] = __builtin_bit_cast(float, 0x7f800000u);
     hi[e] = __builtin_bit_cast(float, 0xff800000u);
   }
+  // values: pieces of all tokens and heads, the first ones requested before the keys
+  const int pieces = dim / 8, v_per = heads * pieces, v_total = n * v_per;
+  typedef uint32_t v4_t __attribute__((ext_vector_type(4)));
+  v4_t y[kAhead];
+  auto load_v = [&](int i) __attribute__((always_inline)) {
+    each_of<kAhead>([&](auto index) __attribute__((always_inline)) {
+      constexpr int a = index;
+      const int j = min(i + a * 256, v_total - 1), tk = j / v_per, r = j - tk * v_per, h = r / pieces;
+      y[a] = *reinterpret_cast<const v4_t*>(v + (int64_t)tk * P.v_token + h * P.v_head + 8 * (r - h * pieces));
+    });
+  };
+  auto store_v = [&](int i) __attribute__((always_inline)) {
+    each_of<kAhead>([&](auto index) __attribute__((always_inline)) {
+      constexpr int a = index;
+      const int j = i + a * 256, tk = j / v_per, r = j - tk * v_per, h = r / pieces;
+      if (j < v_total) *reinterpret_cast<v4_t*>(vp + (int64_t)tk * P.c.v_token + h * P.c.v_head + 8 * (r - h * pieces)) = y[a];
+    });
+  };
+  load_v(tid);
   const int chunk = P.rotary > 0 ? min(n, kTurnFloats / P.rotary) : n;
   for (int c0 = 0; c0 < n; c0 += chunk) {
     const int end = min(c0 + chunk, n);
@@ -223,10 +252,10 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
     if (works)
       for (int t = c0 + tk0; t < end; t += kAhead * lanes) {
         if (t != c0 + tk0) load(t);
-#pragma unroll
-        for (int i = 0; i < kAhead; i++) {
+        each_of<kAhead>([&](auto index) __attribute__((always_inline)) {
+          constexpr int i = index;
           const int tt = t + i * lanes;
-          if (tt >= end) break;
+          if (tt >= end) return;
           if (!copy) x[i].turn(turn_s + (tt - c0) * P.rotary, half, u);
           x[i].store(kp + (int64_t)tt * P.c.k_token + head * P.c.k_head, d0, d1, copy);
           if (P.c.k_bounds) {
@@ -240,33 +269,13 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
               }
             }
           }
-        }
+        });
       }
   }
-  {
-    const int pieces = dim / 8, per = heads * pieces;
-    const int total = n * per;
-    for (int i = tid; i < total; i += kAhead * 256) {
-      Eight<T> y[kAhead];
-      auto at = [&](int j, int* tk, int* h) __attribute__((always_inline)) {
-        *tk = j / per;
-        *h = (j - *tk * per) / pieces;
-        return 8 * (j % pieces);
-      };
-#pragma unroll
-      for (int a = 0; a < kAhead; a++) {
-        int tk, h;
-        const int d = at(min(i + a * 256, total - 1), &tk, &h);
-        y[a].load(v + (int64_t)tk * P.v_token + h * P.v_head + d);
-      }
-#pragma unroll
-      for (int a = 0; a < kAhead; a++) {
-        if (i + a * 256 >= total) break;
-        int tk, h;
-        const int d = at(i + a * 256, &tk, &h);
-        y[a].store(vp + (int64_t)tk * P.c.v_token + h * P.c.v_head + d);
-      }
-    }
+  store_v(tid);
+  for (int i = tid + kAhead * 256; i < v_total; i += kAhead * 256) {
+    load_v(i);
+    store_v(i);
   }
   if (P.c.k_bounds == nullptr) return;
   // ---- a dim's extremes over the token lanes: first those of low, then those of high, in the angles' LDS
