@@ -53,6 +53,18 @@ struct PagedRegions {
   bool apart_from(const Region& r) const { return apart(of[0], r) && apart(of[1], r) && apart(of[2], r); }
 };
 
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+
+// Two binary32 values rounded to a 16-bit type, to nearest even.
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack_pair<f16_t>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){pin_f32(a), pin_f32(b)}, h2));
+}
+template <> __device__ __forceinline__ uint32_t pack_pair<bf16_t>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, b2_t));
+}
+
 // Sum over the lanes up to this one.
 __device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
 #define TT_STEP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);

@@ -86,6 +86,31 @@ __device__ __forceinline__ void form_turns(const AppendParams& P, float* turn, i
   }
 }
 
+// Eight binary32 values rounded to a 16-bit type by the conversion instruction.
+template <typename T> __device__ __forceinline__ uint4 rounded(const float* v) {
+  return make_uint4(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]), pack_pair<T>(v[4], v[5]), pack_pair<T>(v[6], v[7]));
+}
+
+template <typename T> constexpr uint32_t kInfinity = 0x7c00;
+template <> constexpr uint32_t kInfinity<bf16_t> = 0x7f80;
+
+// Two 16-bit floats as integers in their order (-0 below +0; NaN beyond the infinity of its sign), and back.
+typedef short ss2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t to_keys(uint32_t w) {
+  return w ^ (__builtin_bit_cast(uint32_t, __builtin_bit_cast(ss2_t, w) >> 15) | 0x80008000u);
+}
+__device__ __forceinline__ uint32_t from_keys(uint32_t k) {
+  return k ^ (~__builtin_bit_cast(uint32_t, __builtin_bit_cast(ss2_t, k) >> 15) | 0x80008000u);
+}
+__device__ __forceinline__ uint32_t keys_min(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(us2_t, a), __builtin_bit_cast(us2_t, b)));
+}
+__device__ __forceinline__ uint32_t keys_max(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2_t, a), __builtin_bit_cast(us2_t, b)));
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
 // A place of a head: eight pairs of the half layout (two pieces of eight dims), four of the interleaved one (one
 // piece), or a piece to copy.
 template <typename T, bool INTERLEAVED> struct Turned {
@@ -111,9 +136,9 @@ template <typename T, bool INTERLEAVED> struct Turned {
         ra[e] = x * c - y * s;
         rb[e] = y * c + x * s;
       }
-      b.set(rb);
+      b.v = rounded<T>(rb);
     }
-    a.set(ra);
+    a.v = rounded<T>(ra);
   }
   __device__ __forceinline__ void store(T* o, int d0, int d1, bool copy) const {
     if (NP == 2 && !copy) b.store(o + d1);
@@ -211,11 +236,11 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
   // a thread keeps one place of one head and walks over the tokens
   const int lanes = rows / heads, tk0 = r0 / heads, head = r0 - tk0 * heads;
   const bool works = tk0 < lanes;
-  float lo[8 * NP], hi[8 * NP];
+  uint32_t lo[4 * NP], hi[4 * NP];         // extremes of its places, as integers
 #pragma unroll
-  for (int e = 0; e < 8 * NP; e++) {
-    lo[e] = __builtin_bit_cast(float, 0x7f800000u);
-    hi[e] = __builtin_bit_cast(float, 0xff800000u);
+  for (int e = 0; e < 4 * NP; e++) {
+    lo[e] = 0xffffffffu;
+    hi[e] = 0u;
   }
   // values: pieces of all tokens and heads, the first ones requested before the keys
   const int pieces = dim / 8, v_per = heads * pieces, v_total = n * v_per;
@@ -260,13 +285,11 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
           x[i].store(kp + (int64_t)tt * P.c.k_token + head * P.c.k_head, d0, d1, copy);
           if (P.c.k_bounds) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {                     // of the keys as they are stored; NaN stays
-              lo[e] = __builtin_elementwise_minimum(lo[e], x[i].a.get(e));
-              hi[e] = __builtin_elementwise_maximum(hi[e], x[i].a.get(e));
-              if (NP == 2 && !copy) {
-                lo[8 * (NP - 1) + e] = __builtin_elementwise_minimum(lo[8 * (NP - 1) + e], x[i].b.get(e));
-                hi[8 * (NP - 1) + e] = __builtin_elementwise_maximum(hi[8 * (NP - 1) + e], x[i].b.get(e));
-              }
+            for (int e = 0; e < 4 * NP; e++) {                // of the keys as they are stored
+              if (e >= 4 && copy) break;
+              const uint32_t k = to_keys(word_of(e < 4 ? x[i].a.v : x[i].b.v, e & 3));
+              lo[e] = keys_min(lo[e], k);
+              hi[e] = keys_max(hi[e], k);
             }
           }
         });
@@ -278,30 +301,52 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
     store_v(i);
   }
   if (P.c.k_bounds == nullptr) return;
-  // ---- a dim's extremes over the token lanes: first those of low, then those of high, in the angles' LDS
+  // ---- a dim's extremes over the token lanes, where the angles were
   T* bp = reinterpret_cast<T*>(P.c.k_bounds) + (int64_t)run.id * P.c.b_page + kvh0 * P.c.b_head;
   const bool anew = slot0 == 0;
+  const int words = heads * dim / 2;                         // (of all lanes no more than half of kTurnFloats)
+  uint32_t* const lo_s = reinterpret_cast<uint32_t*>(turn_s);
+  uint32_t* const hi_s = lo_s + kTurnFloats / 2;
+  lds_barrier();
+  if (works)
 #pragma unroll
-  for (int side = 0; side < 2; side++) {
-    __syncthreads();
-    if (works)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        float* const to = turn_s + (tk0 * heads + head) * dim;
-        to[d0 + e] = side ? hi[e] : lo[e];
-        if (NP == 2 && !copy) to[d1 + e] = side ? hi[8 * (NP - 1) + e] : lo[8 * (NP - 1) + e];
-      }
-    __syncthreads();
-    for (int i = tid; i < heads * dim; i += 256) {
-      const int h = i / dim, d = i - h * dim;
-      T* const b = bp + h * P.c.b_head + side * dim + d;
-      float r = anew ? turn_s[i] : to_f32(*b);
-      for (int t = 0; t < lanes; t++) {
-        const float y = turn_s[t * heads * dim + i];
-        r = side ? __builtin_elementwise_maximum(r, y) : __builtin_elementwise_minimum(r, y);
-      }
-      store<T>(b, r);
+    for (int e = 0; e < 4 * NP; e++) {
+      if (e >= 4 && copy) break;
+      const int at = tk0 * words + (head * dim + (e < 4 ? d0 : d1)) / 2 + (e & 3);
+      lo_s[at] = lo[e];
+      hi_s[at] = hi[e];
     }
+  lds_barrier();
+  for (int i = tid; i < words; i += 256) {
+    const int h = 2 * i / dim, d = 2 * i - h * dim;
+    uint32_t* const b = reinterpret_cast<uint32_t*>(bp + h * P.c.b_head + d);
+    uint32_t l = 0xffffffffu, m = 0u, old_l = 0, old_m = 0;
+    if (!anew) {
+      old_l = b[0];
+      old_m = b[dim / 2];
+    }
+    for (int t = 0; t < lanes; t++) {
+      l = keys_min(l, lo_s[t * words + i]);
+      m = keys_max(m, hi_s[t * words + i]);
+    }
+    const uint32_t new_l = from_keys(l), new_m = from_keys(m);
+    if (!anew) {
+      l = keys_min(l, to_keys(old_l));
+      m = keys_max(m, to_keys(old_m));
+    }
+    l = from_keys(l);
+    m = from_keys(m);
+#pragma unroll
+    for (int s = 0; s < 32; s += 16) {     // a NaN stays: of the page's own extreme, of a key in both
+      const uint32_t part = 0xffffu << s;
+      auto nan = [&](uint32_t w) __attribute__((always_inline)) { return ((w >> s) & 0x7fffu) > kInfinity<T>; };
+      const bool both = nan(new_l) || nan(new_m);
+      const uint32_t quiet = 0x7fffu << s;
+      if (both || nan(old_l)) l = (l & ~part) | quiet;
+      if (both || nan(old_m)) m = (m & ~part) | quiet;
+    }
+    b[0] = l;
+    b[dim / 2] = m;
   }
 }
 

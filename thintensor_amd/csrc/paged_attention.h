@@ -17,8 +17,6 @@ typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
-typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
 
 // Weights are 2^7 exp(s - m), where m follows the running maximum only when that is more than 2^8 past it: they
@@ -56,9 +54,7 @@ struct PagedParams {
 template <typename T> struct Bits16;
 template <> struct Bits16<f16_t> {
   static constexpr uint32_t kExp = 0x7c00;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){pin_f32(a), pin_f32(b)}, h2));
-  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_pair<f16_t>(a, b); }
   static __device__ __forceinline__ float add_pair(uint32_t w, float c) {      // c + both halves
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), (h2){(_Float16)1.0f, (_Float16)1.0f}, c, false);
   }
@@ -71,9 +67,7 @@ template <> struct Bits16<f16_t> {
 };
 template <> struct Bits16<bf16_t> {
   static constexpr uint32_t kExp = 0x7f80;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, b2_t));
-  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_pair<bf16_t>(a, b); }
   static __device__ __forceinline__ float add_pair(uint32_t w, float c) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2_t, w), (b2_t){(__bf16)1.0f, (__bf16)1.0f}, c, false);
   }
