@@ -25,6 +25,12 @@ constexpr float kPScale = 7.0f;
 constexpr float kSlack = 8.0f;
 constexpr int kMostParts = 1024;       // parts of a query that the join takes
 
+// One job of a launch for few columns: workgroups in all and for a row (of 16 columns times the kernel's blocks each), the
+// rows, tiles of a workgroup, the first of the parts that they leave.
+struct FewJob {
+  int blocks, row_tiles, rows, share, part0;
+};
+
 struct PagedParams {
   tt_paged_cache c;
   const void* q;
@@ -47,8 +53,11 @@ struct PagedParams {
   float* part_o;
   float2* part_ml;
   int parts;
-  // the launch: which job, its first part, tiles of a workgroup, column tiles of a row and in all
-  int shared_job, part0, share, row_tiles, tiles, ordered, wide;
+  int shared_entries;                                // of the table: read from row 0's
+  // a launch for few columns: the rows' own pages [0], the shared pages [1]; or for many, of one of them
+  FewJob few[2];
+  int wide;
+  int shared_job, part0, share, row_tiles, tiles, ordered;
 };
 
 template <typename T> struct Bits16;
@@ -111,11 +120,11 @@ __device__ __forceinline__ float finish_scale(const PagedParams& P, int h, float
 struct Seen {
   int lo, hi;
 };
-__device__ __forceinline__ Seen seen_of(const PagedParams& P, int n, int place, int count) {
+__device__ __forceinline__ Seen seen_of(const PagedParams& P, bool shared_job, int n, int place, int count) {
   Seen s;
   s.hi = n - (count - 1 - place);
   s.lo = P.window > 0 ? max(0, s.hi - P.window) : 0;
-  if (P.shared_job) s.hi = min(s.hi, P.shared);
+  if (shared_job) s.hi = min(s.hi, P.shared);
   else s.lo = max(s.lo, P.shared);
   return s;
 }
@@ -126,8 +135,9 @@ __device__ __forceinline__ int row_length(const PagedParams& P, int row) { retur
 // with every read of LDS.)
 struct PageLanes {
   const int32_t* table;
+  const int32_t* shared_table;   // of the first `shared` entries
   const int32_t* sel;
-  int pages, count, valid;       // of the table, of the selection; of the cache
+  int shared, pages, count, valid;       // entries; of the table, of the selection; of the cache
   int base, id[2], logical[2];
   __device__ __forceinline__ void load(int slot, int from) {
     const int e = from + (int)(threadIdx.x & 63);
@@ -137,7 +147,7 @@ struct PageLanes {
       logical[slot] = ok ? l : -1;
       id[slot] = table[ok ? l : 0];
     } else {
-      id[slot] = table[min(e, pages - 1)];
+      id[slot] = (e < shared ? shared_table : table)[min(e, pages - 1)];
     }
   }
   __device__ __forceinline__ void start(int entry) {
@@ -245,7 +255,7 @@ struct Marks {
 
 // paged_few.hip: up to few_columns() columns of a row and KV head; paged_many.hip: any number
 constexpr int few_columns(int64_t head_dim) { return head_dim == 64 ? 64 : head_dim == 128 ? 32 : 16; }
-int launch_paged_few(const PagedParams& P, int blocks16, int rows, int splits, hipStream_t st, const char* what);
+int launch_paged_few(const PagedParams& P, int blocks16, hipStream_t st, const char* what);
 int launch_paged_many(const PagedParams& P, int waves, int splits, hipStream_t st, const char* what);
 inline int many_tile_tokens(int64_t head_dim) { return head_dim == 256 ? 32 : 64; }
 

@@ -119,12 +119,66 @@ static int many_waves(int64_t head_dim, int64_t cols) { return head_dim == 256 |
 // Workgroups of them that a CU holds (registers, LDS).
 static int many_per_cu(int64_t head_dim, int waves) { return waves == 8 ? (head_dim == 64 ? 2 : 1) : (head_dim == 64 ? 3 : 2); }
 
+// Workgroups that share a column tile's tokens, enough to fill the card, with at least six tiles each: a part costs the
+// write and the reading of its sums, and the join its launch (one row of 512 tokens, 40 heads of 128: 32.3 us in two parts of
+// four tiles, 24.7 in one; 512 behind 4096 70.5 with at least four tiles, 66.8 with six, 65.8 with eight; 49 rows of eight
+// heads behind 30496 shared tokens 40.8, 42.6 and 45.7).
 static void split_many(int64_t groups, int64_t tiles, int per_cu, PagedJob* j) {
-  const int64_t most = tiles / 4, fill = per_cu * device_cus() / (groups > 0 ? groups : 1);
+  const int64_t most = tiles / 6, fill = per_cu * device_cus() / (groups > 0 ? groups : 1);
   int64_t s = most < fill ? most : fill;
   s = s < 1 ? 1 : s > 256 ? 256 : s;
   j->splits = (int)s;
   j->share = 1;
+}
+
+// Whether the rows' own pages go to the kernel for many columns.  That for few takes a row's columns in blocks, each with all
+// of the row's tokens; it starts sooner and costs less per workgroup, so what decides is the K and V that all its blocks
+// would read, in MB, and their number.  us of few and many (8, 10, 2 KV heads at x 64, 128, 256):
+//   x 64, blocks of 64: 64 columns behind 1024 tokens, 4 rows 13.9 and 15.9 (8 MB), 16 rows 26.5 and 23.2 (33); 128 behind
+//     4096 17.2 and 17.4 (17), 256 behind 4096 25.3 and 20.7 (33)
+//   x 128, of 32: 128 behind 1024 14.4 and 20.6 (21), behind 4096 30.1 and 24.8 (84); 64 behind 4096 21.0 and 23.0 (42)
+//   x 256, of 16: 64 behind 4096 18.3 and 28.6 (67), 128 31.3 and 31.4 (134), 512 60.8 and 37.8 (537)
+// One block of a row reads no more than the row has to: with less than half of the CUs taken, or half a block, it stays
+// ahead at any length (x 64, 4 rows of 64 behind 16384: 34.3 and 37.9; x 128, 16 columns of 16 rows behind 4096: 84 and 79,
+// 32 columns 100 and 82).  Many short blocks queue (x 128, 16 rows of 160 columns, 16 tokens each: 21.8 and 12.9).
+// Rows of unequal counts get blocks for all tokens each, most without columns.
+static bool own_by_many(const tt_paged_cache* c, bool ragged, int64_t rows, int64_t tokens, int64_t G, int64_t reach) {
+  const int64_t D = c->head_dim, width = few_columns(D), cols = (ragged ? tokens : tokens / rows) * G, cus = device_cus();
+  const int64_t blocks = (cols + width - 1) / width;
+  if (!ragged && blocks == 1 && (2 * cols <= width || D == 256 || 2 * rows * c->kv_heads < cus)) return false;
+  if (rows * blocks * c->kv_heads > (ragged && D != 256 ? cus : 2 * cus)) return true;
+  return 4e-6 * reach * c->kv_heads * D * (ragged ? rows + blocks : rows * blocks) > (D == 64 ? 20 : D == 128 ? 50 : 140);
+}
+
+// Who computes the shared pages once for all rows: nobody (every row for itself, from row 0's pages, most of which then
+// come from the caches), the kernel for few columns in blocks, in one launch with the rows' own pages, or that for many in
+// a launch before it.  Times are estimated from the MB that a row shares: what a row or a block of sixteen columns costs
+// for each, what a column costs in the kernel for many, and what each way costs to begin with (less where the rows alone
+// would be split and joined too).  us of nobody, few, many in a row of calls:
+//   x 64, 8 KV heads: 16 rows of 4 columns behind 1024 tokens (2 MB) 11.0, 14.1 and 18.4, behind 16384 (34 MB) 41.9,
+//     21.8 and 26.6; 64 rows of 16 behind 4096 (8 MB) 46.0, 49.9 and 40.9, behind 16384 116.6, 94.7 and 67.0
+//   x 128, 10: 8 rows of 4 behind 1024 (5 MB) 12.3, 13.6 and 23.2, behind 4096 23.6, 15.2 and 25.7; 32 rows behind 4096 (21
+//     MB) 55.0, 33.6 and 33.7, behind 16384 150, 70 and 45
+//   x 256, 2: 32 rows of 8 behind 1024 (4 MB) 22.3, 17.9 and 37.7, behind 16384 80, 64 and 62
+// Rows that go to the kernel for many columns by themselves have their matrix products in any case; sharing saves them
+// the padding of their column tiles (16 rows of 80 columns, x 128, 8 KV heads, behind 16384 tokens: 175 us by themselves, 123
+// shared; behind 4096 60 and 57; 16 rows of 128 columns, x 64, 64 and 73).
+enum SharedBy { kNobody, kFew, kMany };
+static SharedBy shared_by(const tt_paged_cache* c, bool own_many, bool ragged, int64_t rows, int64_t tokens, int64_t G,
+                          int64_t window, int64_t reach) {
+  const int64_t D = c->head_dim, cols = tokens * G, each = tokens / rows;
+  if (window > 0 && window + each < reach) reach = window + each;
+  const double mb = 4e-6 * reach * c->kv_heads * D;
+  if (own_many) {
+    const int64_t mc = 32 * many_waves(D, each * G), padded = ragged ? cols + rows * mc / 2 : rows * ((each * G + mc - 1) / mc * mc);
+    return 8 + 0.1 * D + mb * (0.2 + 0.001 * cols) < mb * (0.2 + 0.001 * padded) ? kMany : kNobody;
+  }
+  const int64_t tiles = (reach + 31) / 32;
+  const bool parts = tiles > (rows * c->kv_heads >= device_cus() ? 64 : 24);
+  const double none = mb * (0.25 + 0.05 * (ragged ? (cols + 8 * rows) / 16.0 : rows * ((each * G + 15) / 16)));
+  const double few = (parts ? 2 : 6) + mb * (0.25 + 0.05 * ((cols + 15) / 16));
+  const double many = (parts ? 13 : 16) + mb * (0.2 + 0.001 * cols);
+  return none <= few && none <= many ? kNobody : few <= many ? kFew : kMany;
 }
 
 static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged, int64_t rows, int64_t tokens, int64_t heads,
@@ -133,40 +187,51 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
   const int64_t holds = table_pages * c->page_size, G = heads / c->kv_heads;
   p.limit = max_length < holds ? max_length : holds;
   p.window = window < p.limit ? window : 0;
-  p.shared = rows > 1 ? shared_pages * c->page_size : 0;
   const int64_t each = ragged ? 0 : tokens / rows;
-  const int tt = many_tile_tokens(c->head_dim);
-  if (p.shared > 0) {
-    const int64_t cols = tokens * G, reach = p.shared < p.limit ? p.shared : p.limit;
-    p.prefix.many = cols > few_columns(c->head_dim);
-    if (p.prefix.many) {
-      p.prefix.waves = many_waves(c->head_dim, cols);
-      const int mc = 32 * p.prefix.waves;
-      p.prefix.tiles = (cols + mc - 1) / mc;
-      split_many(p.prefix.tiles * c->kv_heads, (reach + tt - 1) / tt, many_per_cu(c->head_dim, p.prefix.waves), &p.prefix);
-    } else {
-      p.prefix.blocks16 = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-      p.prefix.row_tiles = p.prefix.rows = 1;
-      split_few(c->kv_heads, (reach + 31) / 32, true, &p.prefix);
-    }
+  const int tt = many_tile_tokens(c->head_dim), few = few_columns(c->head_dim);
+  const auto blocks16 = [&](int64_t cols) { return cols <= 16 || few == 16 ? 1 : cols <= 32 || few == 32 ? 2 : 4; };
+  int64_t reach = p.limit;
+  if (p.window > 0 && p.window + (ragged ? tokens : each) < reach) reach = p.window + (ragged ? tokens : each);
+  p.own.many = selected_count == 0 && own_by_many(c, ragged, rows, tokens, G, reach);
+  const int64_t cols = tokens * G, prefix = shared_pages * c->page_size, reach_shared = prefix < p.limit ? prefix : p.limit;
+  const SharedBy by = rows > 1 && shared_pages > 0 ? shared_by(c, p.own.many, ragged, rows, tokens, G, p.window, reach_shared) : kNobody;
+  p.shared = by == kNobody ? 0 : prefix;
+  if (by == kMany) {
+    p.prefix.many = true;
+    p.prefix.waves = many_waves(c->head_dim, cols);
+    const int mc = 32 * p.prefix.waves;
+    p.prefix.tiles = (cols + mc - 1) / mc;
+    split_many(p.prefix.tiles * c->kv_heads, (reach_shared + tt - 1) / tt, many_per_cu(c->head_dim, p.prefix.waves), &p.prefix);
+  } else if (by == kFew) {
+    p.prefix.blocks16 = 4e-6 * reach_shared * c->kv_heads * c->head_dim < 8 ? 1 : blocks16(cols < 32 ? cols : 32);
+    p.prefix.row_tiles = (int)((cols + 16 * p.prefix.blocks16 - 1) / (16 * p.prefix.blocks16));
+    p.prefix.rows = 1;
+    split_few(c->kv_heads * p.prefix.row_tiles, (reach_shared + 31) / 32, true, &p.prefix);
   }
   // tokens of its own that a row's queries may see
-  int64_t reach = p.limit > p.shared ? p.limit - p.shared : 0;
+  reach = p.limit > p.shared ? p.limit - p.shared : 0;
   if (p.window > 0 && p.window + (ragged ? tokens : each) < reach) reach = p.window + (ragged ? tokens : each);
-  if (selected_count > 0) reach = selected_count * c->page_size;
-  p.own.many = ragged || each * G > few_columns(c->head_dim);
+  if (selected_count > 0) {
+    const int64_t pages = (p.limit - 1) / c->page_size + 1;
+    reach = (selected_count < pages ? selected_count : pages) * c->page_size;
+  }
   if (p.own.many) {
     p.own.waves = many_waves(c->head_dim, ragged ? tokens * G / rows : each * G);
     const int mc = 32 * p.own.waves;
+    if (p.window > 0 && p.window + mc / G + 1 < reach) reach = p.window + mc / G + 1;      // of a column tile
     p.own.row_tiles = (int)((each * G + mc - 1) / mc);
     p.own.tiles = ragged ? tokens * G / mc + rows : rows * p.own.row_tiles;
     split_many(p.own.tiles * c->kv_heads, (reach + tt - 1) / tt + 1, many_per_cu(c->head_dim, p.own.waves), &p.own);
   } else {
-    p.own.blocks16 = each * G <= 16 ? 1 : each * G <= 32 ? 2 : 4;
-    p.own.row_tiles = 1;
+    const int64_t most = ragged ? cols : each * G;
+    p.own.blocks16 = by == kFew ? p.prefix.blocks16 : blocks16(most);      // (one kernel for both)
+    p.own.row_tiles = (int)((most + 16 * p.own.blocks16 - 1) / (16 * p.own.blocks16));
     p.own.rows = (int)rows;
     // (one tile more where they may begin inside one)
     split_few(rows * c->kv_heads, (reach + 31) / 32 + (p.window > 0 || p.shared % 32 != 0 ? 1 : 0), false, &p.own);
+    // a selection may name its pages anywhere in it
+    const int64_t listed = (selected_count * c->page_size + 31) / 32;
+    if (listed > p.own.splits * p.own.share) p.own.share = (int)((listed + p.own.splits - 1) / p.own.splits);
   }
   p.parts = p.own.splits + (p.shared > 0 ? p.prefix.splits : 0);
   return p;
@@ -176,16 +241,19 @@ static int64_t scratch_floats_of(const PagedPlan& p, const tt_paged_cache* c, in
   return p.parts == 1 ? 0 : tokens * heads * p.parts * (c->head_dim + 2);
 }
 
-static int launch_job(PagedParams P, const PagedJob& j, bool shared, int part0, hipStream_t st, const char* what) {
+static int launch_many(PagedParams P, const PagedJob& j, bool shared, int part0, hipStream_t st, const char* what) {
   P.shared_job = shared;
   P.part0 = part0;
   P.share = j.share;
   P.row_tiles = j.row_tiles;
   P.tiles = (int)j.tiles;
-  P.wide = j.wide;
   // in order of their length where they do not all run at once
-  P.ordered = j.many && !shared && P.window == 0 && P.of.rows <= 64 && j.tiles * P.c.kv_heads * j.splits > many_per_cu(P.c.head_dim, j.waves) * device_cus();
-  return j.many ? launch_paged_many(P, j.waves, j.splits, st, what) : launch_paged_few(P, j.blocks16, j.rows, j.splits, st, what);
+  P.ordered = !shared && P.window == 0 && P.of.rows <= 64 && j.tiles * P.c.kv_heads * j.splits > many_per_cu(P.c.head_dim, j.waves) * device_cus();
+  return launch_paged_many(P, j.waves, j.splits, st, what);
+}
+
+static FewJob few_job(const PagedParams& P, const PagedJob& j, int part0) {
+  return FewJob{(int)(P.c.kv_heads * j.row_tiles * j.rows * j.splits), j.row_tiles, j.rows, j.share, part0};
 }
 
 static int check_attention(const tt_paged_cache* c, int64_t table_pages, bool ragged, int64_t rows, int64_t tokens,
@@ -196,7 +264,7 @@ static int check_attention(const tt_paged_cache* c, int64_t table_pages, bool ra
   TT_REQUIRE(heads > 0, "%s: heads must be a multiple of kv_heads", what);
   TT_REQUIRE(window >= 0 && max_length > 0, "%s: window must not be negative, max_length at least 1", what);
   TT_REQUIRE(shared_pages >= 0 && shared_pages <= table_pages, "%s: shared_pages outside the table", what);
-  TT_REQUIRE((tokens * heads) / 128 + (ragged ? rows * c->kv_heads : 0) < (1 << 23), "%s: too many queries for one call", what);
+  TT_REQUIRE((tokens * heads) / 128 + rows * c->kv_heads < (1 << 23), "%s: too many queries for one call", what);
   TT_REQUIRE(selected_count >= 0 && selected_count <= 65536 && (selected_count == 0 || (!ragged && tokens == rows && shared_pages == 0)),
              "%s: selected pages (65536 at most) are for one query per row, without shared pages", what);
   return TT_OK;
@@ -250,6 +318,7 @@ extern "C" int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q
   P.selected = selected; P.selected_count = (int)selected_count;
   P.heads = (int)heads; P.per_kv = (int)(heads / cache->kv_heads);
   P.max_length = (int)p.limit; P.window = (int)p.window; P.shared = (int)p.shared;
+  P.shared_entries = (int)shared_pages;
   P.q_vec = aligned(q, 16) && ((q_token | q_head) & 7) == 0;
   P.out_vec = aligned(out, 8) && ((out_token | out_head) & 3) == 0;
   P.scale_log2 = (float)((double)scale * 1.4426950408889634);
@@ -260,8 +329,14 @@ extern "C" int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q
   P.part_o = scratch;
   P.part_ml = reinterpret_cast<float2*>(scratch + tokens * heads * p.parts * cache->head_dim);
   int err = TT_OK;
-  if (p.shared > 0) err = launch_job(P, p.prefix, true, p.own.splits, st, what);
-  if (err == TT_OK) err = launch_job(P, p.own, false, 0, st, what);
+  if (p.shared > 0 && p.prefix.many) err = launch_many(P, p.prefix, true, p.own.splits, st, what);
+  if (p.shared > 0 && !p.prefix.many) P.few[1] = few_job(P, p.prefix, p.own.splits);
+  if (err == TT_OK && p.own.many) err = launch_many(P, p.own, false, 0, st, what);
+  if (err == TT_OK && !p.own.many) {
+    P.few[0] = few_job(P, p.own, 0);
+    P.wide = p.own.wide;
+    err = launch_paged_few(P, p.own.blocks16, st, what);
+  }
   if (err != TT_OK || p.parts == 1) return err;
   return cache->dtype == TT_F16 ? launch_join<f16_t>(P, st, what) : launch_join<bf16_t>(P, st, what);
 }

@@ -46,13 +46,24 @@ void paged_few_kernel(PagedParams P) {
   __shared__ Seen see_s[MIXED ? 16 * NB : 1];
   __shared__ uint32_t marks_s[16 * NB * (D / 16)];
   __shared__ int marked;
-  const int kvh = blockIdx.x / P.row_tiles, cb = blockIdx.x % P.row_tiles, row = blockIdx.y, split = blockIdx.z;
+  // the shared pages' workgroups first, then the rows'; of each KV heads and column blocks, then rows, then splits
+  const bool shared_job = MIXED && (int)blockIdx.x < P.few[1].blocks;
+  const FewJob J = P.few[shared_job ? 1 : 0];
+  const int block = (int)blockIdx.x - (MIXED && !shared_job ? P.few[1].blocks : 0);
+  const int kvhs = (int)P.c.kv_heads * J.row_tiles, rest = block / kvhs, split = rest / J.rows, row = rest - split * J.rows;
+  const int kvh = (block - rest * kvhs) / J.row_tiles, cb = block - rest * kvhs - kvh * J.row_tiles;
   const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int G = P.per_kv;
-  const int first = P.shared_job ? 0 : row * P.of.each, count = P.shared_job ? P.of.tokens : P.of.each;
+  int first = 0, count = P.of.tokens;
+  if (!shared_job) {
+    first = row * P.of.each;
+    count = P.of.each;
+    if (MIXED && P.of.cu) count = P.of.count(row, &first);
+  }
   const int c0 = cb * 16 * NB, cols = min(16 * NB, count * G - c0);
-  const int32_t* table = P.table + (P.shared_job ? 0 : row * P.table_row);
+  if (MIXED && cols <= 0) return;
+  const int32_t* table = P.table + (shared_job ? 0 : row * P.table_row);
   const int32_t* sel = P.selected ? P.selected + ((int64_t)row * P.c.kv_heads + kvh) * P.selected_count : nullptr;
 
   // ---- q, and the first tile where it does not depend on the row's length, are requested before anything else
@@ -92,7 +103,7 @@ void paged_few_kernel(PagedParams P) {
       vr[k] = *reinterpret_cast<const u4_t*>(p[h].v + (size_t)((uint32_t)(k * VR - 16 * h + v_row) * v_step + 16 * v_piece));
     }
   };
-  PageLanes lanes{table, sel, P.table_pages, P.selected_count, (int)P.c.pages, 0, {0, 0}, {0, 0}};
+  PageLanes lanes{table, P.table, sel, P.shared_entries, P.table_pages, P.selected_count, (int)P.c.pages, 0, {0, 0}, {0, 0}};
   const char* const kbase = reinterpret_cast<const char*>(P.c.k_pages) + 2 * kvh * P.c.k_head;
   const char* const vbase = reinterpret_cast<const char*>(P.c.v_pages) + 2 * kvh * P.c.v_head;
   auto place = [&](int j, Place (&p)[2]) __attribute__((always_inline)) {
@@ -101,7 +112,7 @@ void paged_few_kernel(PagedParams P) {
     p[1] = place_of(P, lanes, kbase, vbase, kTile * j + 16);
   };
   // (a place past the table is one in page 0 that nobody sees; a row's first split has a tile unless the row is empty)
-  int tile0 = sel || P.shared_job ? 0 : P.shared / kTile;
+  int tile0 = sel || shared_job ? 0 : P.shared / kTile;
   const bool early = split == 0 && (P.window == 0 || sel);
   Place now[2], next[2];
   if (early) {
@@ -114,13 +125,13 @@ void paged_few_kernel(PagedParams P) {
 
   Seen see[NB];
   int hi_most = 0, hi_least, lo_least, lo_most;             // over the columns
-  if (MIXED && P.shared_job) {
+  if (shared_job) {
     int hl = 0x7fffffff, ll = 0x7fffffff, lm = 0;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
       int place, each;
       const int r = row_of(P.of, token[b], &place, &each);
-      see[b] = r < P.of.rows ? seen_of(P, row_length(P, r), place, each) : Seen{0, 0};
+      see[b] = r < P.of.rows ? seen_of(P, true, row_length(P, r), place, each) : Seen{0, 0};
       see[b].hi = max(see[b].hi, 0);
       if (see[b].hi > see[b].lo) {         // (one that sees nothing may compute what it will, it ends without weight)
         hi_most = max(hi_most, see[b].hi); hl = min(hl, see[b].hi);
@@ -135,21 +146,31 @@ void paged_few_kernel(PagedParams P) {
     const int len = row_length(P, row);
     const int z0 = MIXED ? c0 / G : 0, z1 = MIXED ? (c0 + cols - 1) / G : 0;
 #pragma unroll
-    for (int b = 0; b < NB; b++) see[b] = seen_of(P, len, token[b] - first, count);
-    const Seen a = seen_of(P, len, z0, count), z = seen_of(P, len, z1, count);
+    for (int b = 0; b < NB; b++) see[b] = seen_of(P, false, len, token[b] - first, count);
+    const Seen a = seen_of(P, false, len, z0, count), z = seen_of(P, false, len, z1, count);
     hi_most = max(z.hi, 0); hi_least = a.hi; lo_least = a.lo; lo_most = z.lo;
   }
   int tile1 = (hi_most + kTile - 1) / kTile;
-  if (sel) tile1 = hi_most == 0 ? 0 : ((P.selected_count << P.page_shift) + kTile - 1) / kTile;
-  else tile0 = lo_least / kTile;
-  tile0 += split * P.share;
-  tile1 = min(tile1, tile0 + P.share);
+  if (sel) {
+    int named = 0;                                           // places of the selection, without those of none at its end
+    if (hi_most > 0) {
+      for (int e = (P.selected_count - 1) & ~63; e >= 0 && named == 0; e -= 64) {
+        const uint64_t any = __builtin_amdgcn_ballot_w64(e + lane < P.selected_count && sel[min(e + lane, P.selected_count - 1)] >= 0);
+        if (any != 0) named = e + 64 - __builtin_clzll(any);
+      }
+    }
+    tile1 = ((named << P.page_shift) + kTile - 1) / kTile;
+  } else {
+    tile0 = lo_least / kTile;
+  }
+  tile0 += split * J.share;
+  tile1 = min(tile1, tile0 + J.share);
   const bool only = P.parts == 1;
   if (tile0 >= tile1) {
     if (!only) {                                             // nothing here: no weight
       for (int c = threadIdx.x; c < cols; c += 64 * WAVES) {
         const int i = (c0 + c) / G;
-        P.part_ml[((int64_t)(first + i) * P.heads + kvh * G + (c0 + c - i * G)) * P.parts + P.part0 + split] =
+        P.part_ml[((int64_t)(first + i) * P.heads + kvh * G + (c0 + c - i * G)) * P.parts + J.part0 + split] =
             make_float2(__builtin_bit_cast(float, 0xff800000u), 0.0f);
       }
       return;
@@ -340,7 +361,7 @@ void paged_few_kernel(PagedParams P) {
         const float f = finish_scale(P, hd, M, l);
         store_four<T>(reinterpret_cast<T*>(P.out) + tok * P.out_token + hd * P.out_head + d, acc * f, P.out_vec);
       } else {
-        const int64_t part = ((int64_t)tok * P.heads + hd) * P.parts + P.part0 + split;
+        const int64_t part = ((int64_t)tok * P.heads + hd) * P.parts + J.part0 + split;
         *reinterpret_cast<f4_t*>(P.part_o + part * D + d) = acc;
         if (d == 0) P.part_ml[part] = make_float2(M, l);
       }
@@ -349,9 +370,9 @@ void paged_few_kernel(PagedParams P) {
 }
 
 template <typename T, int D, int NB>
-static int launch_blocks(const PagedParams& P, int rows, int splits, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)(P.c.kv_heads * P.row_tiles), (unsigned)rows, (unsigned)splits);
-  const bool mixed = P.shared_job || P.of.each > 1;
+static int launch_blocks(const PagedParams& P, hipStream_t st, const char* what) {
+  const dim3 grid((unsigned)(P.few[0].blocks + P.few[1].blocks));
+  const bool mixed = P.few[1].blocks > 0 || P.of.each != 1;
   if constexpr (NB == 1 && D < 256) {
     if (P.wide && !mixed) {
       hipLaunchKernelGGL((paged_few_kernel<T, D, NB, false, 8>), grid, dim3(64 * 8), 0, st, P);
@@ -364,19 +385,17 @@ static int launch_blocks(const PagedParams& P, int rows, int splits, hipStream_t
 }
 
 template <typename T>
-static int launch_type(const PagedParams& P, int blocks16, int rows, int splits, hipStream_t st, const char* what) {
+static int launch_type(const PagedParams& P, int blocks16, hipStream_t st, const char* what) {
   if (P.c.head_dim == 64)
-    return blocks16 == 1   ? launch_blocks<T, 64, 1>(P, rows, splits, st, what)
-           : blocks16 == 2 ? launch_blocks<T, 64, 2>(P, rows, splits, st, what)
-                           : launch_blocks<T, 64, 4>(P, rows, splits, st, what);
-  if (P.c.head_dim == 128)
-    return blocks16 == 1 ? launch_blocks<T, 128, 1>(P, rows, splits, st, what) : launch_blocks<T, 128, 2>(P, rows, splits, st, what);
-  return launch_blocks<T, 256, 1>(P, rows, splits, st, what);
+    return blocks16 == 1   ? launch_blocks<T, 64, 1>(P, st, what)
+           : blocks16 == 2 ? launch_blocks<T, 64, 2>(P, st, what)
+                           : launch_blocks<T, 64, 4>(P, st, what);
+  if (P.c.head_dim == 128) return blocks16 == 1 ? launch_blocks<T, 128, 1>(P, st, what) : launch_blocks<T, 128, 2>(P, st, what);
+  return launch_blocks<T, 256, 1>(P, st, what);
 }
 
-int launch_paged_few(const PagedParams& P, int blocks16, int rows, int splits, hipStream_t st, const char* what) {
-  return P.c.dtype == TT_F16 ? launch_type<f16_t>(P, blocks16, rows, splits, st, what)
-                             : launch_type<bf16_t>(P, blocks16, rows, splits, st, what);
+int launch_paged_few(const PagedParams& P, int blocks16, hipStream_t st, const char* what) {
+  return P.c.dtype == TT_F16 ? launch_type<f16_t>(P, blocks16, st, what) : launch_type<bf16_t>(P, blocks16, st, what);
 }
 
 }  // namespace tt

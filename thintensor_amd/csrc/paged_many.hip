@@ -136,9 +136,9 @@ void paged_many_kernel(PagedParams P, int splits) {
   if (P.shared_job) {
     int place, each;
     const int r = row_of(P.of, token, &place, &each);
-    see = r < P.of.rows ? seen_of(P, row_length(P, r), place, each) : Seen{0, 0};
+    see = r < P.of.rows ? seen_of(P, P.shared_job != 0, row_length(P, r), place, each) : Seen{0, 0};
   } else {
-    see = seen_of(P, len, at, count);
+    see = seen_of(P, P.shared_job != 0, len, at, count);
   }
   see.hi = max(see.hi, 0);
   // of this wave's columns, and of all of them
@@ -203,7 +203,7 @@ void paged_many_kernel(PagedParams P, int splits) {
   const char* const kbase = reinterpret_cast<const char*>(P.c.k_pages) + 2 * kvh * P.c.k_head;
   const char* const vbase = reinterpret_cast<const char*>(P.c.v_pages) + 2 * kvh * P.c.v_head;
   u4_t kr[NK], vr[NK];
-  PageLanes lanes{table, nullptr, P.table_pages, 0, (int)P.c.pages, 0, {0, 0}, {0, 0}};
+  PageLanes lanes{table, P.table, nullptr, P.shared_entries, P.table_pages, 0, (int)P.c.pages, 0, {0, 0}, {0, 0}};
   auto load = [&](int tile) __attribute__((always_inline)) {
     lanes.reach((min(tile, tile1 - 1) * TT) >> P.page_shift);
 #pragma unroll

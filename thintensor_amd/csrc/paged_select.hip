@@ -56,6 +56,18 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectParams P) {
     return id < 0 || id >= P.c.pages ? -1 : id;
   };
   if (p0 > 0 && p0 >= pages) return;       // the first ones do not wait for the length
+  // the queries of a turn: heads past the last repeat it, which changes no maximum
+  constexpr int MINE = (GH * D + 255) / 256;
+  T qv[MINE];
+  auto load_q = [&](int h0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+      const int u = threadIdx.x + 256 * i;
+      const int h = min(h0 + u / D, P.per_kv - 1), d = u % D;
+      qv[i] = reinterpret_cast<const T*>(P.q)[row * P.q_token + (kvh * P.per_kv + h) * P.q_head + d];
+    }
+  };
+  load_q(0);
   {
     const int l_row = threadIdx.x / RP, l_piece = threadIdx.x % RP;
     const char* base = reinterpret_cast<const char*>(P.c.k_bounds) + 2 * kvh * P.c.b_head + 16 * l_piece;
@@ -70,18 +82,21 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectParams P) {
       for (int r = 0; r < AT_ONCE; r++) *reinterpret_cast<u4_t*>(b_s + ((r0 + r) * RR + l_row) * BS + 16 * l_piece) = v[r];
     }
   }
+  if (pages <= P.count) return;            // every page is kept, whatever its score
   const char* const mine = b_s + lane * BS + 2 * wave * QD;
   uint32_t best = 0;
   for (int h0 = 0; h0 < P.per_kv; h0 += GH) {
     __syncthreads();
     if (threadIdx.x == 0) odd_q = 0;
     __syncthreads();
-    for (int u = threadIdx.x; u < GH * D; u += 256) {      // heads past the last repeat it, which changes no maximum
-      const int h = min(h0 + u / D, P.per_kv - 1), d = u % D;
-      const float x = to_f32(reinterpret_cast<const T*>(P.q)[row * P.q_token + (kvh * P.per_kv + h) * P.q_head + d]);
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+      const int u = threadIdx.x + 256 * i;
+      const float x = to_f32(qv[i]);
       if (!(__builtin_fabsf(x) < __builtin_bit_cast(float, 0x7f800000u))) odd_q = 1;
-      q_s[d][u / D] = 0.5 * (double)x;
+      q_s[u % D][u / D] = 0.5 * (double)x;
     }
+    if (h0 + GH < P.per_kv) load_q(h0 + GH);
     __syncthreads();
     double sum[GH];
 #pragma unroll
@@ -335,10 +350,12 @@ extern "C" int tt_select_pages(const tt_paged_cache* cache, const void* q, int64
   P.count = (int)selected_count;
   P.keys = reinterpret_cast<uint32_t*>(scratch); P.keys_row = most; P.selected = selected;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache->dtype == TT_F16) launch_score<f16_t>(P, most, rows, st);
-  else launch_score<bf16_t>(P, most, rows, st);
-  const int err = check_launch(what);
-  if (err) return err;
+  if (most > selected_count) {             // (otherwise every page is kept)
+    if (cache->dtype == TT_F16) launch_score<f16_t>(P, most, rows, st);
+    else launch_score<bf16_t>(P, most, rows, st);
+    const int err = check_launch(what);
+    if (err) return err;
+  }
   const dim3 pairs((unsigned)cache->kv_heads, (unsigned)rows);
   if (most <= 256 * 8) hipLaunchKernelGGL((page_pick_kernel<256, 8>), pairs, dim3(256), 0, st, P);
   else hipLaunchKernelGGL((page_pick_kernel<1024, 8>), pairs, dim3(1024), 0, st, P);
