@@ -111,10 +111,17 @@ static void split_few(int64_t groups, int64_t tiles, bool parts, PagedJob* j) {
   if (j->splits < 1) j->splits = 1;
 }
 
-// Waves of a workgroup for rows of `cols` columns, 32 each: eight share what comes to LDS further (4096 queries behind
-// 16384 tokens, 64 / 8 heads: x 128 2212 us with four, 2075 with eight, x 64 1271 and 1217; 512 rows of heads behind 32768
-// shared tokens 143 and 140; x 256, with registers for one wave of a SIMD or two, 1957 and 1109 us for 2048 behind 8192).
-static int many_waves(int64_t head_dim, int64_t cols) { return head_dim == 256 || cols > 128 ? 8 : 4; }
+// Waves of a workgroup, 32 columns each, for rows of `cols` columns, `groups` of them times KV heads.  Eight share what
+// comes to LDS further, and a split prefix fills the card with either (4096 queries behind 16384 tokens, 64 / 8 heads: x 128
+// 2212 us with four, 2075 with eight; 512 columns behind 32768 shared tokens 143 and 140; x 256, with registers for one wave
+// of a SIMD or two, 1957 and 1109 us for 2048 behind 8192).  Four lose less to the ends of rows and, at x 64 with its three
+// workgroups of four on a CU, spread over the CUs better until there are four workgroups of eight for each (64 / 8 heads x 64,
+// 1027 tokens of 4099: 107 us with four, 126 with eight, a window of 2048 70 and 81, 4096 tokens 197 and 188; x 128, 40 / 10
+// heads, eight rows of 100 tokens and less 67 and 79, four of 512 and less 143 and 130).
+static int many_waves(int64_t head_dim, int64_t cols, int64_t groups) {
+  if (head_dim == 256) return 8;
+  return head_dim == 128 ? (cols > 256 ? 8 : 4) : cols > 128 && groups * ((cols + 255) / 256) >= 4 * device_cus() ? 8 : 4;
+}
 
 // Workgroups of them that a CU holds (registers, LDS).
 static int many_per_cu(int64_t head_dim, int waves) { return waves == 8 ? (head_dim == 64 ? 2 : 1) : (head_dim == 64 ? 3 : 2); }
@@ -170,7 +177,7 @@ static SharedBy shared_by(const tt_paged_cache* c, bool own_many, bool ragged, i
   if (window > 0 && window + each < reach) reach = window + each;
   const double mb = 4e-6 * reach * c->kv_heads * D;
   if (own_many) {
-    const int64_t mc = 32 * many_waves(D, each * G), padded = ragged ? cols + rows * mc / 2 : rows * ((each * G + mc - 1) / mc * mc);
+    const int64_t mc = 32 * many_waves(D, each * G, rows * c->kv_heads), padded = ragged ? cols + rows * mc / 2 : rows * ((each * G + mc - 1) / mc * mc);
     return 8 + 0.1 * D + mb * (0.2 + 0.001 * cols) < mb * (0.2 + 0.001 * padded) ? kMany : kNobody;
   }
   const int64_t tiles = (reach + 31) / 32;
@@ -198,7 +205,7 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
   p.shared = by == kNobody ? 0 : prefix;
   if (by == kMany) {
     p.prefix.many = true;
-    p.prefix.waves = many_waves(c->head_dim, cols);
+    p.prefix.waves = c->head_dim == 256 || cols > 128 ? 8 : 4;
     const int mc = 32 * p.prefix.waves;
     p.prefix.tiles = (cols + mc - 1) / mc;
     split_many(p.prefix.tiles * c->kv_heads, (reach_shared + tt - 1) / tt, many_per_cu(c->head_dim, p.prefix.waves), &p.prefix);
@@ -216,7 +223,7 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
     reach = (selected_count < pages ? selected_count : pages) * c->page_size;
   }
   if (p.own.many) {
-    p.own.waves = many_waves(c->head_dim, ragged ? tokens * G / rows : each * G);
+    p.own.waves = many_waves(c->head_dim, tokens / rows * G, rows * c->kv_heads);
     const int mc = 32 * p.own.waves;
     if (p.window > 0 && p.window + mc / G + 1 < reach) reach = p.window + mc / G + 1;      // of a column tile
     p.own.row_tiles = (int)((each * G + mc - 1) / mc);
