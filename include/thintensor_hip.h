@@ -870,7 +870,8 @@ int tt_sample_rows(const void* logits, int64_t row_stride, int dtype, int64_t ro
  * (elements) of pages, heads and tokens, the last axis contiguous; every vector starts on a 16-byte
  * boundary.  k_bounds (or NULL) [pages, kv_heads, 2, head_dim], the last two axes contiguous: of
  * every dim the least and the greatest key of the page.  page_size 16, 32, 64, 128 or 256; head_dim
- * 64, 128 or 256.  Token t of a row lies in page table[row, t / page_size], slot t % page_size. */
+ * 64, 128 or 256; a page's tokens lie in order (strides not negative) within 2 GiB.  Token t of a row lies in
+ * page table[row, t / page_size], slot t % page_size. */
 typedef struct {
   void *k_pages, *v_pages, *k_bounds;
   int64_t k_page, k_head, k_token, v_page, v_head, v_token, b_page, b_head;
@@ -902,11 +903,16 @@ int tt_rotary_append_paged(const tt_paged_cache* cache, const void* q, int64_t q
  * n_r sees the tokens t < e = N - (n_r - 1 - i), N = min(max(lengths[r], 0), max_length, table_pages page_size),
  * and with window > 0 only t >= e - window.  out = sum p v with p the softmax of scale q.k and, where sinks
  * [heads] is given, of the sink's logit, which carries no value; a query that sees nothing is 0.  Queries behind
- * the last row are left as they were.  A query that sees a token whose table entry is no page is NaN.
- * shared_pages: the first ones of every row's table are the same pages (row 0's entries are used): they are read
- * once for all rows, and rows end where their lengths say, inside them too.
+ * the last row are left as they were.  A query that sees a token whose table entry is no page is NaN; one whose
+ * scores are all -inf counts as seeing nothing.
+ * shared_pages: the first ones of every row's table are the same pages (only row 0's entries are used): they are
+ * computed once for all rows where that costs less, and rows end where their lengths say, inside them too.
  * selected (or NULL) int32 [rows, kv_heads, selected_count], one query a row, no shared pages: only the tokens
- * of these pages (places in the table, each once) are seen; negative entries and those past the length are skipped.
+ * of these pages (places in the table, each at most once, in any order) are seen; negative entries and those past the
+ * length are skipped.
+ * Results go by the values, not by the batch: which kernel a call takes, and in how many parts, follows its
+ * sizes, and sums are added in another order then.  The same call gives the same bits.
+ * At most 65535 rows and 2^22 tokens, and tokens heads / 128 + rows kv_heads below 2^23.
  * out may be q; otherwise it shares no memory with q, the cache or itself, which is refused.  max_length
  * (at least 1) bounds what the launch is sized for.  scratch: tt_gqa_attention_paged_scratch_floats of the same
  * arguments with the same GPU current (0: none is needed), for one call at a time, 16-byte aligned. */
@@ -927,8 +933,8 @@ int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q, int64_t q
  * greatest product that a key within its k_bounds can have with one of the KV head's queries,
  *   max over its heads of sum_d max(q_d low_d, q_d high_d),
  * summed in binary64 (to 2^-50 of the sum of |q_d| max(|low_d|, |high_d|)) and rounded to binary32; of equal scores
- * the lower page is taken, NaN counts as the greatest, and so does the score of a table entry that is no page.  scratch: tt_select_pages_scratch_floats, for one call
- * at a time. */
+ * the lower page is taken, NaN counts as the greatest, and so does the score of a table entry that is no page.
+ * scratch: tt_select_pages_scratch_floats, for one call at a time. */
 int64_t tt_select_pages_scratch_floats(const tt_paged_cache* cache, int64_t table_pages, int64_t rows, int64_t max_length);
 int tt_select_pages(const tt_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head, const int32_t* table,
                     int64_t table_row, int64_t table_pages, const int32_t* lengths, int64_t rows, int64_t heads,

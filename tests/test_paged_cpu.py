@@ -64,6 +64,8 @@ def test_cache_descriptor():
     assert c.desc.v_pages - c.desc.k_pages == 2 * 192 and c.desc.k_bounds is None
     assert c.nbytes() == both.numel() * 2
     assert _cache().nbytes() == 2 * (2 * 6 * 2 * 16 * 64 + 6 * 2 * 2 * 64)
+    with pytest.raises(AttributeError):                       # the descriptor holds the addresses
+        c.k_pages = both[:, :, 0].transpose(1, 2).clone()
 
 
 # ------------------------------------------------------------------ refusals of the backend

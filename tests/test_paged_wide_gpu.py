@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from tests.paged_ref import same_bits
-from tests.test_paged_attention_gpu import _DT, _RAGGED, _check, _make, _run
+from tests.test_paged_attention_gpu import _DT, _RAGGED, _check, _i32, _make, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -154,3 +154,22 @@ def test_ignored_sharing_reads_row_0s_entries(backend, device):
         other = table.copy()
         other[1:, :5] = -1
         assert same_bits(out, _run(backend, device, cache, other, lengths, q, shared_pages=5))
+
+
+def test_the_same_call_gives_the_same_bits(backend, device):
+    cache, table, lengths, g = _prefix(device, 27, 8, 128, 64, 20, "bf16", 1)
+    counts = [1, 0, 3, 1, 2, 1, 1, 1, 300] * 3
+    cu = np.concatenate(([0], np.cumsum(counts))).tolist()
+    sel = torch.empty((27, 8, 9), device=device, dtype=torch.int32)
+    one, chunk = (torch.randn((n, 16, 128), generator=g, device=device).bfloat16() for n in (27, cu[-1]))
+    cache.k_bounds.normal_(generator=g)
+
+    def run():
+        backend.select_pages(one, cache, _i32(table, device), _i32(lengths, device), sel)
+        return [sel.clone(), _run(backend, device, cache, table, lengths, one), _run(backend, device, cache, table, lengths, one, shared_pages=20),
+                _run(backend, device, cache, table, lengths, chunk, cu, shared_pages=20),
+                _run(backend, device, cache, table, lengths, one, selected=sel.cpu().numpy())]
+
+    first = run()
+    for _ in range(3):
+        assert all(same_bits(a, b) for a, b in zip(first, run()))

@@ -1787,11 +1787,12 @@ class HipDecodeBackend:
         head_dim] of the cache's type, ``lengths`` int32 [rows] the tokens that a row holds, its queries included;
         tokens belong to rows as in :meth:`rotary_append_paged`.  With ``window`` > 0 a query sees the last
         ``window`` tokens up to its own.  ``sinks`` [heads] are logits that join the softmax and carry no value;
-        ``scale`` is head_dim ** -0.5 by default.  A query that sees nothing is 0, one that needs an entry of the table
-        that is no page NaN; queries behind the last row are left as they were.
+        ``scale`` is head_dim ** -0.5 by default.  A query that sees nothing, or only scores of -inf, is 0, one that
+        needs an entry of the table that is no page NaN; queries behind the last row are left as they were.
         ``shared_pages``: so many first entries of the table are the same in every row (row 0's are read), and
-        these pages are read and multiplied once for the whole batch.  ``selected`` (int32 [rows, kv_heads, count],
-        from :meth:`select_pages`; one query per row): only these pages are read.  ``max_length`` (by default
+        these pages are computed once for the whole batch where that costs less.  ``selected`` (int32 [rows,
+        kv_heads, count], as from :meth:`select_pages`: places in the table, each at most once, negative ones skipped; one
+        query per row): only these pages are read.  ``max_length`` (by default
         what the table holds) bounds the lengths, longer ones count as it, and sizes the launch.  ``out`` may be q;
         otherwise it shares no memory with q, the cache or itself.  Scratch comes from the current stream's
         allocator with every call."""

@@ -46,7 +46,7 @@ class PagedKvCache:
         tensors = (k_pages, v_pages) if k_bounds is None else (k_pages, v_pages, k_bounds)
         if len({t.device for t in tensors}) != 1:
             raise ValueError("paged cache tensors must be on one device")
-        self.k_pages, self.v_pages, self.k_bounds = k_pages, v_pages, k_bounds
+        self._tensors = k_pages, v_pages, k_bounds         # the descriptor holds their addresses: they stay
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, head_dim
         self.dtype, self.device = k_pages.dtype, k_pages.device
         ks, vs, bs = k_pages.stride(), v_pages.stride(), (0, 0) if k_bounds is None else k_bounds.stride()
@@ -54,6 +54,18 @@ class PagedKvCache:
             k_pages.data_ptr(), v_pages.data_ptr(), None if k_bounds is None else k_bounds.data_ptr(),
             ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], bs[0], bs[1], pages, kv_heads, page_size, head_dim,
             _DTYPES[self.dtype])
+
+    @property
+    def k_pages(self) -> torch.Tensor:
+        return self._tensors[0]
+
+    @property
+    def v_pages(self) -> torch.Tensor:
+        return self._tensors[1]
+
+    @property
+    def k_bounds(self) -> torch.Tensor | None:
+        return self._tensors[2]
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.float16, *,
@@ -68,5 +80,4 @@ class PagedKvCache:
                    zeros(pages, kv_heads, 2, head_dim) if bounds else None)
 
     def nbytes(self) -> int:
-        tensors = (self.k_pages, self.v_pages) if self.k_bounds is None else (self.k_pages, self.v_pages, self.k_bounds)
-        return sum(t.numel() * t.element_size() for t in tensors)
+        return sum(t.numel() * t.element_size() for t in self._tensors if t is not None)
