@@ -1,19 +1,25 @@
-// Paged attention for few columns (a row's queries of one KV head: single tokens, drafts; or a small
-// batch against its shared pages): one wave takes 32 tokens at a time for 16 NB columns, the waves of a
-// workgroup take turns and are joined in LDS, a long row is split over workgroups.
+// Paged attention for few columns (a row's queries of one KV head: single tokens, drafts, short chunks; or a
+// small batch against its shared pages): one wave takes 32 tokens at a time for 16 NB columns, the waves of a workgroup
+// take turns and are joined in LDS, a long row is split over workgroups.  One launch holds the rows' own and the
+// shared pages.
 //
-// What bounds it is memory: a tile's K and V are read once, 4 D bytes a token.
-//   * scores are rows = tokens, columns = query heads (v_mfma_f32_16x16x32, K straight from memory as
-//     the first operand); a lane then holds 4 + 4 tokens of one column, which is the second operand of the product
-//     with V, so weights stay in registers;
-//   * V comes in whole rows, goes through the wave's own LDS and is read back transposed
-//     (ds_read_b64_tr_b16: four tokens of a dim to a lane), rows 32 bytes further apart than they are
-//     long, so that the sixteen rows of a read take all banks alike; no barrier;
-//   * K of the next tile is requested once the scores hold the present one's, V once LDS does;
+// What bounds it is memory where rows are long, 4 D bytes a token and KV head (32 rows to 8001 tokens, 64 / 8 heads x 128:
+// 135 us, 4.9 TB/s of a large copy's 5.0), and otherwise its chain of round trips: queries and lengths, table, first tile,
+// join (575 tokens of one row, 32 / 8 x 64: 6 to 6.6 us in a graph, where a launch is 2).
+//   * scores are rows = tokens, columns = query heads (v_mfma_f32_16x16x32); a lane then holds 4 + 4 tokens of
+//     one column, which is the second operand of the product with V, so weights stay in registers;
+//   * K and V come in whole rows and go through the wave's own LDS one after the other, without a barrier: K is read as
+//     the first operand, rows 16 bytes further apart than they are long, V back transposed (ds_read_b64_tr_b16: four
+//     tokens of a dim to a lane), 32 bytes, so that the rows of a read take all banks alike (operands straight from memory,
+//     sixteen bytes of sixteen rows at a time: the batch above 137 us instead of 132);
+//   * K of the next tile is requested once LDS holds the present one's, V likewise; the first tile, which every row has,
+//     before the row's length is known;
 //   * a weight is rounded once to the 16-bit type, half a step, and its sum adds the rounded ones, so that
 //     what weights have in common cancels in the quotient; the rest averages out to about what the store's own
 //     rounding costs.  (A second part of a weight would be exact to 2^-17, but its product with an infinite value
 //     is NaN.)
+// Waves: four; eight for lone rows of sixteen columns (see split_few).  Registers: 117 for one block of columns at D = 64 to
+// 255 at 256, whose sums lie in the accumulators.
 #include "paged_attention.h"
 
 namespace tt {
@@ -46,12 +52,18 @@ void paged_few_kernel(PagedParams P) {
   __shared__ Seen see_s[MIXED ? 16 * NB : 1];
   __shared__ uint32_t marks_s[16 * NB * (D / 16)];
   __shared__ int marked;
-  // the shared pages' workgroups first, then the rows'; of each KV heads and column blocks, then rows, then splits
-  const bool shared_job = MIXED && (int)blockIdx.x < P.few[1].blocks;
+  // KV heads and column blocks, rows, splits are the grid's axes; where it holds two jobs, all in x, the shared pages' first
+  int x = blockIdx.x, row = blockIdx.y, split = blockIdx.z;
+  const bool both = MIXED && P.few[1].blocks > 0, shared_job = both && x < P.few[1].blocks;
   const FewJob J = P.few[shared_job ? 1 : 0];
-  const int block = (int)blockIdx.x - (MIXED && !shared_job ? P.few[1].blocks : 0);
-  const int kvhs = (int)P.c.kv_heads * J.row_tiles, rest = block / kvhs, split = rest / J.rows, row = rest - split * J.rows;
-  const int kvh = (block - rest * kvhs) / J.row_tiles, cb = block - rest * kvhs - kvh * J.row_tiles;
+  if (both) {
+    if (!shared_job) x -= P.few[1].blocks;
+    const int kvhs = (int)P.c.kv_heads * J.row_tiles, rest = x / kvhs;
+    split = rest / J.rows;
+    row = rest - split * J.rows;
+    x -= rest * kvhs;
+  }
+  const int kvh = J.row_tiles == 1 ? x : x / J.row_tiles, cb = x - kvh * J.row_tiles;
   const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int G = P.per_kv;
@@ -371,7 +383,10 @@ void paged_few_kernel(PagedParams P) {
 
 template <typename T, int D, int NB>
 static int launch_blocks(const PagedParams& P, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)(P.few[0].blocks + P.few[1].blocks));
+  const FewJob& own = P.few[0];
+  const int kvhs = (int)P.c.kv_heads * own.row_tiles;
+  const dim3 grid = P.few[1].blocks > 0 ? dim3((unsigned)(own.blocks + P.few[1].blocks))
+                                        : dim3((unsigned)kvhs, (unsigned)own.rows, (unsigned)(own.blocks / kvhs / own.rows));
   const bool mixed = P.few[1].blocks > 0 || P.of.each != 1;
   if constexpr (NB == 1 && D < 256) {
     if (P.wide && !mixed) {
