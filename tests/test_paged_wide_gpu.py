@@ -10,6 +10,7 @@ import torch
 
 from tests.paged_ref import same_bits
 from tests.test_paged_attention_gpu import _DT, _RAGGED, _check, _i32, _make, _run
+from thintensor_amd.paged_cache import PagedKvCache
 
 pytestmark = pytest.mark.gpu
 
@@ -173,3 +174,49 @@ def test_the_same_call_gives_the_same_bits(backend, device):
     first = run()
     for _ in range(3):
         assert all(same_bits(a, b) for a, b in zip(first, run()))
+
+
+def test_strided_operands_in_place(backend, device):
+    """q as an odd part of a fused row, out in place and as a view, a cache with its tokens before its heads."""
+    lengths, cu = [150, 131], [0, 130, 262]
+    cache, table, g = _make(device, 9, lengths, 16, 20, 64, "f16")
+    turned = PagedKvCache(cache.k_pages.transpose(1, 2).contiguous().transpose(1, 2), cache.v_pages.transpose(1, 2).contiguous().transpose(1, 2))
+    rows = torch.randn((262, 3 + 48 * 64), generator=g, device=device).half()
+    q = rows[:, 3:3 + 40 * 64].view(262, 40, 64)
+    q0 = q.contiguous()
+    out = _run(backend, device, cache, table, lengths, q0, cu)
+    _check(cache, table, lengths, q0, out, cu)
+    assert same_bits(out, _run(backend, device, turned, table, lengths, q, cu))
+    wide = torch.full((262, 40, 70), 5.0, device=device, dtype=torch.float16)
+    call = lambda to: backend.gqa_attention_paged(q, cache, _i32(table, device), _i32(lengths, device), to, cu_tokens=_i32(cu, device))  # noqa: E731
+    call(wide[..., 3:67])
+    assert same_bits(wide[..., 3:67], out) and torch.all(wide[..., :3] == 5.0) and torch.all(wide[..., 67:] == 5.0)
+    call(q)
+    assert same_bits(q, out)
+
+
+def test_far_pages(backend, device):
+    """Pages past 2^31 elements; more queries than tokens."""
+    page, kvh, dim = 256, 8, 256
+    pages = (1 << 31) // (page * kvh * dim) + 3
+    cache = PagedKvCache.allocate(pages, kvh, page, dim, device=device)
+    g = torch.Generator(device=device).manual_seed(1)
+    table = np.array([[pages - 1, 3, pages - 2]], dtype=np.int32)
+    for p in table[0]:
+        cache.k_pages[int(p)].normal_(generator=g)
+        cache.v_pages[int(p)].normal_(generator=g)
+    small = PagedKvCache(cache.k_pages[table[0].tolist()], cache.v_pages[table[0].tolist()])
+    q = torch.randn((1100, 8, dim), generator=g, device=device).half()
+    out = _run(backend, device, cache, table, [700], q)
+    assert same_bits(out, _run(backend, device, small, [[0, 1, 2]], [700], q)) and torch.all(out[:400] == 0)
+    _check(small, np.array([[0, 1, 2]]), [700], q[-90:], out[-90:])
+
+
+def test_wild_counts(backend, device):
+    """cu_tokens that no program should give: nothing outside the operands is touched."""
+    cache, table, g = _make(device, 3, [400, 400], 16, 20, 64, "f16")
+    for cu in ([-5, 3, 900], [300, 2, 390], [0, 0, 0], [4, 4, 2], [200, 100, 400]):
+        q = torch.randn((400, 40, 64), generator=g, device=device).half()
+        out = torch.full((402, 40, 64), 9.0, device=device, dtype=torch.float16)
+        backend.gqa_attention_paged(q, cache, _i32(table, device), _i32([400, 400], device), out[1:401], cu_tokens=_i32(cu, device))
+        assert torch.all(out[0] == 9.0) and torch.all(out[401] == 9.0)
