@@ -94,20 +94,30 @@ struct PagedPlan {
 // Workgroups that share a row's tokens, for `groups` of them that each may take up to `tiles` tiles of 32.  A
 // workgroup alone saves the join (3.7 us in a row of calls).  With a CU for each, eight waves instead of four have more on
 // its way (one row of 8 KV heads in a graph, us: x 64, 256 tokens 5.1 and 5.4, 512 7.0 and 6.1, 768 9.0 and 7.4, shared 8.6;
-// x 128, 256 tokens 6.9 and 6.6, 512 9.6 and 7.8, 768 12.3 and 9.6, shared 10.0).
-static void split_few(int64_t groups, int64_t tiles, bool parts, PagedJob* j) {
+// x 128, 256 tokens 6.9 and 6.6, 512 9.6 and 7.8, 768 12.3 and 9.6, shared 10.0).  Where rows are split, few and long
+// workgroups are best, two for each CU, or three for every four CUs where the rows alone are few: parts cost their sums,
+// short workgroups their start (us with 12, 4 and 2 a CU: 16 rows of 4001 tokens, 40 / 10 heads x 128, 75, 68 and 64, 64 rows
+// to 8001, 16 / 2 x 256, 167, 137 and 139; with 2, 1 and 3/4 a CU: one row of 120000, 64 / 8 x 128, 94.8, 92.2 and 90.4).
+// Lengths are on the device, so where a bound leaves room for rows much longer than others (past 8192 tokens) rows are
+// cut finer, and by 8192 tokens at the least (64 rows, 64 / 8 x 128: one of 65536 tokens among 500s 192 us, 642 with two
+// workgroups a CU; all of 500 30.7 and 24.6).  `cached`: at x 64, where rows read the same pages for themselves,
+// which come from the caches, a CU's own pace decides (eight rows of 16 columns behind 16384 tokens, 32 / 8 heads: 28 us with
+// two workgroups a CU, 43 with 3/4; wider heads and more rows are not slower by the rule above).
+static void split_few(int64_t groups, int64_t tiles, bool parts, bool cached, PagedJob* j) {
   const int64_t cus = device_cus();
   j->splits = 1;
   j->share = (int)tiles;
   j->wide = !parts && groups <= cus && tiles > 8;
   if (!parts && (tiles <= 24 || (groups >= cus && tiles <= 64))) return;
   j->wide = 0;
-  const int64_t want = groups >= cus / 2 ? 12 * cus : 2 * cus;
+  const bool uneven = !parts && tiles > 256;
+  const int64_t want = groups < cus / 2 ? (cached ? 2 * cus : 3 * cus / 4) : uneven ? 12 * cus : 2 * cus;
   int64_t share = (tiles * groups + want - 1) / want;
   if (share < 8) share = 8;
+  if (uneven && share > 256) share = 256;
   if (share < (tiles + 511) / 512) share = (tiles + 511) / 512;
   j->share = (int)share;
-  j->splits = (int)((tiles + share - 1) / share);
+  j->splits = (int)((tiles + share - 1) / share);        // (a short last one fills what the others leave)
   if (j->splits < 1) j->splits = 1;
 }
 
@@ -213,7 +223,7 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
     p.prefix.blocks16 = 4e-6 * reach_shared * c->kv_heads * c->head_dim < 8 ? 1 : blocks16(cols < 32 ? cols : 32);
     p.prefix.row_tiles = (int)((cols + 16 * p.prefix.blocks16 - 1) / (16 * p.prefix.blocks16));
     p.prefix.rows = 1;
-    split_few(c->kv_heads * p.prefix.row_tiles, (reach_shared + 31) / 32, true, &p.prefix);
+    split_few(c->kv_heads * p.prefix.row_tiles, (reach_shared + 31) / 32, true, false, &p.prefix);
   }
   // tokens of its own that a row's queries may see
   reach = p.limit > p.shared ? p.limit - p.shared : 0;
@@ -235,7 +245,8 @@ static PagedPlan plan(const tt_paged_cache* c, int64_t table_pages, bool ragged,
     p.own.row_tiles = (int)((most + 16 * p.own.blocks16 - 1) / (16 * p.own.blocks16));
     p.own.rows = (int)rows;
     // (one tile more where they may begin inside one)
-    split_few(rows * c->kv_heads, (reach + 31) / 32 + (p.window > 0 || p.shared % 32 != 0 ? 1 : 0), false, &p.own);
+    split_few(rows * c->kv_heads, (reach + 31) / 32 + (p.window > 0 || p.shared % 32 != 0 ? 1 : 0), false,
+              c->head_dim == 64 && shared_pages > 0 && p.shared == 0, &p.own);
     // a selection may name its pages anywhere in it
     const int64_t listed = (selected_count * c->page_size + 31) / 32;
     if (listed > p.own.splits * p.own.share) p.own.share = (int)((listed + p.own.splits - 1) / p.own.splits);

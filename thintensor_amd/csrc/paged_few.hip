@@ -4,7 +4,7 @@
 // shared pages.
 //
 // What bounds it is memory where rows are long, 4 D bytes a token and KV head (32 rows to 8001 tokens, 64 / 8 heads x 128:
-// 135 us, 4.9 TB/s of a large copy's 5.0), and otherwise its chain of round trips: queries and lengths, table, first tile,
+// 131 us, 5.1 TB/s of a large copy's 5.0), and otherwise its chain of round trips: queries and lengths, table, first tile,
 // join (575 tokens of one row, 32 / 8 x 64: 6 to 6.6 us in a graph, where a launch is 2).
 //   * scores are rows = tokens, columns = query heads (v_mfma_f32_16x16x32); a lane then holds 4 + 4 tokens of
 //     one column, which is the second operand of the product with V, so weights stay in registers;
