@@ -1713,8 +1713,9 @@ class HipDecodeBackend:
     def _paged_rows(what: str, page_table: torch.Tensor, per_row: torch.Tensor, name: str, cu_tokens: torch.Tensor | None,
                     tokens: int) -> int:
         """Checks the table, its rows' int32 values and their tokens; the number of rows."""
-        rows = page_table.shape[0] if page_table.ndim == 2 else -1
-        if rows < 0 or page_table.dtype != torch.int32 or (rows and (page_table.shape[1] < 1 or page_table.stride(1) != 1)):
+        shape = page_table.shape
+        rows = shape[0] if len(shape) == 2 else -1
+        if rows < 0 or page_table.dtype != torch.int32 or (rows and (shape[1] < 1 or page_table.stride(1) != 1)):
             raise ValueError(f"{what}: page_table must be int32 [rows, pages], contiguous in its last axis")
         if per_row.dtype != torch.int32 or per_row.numel() != rows or not per_row.is_contiguous():
             raise ValueError(f"{what}: {name} must be int32, one per row")
@@ -1754,8 +1755,9 @@ class HipDecodeBackend:
         else:
             if q_out is None:
                 q_out = q
-            qs, qos, heads = q.stride(), q_out.stride(), q.shape[1] if q.ndim == 3 else 0
-            if heads < 1 or tuple(q.shape) != (tokens, heads, head_dim) or q_out.shape != q.shape:
+            qs, qos, turned = q.stride(), q_out.stride(), q.shape
+            heads = turned[1] if len(turned) == 3 else 0
+            if heads < 1 or turned[0] != tokens or turned[2] != head_dim or q_out.shape != turned:
                 raise ValueError(f"{what} takes q and its output [tokens, heads, {head_dim}]")
             if q.dtype != dtype or q_out.dtype != dtype:
                 raise ValueError(f"{what} operands must have the cache's dtype {dtype}")
@@ -1809,12 +1811,13 @@ class HipDecodeBackend:
         table_pages = page_table.shape[1]
         count, sel_ptr, sink_ptr, sink_code = 0, None, None, _lib.F32
         if selected is not None:
-            if selected.dtype != torch.int32 or selected.ndim != 3 or tuple(selected.shape[:2]) != (rows, cache.kv_heads) or \
-                    selected.shape[2] < 1 or not selected.is_contiguous():
+            picked = selected.shape
+            if selected.dtype != torch.int32 or len(picked) != 3 or picked[0] != rows or picked[1] != cache.kv_heads or \
+                    picked[2] < 1 or not selected.is_contiguous():
                 raise ValueError(f"{what}: selected must be contiguous int32 [rows, kv_heads, count]")
             if tokens != rows or cu_tokens is not None or shared_pages:
                 raise ValueError(f"{what}: selected pages are for one query per row, without shared pages")
-            count, sel_ptr = selected.shape[2], selected.data_ptr()
+            count, sel_ptr = picked[2], selected.data_ptr()
         if sinks is not None:
             if sinks.numel() != heads or not sinks.is_contiguous():
                 raise ValueError(f"{what}: sinks must hold one logit per query head")
@@ -1856,7 +1859,8 @@ class HipDecodeBackend:
             raise ValueError(f"{what}: the cache keeps no k_bounds")
         if self._paged_rows(what, page_table, lengths, "lengths", None, rows) != rows:
             raise ValueError(f"{what} takes one query per row of the table")
-        if selected.dtype != torch.int32 or selected.ndim != 3 or tuple(selected.shape[:2]) != (rows, cache.kv_heads) or \
+        picked = selected.shape
+        if selected.dtype != torch.int32 or len(picked) != 3 or picked[0] != rows or picked[1] != cache.kv_heads or \
                 not selected.is_contiguous():
             raise ValueError(f"{what}: selected must be contiguous int32 [rows, kv_heads, count]")
         table_pages = page_table.shape[1]
@@ -1869,7 +1873,7 @@ class HipDecodeBackend:
         rc = _on_gpu(gpu, self.lib.tt_select_pages,
                      cache.desc, q.data_ptr(), qs[0], qs[1], page_table.data_ptr(), page_table.stride(0), table_pages,
                      lengths.data_ptr(), rows, heads, first_pages, last_pages, limit,
-                     scratch.data_ptr() if need else None, need, selected.data_ptr(), selected.shape[2])
+                     scratch.data_ptr() if need else None, need, selected.data_ptr(), picked[2])
         if rc:
             _lib.check(rc, what)
         return selected

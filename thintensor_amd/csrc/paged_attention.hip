@@ -99,7 +99,7 @@ struct PagedPlan {
 // short workgroups their start (us with 12, 4 and 2 a CU: 16 rows of 4001 tokens, 40 / 10 heads x 128, 75, 68 and 64, 64 rows
 // to 8001, 16 / 2 x 256, 167, 137 and 139; with 2, 1 and 3/4 a CU: one row of 120000, 64 / 8 x 128, 94.8, 92.2 and 90.4).
 // Lengths are on the device, so where a bound leaves room for rows much longer than others (past 8192 tokens) rows are
-// cut finer, and by 8192 tokens at the least (64 rows, 64 / 8 x 128: one of 65536 tokens among 500s 192 us, 642 with two
+// cut finer, and by 8192 tokens at the least while that is no more than 32 workgroups a CU (64 rows, 64 / 8 x 128: one of 65536 tokens among 500s 192 us, 642 with two
 // workgroups a CU; all of 500 30.7 and 24.6).  `cached`: at x 64, where rows read the same pages for themselves,
 // which come from the caches, a CU's own pace decides (eight rows of 16 columns behind 16384 tokens, 32 / 8 heads: 28 us with
 // two workgroups a CU, 43 with 3/4; wider heads and more rows are not slower by the rule above).
@@ -114,7 +114,8 @@ static void split_few(int64_t groups, int64_t tiles, bool parts, bool cached, Pa
   const int64_t want = groups < cus / 2 ? (cached ? 2 * cus : 3 * cus / 4) : uneven ? 12 * cus : 2 * cus;
   int64_t share = (tiles * groups + want - 1) / want;
   if (share < 8) share = 8;
-  if (uneven && share > 256) share = 256;
+  const int64_t finest = (tiles * groups + 32 * cus - 1) / (32 * cus);      // (most of these workgroups find nothing to do)
+  if (uneven && share > 256) share = finest > 256 ? finest : 256;
   if (share < (tiles + 511) / 512) share = (tiles + 511) / 512;
   j->share = (int)share;
   j->splits = (int)((tiles + share - 1) / share);        // (a short last one fills what the others leave)
