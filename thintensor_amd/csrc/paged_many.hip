@@ -66,17 +66,17 @@ void paged_many_kernel(PagedParams P, int splits) {
 
   // Workgroups go to the eight XCDs in turn.  Of kvhs = 8 F + R heads an XCD takes F by itself, so that their K and V come
   // to its L2 alone, and an eighth of the tiles of the others; eight tiles of all heads follow the eight before.
-  const int kvhs = (int)P.c.kv_heads, xcd = blockIdx.x & 7, turn = blockIdx.x >> 3, full = kvhs >> 3;
-  const int eight = turn / kvhs, i = turn - eight * kvhs;
-  int kvh, rest = 8 * eight;
+  const int kvhs = (int)P.c.kv_heads, xcd = blockIdx.x & 7, i = blockIdx.x >> 3, full = kvhs >> 3;
+  int kvh, rest = 8 * (blockIdx.y + gridDim.y * blockIdx.z);
   if (i < 8 * full) {
-    kvh = xcd * full + i % full;
-    rest += i / full;
+    const int of = full == 1 ? i : i / full;
+    kvh = xcd * full + i - of * full;
+    rest += of;
   } else {
     kvh = i;
     rest += (xcd + i) & 7;
   }
-  const int split = rest % splits, x_first = rest / splits, x = P.tiles - 1 - x_first;
+  const int x_first = splits == 1 ? rest : rest / splits, split = rest - x_first * splits, x = P.tiles - 1 - x_first;
   if (x < 0) return;
   const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -384,7 +384,8 @@ void paged_many_kernel(PagedParams P, int splits) {
 
 template <typename T, int D>
 static int launch_dim(const PagedParams& P, int waves, int splits, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)(P.c.kv_heads * 8 * ((P.tiles * splits + 7) / 8)));
+  const unsigned eights = ((unsigned)P.tiles * splits + 7) / 8, most = 32768;
+  const dim3 grid((unsigned)P.c.kv_heads * 8, eights < most ? eights : most, (eights + most - 1) / most);
   if constexpr (D < 256) {
     if (waves == 4) {
       hipLaunchKernelGGL((paged_many_kernel<T, D, 4>), grid, dim3(64 * 4), 0, st, P, splits);
