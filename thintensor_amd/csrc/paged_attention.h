@@ -1,9 +1,10 @@
 // Attention over the paged cache: what its kernels share.
 //
-// A launch serves one job: the rows' own pages (every row's queries against the tokens that the row
-// does not share), or the shared pages (all rows' queries against them, from row 0's table).  Either
-// way the queries of a KV head are columns: column c is query head c % per_kv of the job's token
-// c / per_kv, sees the tokens lo <= t < hi, and a row's keys meet all its columns at once.
+// There are two jobs: the rows' own pages (every row's queries against the tokens that the row does not
+// share), and the shared pages (all rows' queries against them, from row 0's table).  A launch of the kernel for many
+// columns serves one, that for few may serve both.  Either way the queries of a KV head are columns: column c is
+// query head c % per_kv of the job's token c / per_kv, sees the tokens lo <= t < hi, and a tile of keys meets
+// all columns of a workgroup at once.
 #pragma once
 
 #include "paged.h"
@@ -253,7 +254,7 @@ struct Marks {
   }
 };
 
-// paged_few.hip: up to few_columns() columns of a row and KV head; paged_many.hip: any number
+// paged_few.hip: blocks of up to few_columns() columns of a row and KV head; paged_many.hip: 128 or 256
 constexpr int few_columns(int64_t head_dim) { return head_dim == 64 ? 64 : head_dim == 128 ? 32 : 16; }
 int launch_paged_few(const PagedParams& P, int blocks16, hipStream_t st, const char* what);
 int launch_paged_many(const PagedParams& P, int waves, int splits, hipStream_t st, const char* what);
