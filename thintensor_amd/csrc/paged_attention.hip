@@ -4,7 +4,8 @@
 namespace tt {
 
 // Joins the parts of one (token, head).  Every wave forms all weights; sixteen bytes of a part's sum per
-// thread, the parts dealt over the threads' rows and joined in LDS.  A part without weight is not read.
+// thread, the parts dealt over the threads' rows and joined in LDS.  A part without weight is not read,
+// nor does its maximum count.
 template <typename T, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedParams P) {
   constexpr int PIECES = D / 4, ROWS = THREADS / PIECES;
@@ -23,7 +24,10 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedParams P) {
   }
   const float ninf = __builtin_bit_cast(float, 0xff800000u);
   float M = ninf;
-  for (int k = lane; k < P.parts; k += 64) M = fmaxf(M, ml[k].x);
+  for (int k = lane; k < P.parts; k += 64) {
+    const float2 v = ml[k];
+    if (v.y != 0.0f) M = fmaxf(M, v.x);                // (NaN counts)
+  }
 #define TT_LEVEL(X) M = fmaxf(M, xor_partner<X>(M));
   TT_LEVEL(1) TT_LEVEL(2) TT_LEVEL(4) TT_LEVEL(8) TT_LEVEL(16) TT_LEVEL(32)
 #undef TT_LEVEL

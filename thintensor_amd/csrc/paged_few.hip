@@ -145,7 +145,7 @@ void paged_few_kernel(PagedParams P) {
       const int r = row_of(P.of, token[b], &place, &each);
       see[b] = r < P.of.rows ? seen_of(P, true, row_length(P, r), place, each) : Seen{0, 0};
       see[b].hi = max(see[b].hi, 0);
-      if (see[b].hi > see[b].lo) {         // (one that sees nothing may compute what it will, it ends without weight)
+      if (see[b].hi > see[b].lo) {         // (one that sees nothing may compute what it will, it ends without weight and maximum)
         hi_most = max(hi_most, see[b].hi); hl = min(hl, see[b].hi);
         ll = min(ll, see[b].lo); lm = max(lm, see[b].lo);
       }
@@ -338,12 +338,13 @@ void paged_few_kernel(PagedParams P) {
   float* const o_s = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int b = 0; b < NB; b++) {
-    const float l_col = see[b].hi <= see[b].lo ? 0.0f : bfly<32>(bfly<16>(l_run[b]));
+    const bool blind = see[b].hi <= see[b].lo;
+    const float l_col = blind ? 0.0f : bfly<32>(bfly<16>(l_run[b]));
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < VT; x++) *reinterpret_cast<f4_t*>(o_s + (wave * 16 + n) * OS + 16 * x + 4 * quad) = o[b][x];
     if (quad == 0) {
-      m_s[wave][n] = m_run[b];
+      m_s[wave][n] = blind ? ninf : m_run[b];
       l_s[wave][n] = l_col;
     }
     __syncthreads();

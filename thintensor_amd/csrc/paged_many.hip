@@ -154,7 +154,7 @@ void paged_many_kernel(PagedParams P, int splits) {
 #undef TT_LEVEL
     return __builtin_amdgcn_readfirstlane(v);
   };
-  // (a column that sees nothing may compute what it will, it ends without weight)
+  // (a column that sees nothing may compute what it will, it ends without weight and maximum)
   constexpr int kFar = 0x7fffffff;
   const bool blind = see.hi <= see.lo;
   const int hi_most = most(blind ? 0 : see.hi), hi_least = -most(blind ? -kFar : -see.hi);
@@ -347,7 +347,7 @@ void paged_many_kernel(PagedParams P, int splits) {
   // ---- through LDS, so that whole vectors are written: up to 128 dims of the wave's columns at a time
   const float l = blind ? 0.0f : bfly<32>(l_run);
   const float f = only ? finish_scale(P, head, m_run, l) : 1.0f;
-  if (!only && mine && half == 0) P.part_ml[part] = make_float2(m_run, l);
+  if (!only && mine && half == 0) P.part_ml[part] = make_float2(blind ? ninf : m_run, l);
   const bool any_marks = marked != 0;
   constexpr int DD = WAVES == 8 ? 32 : D, OS = DD + 4, LANES = DD / 4, COLS = 64 / LANES;
   static_assert(WAVES * 32 * OS * 4 <= 2 * BUF, "the wave's sums fit where tiles were");
