@@ -871,7 +871,8 @@ int tt_sample_rows(const void* logits, int64_t row_stride, int dtype, int64_t ro
  * boundary.  k_bounds (or NULL) [pages, kv_heads, 2, head_dim], the last two axes contiguous: of
  * every dim the least and the greatest key of the page.  page_size 16, 32, 64, 128 or 256; head_dim
  * 64, 128 or 256; a page's tokens lie in order (strides not negative) within 2 GiB.  Token t of a row lies in
- * page table[row, t / page_size], slot t % page_size. */
+ * page table[row, t / page_size], slot t % page_size.  A call without rows does nothing; its table may be without
+ * pages then, and max_length 0. */
 typedef struct {
   void *k_pages, *v_pages, *k_bounds;
   int64_t k_page, k_head, k_token, v_page, v_head, v_token, b_page, b_head;

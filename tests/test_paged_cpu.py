@@ -209,6 +209,17 @@ def test_nothing_to_do(be):
     assert _call_select(be.lib, rows=0) == 0
 
 
+def test_an_empty_batch_may_have_a_table_of_no_pages(be):
+    c = _desc()
+    assert _call_append(be.lib, rows=0, tokens=0, tr=0, tp=0) == 0
+    assert be.lib.tt_gqa_attention_paged_scratch_floats(c, 0, 0, 0, 0, 4, 0, 0, 0, 0) == 0
+    assert _call_attention(be.lib, rows=0, tokens=0, tr=0, tp=0, limit=0) == 0
+    assert be.lib.tt_select_pages_scratch_floats(c, 0, 0, 0) == 0
+    assert _call_select(be.lib, rows=0, tr=0, tp=0, limit=0) == 0
+    for f in (_call_append, _call_attention, _call_select):
+        assert f(be.lib, rows=0, tp=-1, **({} if f is _call_select else dict(tokens=0))) == -1
+
+
 # ------------------------------------------------------------------ the restatements on known rows
 def test_restated_attention_on_known_rows():
     rng = np.random.default_rng(0)

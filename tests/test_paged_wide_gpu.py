@@ -176,6 +176,23 @@ def test_the_same_call_gives_the_same_bits(backend, device):
         assert all(same_bits(a, b) for a, b in zip(first, run()))
 
 
+def test_empty_batches(backend, device):
+    """No rows, and a table without pages: nothing happens; tokens behind the last row stay."""
+    cache, _, g = _make(device, 4, [20], 16, 2, 64, "f16")
+    before = [t.clone() for t in (cache.k_pages, cache.v_pages, cache.k_bounds)]
+    for width in (0, 3):
+        for tokens in (0, 4):
+            cu = _i32([0], device) if tokens else None
+            table, none = _i32(np.zeros((0, width)), device), _i32([], device)
+            q, kv = (torch.randn((tokens, h, 64), generator=g, device=device).half() for h in (4, 2))
+            turned, out = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+            backend.rotary_append_paged(cache, q, kv, kv.clone(), table, none, None, turned, cu_tokens=cu)
+            backend.gqa_attention_paged(q, cache, table, none, out, cu_tokens=cu)
+            backend.select_pages(q[:0], cache, table, none, _i32(np.zeros((0, 2, 5)), device))
+            assert torch.all(out == 9.0) and torch.all(turned == 9.0)
+    assert all(same_bits(a, b) for a, b in zip(before, (cache.k_pages, cache.v_pages, cache.k_bounds)))
+
+
 def test_strided_operands_in_place(backend, device):
     """q as an odd part of a fused row, out in place and as a view, a cache with its tokens before its heads."""
     lengths, cu = [150, 131], [0, 130, 262]

@@ -27,7 +27,7 @@ inline int check_paged(const tt_paged_cache* c, const char* what) {
   return TT_OK;
 }
 
-// The table and the rows' tokens: what every operator on pages takes.
+// The table (of no pages where there are no rows) and the rows' tokens: what every operator on pages takes.
 inline int check_rows(const tt_paged_cache* c, int64_t table_pages, bool ragged, int64_t rows, int64_t tokens, int64_t heads,
                       const char* what) {
   const int rc = check_paged(c, what);
@@ -36,7 +36,7 @@ inline int check_rows(const tt_paged_cache* c, int64_t table_pages, bool ragged,
   TT_REQUIRE(tokens >= 0 && tokens <= (1 << 22), "%s: at most 2^22 tokens", what);
   TT_REQUIRE(ragged || tokens == 0 || (rows > 0 && tokens % rows == 0), "%s: tokens must divide over the rows", what);
   TT_REQUIRE(heads % c->kv_heads == 0 && heads <= 65535, "%s: heads must be a multiple of kv_heads (65535 at most)", what);
-  TT_REQUIRE(table_pages > 0 && table_pages * c->page_size < (1LL << 30), "%s: a row's pages must hold fewer than 2^30 tokens", what);
+  TT_REQUIRE(table_pages >= (rows > 0) && table_pages * c->page_size < (1LL << 30), "%s: a row's pages must hold fewer than 2^30 tokens", what);
   return TT_OK;
 }
 

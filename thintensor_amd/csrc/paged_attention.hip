@@ -285,7 +285,7 @@ static int check_attention(const tt_paged_cache* c, int64_t table_pages, bool ra
   const int rc = check_rows(c, table_pages, ragged, rows, tokens, heads, what);
   if (rc) return rc;
   TT_REQUIRE(heads > 0, "%s: heads must be a multiple of kv_heads", what);
-  TT_REQUIRE(window >= 0 && max_length > 0, "%s: window must not be negative, max_length at least 1", what);
+  TT_REQUIRE(window >= 0 && max_length >= (rows > 0), "%s: window must not be negative, max_length at least 1", what);
   TT_REQUIRE(shared_pages >= 0 && shared_pages <= table_pages, "%s: shared_pages outside the table", what);
   TT_REQUIRE((tokens * heads) / 128 + rows * c->kv_heads < (1 << 23), "%s: too many queries for one call", what);
   TT_REQUIRE(selected_count >= 0 && selected_count <= 65536 && (selected_count == 0 || (!ragged && tokens == rows && shared_pages == 0)),

@@ -305,7 +305,7 @@ static int check_select(const tt_paged_cache* c, int64_t table_pages, int64_t ro
   const int rc = check_rows(c, table_pages, false, rows, rows, heads, what);
   if (rc) return rc;
   TT_REQUIRE(c->k_bounds, "%s: the cache keeps no k_bounds", what);
-  TT_REQUIRE(max_length > 0, "%s: max_length must be at least 1", what);
+  TT_REQUIRE(max_length >= (rows > 0), "%s: max_length must be at least 1", what);
   return TT_OK;
 }
 
