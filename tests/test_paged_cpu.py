@@ -87,6 +87,16 @@ def test_append_refusals(be, change):
         be.rotary_append_paged(**{**_append_args(), **change})
 
 
+@pytest.mark.parametrize("width,right", [(1, True), (2, False)])
+def test_tables_of_one_page_have_any_stride_there(be, width, right):
+    table = _i32(3, 2).t()[:, :width]
+    assert table.stride() == (1, 2)
+    with pytest.raises(ValueError, match="device tensors" if right else "page_table"):
+        be.rotary_append_paged(**{**_append_args(), "page_table": table})
+    with pytest.raises(ValueError, match="device tensors" if right else "page_table"):
+        be.gqa_attention_paged(**{**_attention_args(), "page_table": table})
+
+
 def _attention_args():
     return {"q": _f16(4, 4, 64), "cache": _cache(), "page_table": _i32(2, 3), "lengths": _i32(2), "out": _f16(4, 4, 64)}
 

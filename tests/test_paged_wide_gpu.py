@@ -193,6 +193,22 @@ def test_empty_batches(backend, device):
     assert all(same_bits(a, b) for a, b in zip(before, (cache.k_pages, cache.v_pages, cache.k_bounds)))
 
 
+def test_a_table_that_is_a_column(backend, device):
+    cache, table, g = _make(device, 5, [13, 16], 16, 2, 64, "f16")
+    q, k, v = (torch.randn((2, h, 64), generator=g, device=device).half() for h in (4, 2, 2))
+    plain = _run(backend, device, cache, table, [13, 16], q)
+    column = torch.stack((_i32(table[:, 0], device), _i32([-1, -1], device)), 0).t()[:, :1]
+    assert column.stride() == (1, 2)
+    out = torch.empty_like(q)
+    backend.gqa_attention_paged(q, cache, column, _i32([13, 16], device), out)
+    assert same_bits(plain, out)
+    backend.rotary_append_paged(cache, None, k, v, column, _i32([3, 9], device), None)
+    for r, slot in enumerate((3, 9)):
+        assert same_bits(cache.k_pages[int(table[r, 0]), :, slot], k[r]) and same_bits(cache.v_pages[int(table[r, 0]), :, slot], v[r])
+    sel = backend.select_pages(q, cache, column, _i32([13, 0], device), _i32(np.zeros((2, 2, 2)), device), first_pages=0, last_pages=1)
+    assert sel.tolist() == [[[0, -1]] * 2, [[-1, -1]] * 2]
+
+
 def test_strided_operands_in_place(backend, device):
     """q as an odd part of a fused row, out in place and as a view, a cache with its tokens before its heads."""
     lengths, cu = [150, 131], [0, 130, 262]

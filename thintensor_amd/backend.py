@@ -1715,7 +1715,7 @@ class HipDecodeBackend:
         """Checks the table, its rows' int32 values and their tokens; the number of rows."""
         shape = page_table.shape
         rows = shape[0] if len(shape) == 2 else -1
-        if rows < 0 or page_table.dtype != torch.int32 or (rows and (shape[1] < 1 or page_table.stride(1) != 1)):
+        if rows < 0 or page_table.dtype != torch.int32 or (rows and (shape[1] < 1 or (shape[1] > 1 and page_table.stride(1) != 1))):
             raise ValueError(f"{what}: page_table must be int32 [rows, pages], contiguous in its last axis")
         if per_row.dtype != torch.int32 or per_row.numel() != rows or not per_row.is_contiguous():
             raise ValueError(f"{what}: {name} must be int32, one per row")
