@@ -935,6 +935,7 @@ int tt_gqa_attention_paged(const tt_paged_cache* cache, const void* q, int64_t q
  *   max over its heads of sum_d max(q_d low_d, q_d high_d),
  * summed in binary64 (to 2^-50 of the sum of |q_d| max(|low_d|, |high_d|)) and rounded to binary32; of equal scores
  * the lower page is taken, NaN counts as the greatest, and so does the score of a table entry that is no page.
+ * selected shares no memory with what is read here, the cache or scratch, which is refused.
  * scratch: tt_select_pages_scratch_floats, for one call at a time. */
 int64_t tt_select_pages_scratch_floats(const tt_paged_cache* cache, int64_t table_pages, int64_t rows, int64_t max_length);
 int tt_select_pages(const tt_paged_cache* cache, const void* q, int64_t q_token, int64_t q_head, const int32_t* table,

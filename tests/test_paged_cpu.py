@@ -213,6 +213,12 @@ def test_select_entry_refuses(be, change):
     assert be.lib.tt_last_error()
 
 
+@pytest.mark.parametrize("sel", [_P, _P + 2 * 192, (_P << 3) + 20, _P << 4, (_P << 4) + 4, _BASE << 8, _BASE + 4096, (_BASE << 4) + 24000])
+def test_selection_shares_no_memory(be, sel):
+    assert _call_select(be.lib, sel=sel) == -1
+    assert b"share memory" in be.lib.tt_last_error()
+
+
 def test_nothing_to_do(be):
     for f in (_call_append, _call_attention):
         assert f(be.lib, rows=0, tokens=0) == 0 and f(be.lib, tokens=0) == 0

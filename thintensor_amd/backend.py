@@ -1847,7 +1847,7 @@ class HipDecodeBackend:
         with the greatest score, as many as ``selected`` (int32 [rows, kv_heads, count]) takes, in ascending order, -1
         behind them.  A page's score is the greatest product that a key within the cache's ``k_bounds`` of that page can
         have with one of the KV head's queries, summed in float64 and rounded to float32; of equal ones the lower page is
-        taken.  ``max_length`` as in :meth:`gqa_attention_paged`."""
+        taken.  ``selected`` shares no memory with the other tensors.  ``max_length`` as in :meth:`gqa_attention_paged`."""
         what = "select_pages"
         shape, qs = q.shape, q.stride()
         if len(shape) != 3 or q.dtype != cache.dtype or qs[2] != 1:

@@ -339,6 +339,11 @@ extern "C" int tt_select_pages(const tt_paged_cache* cache, const void* q, int64
   TT_REQUIRE(q && table && lengths && selected && scratch, "%s: null pointer", what);
   const int64_t most = most_pages(cache, table_pages, max_length);
   TT_REQUIRE(scratch_floats >= rows * cache->kv_heads * most, "%s: scratch too small", what);
+  const Region made(selected, 4, selected_count, {{rows, cache->kv_heads * selected_count}, {cache->kv_heads, selected_count}});
+  TT_REQUIRE(PagedRegions(cache).apart_from(made) && apart(made, {q, 2, cache->head_dim, {{rows, q_token}, {heads, q_head}}}) &&
+                 apart(made, {table, 4, table_pages, {{rows, table_row}}}) && apart(made, {lengths, 4, rows, {}}) &&
+                 apart(made, {scratch, 4, rows * cache->kv_heads * most, {}}),
+             "%s: selected must not share memory with q, the cache, the table, lengths or scratch", what);
   SelectParams P{};
   P.c = *cache;
   P.q = q; P.q_token = q_token; P.q_head = q_head;
