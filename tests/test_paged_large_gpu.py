@@ -121,3 +121,19 @@ def test_a_bound_on_lengths(backend, device):
     lengths = [500, 33, 1200, 0]
     for limit in (None, 1200, 4096):
         _check(backend, device, lengths, [1] * 4, 16, 2, 128, 16, torch.bfloat16, uniform=True, max_length=limit)
+
+
+@pytest.mark.parametrize("kvh,window", [(16, 0), (32, 5)])
+def test_most_rows_and_the_widest_table(backend, device, kvh, window):
+    """65535 rows and tables of 2^30 - 256 tokens, which all rows share: by themselves and, with a window,
+    by the kernel for few columns.  Slot t holds t + 1, and an odd number of tokens are seen: the mean is exact."""
+    rows, pages = 65535, (1 << 22) - 1
+    cache = PagedKvCache.allocate(1, kvh, 256, 64, device=device)
+    cache.v_pages.copy_(torch.arange(1, 257, device=device)[:, None])
+    table = torch.zeros((1, pages), device=device, dtype=torch.int32).expand(rows, pages)
+    lengths = 1 + 2 * (torch.arange(rows, device=device, dtype=torch.int32) % 100)
+    q = torch.ones((rows, kvh, 64), device=device, dtype=torch.float16)
+    out = torch.full_like(q, float("nan"))
+    backend.gqa_attention_paged(q, cache, table, lengths, out, window=window, shared_pages=pages if window else 0)
+    want = (lengths + (lengths - window).clamp_min(0) + 1) / 2 if window else (lengths + 1) / 2
+    assert int((out != want.half()[:, None, None]).sum()) == 0

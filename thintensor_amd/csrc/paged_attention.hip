@@ -121,6 +121,7 @@ static void split_few(int64_t groups, int64_t tiles, bool parts, bool cached, Pa
   const int64_t finest = (tiles * groups + 32 * cus - 1) / (32 * cus);      // (most of these workgroups find nothing to do)
   if (uneven && share > 256) share = finest > 256 ? finest : 256;
   if (share < (tiles + 511) / 512) share = (tiles + 511) / 512;
+  if (share > tiles) share = tiles;                      // (rows enough for one part each ask for any share)
   j->share = (int)share;
   j->splits = (int)((tiles + share - 1) / share);        // (a short last one fills what the others leave)
   if (j->splits < 1) j->splits = 1;
