@@ -137,3 +137,16 @@ def test_most_rows_and_the_widest_table(backend, device, kvh, window):
     backend.gqa_attention_paged(q, cache, table, lengths, out, window=window, shared_pages=pages if window else 0)
     want = (lengths + (lengths - window).clamp_min(0) + 1) / 2 if window else (lengths + 1) / 2
     assert int((out != want.half()[:, None, None]).sum()) == 0
+
+
+def test_most_heads_of_a_kv_head_behind_many_tokens(backend, device):
+    """65535 query heads of one KV head, with 2^23 + 2^18 tokens in one row and few in three: the longest column tiles begin
+    first.  Values are 1 and 3 in turn, so the mean of an even number is exact."""
+    heads, lengths = 65535, [256, (1 << 23) + (1 << 18), 2, 258]
+    cache = PagedKvCache.allocate(1, 1, 256, 64, device=device)
+    cache.v_pages.copy_(1 + 2 * (torch.arange(256, device=device) % 2)[:, None])
+    table = torch.zeros((4, max(lengths) // 256), device=device, dtype=torch.int32)
+    q = torch.ones((4, heads, 64), device=device, dtype=torch.float16)
+    out = torch.full_like(q, float("nan"))
+    backend.gqa_attention_paged(q, cache, table, torch.tensor(lengths, device=device, dtype=torch.int32), out)
+    assert (out != 2).sum((1, 2)).tolist() == [0, 0, 0, 0]

@@ -26,7 +26,8 @@ template <int COLUMNS>
 __device__ __forceinline__ bool longest(const PagedParams& P, int x, int count, int len, int* row, int* tile) {
   const int lane = threadIdx.x & 63;
   int n = count;
-  const int b = (int)(((int64_t)max(len - n, 0) * P.per_kv) / COLUMNS);
+  const int64_t before = ((int64_t)max(len - n, 0) * P.per_kv) / COLUMNS;
+  const int b = (int)min(before, (int64_t)1 << 29);        // (longer ones need no order, sums of it have to stay in range)
   n = lane < P.of.rows ? (int)(((int64_t)n * P.per_kv + COLUMNS - 1) / COLUMNS) : 0;
   auto at_least = [&](int h) __attribute__((always_inline)) {
     return (int)__builtin_amdgcn_readlane((int)lanes_before((uint32_t)min(max(b + n - h + 1, 0), n)), 63);
