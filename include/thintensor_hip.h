@@ -905,7 +905,9 @@ int tt_rotary_append_paged(const tt_paged_cache* cache, const void* q, int64_t q
  * and with window > 0 only t >= e - window.  out = sum p v with p the softmax of scale q.k and, where sinks
  * [heads] is given, of the sink's logit, which carries no value; a query that sees nothing is 0.  Queries behind
  * the last row are left as they were.  A query that sees a token whose table entry is no page is NaN; one whose
- * scores are all -inf counts as seeing nothing.
+ * scores are all -inf counts as seeing nothing.  Weights are rounded once to the cache's dtype, half a step of it, for
+ * the product with v and for their sum alike.  An infinite value that a query sees makes that dim of its output infinite, or
+ * NaN where its weight is rounded to 0.  What a query does not see has no part in it.
  * shared_pages: the first ones of every row's table are the same pages (only row 0's entries are used): they are
  * computed once for all rows where that costs less, and rows end where their lengths say, inside them too.
  * selected (or NULL) int32 [rows, kv_heads, selected_count], one query a row, no shared pages: only the tokens

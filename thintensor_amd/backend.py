@@ -1790,7 +1790,9 @@ class HipDecodeBackend:
         tokens belong to rows as in :meth:`rotary_append_paged`.  With ``window`` > 0 a query sees the last
         ``window`` tokens up to its own.  ``sinks`` [heads] are logits that join the softmax and carry no value;
         ``scale`` is head_dim ** -0.5 by default.  A query that sees nothing, or only scores of -inf, is 0, one that
-        needs an entry of the table that is no page NaN; queries behind the last row are left as they were.
+        needs an entry of the table that is no page NaN; queries behind the last row are left as they were.  Weights of the
+        softmax are rounded once to the cache's type, so an infinite value that a query sees makes its output infinite, or NaN
+        where its weight is rounded to 0.
         ``shared_pages``: so many first entries of the table are the same in every row (row 0's are read), and
         these pages are computed once for the whole batch where that costs less.  ``selected`` (int32 [rows,
         kv_heads, count], as from :meth:`select_pages`: places in the table, each at most once, negative ones skipped; one

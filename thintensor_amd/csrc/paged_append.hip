@@ -5,8 +5,10 @@
 // then have one writer, which keeps the extremes of its places in registers and joins them in LDS, and no atomics
 // are needed.  Those of queries take a few tokens with all their heads.
 // 16384 tokens, 64 + 8 heads x 128, take 136 to 144 us (4.8 TB/s; a large copy 5.0), 517 and less of 12 rows with bounds, 40 +
-// 10 heads, 15 to 17; one token of eight rows 4.9 in a graph.  One workgroup for each head and page instead of several heads
-// leaves short runs to the launch; one piece requested at a time 20.6 and 146 (loads wait behind stores).
+// 10 heads, 15 to 17; one token of eight rows 4.8 (4.5 a call in a graph).  One workgroup for each head and page instead of
+// several heads leaves short runs to the launch; one piece requested at a time 20.6 and 146 (loads wait behind stores).
+// A page's tokens are not divided, so few heads and large pages leave CUs without work: 2048 tokens of one row, 16 + 2 heads
+// x 256, take 63 us in pages of 256 tokens (18 workgroups) and 11 in pages of 16, 32 + 8 heads x 128 36 and 16.
 #include "paged.h"
 #include "tt_common.h"
 #include "tt_eight.h"
@@ -353,7 +355,9 @@ __global__ __launch_bounds__(256) void append_vec_kernel(AppendParams P) {
   }
 }
 
-// Any strides, alignment and rotary dims: a thread per pair or copied dim, one token after another.
+// Any strides, alignment and rotary dims: a thread per pair or copied dim, one token after another, all heads of a row's
+// page by one workgroup.  (16384 tokens, 64 + 8 heads x 128, with q, or k and v, an element off a 16-byte boundary: 944 us instead
+// of 129; 512, 32 + 8 heads, 327 instead of 11.)
 template <typename T>
 __global__ __launch_bounds__(256) void append_kernel(AppendParams P) {
   __shared__ float2 turn[128];

@@ -104,7 +104,9 @@ struct PagedPlan {
 // to 8001, 16 / 2 x 256, 167, 137 and 139; with 2, 1 and 3/4 a CU: one row of 120000, 64 / 8 x 128, 94.8, 92.2 and 90.4).
 // Lengths are on the device, so where a bound leaves room for rows much longer than others (past 8192 tokens) rows are
 // cut finer, and by 8192 tokens at the least while that is no more than 32 workgroups a CU (64 rows, 64 / 8 x 128: one of 65536 tokens among 500s 192 us, 642 with two
-// workgroups a CU; all of 500 30.7 and 24.6).  `cached`: at x 64, where rows read the same pages for themselves,
+// workgroups a CU; all of 500 30.7 and 24.6).  Rows of like length lose little to it where tables are wider than they need
+// (32 rows of 4001 to 8001 tokens, 64 / 8 x 128, bound at 8192, 8256, 32768 and 131072: 154, 162, 156 and 152 us in 2, 12, 12 and
+// 16 parts; 4000 tokens each, bound at 4032 and 32768, 98 and 100).  `cached`: at x 64, where rows read the same pages for themselves,
 // which come from the caches, a CU's own pace decides (eight rows of 16 columns behind 16384 tokens, 32 / 8 heads: 28 us with
 // two workgroups a CU, 43 with 3/4; wider heads and more rows are not slower by the rule above).
 static void split_few(int64_t groups, int64_t tiles, bool parts, bool cached, PagedJob* j) {
@@ -145,7 +147,9 @@ static int many_per_cu(int64_t head_dim, int waves) { return waves == 8 ? (head_
 // Workgroups that share a column tile's tokens, enough to fill the card, with at least six tiles each: a part costs the
 // write and the reading of its sums, and the join its launch (one row of 512 tokens, 40 heads of 128: 32.3 us in two parts of
 // four tiles, 24.7 in one; 512 behind 4096 70.5 with at least four tiles, 66.8 with six, 65.8 with eight; 49 rows of eight
-// heads behind 30496 shared tokens 40.8, 42.6 and 45.7).
+// heads behind 30496 shared tokens 40.8, 42.6 and 45.7).  Lengths are on the device, so one long row among short ones is one
+// workgroup a KV head where the tiles of all rows fill the card: seven single tokens behind 65536 beside a chunk of 512 of
+// another row, 64 / 8 x 128, take 1871 us, as two calls 321 and 26.
 static void split_many(int64_t groups, int64_t tiles, int per_cu, PagedJob* j) {
   const int64_t most = tiles / 6, fill = per_cu * device_cus() / (groups > 0 ? groups : 1);
   int64_t s = most < fill ? most : fill;
